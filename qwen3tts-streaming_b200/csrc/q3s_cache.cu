@@ -1,0 +1,407 @@
+// q3s_cache.cu -- the paged key/value cache's bookkeeping (q3s_cache_tables)
+// and append (q3s_cache_append).
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "q3s_args.cuh"
+#include "q3s_decode.h"
+#include "q3s_device.cuh"
+
+namespace q3s {
+
+struct TablesArgs {
+  int B, bs, max_blocks, ring, max_tokens;
+  const int32_t* context;
+  const int32_t* fresh;  // new tokens per row
+  const uint8_t* released;
+  int32_t* table;
+  int64_t table_stride;
+  int32_t* free_blocks;
+  const int32_t* free_state;
+  int32_t* free_state_out;
+  int32_t* lengths_out;
+  int32_t* offsets;
+  int64_t* slots;
+  int32_t* positions;
+  int32_t* error_word;
+};
+
+constexpr uint32_t SAT = 0x7fffffffu;
+// Sum of two values in [0, 2^31) that stays there: associative, so a scan of
+// lengths that add up to more than 31 bits ends at the cap instead of wrapping.
+Q3S_DEV uint32_t sat_add(uint32_t a, uint32_t b) { return min(a + b, SAT); }
+
+struct Sums {
+  uint32_t tokens, need, back;
+};
+Q3S_DEV Sums operator+(const Sums& a, const Sums& b) {
+  return {sat_add(a.tokens, b.tokens), sat_add(a.need, b.need), sat_add(a.back, b.back)};
+}
+
+// One launch, no waiting between CTAs.  Everything a row or a token gets is a
+// function of three prefix sums over the rows (new tokens, blocks needed,
+// blocks given back), so every CTA scans all rows by itself (9 bytes a row,
+// from L2 after the first CTA) and then writes its share: the tokens
+// [c * chunk, (c + 1) * chunk), found in the scanned offsets by bisection, and
+// the rows r with r % gridDim.x == c.  Inputs that other CTAs still read are
+// never written: lengths and ring state have separate outputs, table entries
+// that the step writes are at or past the row's held blocks while slots read
+// the last held one, and the ring is read at its front and written at its
+// back.  A row's own table entries are read (given back) and rewritten
+// (readmitted) by the same lane.  Bound by launch and memory latency: two
+// dependent loads (lengths, then block ids) and a scan of two barriers for
+// each NT * R rows. 
+template <int NT, int R>
+__global__ void __launch_bounds__(NT) cache_tables_kernel(const TablesArgs a) {
+  constexpr int TILE = NT * R, WARPS = NT / 32;
+  __shared__ uint32_t s_off[TILE];    // first token of the row
+  __shared__ int32_t s_context[TILE]; // tokens the row already holds
+  __shared__ int32_t s_first[TILE];   // rank in the ring of its first fresh block; -1: refused
+  __shared__ Sums s_warp[WARPS];
+  const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
+  const int cta = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
+  const int chunk = (a.max_tokens + ctas - 1) / ctas;
+  const uint32_t tok0 = static_cast<uint32_t>(min(static_cast<int64_t>(cta) * chunk, static_cast<int64_t>(a.max_tokens)));
+  const uint32_t tok1 = min(tok0 + static_cast<uint32_t>(chunk), static_cast<uint32_t>(a.max_tokens));
+  const int head = min(max(a.free_state[0], 0), a.ring - 1);
+  const int count = min(max(a.free_state[1], 0), a.ring);
+  const int bs = a.bs;
+  const int64_t room = static_cast<int64_t>(a.max_blocks) * bs;
+  int bad = 0;
+  uint32_t taken = 0;
+  Sums carry = {0, 0, 0};
+  auto ring_at = [&](uint32_t rank) {  // ring index `rank` places after the front
+    return static_cast<int>((static_cast<uint64_t>(head) + rank) % static_cast<uint32_t>(a.ring));
+  };
+
+  for (int row0 = 0; row0 < a.B; row0 += TILE) {
+    Sums mine[R], total = {0, 0, 0};
+    int context[R], back[R];
+    bool fits[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int row = row0 + t * R + i;
+      const bool in = row < a.B;
+      const int c = in ? a.context[row] : 0, n = in ? a.fresh[row] : 0;
+      const bool gone = in && a.released && a.released[row];
+      if (c < 0 || n < 0 || c > room) bad |= Q3S_DECERR_LENGTHS;
+      const int held_tokens = static_cast<int>(min(static_cast<int64_t>(max(c, 0)), room));
+      const uint32_t fresh = static_cast<uint32_t>(max(n, 0));
+      context[i] = gone ? 0 : held_tokens;
+      back[i] = gone ? static_cast<int>((static_cast<int64_t>(held_tokens) + bs - 1) / bs) : 0;
+      const int64_t end = static_cast<int64_t>(context[i]) + fresh;
+      fits[i] = end <= room;
+      if (!fits[i]) bad |= Q3S_DECERR_TABLE;
+      const uint32_t need = fits[i] ? static_cast<uint32_t>((end + bs - 1) / bs - (static_cast<int64_t>(context[i]) + bs - 1) / bs) : 0u;
+      mine[i] = {fresh, need, static_cast<uint32_t>(back[i])};
+      total = total + mine[i];
+    }
+    // block-wide exclusive scan of `total`
+    Sums up = total;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const Sums o = {__shfl_up_sync(FULL, up.tokens, d), __shfl_up_sync(FULL, up.need, d),
+                      __shfl_up_sync(FULL, up.back, d)};
+      if (lane >= d) up = up + o;
+    }
+    if (lane == 31) s_warp[w] = up;
+    Sums before = {__shfl_up_sync(FULL, up.tokens, 1), __shfl_up_sync(FULL, up.need, 1),
+                   __shfl_up_sync(FULL, up.back, 1)};
+    if (lane == 0) before = {0, 0, 0};
+    __syncthreads();
+    {
+      Sums x = lane < WARPS ? s_warp[lane] : Sums{0, 0, 0};
+#pragma unroll
+      for (int d = 1; d < WARPS; d <<= 1) {
+        const Sums o = {__shfl_up_sync(FULL, x.tokens, d), __shfl_up_sync(FULL, x.need, d),
+                        __shfl_up_sync(FULL, x.back, d)};
+        if (lane >= d) x = x + o;
+      }
+      const int src = max(w - 1, 0);
+      Sums base = {__shfl_sync(FULL, x.tokens, src), __shfl_sync(FULL, x.need, src), __shfl_sync(FULL, x.back, src)};
+      if (w == 0) base = {0, 0, 0};
+      before = carry + base + before;
+      const Sums all = {__shfl_sync(FULL, x.tokens, WARPS - 1), __shfl_sync(FULL, x.need, WARPS - 1),
+                        __shfl_sync(FULL, x.back, WARPS - 1)};
+      carry = carry + all;
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int k = t * R + i, row = row0 + k;
+      const Sums at = before;
+      before = before + mine[i];
+      const uint32_t need = mine[i].need;
+      const bool granted = fits[i] && (need == 0 || before.need <= static_cast<uint32_t>(count));
+      if (!granted && fits[i]) bad |= Q3S_DECERR_POOL;
+      if (granted && need) taken = max(taken, before.need);
+      s_off[k] = at.tokens;
+      s_context[k] = context[i];
+      s_first[k] = granted ? static_cast<int>(at.need) : -1;
+      // the row's own entries: lane by lane when short, the whole warp when long
+      const bool here = row < a.B && row % ctas == cta;
+      const int take = granted ? static_cast<int>(need) : 0;
+      const int held = (context[i] + bs - 1) / bs;
+      if (here) {
+        a.lengths_out[row] = granted ? static_cast<int>(context[i] + mine[i].tokens) : context[i];
+        a.offsets[row + 1] = static_cast<int>(before.tokens);
+        if (row == 0) a.offsets[0] = 0;
+        if (take == 1 && back[i] == 0)
+          a.table[row * a.table_stride + held] = a.free_blocks[ring_at(at.need)];
+      }
+      unsigned longer = __ballot_sync(FULL, here && (take > 1 || back[i] > 0));
+      while (longer) {
+        const int src = __ffs(longer) - 1;
+        longer &= longer - 1;
+        const int r = __shfl_sync(FULL, row, src), nb = __shfl_sync(FULL, back[i], src);
+        const int nt = __shfl_sync(FULL, take, src), h0 = __shfl_sync(FULL, held, src);
+        const uint32_t first = __shfl_sync(FULL, at.need, src), behind = __shfl_sync(FULL, at.back, src);
+        int32_t* entries = a.table + r * a.table_stride;
+        for (int j = lane; j < nb; j += 32) a.free_blocks[ring_at(sat_add(count, behind) + j)] = entries[j];
+        // h0 > 0 only when nothing was given back; with h0 == 0 lane j wrote entry j back above
+        for (int j = lane; j < nt; j += 32) entries[h0 + j] = a.free_blocks[ring_at(first + j)];
+      }
+    }
+    __syncthreads();  // the tile's rows are in shared memory
+    // tokens of this CTA that belong to the tile's rows
+    const uint32_t lo = max(tok0, s_off[0]), hi = min(tok1, carry.tokens);
+    const int rows = min(TILE, a.B - row0);
+    for (uint32_t tok = lo + t; tok < hi; tok += NT) {
+      int l = 0, r = rows;  // the last row that starts at or before tok (rows without tokens start where the next one does)
+      while (r - l > 1) {
+        const int m = (l + r) >> 1;
+        if (s_off[m] <= tok) l = m; else r = m;
+      }
+      const int first = s_first[l], c = s_context[l];
+      const int pos = static_cast<int>(min(static_cast<uint32_t>(c) + (tok - s_off[l]), SAT));
+      int64_t slot = -1;
+      if (first >= 0) {
+        const int j = pos / bs, held = (c + bs - 1) / bs;
+        const int id = j < held ? a.table[(row0 + l) * a.table_stride + j] : a.free_blocks[ring_at(first + (j - held))];
+        slot = static_cast<int64_t>(id) * bs + (pos - j * bs);
+      }
+      a.slots[tok] = slot;
+      a.positions[tok] = pos;
+    }
+    if (row0 + TILE < a.B) __syncthreads();  // before the next tile's rows replace these
+  }
+  for (uint32_t tok = max(tok0, carry.tokens) + t; tok < tok1; tok += NT) {  // past the last token
+    a.slots[tok] = -1;
+    a.positions[tok] = 0;
+  }
+  if (cta == 0) {
+    if (carry.tokens > static_cast<uint32_t>(a.max_tokens)) bad |= Q3S_DECERR_TOKENS;
+    __shared__ unsigned s_taken, s_bad;
+    if (t == 0) s_taken = 0, s_bad = 0;
+    __syncthreads();
+    taken = __reduce_max_sync(FULL, taken);
+    bad = __reduce_or_sync(FULL, bad);
+    if (lane == 0) {
+      if (taken) atomicMax(&s_taken, taken);
+      if (bad) atomicOr(&s_bad, static_cast<unsigned>(bad));
+    }
+    __syncthreads();
+    if (t == 0) {
+      const uint32_t left = static_cast<uint32_t>(count) - s_taken;
+      a.free_state_out[0] = ring_at(s_taken);
+      a.free_state_out[1] = static_cast<int>(min(sat_add(left, carry.back), static_cast<uint32_t>(a.ring)));
+      if (a.B == 0) a.offsets[0] = 0;
+      if (a.error_word) *a.error_word = static_cast<int>(s_bad);
+    }
+  }
+}
+
+struct AppendArgs {
+  int T, H, bs, blocks;
+  int units;  // copies of one head's row: dim / 8 (16-byte units) or dim (single elements)
+  const void *k, *v;
+  int64_t kt, kh, vt, vh;
+  const int64_t* slots;
+  void *kc, *vc;
+  int64_t kb, kch, kp, vb, vch, vp;
+  int32_t* error_word;
+};
+
+// A copy of 4 * T * H * dim bytes each way, bound by HBM.  A thread's unit is
+// 16 bytes where every base and stride allows it (UNIT = uint4), one element
+// otherwise; consecutive threads take consecutive units of one head's row, so
+// both sides of the copy are whole rows of dim elements.  U units a thread are
+// all loaded before the first is stored.  APPEND_TIMES.
+template <typename UNIT, int U>
+__global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
+  constexpr int E = sizeof(UNIT) == 16 ? 8 : 1;  // elements per unit (2-byte elements) or 1
+  const uint32_t per_part = static_cast<uint32_t>(a.H) * a.units, per_token = 2 * per_part;
+  const uint64_t all = static_cast<uint64_t>(a.T) * per_token;
+  const uint64_t base = static_cast<uint64_t>(blockIdx.x) * (256 * U) + threadIdx.x;
+  UNIT x[U];
+  UNIT* to[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const uint64_t at = base + 256u * i;
+    to[i] = nullptr;
+    if (at >= all) continue;
+    const uint32_t token = static_cast<uint32_t>(at / per_token);
+    uint32_t rest = static_cast<uint32_t>(at - static_cast<uint64_t>(token) * per_token);
+    const bool value = rest >= per_part;
+    if (value) rest -= per_part;
+    const uint32_t h = rest / a.units, e = (rest - h * a.units) * E;
+    const int64_t slot = a.slots[token];
+    if (slot < 0) continue;
+    const int64_t block = slot / a.bs, place = slot - block * a.bs;
+    if (block >= a.blocks) {
+      if (a.error_word) atomicOr(a.error_word, Q3S_DECERR_BLOCK_ID);
+      continue;
+    }
+    using ELEM = typename std::conditional<sizeof(UNIT) == 16, uint16_t, UNIT>::type;
+    const ELEM* from = static_cast<const ELEM*>(value ? a.v : a.k) +
+                       (value ? token * a.vt + h * a.vh : token * a.kt + h * a.kh) + e;
+    x[i] = *reinterpret_cast<const UNIT*>(from);
+    to[i] = reinterpret_cast<UNIT*>(static_cast<ELEM*>(value ? a.vc : a.kc) +
+                                    (value ? block * a.vb + h * a.vch + place * a.vp
+                                           : block * a.kb + h * a.kch + place * a.kp) + e);
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i)
+    if (to[i]) *to[i] = x[i];
+}
+
+template <typename UNIT>
+cudaError_t launch_append(const AppendArgs& a, cudaStream_t st) {
+  const uint64_t all = static_cast<uint64_t>(a.T) * 2 * a.H * a.units;
+  constexpr int U = 4;
+  // few units: one a thread, so that they spread over all SMs
+  if (all <= 256ull * 148 * 4) {
+    cache_append_kernel<UNIT, 1><<<static_cast<unsigned>((all + 255) / 256), 256, 0, st>>>(a);
+  } else {
+    cache_append_kernel<UNIT, U><<<static_cast<unsigned>((all + 256 * U - 1) / (256 * U)), 256, 0, st>>>(a);
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace q3s
+
+extern "C" q3s_status q3s_cache_tables(const q3s_cache_tables_desc* d, void* stream) {
+  using q3s::report;
+  if (!d) return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_tables: desc is NULL");
+  if (d->struct_size != sizeof(q3s_cache_tables_desc))
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_tables: struct_size %u != %u (ABI mismatch)", d->struct_size,
+                  static_cast<unsigned>(sizeof(q3s_cache_tables_desc)));
+  if (d->batch < 0 || d->batch > Q3S_MAX_CACHE_ROWS)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_tables: batch %d is not in [0, %d]", d->batch, Q3S_MAX_CACHE_ROWS);
+  if (d->block_size < 1 || d->max_blocks < 1 || d->ring_size < 1 || d->max_tokens < 0)
+    return report(Q3S_ERR_INVALID_ARGUMENT,
+                  "q3s_cache_tables: block_size, max_blocks and ring_size must be positive and max_tokens not negative");
+  if (static_cast<int64_t>(d->max_blocks) * d->block_size > 0x7fffffffll)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_tables: a table of %d blocks of %d tokens passes 31 bits",
+                  d->max_blocks, d->block_size);
+  if (!d->free_blocks || !d->free_state || !d->free_state_out || !d->query_offsets)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_tables: free_blocks, free_state, free_state_out and query_offsets are required");
+  if (d->batch > 0 && (!d->context_lengths || !d->new_lengths || !d->block_table || !d->lengths_out))
+    return report(Q3S_ERR_INVALID_ARGUMENT,
+                  "q3s_cache_tables: context_lengths, new_lengths, block_table and lengths_out are required");
+  if (d->max_tokens > 0 && (!d->slot_map || !d->positions))
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_tables: slot_map and positions are required");
+  if (d->batch > 1 && d->block_table_stride < d->max_blocks)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_tables: block_table_stride is below max_blocks");
+  if (d->lengths_out && (d->lengths_out == d->context_lengths || d->lengths_out == d->new_lengths))
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_tables: lengths_out must not be an input");
+  if (d->free_state_out == d->free_state)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_tables: free_state_out must not be free_state");
+  q3s::TablesArgs a;
+  a.B = d->batch;
+  a.bs = d->block_size;
+  a.max_blocks = d->max_blocks;
+  a.ring = d->ring_size;
+  a.max_tokens = d->max_tokens;
+  a.context = d->context_lengths;
+  a.fresh = d->new_lengths;
+  a.released = d->released;
+  a.table = d->block_table;
+  a.table_stride = d->block_table_stride;
+  a.free_blocks = d->free_blocks;
+  a.free_state = d->free_state;
+  a.free_state_out = d->free_state_out;
+  a.lengths_out = d->lengths_out;
+  a.offsets = d->query_offsets;
+  a.slots = d->slot_map;
+  a.positions = d->positions;
+  a.error_word = d->error_word;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // CTAs: one per NT tokens or per 32 rows (their entries), up to one per SM
+  const int sms = q3s::sm_count();
+  auto ctas = [&](int nt) {
+    return std::max(1, std::min(sms, std::max(static_cast<int>((static_cast<int64_t>(a.max_tokens) + nt - 1) / nt), (a.B + 31) / 32)));
+  };
+  if (a.B <= 128 && a.max_tokens <= 1024)
+    q3s::cache_tables_kernel<128, 1><<<ctas(128), 128, 0, st>>>(a);
+  else if (a.B <= 1024)
+    q3s::cache_tables_kernel<1024, 1><<<ctas(1024), 1024, 0, st>>>(a);
+  else
+    q3s::cache_tables_kernel<1024, 2><<<ctas(1024), 1024, 0, st>>>(a);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return report(Q3S_ERR_CUDA, "q3s_cache_tables: launch failed: %s", cudaGetErrorString(e));
+  return report(Q3S_OK, "");
+}
+
+extern "C" q3s_status q3s_cache_append(const q3s_cache_append_desc* d, void* stream) {
+  using q3s::report;
+  if (!d) return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_append: desc is NULL");
+  if (d->struct_size != sizeof(q3s_cache_append_desc))
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_append: struct_size %u != %u (ABI mismatch)", d->struct_size,
+                  static_cast<unsigned>(sizeof(q3s_cache_append_desc)));
+  if (d->tokens < 0 || d->kv_heads < 1 || d->dim < 1 || d->block_size < 1 || d->blocks < 1)
+    return report(Q3S_ERR_INVALID_ARGUMENT,
+                  "q3s_cache_append: kv_heads, dim, block_size and blocks must be positive and tokens not negative");
+  if (static_cast<int64_t>(d->kv_heads) * d->dim > (1 << 24))
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_append: kv_heads * dim is above 2^24");
+  if (d->elem != Q3S_ELEM_F32 && d->elem != Q3S_ELEM_BF16 && d->elem != Q3S_ELEM_F16)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_append: unknown elem %d", d->elem);
+  if (d->tokens == 0) return report(Q3S_OK, "");
+  if (!d->k || !d->v || !d->slot_map || !d->k_cache || !d->v_cache)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_append: k, v, slot_map, k_cache and v_cache are required");
+  q3s::AppendArgs a;
+  a.T = d->tokens;
+  a.H = d->kv_heads;
+  a.bs = d->block_size;
+  a.blocks = d->blocks;
+  a.k = d->k;
+  a.v = d->v;
+  a.slots = d->slot_map;
+  a.kc = d->k_cache;
+  a.vc = d->v_cache;
+  a.error_word = d->error_word;
+  // 32-bit elements are copied as pairs of 16-bit ones
+  const int64_t wide = d->elem == Q3S_ELEM_F32 ? 2 : 1;
+  const int64_t strides[10] = {d->k_token_stride, d->k_head_stride,       d->v_token_stride, d->v_head_stride,
+                               d->k_block_stride, d->k_cache_head_stride, d->k_place_stride, d->v_block_stride,
+                               d->v_cache_head_stride, d->v_place_stride};
+  int64_t* to[10] = {&a.kt, &a.kh, &a.vt, &a.vh, &a.kb, &a.kch, &a.kp, &a.vb, &a.vch, &a.vp};
+  const int64_t dim = d->dim * wide;
+  bool vec = dim % 8 == 0;
+  for (int i = 0; i < 10; ++i) {
+    *to[i] = strides[i] * wide;
+    vec = vec && *to[i] % 8 == 0;
+  }
+  for (const void* p : {d->k, d->v, static_cast<const void*>(d->k_cache), static_cast<const void*>(d->v_cache)})
+    vec = vec && (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
+  const int units = static_cast<int>(vec ? dim / 8 : dim);
+  a.units = units;
+  if ((static_cast<uint64_t>(a.T) * 2 * a.H * units + 255) / 256 > 0x7fffffffull)
+    return report(Q3S_ERR_UNSUPPORTED, "q3s_cache_append: %d tokens are too many for one launch", d->tokens);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = vec ? q3s::launch_append<uint4>(a, st) : q3s::launch_append<uint16_t>(a, st);
+  if (e != cudaSuccess) return report(Q3S_ERR_CUDA, "q3s_cache_append: launch failed: %s", cudaGetErrorString(e));
+  return report(Q3S_OK, "");
+}
+
+extern "C" uint32_t q3s_decode_desc_size(int32_t which) {
+  switch (which) {
+    case 0: return sizeof(q3s_cache_tables_desc);
+    case 1: return sizeof(q3s_cache_append_desc);
+    case 2: return sizeof(q3s_prefix_attention_desc);
+    case 3: return sizeof(q3s_quantize_rows_desc);
+    case 4: return sizeof(q3s_int8_matmul_desc);
+  }
+  return 0;
+}

@@ -10,36 +10,14 @@
 #include "q3s_args.cuh"
 #include "q3s_head.cuh"
 #include "q3s_sampler.h"
+#include "q3s_tma.cuh"
 
 namespace {
-
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no link
-// against the driver library); resolved once, racing first callers store the
-// same pointer.
-EncodeTiled encode_tiled() {
-  static std::atomic<EncodeTiled> fn{nullptr};
-  EncodeTiled f = fn.load(std::memory_order_acquire);
-  if (!f) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) !=
-            cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return nullptr;
-    f = reinterpret_cast<EncodeTiled>(p);
-    fn.store(f, std::memory_order_release);
-  }
-  return f;
-}
 
 // 2-D bf16 tensor [rows, cols] (row stride `ld` elements), boxes of
 // [box_rows, 64] in the 128-byte swizzle; rows past the tensor read as zeros.
 bool make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
-  EncodeTiled enc = encode_tiled();
+  const q3s::EncodeTiled enc = q3s::encode_tiled();
   if (!enc) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
@@ -49,8 +27,6 @@ bool make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int6
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <int KS, int BN>
 cudaError_t launch_head(const CUtensorMap& th, const CUtensorMap& tw, const q3s::HeadArgs& a, int mtiles,
@@ -164,7 +140,7 @@ extern "C" q3s_status q3s_head_sample(const q3s_head_desc* d, void* stream) {
   if (B == 0) return report(Q3S_OK, "");
   if (!d->hidden || !d->weight || !d->logits)
     return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_head_sample: hidden, weight and logits are required");
-  if (!aligned16(d->hidden) || !aligned16(d->weight) || !aligned16(d->logits))
+  if (!q3s::aligned16(d->hidden) || !q3s::aligned16(d->weight) || !q3s::aligned16(d->logits))
     return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_head_sample: hidden, weight and logits must be 16-byte aligned");
   if (d->hidden_row_stride < H || d->hidden_row_stride % 8 || d->weight_row_stride < H ||
       d->weight_row_stride % 8 || d->logits_row_stride < V || d->logits_row_stride % 8)

@@ -4,6 +4,17 @@ Python host side over the C ABI of ``include/q3s_sampler.h``; the sampling
 itself runs only in the sm_100a kernels of ``libq3s_sampler.so``.
 """
 from . import _lib
+from .decode import (
+    CacheTables,
+    Int8Linear,
+    PagedCache,
+    cache_append,
+    cache_tables,
+    int8_linear,
+    int8_matmul,
+    prefix_attention,
+    quantize_rows,
+)
 from .step import RowHistory, StepGuard, step_update
 from .ops import (
     CodecSampler,
@@ -24,6 +35,15 @@ from .ops import (
 )
 
 __all__ = [
+    "CacheTables",
+    "Int8Linear",
+    "PagedCache",
+    "cache_append",
+    "cache_tables",
+    "int8_linear",
+    "int8_matmul",
+    "prefix_attention",
+    "quantize_rows",
     "CodecSampler",
     "CpFramePlan",
     "HeadPlan",

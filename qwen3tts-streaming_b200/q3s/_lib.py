@@ -1,4 +1,5 @@
-"""ctypes binding of the C ABI in ``include/q3s_sampler.h``.
+"""ctypes binding of the C ABI in ``include/q3s_sampler.h`` and
+``include/q3s_decode.h``.
 
 The structures below mirror the C descriptors field for field; ``load()``
 checks their sizes against ``q3s_desc_size`` so a stale library or a layout
@@ -164,6 +165,151 @@ class HeadDesc(C.Structure):
     ]
 
 
+# the decode step's operators (include/q3s_decode.h)
+ELEM_F32, ELEM_BF16, ELEM_F16 = 0, 1, 2
+MAX_CACHE_ROWS, MAX_QUERY_GROUP = 65536, 16
+
+
+class CacheTablesDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("batch", C.c_int32),
+        ("block_size", C.c_int32),
+        ("max_blocks", C.c_int32),
+        ("context_lengths", _p),
+        ("new_lengths", _p),
+        ("released", _p),
+        ("block_table", _p),
+        ("block_table_stride", C.c_int64),
+        ("free_blocks", _p),
+        ("free_state", _p),
+        ("free_state_out", _p),
+        ("lengths_out", _p),
+        ("query_offsets", _p),
+        ("slot_map", _p),
+        ("positions", _p),
+        ("error_word", _p),
+        ("ring_size", C.c_int32),
+        ("max_tokens", C.c_int32),
+    ]
+
+
+class CacheAppendDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("tokens", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("dim", C.c_int32),
+        ("block_size", C.c_int32),
+        ("blocks", C.c_int32),
+        ("elem", C.c_int32),
+        ("reserved0", C.c_int32),
+        ("k", _p),
+        ("v", _p),
+        ("k_token_stride", C.c_int64),
+        ("k_head_stride", C.c_int64),
+        ("v_token_stride", C.c_int64),
+        ("v_head_stride", C.c_int64),
+        ("slot_map", _p),
+        ("k_cache", _p),
+        ("v_cache", _p),
+        ("k_block_stride", C.c_int64),
+        ("k_cache_head_stride", C.c_int64),
+        ("k_place_stride", C.c_int64),
+        ("v_block_stride", C.c_int64),
+        ("v_cache_head_stride", C.c_int64),
+        ("v_place_stride", C.c_int64),
+        ("error_word", _p),
+    ]
+
+
+class PrefixAttentionDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("batch", C.c_int32),
+        ("tokens", C.c_int32),
+        ("q_heads", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("dim", C.c_int32),
+        ("block_size", C.c_int32),
+        ("blocks", C.c_int32),
+        ("elem", C.c_int32),
+        ("max_blocks", C.c_int32),
+        ("prefix_length", C.c_int32),
+        ("scale", C.c_float),
+        ("q", _p),
+        ("q_token_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("k_cache", _p),
+        ("v_cache", _p),
+        ("k_block_stride", C.c_int64),
+        ("k_head_stride", C.c_int64),
+        ("k_place_stride", C.c_int64),
+        ("v_block_stride", C.c_int64),
+        ("v_head_stride", C.c_int64),
+        ("v_place_stride", C.c_int64),
+        ("query_offsets", _p),
+        ("block_table", _p),
+        ("block_table_stride", C.c_int64),
+        ("lengths", _p),
+        ("prefix_blocks", _p),
+        ("out", _p),
+        ("out_token_stride", C.c_int64),
+        ("out_head_stride", C.c_int64),
+        ("lse", _p),
+        ("workspace", _p),
+        ("workspace_bytes", C.c_int64),
+        ("error_word", _p),
+    ]
+
+
+class QuantizeRowsDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("rows", C.c_int32),
+        ("cols", C.c_int32),
+        ("elem", C.c_int32),
+        ("x", _p),
+        ("x_row_stride", C.c_int64),
+        ("values", _p),
+        ("values_row_stride", C.c_int64),
+        ("scales", _p),
+    ]
+
+
+class Int8MatmulDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("rows", C.c_int32),
+        ("inputs", C.c_int32),
+        ("outputs", C.c_int32),
+        ("elem", C.c_int32),
+        ("reserved0", C.c_int32),
+        ("a", _p),
+        ("a_row_stride", C.c_int64),
+        ("a_scales", _p),
+        ("w", _p),
+        ("w_row_stride", C.c_int64),
+        ("w_scales", _p),
+        ("bias", _p),
+        ("y", _p),
+        ("y_row_stride", C.c_int64),
+        ("error_word", _p),
+    ]
+
+
+DECODE_DESCS = (CacheTablesDesc, CacheAppendDesc, PrefixAttentionDesc, QuantizeRowsDesc, Int8MatmulDesc)
+# every symbol include/q3s_decode.h declares
+DECODE_EXPORTS = (
+    "q3s_cache_tables",
+    "q3s_cache_append",
+    "q3s_prefix_attention_workspace",
+    "q3s_prefix_attention",
+    "q3s_quantize_rows",
+    "q3s_int8_matmul",
+    "q3s_decode_desc_size",
+)
+
 # every symbol include/q3s_sampler.h declares
 EXPORTS = (
     "q3s_sample",
@@ -216,12 +362,24 @@ def load(path: str | Path | None = None) -> C.CDLL:
         lib.q3s_step_update.restype = C.c_int
         lib.q3s_head_sample.argtypes = [C.POINTER(HeadDesc), _p]
         lib.q3s_head_sample.restype = C.c_int
+        for name, st in zip(("q3s_cache_tables", "q3s_cache_append", "q3s_prefix_attention", "q3s_quantize_rows",
+                             "q3s_int8_matmul"), DECODE_DESCS):
+            getattr(lib, name).argtypes = [C.POINTER(st), _p]
+            getattr(lib, name).restype = C.c_int
+        lib.q3s_prefix_attention_workspace.argtypes = [C.POINTER(PrefixAttentionDesc), C.POINTER(C.c_int64)]
+        lib.q3s_prefix_attention_workspace.restype = C.c_int
+        lib.q3s_decode_desc_size.argtypes = [C.c_int32]
+        lib.q3s_decode_desc_size.restype = C.c_uint32
         if lib.q3s_abi_version() != Q3S_ABI_VERSION:
             raise RuntimeError(f"q3s ABI {lib.q3s_abi_version()} != binding {Q3S_ABI_VERSION}; rebuild")
         for which, st in ((0, SampleDesc), (1, CpFrameDesc), (2, StepDesc), (3, HeadDesc)):
             if lib.q3s_desc_size(which) != C.sizeof(st):
                 raise RuntimeError(f"q3s descriptor {st.__name__} size {C.sizeof(st)} != library "
                                    f"{lib.q3s_desc_size(which)}; rebuild")
+        for which, st in enumerate(DECODE_DESCS):
+            if lib.q3s_decode_desc_size(which) != C.sizeof(st):
+                raise RuntimeError(f"q3s descriptor {st.__name__} size {C.sizeof(st)} != library "
+                                   f"{lib.q3s_decode_desc_size(which)}; rebuild")
         if path is None:
             _lib = lib
         return lib

@@ -2,7 +2,7 @@
 ``torch.ops.q3s`` operator library over it.
 
 ``libq3s_sampler.so`` holds the CUDA kernels and the C ABI declared in
-``include/q3s_sampler.h``; it links the CUDA runtime statically and has no
+``include/q3s_sampler.h`` and ``include/q3s_decode.h``; it links the CUDA runtime statically and has no
 torch dependency, so any FFI (ctypes here) can load it.
 ``libq3s_torch_ops.so`` registers the PyTorch operators (schemas, CUDA and
 Meta kernels) that call that C ABI; it links libq3s_sampler.so through an
@@ -23,9 +23,12 @@ INCLUDE = REPO / "include"
 LIB_PATH = PKG_DIR / "libq3s_sampler.so"
 TORCH_OPS_PATH = PKG_DIR / "libq3s_torch_ops.so"
 TORCH_OPS_SRC = CSRC / "q3s_torch_ops.cpp"
-SOURCES = [CSRC / "q3s_sampler.cu", CSRC / "q3s_warp.cu", CSRC / "q3s_head.cu", CSRC / "q3s_lean.cu"]
+TORCH_DECODE_SRC = CSRC / "q3s_torch_decode.cpp"
+SOURCES = [CSRC / "q3s_sampler.cu", CSRC / "q3s_warp.cu", CSRC / "q3s_head.cu", CSRC / "q3s_lean.cu",
+           CSRC / "q3s_cache.cu", CSRC / "q3s_attn.cu", CSRC / "q3s_int8.cu"]
 DEPS = SOURCES + [CSRC / "q3s_args.cuh", CSRC / "q3s_device.cuh", CSRC / "q3s_warp.cuh", CSRC / "q3s_philox.cuh", CSRC / "q3s_step.cuh", CSRC / "q3s_head.cuh", CSRC / "q3s_lean.cuh", CSRC / "q3s_cp.cuh", CSRC / "q3s_core.cuh",
-                  INCLUDE / "q3s_sampler.h"]
+                  CSRC / "q3s_attn.cuh", CSRC / "q3s_int8.cuh", CSRC / "q3s_tma.cuh",
+                  INCLUDE / "q3s_sampler.h", INCLUDE / "q3s_decode.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -53,7 +56,8 @@ def torch_ops_up_to_date() -> bool:
     if not TORCH_OPS_PATH.exists():
         return False
     t = TORCH_OPS_PATH.stat().st_mtime
-    return all(p.stat().st_mtime <= t for p in (TORCH_OPS_SRC, INCLUDE / "q3s_sampler.h", LIB_PATH))
+    return all(p.stat().st_mtime <= t for p in (TORCH_OPS_SRC, TORCH_DECODE_SRC, INCLUDE / "q3s_sampler.h",
+                                                INCLUDE / "q3s_decode.h", LIB_PATH))
 
 
 def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
@@ -69,7 +73,7 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
     libdirs = [f"-L{p}" for p in ce.library_paths(device_type="cuda")]
     tmp = TORCH_OPS_PATH.with_suffix(".so.tmp")
     cmd = [system_cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           *incs, str(TORCH_OPS_SRC), "-o", str(tmp), *libdirs, f"-L{PKG_DIR}", "-lq3s_sampler",
+           *incs, str(TORCH_OPS_SRC), str(TORCH_DECODE_SRC), "-o", str(tmp), *libdirs, f"-L{PKG_DIR}", "-lq3s_sampler",
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-Wl,-rpath,$ORIGIN"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or res.returncode != 0:
