@@ -1,4 +1,5 @@
 // q3s_attn.cu -- host side of q3s_prefix_attention.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -6,6 +7,7 @@
 #include <cstring>
 
 #include "q3s_attn.cuh"
+#include "q3s_attn_prefix.cuh"
 #include "q3s_tma.cuh"
 
 namespace {
@@ -19,15 +21,46 @@ int split_ctas(int dim) { return q3s::sm_count() * ((227 * 1024) / (split_smem(d
 struct Layout {
   int64_t plan, part_o, part_ml, pre_o, pre_ml, bytes;  // byte offsets
   int64_t slots;
-  int ctas, splits;
+  int ctas;
   bool prefix_here;
+  int per_tile, pairs, steps, per_split, splits;  // the prefix kernel's (splits 0: not used)
 };
+
+// Parts that the prefix kernel cuts the keys into.  A part costs its steps of
+// 128 keys plus about three for its start and end; the CTAs of all parts run
+// in waves of one a SM; and each part writes and the join reads fp32 sums of
+// all queries.  The number with the lowest estimate is taken.
+void plan_prefix(const q3s_prefix_attention_desc* d, Layout* l) {
+  const int G = d->q_heads / d->kv_heads;
+  l->per_tile = q3s::PX_M / G;
+  l->pairs = (d->tokens + 2 * l->per_tile - 1) / (2 * l->per_tile);
+  l->steps = (d->prefix_length + q3s::PX_KEYS - 1) / q3s::PX_KEYS;
+  const int64_t items = static_cast<int64_t>(l->pairs) * d->kv_heads, sms = q3s::sm_count();
+  const double step_us = 1.2, part_us = static_cast<double>(d->tokens) * d->q_heads * d->dim * 8 / 6e6;
+  double best = 0;
+  for (int s = 1; s <= l->steps && s <= 64; ++s) {
+    const int per = (l->steps + s - 1) / s, parts = (l->steps + per - 1) / per;
+    if (parts != s) continue;
+    const double cost = static_cast<double>((items * s + sms - 1) / sms) * (per + 3) * step_us + s * part_us;
+    if (l->splits == 0 || cost < best) {
+      best = cost;
+      l->splits = s;
+      l->per_split = per;
+    }
+  }
+}
 
 Layout layout_of(const q3s_prefix_attention_desc* d) {
   Layout l;
   const int64_t G = d->q_heads / d->kv_heads, queries = static_cast<int64_t>(d->tokens) * G;
-  l.prefix_here = true;
+  // The prefix kernel's tiles are 128 query rows: with fewer than
+  // 64 of them, or fewer than 64 keys, the key-split kernel takes
+  // the prefix as one more row.  A scale that is not positive turns the order
+  // of the scores around, which the prefix kernel's running maximum does not
+  // follow.
   l.splits = 0;
+  l.prefix_here = !(queries >= 64 && d->prefix_length >= 64 && d->scale > 0.0f);
+  if (!l.prefix_here) plan_prefix(d, &l);
   l.ctas = split_ctas(d->dim);
   const int64_t items = (queries + q3s::AT_ROWS - 1) / q3s::AT_ROWS * (l.prefix_here ? 1 : 0) + queries / q3s::AT_ROWS +
                         std::min<int64_t>(d->batch, d->tokens);
@@ -78,14 +111,64 @@ q3s_status check_sizes(const q3s_prefix_attention_desc* d) {
   return Q3S_OK;
 }
 
+// The tensor maps of the prefix kernel: q as [T, q_heads, dim] in boxes of a
+// tile's tokens by a group's heads by 64 dims, a cache as [blocks, kv_heads,
+// block_size, dim] in boxes of one page (at most 128 tokens) by 64 dims; the
+// 128-byte swizzle, zeros outside.
+bool prefix_maps(const q3s::AttnArgs& a, int dim, bool bf16, int per_tile, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v) {
+  const q3s::EncodeTiled enc = q3s::encode_tiled();
+  if (!enc) return false;
+  const CUtensorMapDataType type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  auto u = [](int64_t x) { return static_cast<cuuint64_t>(x); };
+  // an axis of one entry has no stride of its own: any that the encoder takes
+  auto bytes = [&](int64_t stride, int n, int64_t otherwise) { return u(2 * (n > 1 ? stride : otherwise)); };
+  {
+    const cuuint64_t dims[3] = {u(dim), u(a.Hq), u(a.T)};
+    const cuuint64_t strides[2] = {bytes(a.qh, a.Hq, dim), bytes(a.qt, a.T, static_cast<int64_t>(a.Hq) * dim)};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.G), static_cast<cuuint32_t>(per_tile)};
+    if (enc(q, type, 3, const_cast<void*>(a.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return false;
+  }
+  auto cache = [&](CUtensorMap* m, const void* base, int64_t block, int64_t head, int64_t place) {
+    const cuuint64_t dims[4] = {u(dim), u(a.bs), u(a.H), u(a.blocks)};
+    const cuuint64_t strides[3] = {bytes(place, a.bs, dim), bytes(head, a.H, static_cast<int64_t>(a.bs) * dim),
+                                   bytes(block, a.blocks, static_cast<int64_t>(a.H) * a.bs * dim)};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(std::min(a.bs, q3s::PX_KEYS)), 1, 1};
+    return enc(m, type, 4, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  return cache(k, a.k, a.kb, a.kh, a.kp) && cache(v, a.v, a.vb, a.vh, a.vp);
+}
+
 template <int D, bool BF16>
 cudaError_t launch(const q3s::AttnArgs& a, const Layout& l, cudaStream_t st) {
+  cudaError_t e;
+  if (l.splits) {
+    auto prefix = q3s::attn_prefix_kernel<D, BF16>;
+    constexpr int smem = q3s::PrefixTile<D>::SMEM;
+    static std::atomic<uint64_t> prefix_done{0};
+    e = q3s::allow_smem(prefix, smem, prefix_done);
+    if (e != cudaSuccess) return e;
+    CUtensorMap tq, tk, tv;
+    if (!prefix_maps(a, D, BF16, l.per_tile, &tq, &tk, &tv)) return cudaErrorInvalidValue;
+    q3s::PrefixArgs p;
+    p.a = a;
+    p.per_tile = l.per_tile;
+    p.pairs = l.pairs;
+    p.steps = l.steps;
+    p.per_split = l.per_split;
+    prefix<<<dim3(l.pairs, a.H, l.splits), q3s::PX_NT, smem, st>>>(tq, tk, tv, p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
   auto split = q3s::attn_split_kernel<D, BF16>;
   static std::atomic<uint64_t> done{0};
-  cudaError_t e = q3s::allow_smem(split, split_smem(D), done);
+  e = q3s::allow_smem(split, split_smem(D), done);
   if (e != cudaSuccess) return e;
-  split<<<l.ctas, kSplitThreads, split_smem(D), st>>>(a);
-  e = cudaGetLastError();
+  // beside the prefix kernel where there is one: neither reads what the other writes
+  e = q3s::launch_maybe_pdl(split, dim3(l.ctas), dim3(kSplitThreads), split_smem(D), st, l.splits > 0, a);
   if (e != cudaSuccess) return e;
   // a warp joins one query row: rows of a (row, head) spread over gridDim.z CTAs of 4 warps
   const int64_t per = (static_cast<int64_t>(a.T) * a.G + a.B - 1) / std::max(a.B, 1);

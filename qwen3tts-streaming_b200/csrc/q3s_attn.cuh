@@ -243,7 +243,10 @@ __global__ void __launch_bounds__(AT_WARPS * 32) attn_split_kernel(const AttnArg
   // this warp's range: warps of a CTA are neighbours in the list
   const long long gw = static_cast<long long>(blockIdx.x) * AT_WARPS + w;
   const long long u0 = gw * quota, u1 = min(u0 + quota, all);
-  if (u0 >= u1) return;
+  if (u0 >= u1) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
 
   AttnPos p;
   {
@@ -471,6 +474,9 @@ __global__ void __launch_bounds__(AT_WARPS * 32) attn_split_kernel(const AttnArg
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
+  // this grid may have started beside the prefix kernel's: it does not end
+  // before that one, so that the join, which waits for this grid, has both
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (bad_block && a.error_word) atomicOr(a.error_word, Q3S_DECERR_BLOCK_ID);
 }
 

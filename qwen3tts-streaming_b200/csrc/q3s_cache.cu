@@ -227,7 +227,7 @@ struct AppendArgs {
 // 16 bytes where every base and stride allows it (UNIT = uint4), one element
 // otherwise; consecutive threads take consecutive units of one head's row, so
 // both sides of the copy are whole rows of dim elements.  U units a thread are
-// all loaded before the first is stored.  APPEND_TIMES.
+// all loaded before the first is stored.
 template <typename UNIT, int U>
 __global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
   constexpr int E = sizeof(UNIT) == 16 ? 8 : 1;  // elements per unit (2-byte elements) or 1
