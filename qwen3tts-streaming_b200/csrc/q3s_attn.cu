@@ -14,15 +14,16 @@ namespace {
 
 constexpr int kSplitThreads = q3s::AT_WARPS * 32;
 
-int split_smem(int dim) { return q3s::AT_WARPS * q3s::AT_STAGES * 2 * q3s::AT_KEYS * dim * 2; }
+int split_smem(int dim) { return dim == 64 ? q3s::SplitTile<64>::SMEM : q3s::SplitTile<128>::SMEM; }
 // CTAs of the key-split kernel: as many as are resident
 int split_ctas(int dim) { return q3s::sm_count() * ((227 * 1024) / (split_smem(dim) + 4096)); }
 
 struct Layout {
-  int64_t plan, part_o, part_ml, pre_o, pre_ml, bytes;  // byte offsets
-  int64_t slots;
+  int64_t items, part_o, part_ml, pre_o, pre_ml, bytes;  // byte offsets
+  int64_t ids, slots;
   int ctas;
-  bool prefix_here;
+  int nq;      // 8-row query tiles of an item of the key-split kernel: 1, 2 or 4
+  int tiles0;  // tiles of the prefix there (0: none)
   int per_tile, pairs, steps, per_split, splits;  // the prefix kernel's (splits 0: not used)
 };
 
@@ -59,20 +60,24 @@ Layout layout_of(const q3s_prefix_attention_desc* d) {
   // of the scores around, which the prefix kernel's running maximum does not
   // follow.
   l.splits = 0;
-  l.prefix_here = !(queries >= 64 && d->prefix_length >= 64 && d->scale > 0.0f);
-  if (!l.prefix_here) plan_prefix(d, &l);
+  if (queries >= 64 && d->prefix_length >= 64 && d->scale > 0.0f) plan_prefix(d, &l);
   l.ctas = split_ctas(d->dim);
-  const int64_t items = (queries + q3s::AT_ROWS - 1) / q3s::AT_ROWS * (l.prefix_here ? 1 : 0) + queries / q3s::AT_ROWS +
-                        std::min<int64_t>(d->batch, d->tokens);
-  l.slots = items * d->kv_heads + static_cast<int64_t>(l.ctas) * q3s::AT_WARPS;
+  // An item of the key-split kernel holds the query rows of an average row of
+  // the batch (an item reads its keys once), in tiles of 8 to 32.
+  const int64_t mean = (queries + std::max(d->batch, 1) - 1) / std::max(d->batch, 1);
+  l.nq = mean <= 8 ? 1 : mean <= 16 ? 2 : 4;
+  const int64_t R = 8 * l.nq;
+  l.tiles0 = l.splits || d->prefix_length == 0 ? 0 : static_cast<int>((queries + R - 1) / R);
+  l.ids = (l.tiles0 + queries / R + d->batch + 1) * d->kv_heads;
+  l.slots = l.ids + static_cast<int64_t>(l.ctas) * q3s::AT_WARPS;
   auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
   int64_t at = 0;
-  l.plan = at;
-  at += up(12 * (static_cast<int64_t>(d->batch) + 2) + 8);
+  l.items = at;
+  at += up(l.ids * 8);
   l.part_ml = at;
-  at += up(l.slots * q3s::AT_ROWS * 8);
+  at += up(l.slots * R * 8);
   l.part_o = at;
-  at += up(l.slots * q3s::AT_ROWS * d->dim * 4);
+  at += up(l.slots * R * d->dim * 4);
   l.pre_ml = at;
   at += up(static_cast<int64_t>(l.splits) * d->tokens * d->q_heads * 8);
   l.pre_o = at;
@@ -111,39 +116,58 @@ q3s_status check_sizes(const q3s_prefix_attention_desc* d) {
   return Q3S_OK;
 }
 
-// The tensor maps of the prefix kernel: q as [T, q_heads, dim] in boxes of a
-// tile's tokens by a group's heads by 64 dims, a cache as [blocks, kv_heads,
-// block_size, dim] in boxes of one page (at most 128 tokens) by 64 dims; the
-// 128-byte swizzle, zeros outside.
-bool prefix_maps(const q3s::AttnArgs& a, int dim, bool bf16, int per_tile, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v) {
+// Tensor maps: q as [T, q_heads, dim] in boxes of a tile's tokens by a group's
+// heads by 64 dims; a cache as [blocks, kv_heads, dim / 64, block_size, 64]
+// (the dims cut into slices of the swizzle's 128 bytes) in boxes of `slices`
+// slices of one page, at most `tokens` of it; zeros outside.  An axis of one
+// entry has no stride of its own: any that the encoder takes.
+bool encode(CUtensorMap* m, bool bf16, const void* base, int rank, const int64_t* dims, const int64_t* strides,
+            const int* box) {
   const q3s::EncodeTiled enc = q3s::encode_tiled();
   if (!enc) return false;
-  const CUtensorMapDataType type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const cuuint32_t ones[4] = {1, 1, 1, 1};
-  auto u = [](int64_t x) { return static_cast<cuuint64_t>(x); };
-  // an axis of one entry has no stride of its own: any that the encoder takes
-  auto bytes = [&](int64_t stride, int n, int64_t otherwise) { return u(2 * (n > 1 ? stride : otherwise)); };
-  {
-    const cuuint64_t dims[3] = {u(dim), u(a.Hq), u(a.T)};
-    const cuuint64_t strides[2] = {bytes(a.qh, a.Hq, dim), bytes(a.qt, a.T, static_cast<int64_t>(a.Hq) * dim)};
-    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.G), static_cast<cuuint32_t>(per_tile)};
-    if (enc(q, type, 3, const_cast<void*>(a.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return false;
+  cuuint64_t d[5], s[4];
+  cuuint32_t b[5], ones[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = static_cast<cuuint64_t>(dims[i]);
+    b[i] = static_cast<cuuint32_t>(box[i]);
+    if (i) s[i - 1] = static_cast<cuuint64_t>(2 * (dims[i] > 1 ? strides[i - 1] : 64));
   }
-  auto cache = [&](CUtensorMap* m, const void* base, int64_t block, int64_t head, int64_t place) {
-    const cuuint64_t dims[4] = {u(dim), u(a.bs), u(a.H), u(a.blocks)};
-    const cuuint64_t strides[3] = {bytes(place, a.bs, dim), bytes(head, a.H, static_cast<int64_t>(a.bs) * dim),
-                                   bytes(block, a.blocks, static_cast<int64_t>(a.H) * a.bs * dim)};
-    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(std::min(a.bs, q3s::PX_KEYS)), 1, 1};
-    return enc(m, type, 4, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-  };
-  return cache(k, a.k, a.kb, a.kh, a.kp) && cache(v, a.v, a.vb, a.vh, a.vp);
+  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+             const_cast<void*>(base), d, s, b, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool query_map(const q3s::AttnArgs& a, int dim, bool bf16, int per_tile, CUtensorMap* q) {
+  const int64_t dims[3] = {dim, a.Hq, a.T}, strides[2] = {a.qh, a.qt};
+  const int box[3] = {64, a.G, per_tile};
+  return encode(q, bf16, a.q, 3, dims, strides, box);
+}
+bool cache_maps(const q3s::AttnArgs& a, int dim, bool bf16, int tokens, int slices, CUtensorMap* k, CUtensorMap* v) {
+  const int64_t dims[5] = {64, a.bs, dim / 64, a.H, a.blocks};
+  const int64_t ks[4] = {a.kp, 64, a.kh, a.kb}, vs[4] = {a.vp, 64, a.vh, a.vb};
+  const int box[5] = {64, std::min(a.bs, tokens), slices, 1, 1};
+  return encode(k, bf16, a.k, 5, dims, ks, box) && encode(v, bf16, a.v, 5, dims, vs, box);
+}
+
+template <int D, bool BF16, int NQ>
+cudaError_t launch_split(const q3s::AttnArgs& a, const Layout& l, const CUtensorMap& tk, const CUtensorMap& tv,
+                         cudaStream_t st) {
+  auto split = q3s::attn_split_kernel<D, BF16, NQ>;
+  constexpr int smem = q3s::SplitTile<D>::SMEM;
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = q3s::allow_smem(split, smem, done);
+  if (e != cudaSuccess) return e;
+  // beside the prefix kernel where there is one: neither reads what the other writes
+  e = q3s::launch_maybe_pdl(split, dim3(l.ctas), dim3(kSplitThreads), smem, st, l.splits > 0, tk, tv, a);
+  if (e != cudaSuccess) return e;
+  // a warp joins one query row: rows of a (row, head) spread over gridDim.z CTAs of 4 warps
+  const int64_t per = (static_cast<int64_t>(a.T) * a.G + a.B - 1) / std::max(a.B, 1);
+  const int z = static_cast<int>(std::min<int64_t>(64, std::max<int64_t>(1, (per + 3) / 4)));
+  return q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, NQ>, dim3(a.B + 1, a.H, z), dim3(128), 0, st, true, a);
 }
 
 template <int D, bool BF16>
 cudaError_t launch(const q3s::AttnArgs& a, const Layout& l, cudaStream_t st) {
+  CUtensorMap tk, tv;
   cudaError_t e;
   if (l.splits) {
     auto prefix = q3s::attn_prefix_kernel<D, BF16>;
@@ -151,8 +175,8 @@ cudaError_t launch(const q3s::AttnArgs& a, const Layout& l, cudaStream_t st) {
     static std::atomic<uint64_t> prefix_done{0};
     e = q3s::allow_smem(prefix, smem, prefix_done);
     if (e != cudaSuccess) return e;
-    CUtensorMap tq, tk, tv;
-    if (!prefix_maps(a, D, BF16, l.per_tile, &tq, &tk, &tv)) return cudaErrorInvalidValue;
+    CUtensorMap tq;
+    if (!query_map(a, D, BF16, l.per_tile, &tq) || !cache_maps(a, D, BF16, q3s::PX_KEYS, 1, &tk, &tv)) return cudaErrorInvalidValue;
     q3s::PrefixArgs p;
     p.a = a;
     p.per_tile = l.per_tile;
@@ -163,17 +187,10 @@ cudaError_t launch(const q3s::AttnArgs& a, const Layout& l, cudaStream_t st) {
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
-  auto split = q3s::attn_split_kernel<D, BF16>;
-  static std::atomic<uint64_t> done{0};
-  e = q3s::allow_smem(split, split_smem(D), done);
-  if (e != cudaSuccess) return e;
-  // beside the prefix kernel where there is one: neither reads what the other writes
-  e = q3s::launch_maybe_pdl(split, dim3(l.ctas), dim3(kSplitThreads), split_smem(D), st, l.splits > 0, a);
-  if (e != cudaSuccess) return e;
-  // a warp joins one query row: rows of a (row, head) spread over gridDim.z CTAs of 4 warps
-  const int64_t per = (static_cast<int64_t>(a.T) * a.G + a.B - 1) / std::max(a.B, 1);
-  const int z = static_cast<int>(std::min<int64_t>(64, std::max<int64_t>(1, (per + 3) / 4)));
-  return q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16>, dim3(a.B + 1, a.H, z), dim3(128), 0, st, true, a);
+  if (!cache_maps(a, D, BF16, q3s::AT_KEYS, D / 64, &tk, &tv)) return cudaErrorInvalidValue;
+  if (l.nq == 1) return launch_split<D, BF16, 1>(a, l, tk, tv, st);
+  if (l.nq == 2) return launch_split<D, BF16, 2>(a, l, tk, tv, st);
+  return launch_split<D, BF16, 4>(a, l, tk, tv, st);
 }
 
 }  // namespace
@@ -216,10 +233,12 @@ extern "C" q3s_status q3s_prefix_attention(const q3s_prefix_attention_desc* d, v
   a.H = d->kv_heads;
   a.G = d->q_heads / d->kv_heads;
   a.bs = d->block_size;
+  a.bs_log2 = 4;
+  while ((1 << a.bs_log2) < a.bs) ++a.bs_log2;
   a.blocks = d->blocks;
   a.max_blocks = d->max_blocks;
   a.L = d->prefix_length;
-  a.prefix_here = l.prefix_here;
+  a.tiles0 = l.tiles0;
   a.splits = l.splits;
   a.scale_log2 = d->scale * 1.4426950408889634f;
   a.q = d->q;
@@ -244,9 +263,10 @@ extern "C" q3s_status q3s_prefix_attention(const q3s_prefix_attention_desc* d, v
   a.lse = d->lse;
   a.error_word = d->error_word;
   unsigned char* ws = static_cast<unsigned char*>(d->workspace);
-  a.plan = reinterpret_cast<int32_t*>(ws + l.plan);
+  a.items = reinterpret_cast<int2*>(ws + l.items);
   a.part_o = reinterpret_cast<float*>(ws + l.part_o);
   a.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
+  a.ids = l.ids;
   a.slots = l.slots;
   a.pre_o = reinterpret_cast<float*>(ws + l.pre_o);
   a.pre_ml = reinterpret_cast<float2*>(ws + l.pre_ml);

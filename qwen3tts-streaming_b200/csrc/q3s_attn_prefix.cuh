@@ -38,11 +38,12 @@ Q3S_DEV void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
 }
-Q3S_DEV void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int q, uint64_t* bar) {
+// Part of one block of a cache, 64 dims (slice x).
+Q3S_DEV void tma_load_slice(uint32_t dst, const CUtensorMap* map, int x, int place, int h, int block, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::
           "r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(q), "r"(smem_u32(bar))
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(place), "r"(x), "r"(h), "r"(block), "r"(smem_u32(bar))
       : "memory");
 }
 // D += A B with A from TMEM.
@@ -59,6 +60,12 @@ Q3S_DEV void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint3
 Q3S_DEV uint64_t v_smem_desc(uint32_t saddr) {
   return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>((PX_KEYS * 128) >> 4) << 16) |
          (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// One lane of a converged warp (the compiler then knows that the branch is taken by one thread).
+Q3S_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
 }
 Q3S_DEV void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -165,8 +172,8 @@ Q3S_DEV void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
 // what the product takes; the prefix of a large batch has many keys, over
 // which it averages out (the other kernel, for few keys, holds p in two).
 //
-// Keys past the end: whole pages read as zeros (an out-of-range block
-// coordinate), the rest of the last page is cleared in V and masked in S.
+// Keys past the end: whole boxes read as zeros (an out-of-range block
+// coordinate), the rest of the last one is cleared in V and masked in S.
 // Bound by the exponentials (16 a clock and SM: 1024 clocks for 128 x 128
 // scores) and, equally, by the two products (1024 clocks at the tensor peak).
 template <int D, bool BF16>
@@ -190,7 +197,8 @@ __global__ void __launch_bounds__(PX_NT, 1)
   uint64_t* s_full = v_empty + PX_STAGES;  // [2] scores of a tile are in TMEM
   uint64_t* p_full = s_full + 2;           // [2] its probabilities are
   uint64_t* o_done = p_full + 2;           // [2] its second product is
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+  uint64_t* v_clean = o_done + 2;          // V of a part's ragged last step has been cleared past its end
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_clean + 1);
   int* failed = reinterpret_cast<int*>(tmem_slot + 1);
   const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
   asm volatile("griddepcontrol.launch_dependents;");
@@ -202,6 +210,7 @@ __global__ void __launch_bounds__(PX_NT, 1)
 
   if (t == 0) {
     mbar_init(q_full, 1);
+    mbar_init(v_clean, 1);
     for (int s = 0; s < PX_STAGES; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
@@ -235,7 +244,8 @@ __global__ void __launch_bounds__(PX_NT, 1)
   };
 
   if (w == 8) {
-    // ---- copies: lane l copies page l of a step ------------------------------
+    if (lane < 3) prefetch_map(lane == 0 ? &tm_q : lane == 1 ? &tm_k : &tm_v);
+    // ---- copies: lane l copies box l of a step (a page, or 128 tokens of one) ------------------------------
     const int rows = min(a.bs, PX_KEYS), pages = PX_KEYS / rows;
     if (lane == 0) {
       mbar_expect_tx(q_full, static_cast<uint32_t>(tiles * HALVES * p.per_tile * a.G * 128));
@@ -246,9 +256,9 @@ __global__ void __launch_bounds__(PX_NT, 1)
     int j = 0, bad = 0;
     for (; j < steps; ++j) {
       const int s = j % PX_STAGES;
-      int id = a.blocks;  // past the cache: the page reads as zeros
+      int id = a.blocks;  // past the cache: it reads as zeros
+      const int key = (step0 + j) * PX_KEYS + lane * rows, place = key % a.bs;
       if (lane < pages) {
-        const int key = (step0 + j) * PX_KEYS + lane * rows;
         if (key < a.L) {
           id = a.prefix_blocks[key / a.bs];
           if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.blocks)) {
@@ -263,13 +273,25 @@ __global__ void __launch_bounds__(PX_NT, 1)
         __syncwarp();
         if (lane < pages)
           for (int x = 0; x < HALVES; ++x)
-            tma_load_4d(smem_u32(ring + s * Tile::KV_BYTES + x * PX_KEYS * 128 + lane * rows * 128), map, 64 * x, 0, h, id, &full[s]);
+            tma_load_slice(smem_u32(ring + s * Tile::KV_BYTES + x * PX_KEYS * 128 + lane * rows * 128), map, x, place, h, id, &full[s]);
         return true;
       };
       if (!copy(&tm_k, s_k, k_full, k_empty)) break;
       if (!copy(&tm_v, s_v, v_full, v_empty)) break;
     }
     if (bad && a.error_word) atomicOr(a.error_word, Q3S_DECERR_BLOCK_ID);
+    const int valid = a.L - (step0 + steps - 1) * PX_KEYS;  // keys of the last step
+    if (j == steps && valid < PX_KEYS) {  // clear V past the end, up to the end of its box
+      const int last = steps - 1, s = last % PX_STAGES, end = (valid + rows - 1) / rows * rows;
+      if (__all_sync(FULL, wait(&v_full[s], (last / PX_STAGES) & 1))) {
+        for (int c = lane; c < (end - valid) * 8; c += 32)
+          for (int x = 0; x < HALVES; ++x)
+            *reinterpret_cast<uint4*>(s_v + s * Tile::KV_BYTES + x * PX_KEYS * 128 + valid * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_clean);
+      }
+    }
     // no copy may be in flight when the CTA leaves: wait for each stage's last one
     if (lane == 0) {
       (void)mbar_wait_bounded(q_full, 0);
@@ -285,62 +307,51 @@ __global__ void __launch_bounds__(PX_NT, 1)
                               (static_cast<uint32_t>(PX_M >> 4) << 24);
     constexpr uint32_t ID_O = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) |
                               (static_cast<uint32_t>(PX_M >> 4) << 24);  // bit 16: B's rows are the contraction
-    auto scores = [&](int i, int s) {
-      if (lane == 0) {
-        const uint32_t q0 = smem_u32(s_q + i * Tile::Q_BYTES), k0 = smem_u32(s_k + s * Tile::KV_BYTES);
+    if (elect_one()) {
+      const uint64_t q_desc = head_smem_desc(smem_u32(s_q)), k_desc = head_smem_desc(smem_u32(s_k)), v_desc = v_smem_desc(smem_u32(s_v));
+      auto scores = [&](int i, int s) {  // S_i = Q_i K^T
+        const uint64_t dq = q_desc + static_cast<uint64_t>(i * (Tile::Q_BYTES >> 4)), dk = k_desc + static_cast<uint64_t>(s * (Tile::KV_BYTES >> 4));
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
-          const uint32_t off = static_cast<uint32_t>((c / 4) * PX_KEYS * 128 + (c % 4) * 32);
-          umma_f16(tmem + static_cast<uint32_t>(128 * i), head_smem_desc(q0 + off), head_smem_desc(k0 + off), ID_S, c != 0);
+          constexpr int SLICE = (PX_KEYS * 128) >> 4;
+          umma_f16(tmem + static_cast<uint32_t>(128 * i), dq + (c / 4) * SLICE + (c % 4) * 2, dk + (c / 4) * SLICE + (c % 4) * 2, ID_S, c != 0);
         }
         umma_commit(&s_full[i]);
+      };
+      bool ok = wait(q_full, 0) && wait(&k_full[0], 0);
+      tc_fence_after();
+      if (ok) {
+        for (int i = 0; i < tiles; ++i) scores(i, 0);
+        umma_commit(&k_empty[0]);
       }
-      __syncwarp();
-    };
-    bool ok = __all_sync(FULL, wait(q_full, 0)) && __all_sync(FULL, wait(&k_full[0], 0));
-    tc_fence_after();
-    if (ok) {
-      for (int i = 0; i < tiles; ++i) scores(i, 0);
-      if (lane == 0) umma_commit(&k_empty[0]);
-    }
-    for (int j = 0; ok && j < steps; ++j) {
-      const int s = j % PX_STAGES, s1 = (j + 1) % PX_STAGES;
-      if (!__all_sync(FULL, wait(&v_full[s], (j / PX_STAGES) & 1))) break;
-      const int valid = a.L - (step0 + j) * PX_KEYS;  // keys of this step
-      if (valid < PX_KEYS) {                          // clear V past the end, up to the end of its page
-        const int end = min((valid + a.bs - 1) / a.bs * a.bs, PX_KEYS);
-        for (int c = lane; c < (end - valid) * 8; c += 32)
-          for (int x = 0; x < HALVES; ++x)
-            *reinterpret_cast<uint4*>(s_v + s * Tile::KV_BYTES + x * PX_KEYS * 128 + valid * 128 + c * 16) = make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-      for (int i = 0; ok && i < tiles; ++i) {
-        ok = __all_sync(FULL, wait(&p_full[i], j & 1));
-        if (!ok) break;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t v0 = smem_u32(s_v + s * Tile::KV_BYTES);
+      for (int j = 0; ok && j < steps; ++j) {
+        const int s = j % PX_STAGES, s1 = (j + 1) % PX_STAGES;
+        ok = wait(&v_full[s], (j / PX_STAGES) & 1);
+        if (ok && j + 1 == steps && a.L < (step0 + steps) * PX_KEYS) ok = wait(v_clean, 0);
+        for (int i = 0; ok && i < tiles; ++i) {
+          ok = wait(&p_full[i], j & 1);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t dv = v_desc + static_cast<uint64_t>(s * (Tile::KV_BYTES >> 4));
 #pragma unroll
-          for (int c = 0; c < PX_KEYS / 16; ++c)
+          for (int c = 0; c < PX_KEYS / 16; ++c)  // O_i += P_i V
             umma_f16_ta(tmem + static_cast<uint32_t>(256 + 128 * i), tmem + static_cast<uint32_t>(128 * i + 8 * c),
-                        v_smem_desc(v0 + static_cast<uint32_t>(c * 16 * 128)), ID_O, (j | c) != 0);
+                        dv + c * ((16 * 128) >> 4), ID_O, (j | c) != 0);
           if (i == tiles - 1) umma_commit(&v_empty[s]);
           umma_commit(&o_done[i]);
-        }
-        __syncwarp();
-        if (j + 1 < steps) {
-          if (i == 0) {
-            ok = __all_sync(FULL, wait(&k_full[s1], ((j + 1) / PX_STAGES) & 1));
-            if (!ok) break;
-            tc_fence_after();
+          if (j + 1 < steps) {
+            if (i == 0) {
+              ok = wait(&k_full[s1], ((j + 1) / PX_STAGES) & 1);
+              if (!ok) break;
+              tc_fence_after();
+            }
+            scores(i, s1);
+            if (i == tiles - 1) umma_commit(&k_empty[s1]);
           }
-          scores(i, s1);
         }
       }
-      if (ok && lane == 0 && j + 1 < steps) umma_commit(&k_empty[s1]);
-      __syncwarp();
     }
+    __syncwarp();
   } else {
     // ---- softmax ----------------------------------------------------------------
     const int i = w >> 2, row = (w & 3) * 32 + lane;
@@ -411,21 +422,37 @@ __global__ void __launch_bounds__(PX_NT, 1)
       if (ok) ok = __all_sync(FULL, wait(&o_done[i], (steps - 1) & 1));
       if (ok) {
         tc_fence_after();
-        const int token = token0 + i * p.per_tile + row / a.G, g = row % a.G;
-        const bool in = row < p.per_tile * a.G && token < a.T;
-        const int64_t at = (static_cast<int64_t>(split) * a.T + token) * a.Hq + h * a.G + g;
-        float* dst = a.pre_o + at * D;
+        // O through shared memory, so that a row's stores are whole lines: tile
+        // 0's rows in the K ring, whose last readers came before this tile's last
+        // product, tile 1's in the V ring; a warp stages and stores its own 32
+        // rows (16-byte chunk c of row r at c ^ (r & 7))
+        unsigned char* stage = (i == 0 ? s_k : s_v) + (w & 3) * (32 * D * 4);
 #pragma unroll 1
         for (int k = 0; k < D / 32; ++k) {
           float v[32];
           tmem_ld32(to + static_cast<uint32_t>(32 * k), v);
-          if (in) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(dst + 32 * k + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-          }
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<float4*>(stage + lane * D * 4 + (((8 * k + e) ^ (lane & 7)) << 4)) =
+                make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
         }
-        if (in) a.pre_ml[at] = make_float2(m, l);
+        __syncwarp();
+        auto at = [&](int r) {  // query row r of the tile, in the part's rows (-1: there is none)
+          const int token = token0 + i * p.per_tile + r / a.G;
+          return r < p.per_tile * a.G && token < a.T
+                     ? (static_cast<int64_t>(split) * a.T + token) * a.Hq + h * a.G + r % a.G
+                     : static_cast<int64_t>(-1);
+        };
+        const int64_t mine = at(row);
+        if (mine >= 0) a.pre_ml[mine] = make_float2(m, l);
+        constexpr int LANES = D / 4, ROWS = 32 / LANES;  // lanes of a row, rows at a time
+#pragma unroll 4
+        for (int r0 = 0; r0 < 32; r0 += ROWS) {
+          const int r = r0 + lane / LANES, c = lane % LANES;
+          const int64_t to_row = __shfl_sync(FULL, mine, r);
+          const float4 v = *reinterpret_cast<const float4*>(stage + r * D * 4 + ((c ^ (r & 7)) << 4));
+          if (to_row >= 0) *reinterpret_cast<float4*>(a.pre_o + to_row * D + c * 4) = v;
+        }
       }
     }
   }
