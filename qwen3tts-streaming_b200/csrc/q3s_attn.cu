@@ -12,18 +12,19 @@
 
 namespace {
 
-constexpr int kSplitThreads = q3s::AT_WARPS * 32;
-
-int split_smem(int dim) { return dim == 64 ? q3s::SplitTile<64>::SMEM : q3s::SplitTile<128>::SMEM; }
-// CTAs of the key-split kernel: as many as are resident
-int split_ctas(int dim) { return q3s::sm_count() * ((227 * 1024) / (split_smem(dim) + 4096)); }
+// Computing warps of the key-split kernel's grid.
+template <int D, int NQ>
+int split_warps() {
+  using Tile = q3s::SplitTile<D, NQ>;
+  return q3s::sm_count() * Tile::PER_SM * Tile::WARPS;
+}
 
 struct Layout {
   int64_t items, part_o, part_ml, pre_o, pre_ml, bytes;  // byte offsets
   int64_t ids, slots;
-  int ctas;
-  int nq;      // 8-row query tiles of an item of the key-split kernel: 1, 2 or 4
+  int nq;      // 8-row query tiles of an item of the key-split kernel: 1 or 2
   int tiles0;  // tiles of the prefix there (0: none)
+  int early, lead;
   int per_tile, pairs, steps, per_split, splits;  // the prefix kernel's (splits 0: not used)
 };
 
@@ -37,7 +38,7 @@ void plan_prefix(const q3s_prefix_attention_desc* d, Layout* l) {
   l->pairs = (d->tokens + 2 * l->per_tile - 1) / (2 * l->per_tile);
   l->steps = (d->prefix_length + q3s::PX_KEYS - 1) / q3s::PX_KEYS;
   const int64_t items = static_cast<int64_t>(l->pairs) * d->kv_heads, sms = q3s::sm_count();
-  const double step_us = 1.2, part_us = static_cast<double>(d->tokens) * d->q_heads * d->dim * 8 / 6e6;
+  const double step_us = 1.6, part_us = 0.5 + static_cast<double>(d->tokens) * d->q_heads * d->dim * 8 / 6e6;
   double best = 0;
   for (int s = 1; s <= l->steps && s <= 64; ++s) {
     const int per = (l->steps + s - 1) / s, parts = (l->steps + per - 1) / per;
@@ -61,15 +62,23 @@ Layout layout_of(const q3s_prefix_attention_desc* d) {
   // follow.
   l.splits = 0;
   if (queries >= 64 && d->prefix_length >= 64 && d->scale > 0.0f) plan_prefix(d, &l);
-  l.ctas = split_ctas(d->dim);
   // An item of the key-split kernel holds the query rows of an average row of
-  // the batch (an item reads its keys once), in tiles of 8 to 32.
+  // the batch (an item reads its keys once), in tiles of 8 or 16.
   const int64_t mean = (queries + std::max(d->batch, 1) - 1) / std::max(d->batch, 1);
-  l.nq = mean <= 8 ? 1 : mean <= 16 ? 2 : 4;
+  l.nq = mean <= 8 ? 1 : 2;
+  const int64_t warps = d->dim == 64 ? (l.nq == 1 ? split_warps<64, 1>() : split_warps<64, 2>())
+                                     : (l.nq == 1 ? split_warps<128, 1>() : split_warps<128, 2>());
+  // A CTA of the prefix kernel has a SM for itself: this kernel's CTAs that
+  // would be there start when it ends, about that many units (of a good
+  // microsecond) later.
+  const int64_t busy = l.splits ? std::min<int64_t>(static_cast<int64_t>(l.pairs) * d->kv_heads * l.splits, q3s::sm_count()) : 0;
+  const int64_t ctas = warps / q3s::SplitTile<64, 1>::WARPS;
+  l.early = static_cast<int>(ctas - busy * (ctas / q3s::sm_count()));
+  l.lead = l.splits ? 5 + l.per_split * 3 / 2 : 0;
   const int64_t R = 8 * l.nq;
   l.tiles0 = l.splits || d->prefix_length == 0 ? 0 : static_cast<int>((queries + R - 1) / R);
   l.ids = (l.tiles0 + queries / R + d->batch + 1) * d->kv_heads;
-  l.slots = l.ids + static_cast<int64_t>(l.ctas) * q3s::AT_WARPS;
+  l.slots = l.ids + warps;
   auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
   int64_t at = 0;
   l.items = at;
@@ -149,48 +158,44 @@ bool cache_maps(const q3s::AttnArgs& a, int dim, bool bf16, int tokens, int slic
 }
 
 template <int D, bool BF16, int NQ>
-cudaError_t launch_split(const q3s::AttnArgs& a, const Layout& l, const CUtensorMap& tk, const CUtensorMap& tv,
-                         cudaStream_t st) {
+cudaError_t launch_split(const q3s::AttnArgs& a, bool beside, cudaStream_t st) {
+  using Tile = q3s::SplitTile<D, NQ>;
   auto split = q3s::attn_split_kernel<D, BF16, NQ>;
-  constexpr int smem = q3s::SplitTile<D>::SMEM;
   static std::atomic<uint64_t> done{0};
-  cudaError_t e = q3s::allow_smem(split, smem, done);
+  const cudaError_t e = q3s::allow_smem(split, Tile::SMEM, done);
   if (e != cudaSuccess) return e;
-  // beside the prefix kernel where there is one: neither reads what the other writes
-  e = q3s::launch_maybe_pdl(split, dim3(l.ctas), dim3(kSplitThreads), smem, st, l.splits > 0, tk, tv, a);
+  CUtensorMap tk, tv;
+  if (!cache_maps(a, D, BF16, q3s::AT_KEYS, D / 64, &tk, &tv)) return cudaErrorInvalidValue;
+  return q3s::launch_maybe_pdl(split, dim3(q3s::sm_count() * Tile::PER_SM), dim3(Tile::NT), Tile::SMEM, st, beside, tk, tv, a);
+}
+
+template <int D, bool BF16>
+cudaError_t launch_prefix(const q3s::AttnArgs& a, const Layout& l, cudaStream_t st) {
+  auto prefix = q3s::attn_prefix_kernel<D, BF16>;
+  constexpr int smem = q3s::PrefixTile<D>::SMEM;
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = q3s::allow_smem(prefix, smem, done);
   if (e != cudaSuccess) return e;
-  // a warp joins one query row: rows of a (row, head) spread over gridDim.z CTAs of 4 warps
-  const int64_t per = (static_cast<int64_t>(a.T) * a.G + a.B - 1) / std::max(a.B, 1);
-  const int z = static_cast<int>(std::min<int64_t>(64, std::max<int64_t>(1, (per + 3) / 4)));
-  return q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, NQ>, dim3(a.B + 1, a.H, z), dim3(128), 0, st, true, a);
+  CUtensorMap tq, tk, tv;
+  if (!query_map(a, D, BF16, l.per_tile, &tq) || !cache_maps(a, D, BF16, q3s::PX_KEYS, 1, &tk, &tv)) return cudaErrorInvalidValue;
+  q3s::PrefixArgs p;
+  p.a = a;
+  p.per_tile = l.per_tile;
+  p.steps = l.steps;
+  p.per_split = l.per_split;
+  return q3s::launch_maybe_pdl(prefix, dim3(l.pairs, a.H, l.splits), dim3(q3s::PX_NT), smem, st, false, tq, tk, tv, p);
 }
 
 template <int D, bool BF16>
 cudaError_t launch(const q3s::AttnArgs& a, const Layout& l, cudaStream_t st) {
-  CUtensorMap tk, tv;
-  cudaError_t e;
-  if (l.splits) {
-    auto prefix = q3s::attn_prefix_kernel<D, BF16>;
-    constexpr int smem = q3s::PrefixTile<D>::SMEM;
-    static std::atomic<uint64_t> prefix_done{0};
-    e = q3s::allow_smem(prefix, smem, prefix_done);
-    if (e != cudaSuccess) return e;
-    CUtensorMap tq;
-    if (!query_map(a, D, BF16, l.per_tile, &tq) || !cache_maps(a, D, BF16, q3s::PX_KEYS, 1, &tk, &tv)) return cudaErrorInvalidValue;
-    q3s::PrefixArgs p;
-    p.a = a;
-    p.per_tile = l.per_tile;
-    p.pairs = l.pairs;
-    p.steps = l.steps;
-    p.per_split = l.per_split;
-    prefix<<<dim3(l.pairs, a.H, l.splits), q3s::PX_NT, smem, st>>>(tq, tk, tv, p);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-  }
-  if (!cache_maps(a, D, BF16, q3s::AT_KEYS, D / 64, &tk, &tv)) return cudaErrorInvalidValue;
-  if (l.nq == 1) return launch_split<D, BF16, 1>(a, l, tk, tv, st);
-  if (l.nq == 2) return launch_split<D, BF16, 2>(a, l, tk, tv, st);
-  return launch_split<D, BF16, 4>(a, l, tk, tv, st);
+  cudaError_t e = l.splits ? launch_prefix<D, BF16>(a, l, st) : cudaSuccess;
+  if (e != cudaSuccess) return e;
+  // beside the prefix kernel where there is one: neither reads what the other writes
+  e = l.nq == 1 ? launch_split<D, BF16, 1>(a, l.splits > 0, st) : launch_split<D, BF16, 2>(a, l.splits > 0, st);
+  if (e != cudaSuccess) return e;
+  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(a.T) * a.Hq + 3) / 4));  // a warp a row
+  return l.nq == 1 ? q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, 1>, grid, dim3(128), 0, st, true, a)
+                   : q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, 2>, grid, dim3(128), 0, st, true, a);
 }
 
 }  // namespace
@@ -240,6 +245,8 @@ extern "C" q3s_status q3s_prefix_attention(const q3s_prefix_attention_desc* d, v
   a.L = d->prefix_length;
   a.tiles0 = l.tiles0;
   a.splits = l.splits;
+  a.early = l.early;
+  a.lead = l.lead;
   a.scale_log2 = d->scale * 1.4426950408889634f;
   a.q = d->q;
   a.k = d->k_cache;

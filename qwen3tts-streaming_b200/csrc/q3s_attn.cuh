@@ -22,8 +22,6 @@
 namespace q3s {
 
 constexpr int AT_KEYS = 16;    // keys of a unit (one pipeline stage of a warp); a block is a multiple of it
-constexpr int AT_WARPS = 8;
-constexpr int AT_STAGES = 3;
 constexpr int AT_MIN_UNITS = 3;  // fewest units a warp takes before another one is used
 
 struct AttnArgs {
@@ -31,6 +29,7 @@ struct AttnArgs {
   int L;            // prefix tokens
   int tiles0;       // item tiles of the prefix (0: it is the prefix kernel's, or empty)
   int splits;       // parts of the prefix kernel (0: not used)
+  int early, lead;  // CTAs of the key-split kernel that start at once, and how many units a warp of theirs takes more
   float scale_log2;
   const void *q, *k, *v;
   int64_t qt, qh, kb, kh, kp, vb, vh, vp;
@@ -146,6 +145,19 @@ Q3S_DEV void tma_load_block(uint32_t dst, const CUtensorMap* map, int place, int
       "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(place), "r"(h), "r"(block), "r"(smem_u32(bar))
       : "memory");
 }
+Q3S_DEV void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// Whether the phase of that parity is complete; does not wait.
+Q3S_DEV bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 Q3S_DEV void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -177,60 +189,93 @@ Q3S_DEV bool attn_next(const AttnArgs& a, AttnPos& p, const Rows& row_at) {
   return true;
 }
 
-template <int D>
+// Shapes of the key-split kernel: four computing warps (and one that copies)
+// with rings of three units; two CTAs a SM at dim 128, four or three at 64.
+template <int D, int NQ>
 struct SplitTile {
+  static constexpr int WARPS = 4, STAGES = 3;
+  static constexpr int PER_SM = D == 128 ? 2 : 5 - NQ;
+  static constexpr int NT = (WARPS + 1) * 32;
   static constexpr int HALVES = D / 64;                 // 128-byte slices of a key
   static constexpr int SLICE = AT_KEYS * 128;           // bytes of a unit's keys in one slice
   static constexpr int BYTES = HALVES * SLICE;          // a unit's keys (or values)
-  static constexpr int SMEM = 1024 + AT_WARPS * AT_STAGES * 2 * BYTES;
+  static constexpr int SMEM = 1024 + WARPS * STAGES * 2 * BYTES;
 };
 
+// How the unit list is cut into the warps' ranges.  The CTAs that find a SM
+// free start at once, the others when the prefix kernel leaves theirs: warps of
+// the first `early` CTAs take `lead` units more.
+struct AttnCut {
+  long long all, early, more, less;  // units, early warps, an early and a late warp's units
+  Q3S_DEV long long start(long long warp) const {
+    return min(warp < early ? warp * more : early * more + (warp - early) * less, all);
+  }
+  Q3S_DEV long long warp_of(long long u) const {
+    return u < early * more ? div_nonneg(u, more) : early + div_nonneg(u - early * more, less);
+  }
+};
+Q3S_DEV AttnCut attn_cut(const AttnArgs& a, long long all, long long ctas, long long per_cta) {
+  AttnCut c;
+  const long long warps = ctas * per_cta, rest = all - a.early * per_cta * a.lead, least = AT_MIN_UNITS;
+  c.all = all;
+  c.early = a.early * per_cta;
+  if (rest > 0 || c.early == 0) {
+    c.less = max(div_nonneg(max(rest, 0ll) + warps - 1, warps), least);
+    c.more = c.less + a.lead;
+  } else {  // the early ones can do it all
+    c.less = least;
+    c.more = max(div_nonneg(all + c.early - 1, c.early), least);
+  }
+  return c;
+}
+
 // The key-split kernel.  The keys of every item are cut into units of 16; all
-// units of the batch form one list, cut into equal contiguous ranges, one a
-// warp, so that rows of any lengths load the GPU evenly with no more than one
-// part per item plus one per warp.  Each CTA derives the list from the
-// device's lengths (one scan of the rows), so no host plan is needed and a
-// captured graph follows the lengths.
+// units of the batch form one list, cut into contiguous ranges, one a warp, so
+// that rows of any lengths load the GPU evenly with no more than one part per
+// item plus one per warp.  Each CTA derives the list from the device's lengths
+// (one scan of the rows), so no host plan is needed and a captured graph
+// follows the lengths.
 //
-// A warp works alone: lane 0 copies units into a three-stage ring of the
-// warp's own (TMA, 128-byte swizzle); what lies past the end of a row's last
-// unit is cleared in V (so that nothing that lies there, NaN included, reaches
-// the products) and masked in the scores.  Both products have the keys' side as the matrix
-// instruction's M (m16n8k16): S^T = K Q^T, O^T += V^T P^T, with N = 8 query
-// rows, so one query a row and its group of heads waste little of it.  p is
-// carried as the sum of two 16-bit values: rounding it to one would be the
-// largest error of a query that sees few keys.
+// The computing warps work alone, each on its own range with a ring of
+// its own; one more warp copies for them (lane l for warp l; TMA,
+// 128-byte swizzle), because issuing a unit's copies takes a third as long as
+// computing it.  What lies
+// past the end of a row's last unit is cleared in V (so that nothing that lies
+// there, NaN included, reaches the products) and masked in the scores.  Both
+// products have the keys' side as the matrix instruction's M (m16n8k16):
+// S^T = K Q^T, O^T += V^T P^T, with N = 8 query rows, so one query a row and its
+// group of heads waste little of it.  p is carried as the sum of two 16-bit
+// values: rounding it to one would be the largest error of a query that sees
+// few keys.
 //
 // With one query a row this is bound by reading the cache (2 * G useful
-// operations a byte); a warp's dependent chain of a unit has to stay below the
-// time its 16 KB take, which the query-row form (M = 16 query rows, mostly
-// padding; twice the instructions) did not: 34 us against .. us on 96 rows of
-// 125 to 500 own tokens.  The tcgen05 form, whose M is 128, would be nearly
-// empty; many queries on a long prefix are the other kernel's.
+// operations a byte), as long as a warp's dependent chain of a unit stays below
+// the time that its 8 KB take.  The tcgen05 form, whose M is 128, would be
+// nearly empty; many queries on a long prefix are the other kernel's.
 template <int D, bool BF16, int NQ>
-__global__ void __launch_bounds__(AT_WARPS * 32)
+__global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM)
     attn_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const AttnArgs a) {
-  using Tile = SplitTile<D>;
-  constexpr int R = 8 * NQ;
+  using Tile = SplitTile<D, NQ>;
+  constexpr int R = 8 * NQ, AT_WARPS = Tile::WARPS, AT_NT = Tile::NT, AT_STAGES = Tile::STAGES, BARS = AT_WARPS * AT_STAGES;
   extern __shared__ __align__(1024) unsigned char at_smem[];
-  __shared__ long long s_units[AT_WARPS * 32 + 1];
-  __shared__ AttnRow s_rows[AT_WARPS * 32];  // the rows, where there are no more than threads
-  __shared__ __align__(8) uint64_t s_bar[AT_WARPS * AT_STAGES];
+  __shared__ long long s_units[AT_NT + 1];
+  __shared__ AttnRow s_rows[AT_NT];  // the rows, where there are no more than threads
+  __shared__ __align__(8) uint64_t s_full[BARS], s_empty[BARS];
   const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
   asm volatile("griddepcontrol.launch_dependents;");
   if (t == 0) {
     prefetch_map(&tm_k);
     prefetch_map(&tm_v);
-  }
-  if (lane == 0) {
-    for (int i = 0; i < AT_STAGES; ++i) mbar_init(&s_bar[w * AT_STAGES + i], 1);
+    for (int i = 0; i < BARS; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 1);
+    }
     fence_mbar_init();
   }
 
   // ---- the work list: thread t sums rows [t * per, (t + 1) * per) ------------
-  const int rows = a.B + 1, NT = AT_WARPS * 32;
-  const int per = (rows + NT - 1) / NT;
+  const int rows = a.B + 1, per = (rows + AT_NT - 1) / AT_NT;
   long long mu = 0;
   bool bad = false;
   for (int i = 0; i < per; ++i) {
@@ -245,10 +290,11 @@ __global__ void __launch_bounds__(AT_WARPS * 32)
   s_units[t + 1] = mu;
   if (t == 0) s_units[0] = 0;
   __syncthreads();
-  if (w == 0) {  // inclusive scan of NT values, NT / 32 a lane
-    long long u[AT_WARPS], su = 0;
+  if (w == 0) {  // inclusive scan, AT_NT / 32 values a lane
+    constexpr int V = AT_NT / 32;
+    long long u[V], su = 0;
 #pragma unroll
-    for (int k = 0; k < AT_WARPS; ++k) u[k] = su += s_units[1 + lane * AT_WARPS + k];
+    for (int k = 0; k < V; ++k) u[k] = su += s_units[1 + lane * V + k];
     long long pu = su;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -257,23 +303,21 @@ __global__ void __launch_bounds__(AT_WARPS * 32)
     }
     pu -= su;
 #pragma unroll
-    for (int k = 0; k < AT_WARPS; ++k) s_units[1 + lane * AT_WARPS + k] = pu + u[k];
+    for (int k = 0; k < V; ++k) s_units[1 + lane * V + k] = pu + u[k];
   }
   __syncthreads();
-  const long long all = s_units[NT];
-  const long long warps = static_cast<long long>(gridDim.x) * AT_WARPS;
-  const long long quota = max(div_nonneg(all + warps - 1, warps), static_cast<long long>(AT_MIN_UNITS));
-  const long long gw = static_cast<long long>(blockIdx.x) * AT_WARPS + w;
-  const long long u0 = gw * quota, u1 = min(u0 + quota, all);
-  if (u0 >= u1) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    return;
-  }
+  const AttnCut cuts = attn_cut(a, s_units[AT_NT], gridDim.x, AT_WARPS);
+  // the range of this warp, or, in the copying warp, of warp `lane`
+  const int mine = w == AT_WARPS ? lane : w;
+  const long long gw = static_cast<long long>(blockIdx.x) * AT_WARPS + mine;
+  const long long u0 = cuts.start(gw);
+  const int total = mine < AT_WARPS ? static_cast<int>(cuts.start(gw + 1) - u0) : 0;
 
   auto row_at = [&](int r) { return per == 1 ? s_rows[r] : attn_row<R>(a, r); };
   AttnPos p;
-  {
-    int l = 0, r = NT;  // the last thread chunk that starts at or before u0
+  p.r = p.h = p.tile = p.u = 0;
+  if (total > 0) {
+    int l = 0, r = AT_NT;  // the last thread chunk that starts at or before u0
     while (r - l > 1) {
       const int m = (l + r) >> 1;
       if (s_units[m] <= u0) l = m; else r = m;
@@ -292,41 +336,48 @@ __global__ void __launch_bounds__(AT_WARPS * 32)
     p.h = in / p.x.tiles;
     p.tile = in - p.h * p.x.tiles;
   }
-
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(at_smem) + 1023) &
                                                          ~static_cast<uintptr_t>(1023)) +
-                        w * AT_STAGES * 2 * Tile::BYTES;
-  uint64_t* bars = s_bar + w * AT_STAGES;
-  const int total = static_cast<int>(u1 - u0);
+                        (mine < AT_WARPS ? mine : 0) * AT_STAGES * 2 * Tile::BYTES;
+  uint64_t* full = s_full + (mine < AT_WARPS ? mine : 0) * AT_STAGES;
+  uint64_t* empty = s_empty + (mine < AT_WARPS ? mine : 0) * AT_STAGES;
 
-  // ---- copies ----------------------------------------------------------------
-  AttnPos pf = p;  // the next unit to fetch
-  auto block_of = [&](const AttnPos& q) {  // its cache block, as the table has it
-    const int j = (q.u * AT_KEYS) >> a.bs_log2;
-    return q.r == 0 ? a.prefix_blocks[j] : a.table[(q.r - 1) * a.table_stride + j];
-  };
-  int next_id = block_of(pf), fetched = 0;
-  bool bad_block = false;
-  auto fetch = [&]() {
-    if (fetched >= total) return;
-    const int s = fetched % AT_STAGES;
-    if (lane == 0) {
+  if (w == AT_WARPS) {
+    // ---- copies: lane l for warp l -----------------------------------------------
+    auto block_of = [&](const AttnPos& q) {  // its cache block, as the table has it
+      const int j = (q.u * AT_KEYS) >> a.bs_log2;
+      return q.r == 0 ? a.prefix_blocks[j] : a.table[(q.r - 1) * a.table_stride + j];
+    };
+    int next_id = total > 0 ? block_of(p) : 0, fetched = 0, idle = 0;
+    bool bad_block = false;
+    while (fetched < total) {
+      const int s = fetched % AT_STAGES;
+      if (fetched >= AT_STAGES && !mbar_test(&empty[s], ((fetched / AT_STAGES) - 1) & 1)) {
+        if (++idle == (1 << 24)) break;  // the warp has given up: so does its copier
+        continue;
+      }
+      idle = 0;
       const uint32_t dst = smem_u32(ring + s * 2 * Tile::BYTES);
       const bool inside = static_cast<unsigned>(next_id) < static_cast<unsigned>(a.blocks);
       bad_block |= !inside;
       const int id = inside ? next_id : a.blocks;  // past the cache: reads as zeros
-      const int place = (pf.u * AT_KEYS) & (a.bs - 1);
-      mbar_expect_tx(&bars[s], 2 * Tile::BYTES);
-      tma_load_block(dst, &tm_k, place, pf.h, id, &bars[s]);
-      tma_load_block(dst + Tile::BYTES, &tm_v, place, pf.h, id, &bars[s]);
+      const int place = (p.u * AT_KEYS) & (a.bs - 1);
+      mbar_expect_tx(&full[s], 2 * Tile::BYTES);
+      tma_load_block(dst, &tm_k, place, p.h, id, &full[s]);
+      tma_load_block(dst + Tile::BYTES, &tm_v, place, p.h, id, &full[s]);
+      if (++fetched < total) {
+        attn_next(a, p, row_at);
+        next_id = block_of(p);  // not looked at before the next round: its latency is not waited for
+      }
     }
-    if (++fetched < total) {
-      attn_next(a, pf, row_at);
-      next_id = block_of(pf);  // not looked at before the next call: its latency is not waited for
-    }
-  };
-#pragma unroll
-  for (int s = 0; s < AT_STAGES - 1; ++s) fetch();
+    if (bad_block && a.error_word) atomicOr(a.error_word, Q3S_DECERR_BLOCK_ID);
+    // no copy may be in flight when the CTA leaves: wait for each stage's last one
+    for (int i = max(0, fetched - AT_STAGES); i < fetched; ++i)
+      (void)mbar_wait_bounded(&full[i % AT_STAGES], (i / AT_STAGES) & 1);
+    __syncwarp();
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // as below
+    return;
+  }
 
   // ---- products -----------------------------------------------------------------
   const int g = lane >> 2, tq = lane & 3;
@@ -344,13 +395,13 @@ __global__ void __launch_bounds__(AT_WARPS * 32)
       low = limit(r0);
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
-        const int mine = r0 + 8 * q + g;
-        const uint16_t* src = static_cast<const uint16_t*>(a.q) + static_cast<int64_t>(p.x.t0 + mine / a.G) * a.qt +
-                              (static_cast<int64_t>(p.h) * a.G + mine % a.G) * a.qh + 2 * tq;
+        const int row = r0 + 8 * q + g;
+        const uint16_t* src = static_cast<const uint16_t*>(a.q) + static_cast<int64_t>(p.x.t0 + row / a.G) * a.qt +
+                              (static_cast<int64_t>(p.h) * a.G + row % a.G) * a.qh + 2 * tq;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          qf[q][k][0] = mine < M ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u;
-          qf[q][k][1] = mine < M ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u;
+          qf[q][k][0] = row < M ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u;
+          qf[q][k][1] = row < M ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u;
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -363,10 +414,9 @@ __global__ void __launch_bounds__(AT_WARPS * 32)
       }
     }
     const int st = done % AT_STAGES;
-    if (lane == 0) ok = mbar_wait_bounded(&bars[st], (done / AT_STAGES) & 1);
+    if (lane == 0) ok = mbar_wait_bounded(&full[st], (done / AT_STAGES) & 1);
     ok = __shfl_sync(FULL, ok, 0);
     if (!ok) break;
-    fetch();  // into the stage that the last unit has left
     unsigned char* kt = ring + st * 2 * Tile::BYTES;
     const int j0 = p.u * AT_KEYS, valid = p.x.len - j0;
     if (valid < AT_KEYS) {  // clear V past the end
@@ -379,101 +429,104 @@ __global__ void __launch_bounds__(AT_WARPS * 32)
     }
     const uint32_t ka = smem_u32(kt), va = ka + Tile::BYTES;
 
-    float s[AT_KEYS / 16][NQ][4];
+    float s[2][NQ][4];  // two chains of sums, over every other 16 dims
 #pragma unroll
-    for (int i = 0; i < AT_KEYS / 16; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int q = 0; q < NQ; ++q) s[i][q][0] = s[i][q][1] = s[i][q][2] = s[i][q][3] = 0.0f;
     {
       // the four 8x8 matrices: keys (lane & 7) + 8 ((lane >> 3) & 1), 16-byte chunk + (lane >> 4)
       const int key = (lane & 7) + (((lane >> 3) & 1) << 3), cc = lane >> 4, x7 = key & 7;
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k)
+      for (int k = 0; k < D / 16; ++k) {
+        uint32_t f[4];
+        ldsm4(f, ka + static_cast<uint32_t>((k / 4) * Tile::SLICE + key * 128 + ((((2 * k) & 7) + cc) ^ x7) * 16));
 #pragma unroll
-        for (int i = 0; i < AT_KEYS / 16; ++i) {
-          uint32_t f[4];
-          ldsm4(f, ka + static_cast<uint32_t>((k / 4) * Tile::SLICE + (16 * i + key) * 128 + ((((2 * k) & 7) + cc) ^ x7) * 16));
-#pragma unroll
-          for (int q = 0; q < NQ; ++q) mma16816<BF16>(s[i][q], f, qf[q][k][0], qf[q][k][1]);
-        }
+        for (int q = 0; q < NQ; ++q) mma16816<BF16>(s[k & 1][q], f, qf[q][k][0], qf[q][k][1]);
+      }
     }
     const bool cut = j0 + AT_KEYS - 1 > low;
-    uint32_t ph[AT_KEYS / 16][NQ][2], pl[AT_KEYS / 16][NQ][2];  // p^T, upper and lower part: the B operand
+    float c[NQ][2], base[NQ][2];
+    bool moved = false;
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
       float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < AT_KEYS / 16; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[i][q][e] *= a.scale_log2;
-          if (cut && j0 + 16 * i + g + 8 * (e >> 1) > lim[q][e & 1]) s[i][q][e] = -INFINITY;
-          top[e & 1] = fmaxf(top[e & 1], s[i][q][e]);
-        }
+      for (int e = 0; e < 4; ++e) {
+        s[0][q][e] = (s[0][q][e] + s[1][q][e]) * a.scale_log2;
+        if (cut && j0 + g + 8 * (e >> 1) > lim[q][e & 1]) s[0][q][e] = -INFINITY;
+        top[e & 1] = fmaxf(top[e & 1], s[0][q][e]);
+      }
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) {
         top[0] = fmaxf(top[0], __shfl_xor_sync(FULL, top[0], d));
         top[1] = fmaxf(top[1], __shfl_xor_sync(FULL, top[1], d));
       }
-      const float n0 = fmaxf(m[q][0], top[0]), n1 = fmaxf(m[q][1], top[1]);
-      const float b0 = n0 == -INFINITY ? 0.0f : n0, b1 = n1 == -INFINITY ? 0.0f : n1;
-      if (__any_sync(FULL, n0 != m[q][0] || n1 != m[q][1])) {
-        const float c0 = ex2(m[q][0] - b0), c1 = ex2(m[q][1] - b1);  // 0 for the item's first unit (m = -inf)
-        l[q][0] *= c0;
-        l[q][1] *= c1;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float nm = fmaxf(m[q][e], top[e]);
+        base[q][e] = nm == -INFINITY ? 0.0f : nm;
+        moved |= nm != m[q][e];
+        c[q][e] = ex2(m[q][e] - base[q][e]);  // 0 for the item's first unit (m = -inf)
+        m[q][e] = nm;
+      }
+    }
+    if (__any_sync(FULL, moved)) {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        l[q][0] *= c[q][0];
+        l[q][1] *= c[q][1];
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
-          o[i][q][0] *= c0;
-          o[i][q][1] *= c1;
-          o[i][q][2] *= c0;
-          o[i][q][3] *= c1;
+          o[i][q][0] *= c[q][0];
+          o[i][q][1] *= c[q][1];
+          o[i][q][2] *= c[q][0];
+          o[i][q][3] *= c[q][1];
         }
-        m[q][0] = n0;
-        m[q][1] = n1;
       }
-#pragma unroll
-      for (int i = 0; i < AT_KEYS / 16; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float p0 = ex2(s[i][q][2 * e] - b0), p1 = ex2(s[i][q][2 * e + 1] - b1);
-          l[q][0] += p0;
-          l[q][1] += p1;
-          const uint32_t hi = pack2<BF16>(p0, p1);
-          const float2 back = unpack2<BF16>(hi);
-          ph[i][q][e] = transpose8(hi);
-          pl[i][q][e] = transpose8(pack2<BF16>(p0 - back.x, p1 - back.y));
-        }
     }
+    uint32_t ph[NQ][2], pl[NQ][2];  // p^T, upper and lower part: the B operand
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float p0 = ex2(s[0][q][2 * e] - base[q][0]), p1 = ex2(s[0][q][2 * e + 1] - base[q][1]);
+        l[q][0] += p0;
+        l[q][1] += p1;
+        const uint32_t hi = pack2<BF16>(p0, p1);
+        const float2 back = unpack2<BF16>(hi);
+        ph[q][e] = transpose8(hi);
+        pl[q][e] = transpose8(pack2<BF16>(p0 - back.x, p1 - back.y));
+      }
     {
       // V^T: keys (lane & 7) + 8 (lane >> 4), 16-byte chunk + ((lane >> 3) & 1)
       const int key = (lane & 7) + ((lane >> 4) << 3), cc = (lane >> 3) & 1, x7 = key & 7;
 #pragma unroll
-      for (int i = 0; i < AT_KEYS / 16; ++i)
+      for (int d = 0; d < D / 16; ++d) {
+        uint32_t f[4];
+        ldsm4t(f, va + static_cast<uint32_t>((d / 4) * Tile::SLICE + key * 128 + ((((2 * d) & 7) + cc) ^ x7) * 16));
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
-          uint32_t f[4];
-          ldsm4t(f, va + static_cast<uint32_t>((d / 4) * Tile::SLICE + (16 * i + key) * 128 + ((((2 * d) & 7) + cc) ^ x7) * 16));
+        for (int q = 0; q < NQ; ++q) mma16816<BF16>(o[d][q], f, ph[q][0], ph[q][1]);
 #pragma unroll
-          for (int q = 0; q < NQ; ++q) {
-            mma16816<BF16>(o[d][q], f, ph[i][q][0], ph[i][q][1]);
-            mma16816<BF16>(o[d][q], f, pl[i][q][0], pl[i][q][1]);
-          }
-        }
+        for (int q = 0; q < NQ; ++q) mma16816<BF16>(o[d][q], f, pl[q][0], pl[q][1]);
+      }
     }
-    __syncwarp();  // every lane has read the stage before it is refilled
+    __syncwarp();  // every lane has read the stage
+    if (lane == 0) mbar_arrive(&empty[st]);
 
-    const AttnPos was = p;
+    const int wr = p.r, wh = p.h, wt = p.tile, wu = p.u;
+    const AttnRow wx = p.x;
     const bool last = done + 1 == total;
     if (attn_next(a, p, row_at) || last) {  // the warp's part of this item is complete
       fresh = true;
-      const int64_t id = attn_first_id<R>(a, was.r, was.x) + static_cast<int64_t>(was.h) * was.x.tiles + was.tile;
+      const int64_t id = attn_first_id<R>(a, wr, wx) + static_cast<int64_t>(wh) * wx.tiles + wt;
       const int64_t slot = gw + id;
-      const int M = was.x.n * a.G - was.tile * R;
+      const int M = wx.n * a.G - wt * R;
       if (slot < a.slots && id < a.ids) {
         if (first_u == 0 && lane == 0) {
           int parts = 1;
-          if (was.u + 1 < was.x.units)  // it goes on in other warps' ranges
-            parts = static_cast<int>(div_nonneg(u0 + done + (was.x.units - 1 - was.u), quota) - gw) + 1;
+          if (wu + 1 < wx.units)  // it goes on in other warps' ranges
+            parts = static_cast<int>(cuts.warp_of(u0 + done + (wx.units - 1 - wu)) - gw) + 1;
           a.items[id] = make_int2(static_cast<int>(slot), parts);
         }
         float* po = a.part_o + slot * (R * D);
@@ -497,75 +550,99 @@ __global__ void __launch_bounds__(AT_WARPS * 32)
       }
     }
   }
-  if (!ok) {  // a copy did not arrive: wait (bounded) for those in flight, and say so
-    for (int i = done; i < fetched; ++i) (void)mbar_wait_bounded(&bars[i % AT_STAGES], (i / AT_STAGES) & 1);
-    if (lane == 0 && a.error_word) atomicOr(a.error_word, Q3S_DECERR_WAIT);
-  }
-  if (bad_block && a.error_word) atomicOr(a.error_word, Q3S_DECERR_BLOCK_ID);  // lane 0's
-  // this grid may have started beside the prefix kernel's: it does not end
-  // before that one, so that the join, which waits for this grid, has both
+  if (!ok && lane == 0 && a.error_word) atomicOr(a.error_word, Q3S_DECERR_WAIT);  // a copy did not arrive
+  // this grid starts beside the prefix kernel's: it does not end before that
+  // one, so that the join, which waits for this grid, has both
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // Joins the parts of each query row (m, l, o as above) and writes out and lse.
-// One warp a row; a lane holds D / 32 of its values and, for up to 32 parts at
-// a time, one part's m and l.
-// Block (b, h, z): rows 4 z + warp, ... of batch row b's n * G; b == B: the
-// tokens past the last row, which see nothing.  Bound by latency: one load of
-// the item's record, one of its parts.
+// One warp a row of [T * q_heads]; a lane holds D / 32 of its values and, for up
+// to 32 parts at a time, one part's m and l.  A token's batch row is found in
+// query_offsets by bisection, before the grid waits for the parts; tokens past
+// the last row see nothing.  Bound by latency: the record of the row's own
+// parts, then their sums; the prefix parts' sums are requested before the record
+// has arrived.
 template <int D, bool BF16, int NQ>
-__global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
-  constexpr int E = D / 32, R = 8 * NQ;
-  const int w = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
-  const int b = static_cast<int>(blockIdx.x), h = static_cast<int>(blockIdx.y);
+__global__ void __launch_bounds__(128, 5) attn_join_kernel(const AttnArgs a) {
+  constexpr int E = D / 32, R = 8 * NQ, AHEAD = 8;
+  const int lane = static_cast<int>(threadIdx.x) & 31;
+  const int64_t out_row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int token = static_cast<int>(out_row / a.Hq), head = static_cast<int>(out_row - static_cast<int64_t>(token) * a.Hq);
+  const int h = head / a.G, gq = head - h * a.G;
   AttnRow x;
-  if (b < a.B) {
+  x.units = 0;
+  bool live = false;
+  int b = 0;
+  if (token < a.T && a.B > 0) {
+    int r = a.B;  // offsets[b] <= token < offsets[r], once it is known that there is such a row
+    while (r - b > 1) {
+      const int m = (b + r) >> 1;
+      if (a.offsets[m] <= token) b = m; else r = m;
+    }
     x = attn_row<R>(a, b + 1);
-  } else {
-    x.t0 = a.B ? min(max(a.offsets[a.B], 0), a.T) : 0;
-    x.n = a.T - x.t0;
-    x.units = x.tiles = 0;
+    live = token >= x.t0 && token < x.t0 + x.n;
+    if (!live) x.units = 0;
   }
-  const int M = x.n * a.G;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int row = static_cast<int>(blockIdx.z) * 4 + w; row < M; row += static_cast<int>(gridDim.z) * 4) {
-    const int token = x.t0 + row / a.G, gq = row % a.G;
+  if (token >= a.T) return;
+  {
+    const int row = live ? (token - x.t0) * a.G + gq : 0;  // of the batch row's n * G
     // two runs of parts, the prefix's and the row's own: part i of a run is
     // query row `at + i * step` of `o` and `ml`
     const float* o0 = a.part_o;
     const float2* ml0 = a.part_ml;
     int64_t at0 = 0, step0 = R, at1 = 0;
     int n0 = 0, n1 = 0;
-    if (b < a.B && a.tiles0) {
+    int2 own = make_int2(0, 0);
+    if (x.units) {
+      const int64_t id = attn_first_id<R>(a, b + 1, x) + static_cast<int64_t>(h) * x.tiles + row / R;
+      if (id < a.ids) own = a.items[id];
+    }
+    if (live && a.tiles0) {
       const int r = token * a.G + gq;
       const int2 it = a.items[static_cast<int64_t>(h) * a.tiles0 + r / R];
       at0 = static_cast<int64_t>(it.x) * R + r % R;
       n0 = it.x >= 0 && it.y > 0 && static_cast<int64_t>(it.x) + it.y <= a.slots ? it.y : 0;
-    } else if (b < a.B && a.splits) {
+    } else if (live && a.splits) {
       o0 = a.pre_o;
       ml0 = a.pre_ml;
-      at0 = static_cast<int64_t>(token) * a.Hq + h * a.G + gq;
+      at0 = out_row;
       step0 = static_cast<int64_t>(a.T) * a.Hq;
       n0 = a.splits;
     }
-    if (x.units) {
-      const int64_t id = attn_first_id<R>(a, b + 1, x) + static_cast<int64_t>(h) * x.tiles + row / R;
-      if (id < a.ids) {
-        const int2 it = a.items[id];
-        at1 = static_cast<int64_t>(it.x) * R + row % R;
-        n1 = it.x >= 0 && it.y > 0 && static_cast<int64_t>(it.x) + it.y <= a.slots ? it.y : 0;
+    float y[AHEAD][E], z[2][E];  // sums of the first parts of each run
+    auto fetch = [&](const float* src, float (&v)[E]) {
+      if constexpr (E == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(src);
+        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+      } else {
+        const float2 f = *reinterpret_cast<const float2*>(src);
+        v[0] = f.x, v[1] = f.y;
       }
-    }
+    };
+    const float* src0 = o0 + at0 * D + lane * E;
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (j < n0) fetch(src0 + j * step0 * D, y[j]);
+    n1 = own.x >= 0 && own.y > 0 && static_cast<int64_t>(own.x) + own.y <= a.slots ? own.y : 0;
+    at1 = static_cast<int64_t>(own.x) * R + row % R;
+    const float* src1 = a.part_o + at1 * D + lane * E;
     const int parts = n0 + n1;
     float acc[E], m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
     for (int i0 = 0; i0 < parts; i0 += 32) {
-      const int k = min(parts - i0, 32);
+      const int k = min(parts - i0, 32), k0 = min(max(n0 - i0, 0), k);  // parts of this round, and of the prefix's run
       float2 ml = make_float2(-INFINITY, 0.0f);
       if (lane < k) {
         const int i = i0 + lane;
         ml = i < n0 ? ml0[at0 + i * step0] : a.part_ml[at1 + (i - n0) * static_cast<int64_t>(R)];
+      }
+      if (i0 == 0) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (j < n1 && n0 + j < k) fetch(src1 + j * (R * D), z[j]);
       }
       float top = ml.x;
 #pragma unroll
@@ -580,35 +657,41 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
       l = l * c + lw;
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] *= c;
-      auto add = [&](const float* src, int64_t stride, int i1, int i2) {  // parts i1 .. i2 - 1 of the 32
+      auto add = [&](const float (&v)[E], int i) {
+        const float wi = __shfl_sync(FULL, wt, i);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += wi * v[e];
+      };
+      auto run = [&](const float* src, int64_t stride, int i1, int i2) {  // parts i1 .. i2 - 1 of the round
+        float v[E];
 #pragma unroll 4
         for (int i = i1; i < i2; ++i, src += stride) {
-          const float wi = __shfl_sync(FULL, wt, i);
-          if constexpr (E == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(src);
-            acc[0] += wi * v.x;
-            acc[1] += wi * v.y;
-            acc[2] += wi * v.z;
-            acc[3] += wi * v.w;
-          } else {
-            const float2 v = *reinterpret_cast<const float2*>(src);
-            acc[0] += wi * v.x;
-            acc[1] += wi * v.y;
-          }
+          fetch(src, v);
+          add(v, i);
         }
       };
-      const int k0 = min(max(n0 - i0, 0), k);  // of the prefix's run
-      add(o0 + (at0 + i0 * step0) * D + lane * E, step0 * D, 0, k0);
-      add(a.part_o + (at1 + static_cast<int64_t>(i0 + k0 - n0) * R) * D + lane * E, R * D, k0, k);
+      if (i0 == 0) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+          if (j < k0) add(y[j], j);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (k0 + j < k) add(z[j], k0 + j);
+        run(src0 + AHEAD * step0 * D, step0 * D, AHEAD, k0);
+        run(src1 + 2 * (R * D), R * D, k0 + 2, k);
+      } else {
+        run(src0 + i0 * step0 * D, step0 * D, 0, k0);
+        run(src1 + static_cast<int64_t>(i0 + k0 - n0) * (R * D), R * D, k0, k);
+      }
     }
     const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;  // a NaN stays one
-    uint16_t* dst = static_cast<uint16_t*>(a.out) + token * a.ot + (static_cast<int64_t>(h) * a.G + gq) * a.oh + lane * E;
+    uint16_t* dst = static_cast<uint16_t*>(a.out) + token * a.ot + head * a.oh + lane * E;
     if constexpr (E == 4)
       *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv));
     else
       *reinterpret_cast<uint32_t*>(dst) = pack2<BF16>(acc[0] * inv, acc[1] * inv);
     if (a.lse && lane == 0)
-      a.lse[static_cast<int64_t>(token) * a.Hq + h * a.G + gq] =
+      a.lse[out_row] =
           l > 0.0f ? (m + log2f(l)) * 0.69314718055994531f : l == l ? -INFINITY : l;
   }
 }

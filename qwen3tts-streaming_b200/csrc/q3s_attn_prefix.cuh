@@ -26,7 +26,6 @@ struct PrefixTile {
 struct PrefixArgs {
   AttnArgs a;
   int per_tile;   // tokens of a tile: 128 / G
-  int pairs;      // pairs of tiles that cover the T tokens
   int steps;      // ceil(L / 128)
   int per_split;  // steps of a part
 };
@@ -67,10 +66,6 @@ Q3S_DEV bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n}" : "=r"(p));
   return p != 0;
 }
-Q3S_DEV void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
 // 128 consecutive 32-bit columns of this thread's TMEM lane.
 Q3S_DEV void tmem_ld128(uint32_t addr, uint32_t (&r)[128]) {
   asm volatile(
@@ -155,6 +150,13 @@ Q3S_DEV void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
       : "memory");
 }
 
+// Largest of three.
+Q3S_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // One CTA: 2 * 128 query rows of one key/value head over one part of the
 // prefix.  Rows of a tile are (token, head of the group) pairs, so a group's
 // heads share the keys that are read.
@@ -163,8 +165,9 @@ Q3S_DEV void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
 //   S0 = Q0 K^T, S1 = Q1 K^T, then per step  O0 += P0 V, S0 = Q0 K'^T, O1 += P1 V, S1 = Q1 K'^T,
 // so that one tile's softmax runs while the other tile's products do.  A
 // softmax thread owns a row: it reads the 128 scores from TMEM, writes p over
-// them as 16-bit values (the second product's A operand, straight from TMEM)
-// and keeps m and l in registers.  TMEM: S0 S1 O0 O1, 128 columns each.
+// them as 16-bit values (the second product's A operand, straight from TMEM) in
+// two halves, so that the product starts on the first while the second is
+// computed, and keeps m and l in registers.  TMEM: S0 S1 O0 O1, 128 columns each.
 //
 // The running maximum is allowed to lag by 8 (p up to 256, sums in fp32), so
 // O is rescaled only when a score rises above that: the first step sets it,
@@ -195,8 +198,9 @@ __global__ void __launch_bounds__(PX_NT, 1)
   uint64_t* v_full = k_empty + PX_STAGES;
   uint64_t* v_empty = v_full + PX_STAGES;
   uint64_t* s_full = v_empty + PX_STAGES;  // [2] scores of a tile are in TMEM
-  uint64_t* p_full = s_full + 2;           // [2] its probabilities are
-  uint64_t* o_done = p_full + 2;           // [2] its second product is
+  uint64_t* p_half = s_full + 2;           // [2] the probabilities of its first 64 keys are
+  uint64_t* p_full = p_half + 2;           // [2] all are
+  uint64_t* o_done = p_full + 2;           // [2] its second product is complete
   uint64_t* v_clean = o_done + 2;          // V of a part's ragged last step has been cleared past its end
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_clean + 1);
   int* failed = reinterpret_cast<int*>(tmem_slot + 1);
@@ -219,6 +223,7 @@ __global__ void __launch_bounds__(PX_NT, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
+      mbar_init(&p_half[i], 128);
       mbar_init(&p_full[i], 128);
       mbar_init(&o_done[i], 1);
     }
@@ -237,6 +242,7 @@ __global__ void __launch_bounds__(PX_NT, 1)
 
   // a wait that gives up marks the CTA; every role then stops at its next wait
   auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
     if (*reinterpret_cast<volatile int*>(failed)) return false;
     if (mbar_wait_bounded(bar, parity)) return true;
     atomicOr(failed, 1);
@@ -253,20 +259,17 @@ __global__ void __launch_bounds__(PX_NT, 1)
         for (int x = 0; x < HALVES; ++x)
           tma_load_3d(smem_u32(s_q + i * Tile::Q_BYTES + x * PX_M * 128), &tm_q, 64 * x, h * a.G, token0 + i * p.per_tile, q_full);
     }
-    int j = 0, bad = 0;
+    auto block_of = [&](int j) {  // lane's block of step j; past the cache (it reads as zeros) where there is none
+      const int key = (step0 + j) * PX_KEYS + lane * rows;
+      return lane < pages && key < a.L ? a.prefix_blocks[key >> a.bs_log2] : a.blocks;
+    };
+    int next = block_of(0), j = 0, bad = 0;
     for (; j < steps; ++j) {
       const int s = j % PX_STAGES;
-      int id = a.blocks;  // past the cache: it reads as zeros
-      const int key = (step0 + j) * PX_KEYS + lane * rows, place = key % a.bs;
-      if (lane < pages) {
-        if (key < a.L) {
-          id = a.prefix_blocks[key / a.bs];
-          if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.blocks)) {
-            id = a.blocks;
-            bad = 1;
-          }
-        }
-      }
+      const bool inside = static_cast<unsigned>(next) < static_cast<unsigned>(a.blocks);
+      bad |= !inside && next != a.blocks;
+      const int id = inside ? next : a.blocks, place = ((step0 + j) * PX_KEYS + lane * rows) & (a.bs - 1);
+      if (j + 1 < steps) next = block_of(j + 1);
       auto copy = [&](const CUtensorMap* map, unsigned char* ring, uint64_t* full, uint64_t* empty) {
         if (j >= PX_STAGES && !__all_sync(FULL, wait(&empty[s], ((j / PX_STAGES) - 1) & 1))) return false;
         if (lane == 0) mbar_expect_tx(&full[s], Tile::KV_BYTES);
@@ -329,14 +332,20 @@ __global__ void __launch_bounds__(PX_NT, 1)
         ok = wait(&v_full[s], (j / PX_STAGES) & 1);
         if (ok && j + 1 == steps && a.L < (step0 + steps) * PX_KEYS) ok = wait(v_clean, 0);
         for (int i = 0; ok && i < tiles; ++i) {
-          ok = wait(&p_full[i], j & 1);
-          if (!ok) break;
-          tc_fence_after();
           const uint64_t dv = v_desc + static_cast<uint64_t>(s * (Tile::KV_BYTES >> 4));
 #pragma unroll
-          for (int c = 0; c < PX_KEYS / 16; ++c)  // O_i += P_i V
-            umma_f16_ta(tmem + static_cast<uint32_t>(256 + 128 * i), tmem + static_cast<uint32_t>(128 * i + 8 * c),
-                        dv + c * ((16 * 128) >> 4), ID_O, (j | c) != 0);
+          for (int half = 0; half < 2; ++half) {  // O_i += P_i V
+            ok = ok && wait(half ? &p_full[i] : &p_half[i], j & 1);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < PX_KEYS / 32; ++c) {
+              const int k = half * (PX_KEYS / 32) + c;
+              umma_f16_ta(tmem + static_cast<uint32_t>(256 + 128 * i), tmem + static_cast<uint32_t>(128 * i + 8 * k),
+                          dv + k * ((16 * 128) >> 4), ID_O, (j | k) != 0);
+            }
+          }
+          if (!ok) break;
           if (i == tiles - 1) umma_commit(&v_empty[s]);
           umma_commit(&o_done[i]);
           if (j + 1 < steps) {
@@ -372,15 +381,16 @@ __global__ void __launch_bounds__(PX_NT, 1)
           for (int c = 0; c < 128; ++c)
             if (c >= valid) r[c] = 0xff800000u;
         }
-        float x0 = __uint_as_float(r[0]), x1 = __uint_as_float(r[1]), x2 = __uint_as_float(r[2]), x3 = __uint_as_float(r[3]);
+        auto f = [&](int c) { return __uint_as_float(r[c]); };
+        float x[4] = {f(0), f(1), f(2), f(3)};
 #pragma unroll
-        for (int c = 4; c < 128; c += 4) {
-          x0 = fmaxf(x0, __uint_as_float(r[c]));
-          x1 = fmaxf(x1, __uint_as_float(r[c + 1]));
-          x2 = fmaxf(x2, __uint_as_float(r[c + 2]));
-          x3 = fmaxf(x3, __uint_as_float(r[c + 3]));
+        for (int c = 4; c + 8 <= 128; c += 8) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = max3(x[e], f(c + 2 * e), f(c + 2 * e + 1));
         }
-        const float top = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * a.scale_log2;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = fmaxf(x[e], f(124 + e));
+        const float top = max3(fmaxf(x[0], x[1]), x[2], x[3]) * a.scale_log2;
         const bool rise = top > m + PX_SLACK || (j == 0 && top > m);
         if (__any_sync(FULL, rise)) {
           const float nm = rise ? top : m;
@@ -405,19 +415,22 @@ __global__ void __launch_bounds__(PX_NT, 1)
         const float base = m == -INFINITY ? 0.0f : m;
         const float2 sc = make_float2(a.scale_log2, a.scale_log2), nb = make_float2(-base, -base);
         float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
-        uint32_t pk[64];
 #pragma unroll
-        for (int c = 0; c < 64; ++c) {
-          float2 e = __ffma2_rn(make_float2(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1])), sc, nb);
-          e.x = ex2(e.x);
-          e.y = ex2(e.y);
-          if (c & 1) sum1 = __fadd2_rn(sum1, e); else sum0 = __fadd2_rn(sum0, e);
-          pk[c] = pack2<BF16>(e.x, e.y);
+        for (int half = 0; half < 2; ++half) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            float2 e = __ffma2_rn(make_float2(f(64 * half + 2 * c), f(64 * half + 2 * c + 1)), sc, nb);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            if (c & 1) sum1 = __fadd2_rn(sum1, e); else sum0 = __fadd2_rn(sum0, e);
+            pk[c] = pack2<BF16>(e.x, e.y);
+          }
+          tmem_st32(ts + static_cast<uint32_t>(32 * half), pk);
+          tc_fence_before();
+          mbar_arrive(half ? &p_full[i] : &p_half[i]);
         }
-        tmem_st64(ts, pk);
         l += (sum0.x + sum1.x) + (sum0.y + sum1.y);
-        tc_fence_before();
-        mbar_arrive(&p_full[i]);
       }
       if (ok) ok = __all_sync(FULL, wait(&o_done[i], (steps - 1) & 1));
       if (ok) {
