@@ -196,6 +196,11 @@ typedef struct q3s_int8_matmul_desc {
 
 q3s_status q3s_int8_matmul(const q3s_int8_matmul_desc* desc, void* stream);
 
+/* A Linear: quantise x, then the product of its values and scales (the
+ * product's a and a_scales are the quantisation's outputs, and y has x's
+ * type).  One launch for a few rows, two otherwise. */
+q3s_status q3s_int8_linear(const q3s_quantize_rows_desc* quantize, const q3s_int8_matmul_desc* product, void* stream);
+
 /* sizeof() of the descriptors above as compiled (which: 0 = cache_tables,
  * 1 = cache_append, 2 = prefix_attention, 3 = quantize_rows, 4 = int8_matmul). */
 uint32_t q3s_decode_desc_size(int32_t which);

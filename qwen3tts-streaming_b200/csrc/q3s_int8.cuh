@@ -187,207 +187,578 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const QuantArgs a) {
 
 struct Int8Args {
   int M, N, K;
-  int mtiles, ntiles, kchunks;
+  const int8_t* a;
+  int64_t lda;
   const float* a_scales;
+  const int8_t* w;
+  int64_t ldw;
   const float* w_scales;
   const float* bias;
   void* y;
   int64_t ldy;
-  bool vec_y;  // 16-byte stores of y are aligned
+  bool vec_y;  // 16-byte accesses of y's rows are aligned
   int32_t* error_word;
 };
 
+// An output from its exact sum.
+Q3S_DEV float int8_out(int sum, float a_scale, float w_scale) {
+  return __fmul_rn(__fmul_rn(static_cast<float>(sum), a_scale), w_scale);
+}
+
+// -- few rows: one pass over the weights with 8-bit dot products -----------------
+
+constexpr int GV_NT = 256, GV_WARPS = GV_NT / 32;
+constexpr int GV_MAX_M = 8;
+constexpr int GV_SMEM = 96 * 1024;  // most bytes of activations
+
+// M <= MB <= 8 rows: the product is bound by reading the weights once, and at
+// these sizes by latency.  A warp owns RW outputs and reads their weight rows
+// 512 bytes at a time, the first rounds of all of them before anything else; the
+// activations sit in shared memory as bytes; sums are reduced over the warp by
+// one integer instruction each.  QUANT: the rows of x are quantised here, by
+// every CTA for itself (they are few), with the weights already on their way,
+// so a Linear is one launch; CTA 0 writes the values and scales out.
+template <bool QUANT, int ELEM, int MB, int RW>
+__global__ void __launch_bounds__(GV_NT) int8_gemv_kernel(const Int8Args a, const QuantArgs q) {
+  using E = Elem<ELEM>;
+  constexpr int AHEAD = 4;  // rounds of 512 bytes of each row requested at the start
+  extern __shared__ __align__(16) unsigned char gv_smem[];  // [MB][K] activations
+  __shared__ float s_max[GV_WARPS], s_scale[MB];
+  const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
+  const int n0 = (static_cast<int>(blockIdx.x) * GV_WARPS + w) * RW;
+  const int rounds = (a.K + 511) / 512;
+  uint4 first[RW][AHEAD];
+#pragma unroll
+  for (int r = 0; r < RW; ++r)
+#pragma unroll
+    for (int c = 0; c < AHEAD; ++c) {
+      const int k = 512 * c + 16 * lane;
+      first[r][c] = n0 + r < a.N && k < a.K ? ld_stream16(a.w + (n0 + r) * a.ldw + k) : make_uint4(0, 0, 0, 0);
+    }
+  if constexpr (QUANT) {
+    constexpr int GROUP = GV_NT / MB, KEEP = 4;  // threads of a row; 16-byte loads that stay in registers
+    const int m = t / GROUP, i = t % GROUP, chunks = a.K / E::N;
+    const typename E::T* x = static_cast<const typename E::T*>(q.x) + m * q.ldx;
+    uint4 keep[KEEP];
+    float v[E::N], top = 0.0f;
+#pragma unroll
+    for (int c = 0; c < KEEP; ++c)
+      keep[c] = m < a.M && i + GROUP * c < chunks
+                    ? *reinterpret_cast<const uint4*>(x + static_cast<int64_t>(i + GROUP * c) * E::N)
+                    : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int c = 0; c < KEEP; ++c) {
+      E::widen(keep[c], v);
+#pragma unroll
+      for (int j = 0; j < E::N; ++j) top = absmax(top, v[j]);
+    }
+    if (m < a.M)
+      for (int c = i + GROUP * KEEP; c < chunks; c += GROUP) {
+        E::widen(*reinterpret_cast<const uint4*>(x + static_cast<int64_t>(c) * E::N), v);
+#pragma unroll
+        for (int j = 0; j < E::N; ++j) top = absmax(top, v[j]);
+      }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = absmax(top, __shfl_xor_sync(FULL, top, d));
+    if (lane == 0) s_max[w] = top;
+    __syncthreads();
+    constexpr int WR = GROUP / 32;  // warps of a row
+    top = s_max[(w / WR) * WR];
+#pragma unroll
+    for (int j = 1; j < WR; ++j) top = absmax(top, s_max[(w / WR) * WR + j]);
+    const QuantScale s = quant_scale(top);
+    const bool out = blockIdx.x == 0 && m < a.M;
+    if (i == 0) {
+      s_scale[m] = s.scale;
+      if (out) q.scales[m] = s.scale;
+    }
+    auto store = [&](int c, const uint4& u) {
+      E::widen(u, v);
+      uint32_t p[E::N / 4];
+#pragma unroll
+      for (int j = 0; j < E::N / 4; ++j) {
+        p[j] = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) p[j] |= (static_cast<uint32_t>(quant_one(v[4 * j + b], s.unit)) & 0xffu) << (8 * b);
+      }
+      uint32_t* dst = reinterpret_cast<uint32_t*>(gv_smem + static_cast<size_t>(m) * a.K + static_cast<size_t>(c) * E::N);
+      uint32_t* copy = reinterpret_cast<uint32_t*>(q.values + m * q.ldv + static_cast<int64_t>(c) * E::N);
+#pragma unroll
+      for (int j = 0; j < E::N / 4; ++j) {
+        dst[j] = p[j];
+        if (out) copy[j] = p[j];
+      }
+    };
+#pragma unroll
+    for (int c = 0; c < KEEP; ++c)
+      if (i + GROUP * c < chunks) store(i + GROUP * c, keep[c]);
+    for (int c = i + GROUP * KEEP; c < chunks; c += GROUP)
+      store(c, m < a.M ? *reinterpret_cast<const uint4*>(x + static_cast<int64_t>(c) * E::N) : make_uint4(0, 0, 0, 0));
+  } else {
+    for (int c = t; c < MB * (a.K / 16); c += GV_NT) {
+      const int m = c / (a.K / 16), k = 16 * (c - m * (a.K / 16));
+      reinterpret_cast<uint4*>(gv_smem)[c] = m < a.M ? *reinterpret_cast<const uint4*>(a.a + m * a.lda + k) : make_uint4(0, 0, 0, 0);
+    }
+    if (t < MB) s_scale[t] = t < a.M ? a.a_scales[t] : 0.0f;
+  }
+  __syncthreads();
+
+  int acc[RW][MB];
+#pragma unroll
+  for (int r = 0; r < RW; ++r)
+#pragma unroll
+    for (int m = 0; m < MB; ++m) acc[r][m] = 0;
+  auto round = [&](int k, const uint4 (&wv)[RW]) {  // 16 bytes of K a lane
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+      const uint4 x = *reinterpret_cast<const uint4*>(gv_smem + static_cast<size_t>(m) * a.K + k);
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        acc[r][m] = __dp4a(static_cast<int>(wv[r].x), static_cast<int>(x.x), acc[r][m]);
+        acc[r][m] = __dp4a(static_cast<int>(wv[r].y), static_cast<int>(x.y), acc[r][m]);
+        acc[r][m] = __dp4a(static_cast<int>(wv[r].z), static_cast<int>(x.z), acc[r][m]);
+        acc[r][m] = __dp4a(static_cast<int>(wv[r].w), static_cast<int>(x.w), acc[r][m]);
+      }
+    }
+  };
+#pragma unroll
+  for (int c = 0; c < AHEAD; ++c) {
+    uint4 wv[RW];
+#pragma unroll
+    for (int r = 0; r < RW; ++r) wv[r] = first[r][c];
+    if (512 * c + 16 * lane < a.K) round(512 * c + 16 * lane, wv);
+  }
+#pragma unroll 2
+  for (int c = AHEAD; c < rounds; ++c) {
+    const int k = 512 * c + 16 * lane;
+    if (k >= a.K) break;
+    uint4 wv[RW];
+#pragma unroll
+    for (int r = 0; r < RW; ++r) wv[r] = n0 + r < a.N ? ld_stream16(a.w + (n0 + r) * a.ldw + k) : make_uint4(0, 0, 0, 0);
+    round(k, wv);
+  }
+  __syncwarp();
+  int mine = 0;  // lane r * MB + m: that sum
+#pragma unroll
+  for (int r = 0; r < RW; ++r)
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+      const int sum = __reduce_add_sync(FULL, acc[r][m]);
+      if (lane == r * MB + m) mine = sum;
+    }
+  const int m = lane % MB, n = n0 + lane / MB;
+  if (lane < RW * MB && m < a.M && n < a.N) {
+    float v = int8_out(mine, s_scale[m], a.w_scales[n]);
+    if (a.bias) v += a.bias[n];
+    static_cast<typename E::T*>(a.y)[m * a.ldy + n] = E::narrow(v);
+  }
+}
+
+// -- tensor cores -----------------------------------------------------------------
+
+constexpr int I8_BK = 128;   // bytes of a row in one 128-byte swizzled chunk
+constexpr int I8_TILE = 128 * I8_BK;  // 128 rows of a chunk
+
+// kind::i8: 32-bit integer accumulator (2), A and B signed (1), both K-major,
+// N >> 3 in [17, 23), M >> 4 in [24, 29).
+__host__ __device__ constexpr uint32_t i8_idesc(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
 Q3S_DEV void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(tmem_d),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
 }
+Q3S_DEV void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+// Arrive on `bar` of both CTAs of the pair once the products issued before are complete.
+Q3S_DEV void umma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+// A copy into this CTA's shared memory that completes on the barrier at
+// shared::cluster address `bar` (the pair's leading CTA).
+Q3S_DEV void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
+          "r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+Q3S_DEV void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+Q3S_DEV void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(src)
+               : "memory");
+}
+Q3S_DEV void cluster_arrive_release() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+Q3S_DEV int4 ld_cluster16(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 
-constexpr int I8_BM = 128;   // rows of a tile: the matrix instruction's M
-constexpr int I8_BK = 128;   // bytes of a row in one 128-byte swizzled chunk
-constexpr int I8_NT = 192;   // 4 epilogue warps, the copy warp, the matrix warp
-constexpr int I8_A_BYTES = I8_BM * I8_BK;
-
-template <int BN>
-struct I8Tile {
-  static constexpr int STAGE = I8_A_BYTES + BN * I8_BK;
-  static constexpr int STAGES = (200 * 1024) / STAGE < 8 ? (200 * 1024) / STAGE : 8;
-  static constexpr int SMEM = 1024 + STAGES * STAGE + 256;
-  static constexpr int TMEM = 2 * BN < 32 ? 32 : 2 * BN;  // two accumulators
-  // kind::i8: 32-bit integer accumulator (2), A and B signed (1), both
-  // K-major, N >> 3 in [17, 23), M >> 4 in [24, 29)
-  static constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(BN >> 3) << 17) |
-                                    (static_cast<uint32_t>(I8_BM >> 4) << 24);
+// Up to a few hundred rows: the weights are the matrix instruction's M (128
+// outputs a CTA), the rows of x its N (BT, a multiple of 16), so that one pass
+// over the weights serves all rows of a tile; K is cut over the KS CTAs of a
+// cluster so that all SMs read.  The partial sums (32-bit integers, exact in any
+// order) meet in distributed shared memory: CTA r of a cluster finishes every
+// KS-th group of tokens.  Bound by the latency of that chain (load, products,
+// exchange) and the weights' bytes.
+struct I8Cut {
+  int bt, ks, stages, chunks;  // tokens of a tile, CTAs of a cluster, ring stages, chunks of K
+  int tmem;                    // columns: a power of two >= 32
 };
+constexpr int I8C_NT = 128;
 
-// Persistent tiles of 128 x BN: one warp copies (TMA, 128-byte swizzle), one
-// issues the matrix instructions (one elected thread), four scale and store
-// the previous tile out of the other half of TMEM meanwhile.  The sums are
-// exact 32-bit integers (K <= 131072 keeps them below 2^31), so their order
-// does not matter; each output is rounded once. 
-template <int BN, int ELEM>
-__global__ void __launch_bounds__(I8_NT, 1)
-    int8_matmul_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
-                       const Int8Args a) {
-  using Tile = I8Tile<BN>;
+template <int ELEM>
+__global__ void __launch_bounds__(I8C_NT)
+    int8_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const Int8Args a,
+                      const I8Cut cut) {
   using E = Elem<ELEM>;
-  constexpr int STAGES = Tile::STAGES;
   extern __shared__ __align__(1024) unsigned char i8_smem[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(i8_smem) + 1023) &
                                                          ~static_cast<uintptr_t>(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Tile::STAGE);
-  uint64_t* empty = full + STAGES;
-  uint64_t* ready = empty + STAGES;  // [2] an accumulator is complete
-  uint64_t* drained = ready + 2;     // [2] an accumulator has been read
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
-  int* failed = reinterpret_cast<int*>(tmem_slot + 1);
+  __shared__ __align__(8) uint64_t full[8], empty[8], ready;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
   const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
-  const int tiles = a.mtiles * a.ntiles;
-
+  const int n0 = static_cast<int>(blockIdx.x) * 128, rank = static_cast<int>(cluster_rank());
+  const int token0 = static_cast<int>(blockIdx.z) * cut.bt;
+  const int stage_bytes = I8_TILE + cut.bt * I8_BK;
+  const int c0 = cut.chunks * rank / cut.ks, count = cut.chunks * (rank + 1) / cut.ks - c0;  // this CTA's chunks, >= 1
   if (t == 0) {
-    for (int s = 0; s < STAGES; ++s) {
+    for (int s = 0; s < cut.stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&ready[b], 1);
-      mbar_init(&drained[b], 128);
-    }
-    *failed = 0;
+    mbar_init(&ready, 1);
+    failed = 0;
     fence_mbar_init();
   }
-  if (w == 5) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(Tile::TMEM)
+  if (w == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(cut.tmem)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = tmem_slot;
+  if (t == 0) {
+    auto load_w = [&](int c) { tma_load_2d(smem_u32(smem + (c % cut.stages) * stage_bytes), &tm_w, (c0 + c) * I8_BK, n0, &full[c % cut.stages]); };
+    // the weights do not depend on the kernel before: they are on their way while it ends
+    const int ahead = min(count, cut.stages);
+    for (int c = 0; c < ahead; ++c) {
+      mbar_expect_tx(&full[c], stage_bytes);
+      load_w(c);
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int c = 0; c < count; ++c) {
+      const int s = c % cut.stages;
+      if (c >= ahead) {
+        if (!mbar_wait_bounded(&empty[s], ((c / cut.stages) - 1) & 1)) {
+          atomicOr(&failed, 1);
+          break;
+        }
+        mbar_expect_tx(&full[s], stage_bytes);
+        load_w(c);
+      }
+      tma_load_2d(smem_u32(smem + s * stage_bytes + I8_TILE), &tm_a, (c0 + c) * I8_BK, token0, &full[s]);
+    }
+  } else if (t == 32) {
+    const uint32_t idesc = i8_idesc(128, cut.bt);
+    for (int c = 0; c < count; ++c) {
+      const int s = c % cut.stages;
+      if (!mbar_wait_bounded(&full[s], (c / cut.stages) & 1)) {
+        atomicOr(&failed, 1);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t sa = smem_u32(smem + s * stage_bytes);
+      const uint64_t dw = head_smem_desc(sa), da = head_smem_desc(sa + I8_TILE);
+#pragma unroll
+      for (int j = 0; j < I8_BK / 32; ++j)  // 32 bytes of K = 2 descriptor units per instruction
+        umma_i8(tmem, dw + 2 * j, da + 2 * j, idesc, (c | j) != 0);
+      umma_commit(&empty[s]);
+    }
+    umma_commit(&ready);
+  }
+  __syncwarp();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const bool done = mbar_wait_bounded(&ready, 0);
+  if (!done) atomicOr(&failed, 1);
+  tc_fence_after();
+  // every product is complete: the ring holds the partial sums now, [token][128 outputs]
+  int* part = reinterpret_cast<int*>(smem);
+  for (int c = 0; c < cut.bt; c += 16) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(tmem + (static_cast<uint32_t>(32 * w) << 16) + static_cast<uint32_t>(c))
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) part[(c + i) * 128 + t] = static_cast<int>(r[i]);
+  }
+  tc_fence_before();
+  cluster_arrive_release();
+  cluster_wait();  // every CTA's partial sums are in place
+  {
+    const int n = n0 + 4 * lane;
+    float ws[4], bi[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      ws[j] = n + j < a.N ? a.w_scales[n + j] : 0.0f;
+      bi[j] = a.bias && n + j < a.N ? a.bias[n + j] : 0.0f;
+    }
+    for (int tok = rank * 4 + w; tok < cut.bt; tok += cut.ks * 4) {
+      if (token0 + tok >= a.M) break;
+      const uint32_t at = smem_u32(part + tok * 128 + 4 * lane);
+      int4 sum = make_int4(0, 0, 0, 0);
+      for (int k = 0; k < cut.ks; ++k) {
+        const int4 v = ld_cluster16(cluster_addr(at, k));
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
+      }
+      const float as = a.a_scales[token0 + tok];
+      const float v[4] = {int8_out(sum.x, as, ws[0]) + bi[0], int8_out(sum.y, as, ws[1]) + bi[1],
+                          int8_out(sum.z, as, ws[2]) + bi[2], int8_out(sum.w, as, ws[3]) + bi[3]};
+      typename E::T* y = static_cast<typename E::T*>(a.y) + static_cast<int64_t>(token0 + tok) * a.ldy + n;
+      if (a.vec_y && n + 4 <= a.N) {
+        typename E::T o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = E::narrow(v[j]);
+        if constexpr (sizeof(o) == 8) *reinterpret_cast<uint2*>(y) = *reinterpret_cast<uint2*>(o);
+        else *reinterpret_cast<uint4*>(y) = *reinterpret_cast<uint4*>(o);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < a.N) y[j] = E::narrow(v[j]);
+      }
+    }
+  }
+  cluster_arrive_relaxed();
+  cluster_wait();  // nobody leaves while its sums are being read
+  if (failed && t == 0) {  // copies and products still in flight, bounded
+    for (int s = 0; s < cut.stages && s < count; ++s) (void)mbar_wait_bounded(&full[s], 0);
+    (void)mbar_wait_bounded(&ready, 0);
+    if (a.error_word) atomicOr(a.error_word, Q3S_DECERR_WAIT);
+  }
+  __syncthreads();
+  if (w == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cut.tmem) : "memory");
+  }
+}
+
+// Many rows: persistent 256 x 256 tiles, one a pair of CTAs (cta_group::2: each
+// holds 128 rows of x and 128 of the weights, the instruction reads both
+// halves), because at 8 bits the operands of a one-CTA instruction would take
+// more than the shared memory gives and twice the L2 reads (128 x 128 tiles of
+// one CTA: 200 us for 8192 x 2048 x 8192; 128 x 256: 131 us).  Per CTA: a copy
+// warp, the leading CTA's matrix warp, and four warps that scale and store the
+// previous tile out of the other half of TMEM, through shared memory and TMA
+// stores.
+constexpr int I8P_NT = 192, I8P_STAGES = 5, I8P_N = 256;
+constexpr int I8P_STAGE = 2 * I8_TILE;
+constexpr int I8P_OUT = 4096;  // 32 rows of 128 bytes
+constexpr int I8P_SMEM = 1024 + I8P_STAGES * I8P_STAGE + 4 * 2 * I8P_OUT + 4 * I8P_N * 4;
+
+template <int ELEM>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_NT, 1)
+    int8_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
+                     const __grid_constant__ CUtensorMap tm_y, const Int8Args a) {
+  using E = Elem<ELEM>;
+  constexpr int OC = 128 / static_cast<int>(sizeof(typename E::T));  // output columns in 128 bytes
+  extern __shared__ __align__(1024) unsigned char i8_smem[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(i8_smem) + 1023) &
+                                                         ~static_cast<uintptr_t>(1023));
+  __shared__ __align__(8) uint64_t full[I8P_STAGES], empty[I8P_STAGES], ready[2], drained[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+  const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
+  const int rank = static_cast<int>(cluster_rank()), pairs = static_cast<int>(gridDim.x) / 2, pair = static_cast<int>(blockIdx.x) / 2;
+  const int mtiles = (a.M + 255) / 256, tiles = mtiles * ((a.N + I8P_N - 1) / I8P_N), chunks = (a.K + I8_BK - 1) / I8_BK;
+  if (t == 0) {
+    for (int s = 0; s < I8P_STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&ready[b], 1);
+      mbar_init(&drained[b], 8);  // the epilogue warps of both CTAs
+    }
+    failed = 0;
+    fence_mbar_init();
+  }
+  if (w == 5) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive_release();
+  cluster_wait();  // the pair's barriers are initialised and its TMEM is allocated
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the quantised rows, when this grid is launched behind them
 
   // a wait that gives up marks the CTA; every role then stops at its next wait
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (*reinterpret_cast<volatile int*>(failed)) return false;
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*static_cast<volatile int*>(&failed)) return false;
     if (mbar_wait_bounded(bar, parity)) return true;
-    atomicOr(failed, 1);
+    atomicOr(&failed, 1);
     return false;
   };
 
   if (w == 4) {
     if (lane == 0) {
-      int k = 0;  // chunks so far
+      int k = 0;
       bool ok = true;
-      for (int tile = static_cast<int>(blockIdx.x); ok && tile < tiles; tile += static_cast<int>(gridDim.x)) {
-        const int m0 = (tile % a.mtiles) * I8_BM, n0 = (tile / a.mtiles) * BN;
-        for (int c = 0; c < a.kchunks; ++c, ++k) {
-          const int s = k % STAGES;
-          if (k >= STAGES && !wait(&empty[s], ((k / STAGES) - 1) & 1)) {
+      for (int tile = pair; ok && tile < tiles; tile += pairs) {
+        const int m0 = (tile % mtiles) * 256 + 128 * rank, n0 = (tile / mtiles) * I8P_N + 128 * rank;
+        for (int c = 0; c < chunks; ++c, ++k) {
+          const int s = k % I8P_STAGES;
+          if (k >= I8P_STAGES && !wait(&empty[s], ((k / I8P_STAGES) - 1) & 1)) {
             ok = false;
             break;
           }
-          unsigned char* st = smem + s * Tile::STAGE;
-          mbar_expect_tx(&full[s], Tile::STAGE);
-          tma_load_2d(smem_u32(st), &tm_a, c * I8_BK, m0, &full[s]);
-          tma_load_2d(smem_u32(st + I8_A_BYTES), &tm_w, c * I8_BK, n0, &full[s]);
+          const uint32_t dst = smem_u32(smem + s * I8P_STAGE), bar = cluster_addr(smem_u32(&full[s]), 0);
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * I8P_STAGE);  // both CTAs' copies
+          tma_load_2d_pair(dst, &tm_a, c * I8_BK, m0, bar);
+          tma_load_2d_pair(dst + I8_TILE, &tm_w, c * I8_BK, n0, bar);
         }
       }
-      // no copy may be in flight when the CTA leaves: wait for each stage's last one
-      for (int i = max(0, k - STAGES); i < k; ++i) (void)mbar_wait_bounded(&full[i % STAGES], (i / STAGES) & 1);
+      // no copy may be in flight when the pair leaves: the stages' last ones (they complete on the leading CTA)
+      if (rank == 0)
+        for (int i = max(0, k - I8P_STAGES); i < k; ++i) (void)mbar_wait_bounded(&full[i % I8P_STAGES], (i / I8P_STAGES) & 1);
     }
   } else if (w == 5) {
-    if (lane == 0) {
+    if (rank == 0 && lane == 0) {
+      constexpr uint32_t idesc = i8_idesc(256, I8P_N);
       int k = 0, i = 0;
       bool ok = true;
-      for (int tile = static_cast<int>(blockIdx.x); ok && tile < tiles; tile += static_cast<int>(gridDim.x), ++i) {
+      for (int tile = pair; ok && tile < tiles; tile += pairs, ++i) {
         const int b = i & 1;
         if (i >= 2 && !wait(&drained[b], ((i >> 1) - 1) & 1)) break;
         tc_fence_after();
-        for (int c = 0; c < a.kchunks; ++c, ++k) {
-          const int s = k % STAGES;
-          if (!wait(&full[s], (k / STAGES) & 1)) {
+        for (int c = 0; c < chunks; ++c, ++k) {
+          const int s = k % I8P_STAGES;
+          if (!wait(&full[s], (k / I8P_STAGES) & 1)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * Tile::STAGE);
-          const uint64_t da = head_smem_desc(sa), db = head_smem_desc(sa + I8_A_BYTES);
+          const uint32_t sa = smem_u32(smem + s * I8P_STAGE);
+          const uint64_t da = head_smem_desc(sa), dw = head_smem_desc(sa + I8_TILE);
 #pragma unroll
           for (int j = 0; j < I8_BK / 32; ++j)  // 32 bytes of K = 2 descriptor units per instruction
-            umma_i8(tmem + static_cast<uint32_t>(b * BN), da + 2 * j, db + 2 * j, Tile::IDESC, (c | j) != 0);
-          umma_commit(&empty[s]);
+            umma_i8_pair(tmem + static_cast<uint32_t>(b * I8P_N), da + 2 * j, dw + 2 * j, idesc, (c | j) != 0);
+          umma_commit_pair(&empty[s]);
         }
-        umma_commit(&ready[b]);
+        umma_commit_pair(&ready[b]);
       }
     }
   } else {
-    int i = 0;
-    for (int tile = static_cast<int>(blockIdx.x); tile < tiles; tile += static_cast<int>(gridDim.x), ++i) {
-      const int b = i & 1;
-      const int n0 = (tile / a.mtiles) * BN, row = (tile % a.mtiles) * I8_BM + 32 * w + lane;
-      const bool in = row < a.M;
-      const float as = in ? a.a_scales[row] : 0.0f;
+    unsigned char* out = smem + I8P_STAGES * I8P_STAGE + w * 2 * I8P_OUT;
+    float* s_ws = reinterpret_cast<float*>(smem + I8P_STAGES * I8P_STAGE + 4 * 2 * I8P_OUT) + w * I8P_N;
+    int i = 0, sent = 0;
+    for (int tile = pair; tile < tiles; tile += pairs, ++i) {
+      const int b = i & 1, n0 = (tile / mtiles) * I8P_N, row0 = (tile % mtiles) * 256 + 128 * rank + 32 * w, row = row0 + lane;
+      const float as = row < a.M ? a.a_scales[row] : 0.0f;
+#pragma unroll
+      for (int j = 0; j < I8P_N / 32; ++j) s_ws[32 * j + lane] = n0 + 32 * j + lane < a.N ? a.w_scales[n0 + 32 * j + lane] : 0.0f;
+      __syncwarp();
       if (!__all_sync(FULL, wait(&ready[b], (i >> 1) & 1))) break;
       tc_fence_after();
-      typename E::T* y = static_cast<typename E::T*>(a.y) + row * a.ldy + n0;
 #pragma unroll 1
-      for (int c = 0; c < BN / 32; ++c) {
-        float v[32];
-        tmem_ld32(tmem + (static_cast<uint32_t>(32 * w) << 16) + static_cast<uint32_t>(b * BN + 32 * c), v);
-        if (n0 + 32 * c >= a.N) continue;
-        const int left = a.N - n0 - 32 * c;
-        if (left >= 32 && a.vec_y) {
-          const float* ws = a.w_scales + n0 + 32 * c;
-          const float* bi = a.bias ? a.bias + n0 + 32 * c : nullptr;
+      for (int c = 0; c < I8P_N / OC; ++c) {
+        typename E::T o[OC];
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            v[j] = __fmul_rn(__fmul_rn(static_cast<float>(__float_as_int(v[j])), as), __ldg(ws + j));
-          if (bi) {
+        for (int hc = 0; hc < OC / 32; ++hc) {
+          float v[32];
+          tmem_ld32(tmem + (static_cast<uint32_t>(32 * w) << 16) + static_cast<uint32_t>(b * I8P_N + OC * c + 32 * hc), v);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] += __ldg(bi + j);
-          }
-          if (in) {
-            constexpr int W = 16 / sizeof(typename E::T);
+          for (int j = 0; j < 32; j += 4) {
+            const float4 s4 = *reinterpret_cast<const float4*>(s_ws + OC * c + 32 * hc + j);
+            const float ws[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-            for (int j = 0; j < 32; j += W) {
-              typename E::T p[W];
-#pragma unroll
-              for (int q = 0; q < W; ++q) p[q] = E::narrow(v[j + q]);
-              uint4 u;
-              memcpy(&u, p, 16);
-              *reinterpret_cast<uint4*>(y + 32 * c + j) = u;
+            for (int e = 0; e < 4; ++e) {
+              const int n = n0 + OC * c + 32 * hc + j + e;
+              float x = int8_out(__float_as_int(v[j + e]), as, ws[e]);
+              if (a.bias && n < a.N) x += __ldg(a.bias + n);
+              o[32 * hc + j + e] = E::narrow(x);
             }
           }
-        } else if (in) {
+        }
+        const int n = n0 + OC * c;
+        if (c == I8P_N / OC - 1) {  // the accumulator has been read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(cluster_addr(smem_u32(&drained[b]), 0));
+        }
+        if (n >= a.N || row0 >= a.M) continue;
+        if (a.vec_y) {
+          unsigned char* buf = out + (sent & 1) * I8P_OUT;
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the store before last has left the buffer
+          __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (j >= left) break;
-            float x = __fmul_rn(__fmul_rn(static_cast<float>(__float_as_int(v[j])), as), a.w_scales[n0 + 32 * c + j]);
-            if (a.bias) x += a.bias[n0 + 32 * c + j];
-            y[32 * c + j] = E::narrow(x);
+          for (int q = 0; q < 8; ++q) {
+            uint4 u;
+            memcpy(&u, o + q * (OC / 8), 16);
+            *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) = u;
           }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tm_y, n, row0, smem_u32(buf));
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          ++sent;
+        } else if (row < a.M) {
+          typename E::T* y = static_cast<typename E::T*>(a.y) + row * a.ldy + n;
+#pragma unroll
+          for (int j = 0; j < OC; ++j)
+            if (n + j < a.N) y[j] = o[j];
         }
       }
-      tc_fence_before();
-      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&drained[b])) : "memory");
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  cluster_arrive_release();
+  cluster_wait();  // both CTAs are done with each other's barriers, shared memory and TMEM
   if (w == 5) {
     tc_fence_after();
-    if (*failed) {  // matrix instructions may still be running: their commits (bounded) before the columns go
+    if (failed && rank == 0) {  // products may still be running: their commits (bounded) before the columns go
       if (lane == 0)
         for (int b = 0; b < 2; ++b) (void)mbar_wait_bounded(&ready[b], 0);
       __syncwarp();
     }
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Tile::TMEM) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
-  if (t == 0 && *failed && a.error_word) atomicOr(a.error_word, Q3S_DECERR_WAIT);
+  if (t == 0 && failed && a.error_word) atomicOr(a.error_word, Q3S_DECERR_WAIT);
 }
 
 }  // namespace q3s

@@ -13,6 +13,7 @@
 //   int8_matmul(values, scales, weight, weight_scales, dtype, bias=None) -> y
 //   int8_linear(x, weight, weight_scales, bias=None) -> (y, values, scales)
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -62,6 +63,22 @@ int32_t i32(int64_t x, const char* name) {
   TORCH_CHECK(x >= 0 && x <= INT32_MAX, "q3s: ", name, " is ", x, ", not in [0, 2^31)");
   return static_cast<int32_t>(x);
 }
+// A new contiguous tensor like at::empty's, straight from the CUDA allocator: at a decode step's sizes the dispatcher
+// costs more than the kernels.
+Tensor make(at::IntArrayRef sizes, at::ScalarType dt, const Tensor& ref) {
+  return at::detail::empty_cuda(sizes, dt, ref.device(), c10::nullopt);
+}
+// A tensor of its own over part of `base`'s memory (which stays alive with it): the outputs of a call that always come
+// together share one allocation.  `byte` is a multiple of the element size.
+Tensor part(const Tensor& base, int64_t byte, at::IntArrayRef sizes, at::ScalarType dt) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                      c10::scalarTypeToTypeMeta(dt));
+  t.unsafeGetTensorImpl()->set_storage_offset(byte / static_cast<int64_t>(c10::elementSize(dt)));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
+}
+int64_t round16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
 // Two tensors that a call reads and writes must not share memory.
 void apart(const Tensor& out, const Tensor& in, const char* what) {
   TORCH_CHECK(!out.is_alias_of(in) || out.data_ptr() != in.data_ptr(), "q3s: ", what, " must not be the same tensor");
@@ -105,10 +122,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> cache_tables(
   d.ring_size = i32(free_blocks.size(0), "free_blocks");
   d.free_state = free_state.data_ptr<int32_t>();
   d.max_tokens = i32(max_tokens, "max_tokens");
-  const auto opt = context.options();
-  Tensor offsets = at::empty({B + 1}, opt), slots = at::empty({max_tokens}, opt.dtype(at::kLong));
-  Tensor positions = at::empty({max_tokens}, opt), lengths = at::empty({B}, opt);
-  Tensor state = at::empty({2}, opt), error = at::empty({1}, opt);
+  const int64_t at_slots = 0, at_positions = at_slots + round16(8 * max_tokens), at_offsets = at_positions + round16(4 * max_tokens),
+                at_lengths = at_offsets + round16(4 * (B + 1)), at_state = at_lengths + round16(4 * B), all = at_state + 32;
+  const Tensor arena = make({all}, at::kByte, context);
+  Tensor slots = part(arena, at_slots, {max_tokens}, at::kLong), positions = part(arena, at_positions, {max_tokens}, at::kInt);
+  Tensor offsets = part(arena, at_offsets, {B + 1}, at::kInt), lengths = part(arena, at_lengths, {B}, at::kInt);
+  Tensor state = part(arena, at_state, {2}, at::kInt), error = part(arena, at_state + 16, {1}, at::kInt);
   d.query_offsets = offsets.data_ptr<int32_t>();
   d.slot_map = slots.data_ptr<int64_t>();
   d.positions = positions.data_ptr<int32_t>();
@@ -226,8 +245,7 @@ std::tuple<Tensor, Tensor> prefix_attention(const Tensor& q, const Tensor& k_cac
   d.block_table = block_table.data_ptr<int32_t>();
   d.block_table_stride = B > 1 ? block_table.stride(0) : block_table.size(1);
   d.lengths = lengths.data_ptr<int32_t>();
-  Tensor out = at::empty({T, q.size(1), q.size(2)}, q.options());
-  Tensor lse = at::empty({T, q.size(1)}, q.options().dtype(at::kFloat));
+  Tensor out = make({T, q.size(1), q.size(2)}, q.scalar_type(), q), lse = make({T, q.size(1)}, at::kFloat, q);
   d.out = out.data_ptr();
   d.out_token_stride = q.size(1) * q.size(2);
   d.out_head_stride = q.size(2);
@@ -235,7 +253,7 @@ std::tuple<Tensor, Tensor> prefix_attention(const Tensor& q, const Tensor& k_cac
   d.error_word = error_of(error_word, q);
   int64_t bytes = 0;
   check_status(q3s_prefix_attention_workspace(&d, &bytes), "q3s_prefix_attention");
-  Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  const Tensor ws = make({bytes}, at::kByte, q);
   d.workspace = ws.data_ptr();
   d.workspace_bytes = bytes;
   check_status(q3s_prefix_attention(&d, stream_of(q)), "q3s_prefix_attention");
@@ -251,7 +269,7 @@ Tensor rows_of(const Tensor& x) {
   return r;
 }
 
-void quantize_into(const Tensor& r, const Tensor& values, const Tensor& scales) {
+q3s_quantize_rows_desc quantize_desc(const Tensor& r, const Tensor& values, const Tensor& scales) {
   q3s_quantize_rows_desc d;
   std::memset(&d, 0, sizeof(d));
   d.struct_size = sizeof(d);
@@ -263,21 +281,21 @@ void quantize_into(const Tensor& r, const Tensor& values, const Tensor& scales) 
   d.values = values.data_ptr<int8_t>();
   d.values_row_stride = r.size(1);
   d.scales = scales.data_ptr<float>();
-  check_status(q3s_quantize_rows(&d, stream_of(r)), "q3s_quantize_rows");
+  return d;
 }
 
 std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {
   const Tensor r = rows_of(x);
   c10::cuda::CUDAGuard guard(r.device());
-  Tensor values = at::empty({r.size(0), r.size(1)}, r.options().dtype(at::kChar));
-  Tensor scales = at::empty({r.size(0)}, r.options().dtype(at::kFloat));
-  quantize_into(r, values, scales);
+  Tensor values = make({r.size(0), r.size(1)}, at::kChar, r), scales = make({r.size(0)}, at::kFloat, r);
+  const q3s_quantize_rows_desc d = quantize_desc(r, values, scales);
+  check_status(q3s_quantize_rows(&d, stream_of(r)), "q3s_quantize_rows");
   if (x.dim() == 2) return {values, scales};
   return {values.view(x.sizes()), scales.view(x.sizes().slice(0, x.dim() - 1))};
 }
 
-void matmul_into(const Tensor& a, const Tensor& a_scales, const Tensor& w, const Tensor& w_scales,
-                 const OptTensor& bias, const Tensor& y) {
+q3s_int8_matmul_desc matmul_desc(const Tensor& a, const Tensor& a_scales, const Tensor& w, const Tensor& w_scales,
+                                 const OptTensor& bias, const Tensor& y) {
   const int64_t M = a.size(0), K = a.size(1), N = w.size(0);
   need(w, a, at::kChar, 2, "weight");
   TORCH_CHECK(w.size(1) == K && w.stride(1) == 1, "q3s: weight must be [N, ", K, "] with unit column stride, got ", w.sizes());
@@ -302,7 +320,7 @@ void matmul_into(const Tensor& a, const Tensor& a_scales, const Tensor& w, const
   }
   d.y = y.data_ptr();
   d.y_row_stride = N;
-  check_status(q3s_int8_matmul(&d, stream_of(a)), "q3s_int8_matmul");
+  return d;
 }
 
 Tensor int8_matmul(const Tensor& values, const Tensor& scales, const Tensor& weight, const Tensor& weight_scales,
@@ -312,8 +330,9 @@ Tensor int8_matmul(const Tensor& values, const Tensor& scales, const Tensor& wei
   need(values, values, at::kChar, 2, "values");
   TORCH_CHECK(values.size(1) <= 1 || values.stride(1) == 1, "q3s: values must have unit column stride");
   TORCH_CHECK(weight.dim() == 2, "q3s: weight must be [N, K], got ", weight.sizes());
-  Tensor y = at::empty({values.size(0), weight.size(0)}, values.options().dtype(dtype));
-  matmul_into(values, scales, weight, weight_scales, bias, y);
+  Tensor y = make({values.size(0), weight.size(0)}, dtype, values);
+  const q3s_int8_matmul_desc d = matmul_desc(values, scales, weight, weight_scales, bias, y);
+  check_status(q3s_int8_matmul(&d, stream_of(values)), "q3s_int8_matmul");
   return y;
 }
 
@@ -323,11 +342,13 @@ std::tuple<Tensor, Tensor, Tensor> int8_linear(const Tensor& x, const Tensor& we
   c10::cuda::CUDAGuard guard(r.device());
   TORCH_CHECK(weight.dim() == 2, "q3s: weight must be [N, K], got ", weight.sizes());
   const int64_t M = r.size(0), K = r.size(1), N = weight.size(0);
-  Tensor values = at::empty({M, K}, r.options().dtype(at::kChar));
-  Tensor scales = at::empty({M}, r.options().dtype(at::kFloat));
-  Tensor y = at::empty({M, N}, r.options());
-  quantize_into(r, values, scales);
-  matmul_into(values, scales, weight, weight_scales, bias, y);
+  const int64_t at_scales = round16(M * K);
+  const Tensor arena = make({at_scales + 4 * M}, at::kByte, r);
+  Tensor values = part(arena, 0, {M, K}, at::kChar), scales = part(arena, at_scales, {M}, at::kFloat);
+  Tensor y = make({M, N}, r.scalar_type(), r);
+  const q3s_quantize_rows_desc q = quantize_desc(r, values, scales);
+  const q3s_int8_matmul_desc d = matmul_desc(values, scales, weight, weight_scales, bias, y);
+  check_status(q3s_int8_linear(&q, &d, stream_of(r)), "q3s_int8_linear");
   if (x.dim() == 2) return {y, values, scales};
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = N;

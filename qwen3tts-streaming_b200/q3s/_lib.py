@@ -307,6 +307,7 @@ DECODE_EXPORTS = (
     "q3s_prefix_attention",
     "q3s_quantize_rows",
     "q3s_int8_matmul",
+    "q3s_int8_linear",
     "q3s_decode_desc_size",
 )
 
@@ -366,6 +367,8 @@ def load(path: str | Path | None = None) -> C.CDLL:
                              "q3s_int8_matmul"), DECODE_DESCS):
             getattr(lib, name).argtypes = [C.POINTER(st), _p]
             getattr(lib, name).restype = C.c_int
+        lib.q3s_int8_linear.argtypes = [C.POINTER(QuantizeRowsDesc), C.POINTER(Int8MatmulDesc), _p]
+        lib.q3s_int8_linear.restype = C.c_int
         lib.q3s_prefix_attention_workspace.argtypes = [C.POINTER(PrefixAttentionDesc), C.POINTER(C.c_int64)]
         lib.q3s_prefix_attention_workspace.restype = C.c_int
         lib.q3s_decode_desc_size.argtypes = [C.c_int32]

@@ -74,7 +74,7 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
     tmp = TORCH_OPS_PATH.with_suffix(".so.tmp")
     cmd = [system_cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            *incs, str(TORCH_OPS_SRC), str(TORCH_DECODE_SRC), "-o", str(tmp), *libdirs, f"-L{PKG_DIR}", "-lq3s_sampler",
-           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-Wl,-rpath,$ORIGIN"]
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-Wl,-rpath,$ORIGIN"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or res.returncode != 0:
         print(" ".join(cmd))

@@ -440,7 +440,9 @@ def test_quantize_rows_of_odd_values(dev):
 
 @pytest.mark.parametrize("M,K,N", [(1, 16, 1), (1, 2048, 2048), (2, 64, 100), (7, 144, 33), (8, 2048, 513), (9, 2048, 513),
                                    (16, 4096, 96), (17, 512, 1000), (64, 1040, 257), (128, 2048, 2048), (129, 2048, 96),
-                                   (130, 2064, 5000), (300, 768, 768), (513, 128, 2050), (1000, 16, 130), (2000, 2048, 1024)])
+                                   (130, 2064, 5000), (300, 768, 768), (513, 128, 2050), (1000, 16, 130), (2000, 2048, 1024),
+                                   (3, 16384, 130), (8, 16000, 40), (300, 16400, 96), (2300, 528, 5001), (4096, 2048, 2304),
+                                   (250, 144, 20000)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_int8_matmul(dev, M, K, N, dtype):
     g = torch.Generator(device=dev).manual_seed(M + K + N)
