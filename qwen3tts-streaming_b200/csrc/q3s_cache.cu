@@ -234,32 +234,48 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
   const uint32_t per_part = static_cast<uint32_t>(a.H) * a.units, per_token = 2 * per_part;
   const uint64_t all = static_cast<uint64_t>(a.T) * per_token;
   const uint64_t base = static_cast<uint64_t>(blockIdx.x) * (256 * U) + threadIdx.x;
+  using ELEM = typename std::conditional<sizeof(UNIT) == 16, uint16_t, UNIT>::type;
   UNIT x[U];
+  int64_t slot[U];
   UNIT* to[U];
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
+  for (int i = 0; i < U; ++i) {  // the copies and their slots are requested side by side
     const uint64_t at = base + 256u * i;
     to[i] = nullptr;
+    slot[i] = -1;
     if (at >= all) continue;
     const uint32_t token = static_cast<uint32_t>(at / per_token);
     uint32_t rest = static_cast<uint32_t>(at - static_cast<uint64_t>(token) * per_token);
     const bool value = rest >= per_part;
     if (value) rest -= per_part;
     const uint32_t h = rest / a.units, e = (rest - h * a.units) * E;
-    const int64_t slot = a.slots[token];
-    if (slot < 0) continue;
-    const int64_t block = slot / a.bs, place = slot - block * a.bs;
-    if (block >= a.blocks) {
-      if (a.error_word) atomicOr(a.error_word, Q3S_DECERR_BLOCK_ID);
+    slot[i] = a.slots[token];
+    x[i] = *reinterpret_cast<const UNIT*>(static_cast<const ELEM*>(value ? a.v : a.k) +
+                                          (value ? token * a.vt + h * a.vh : token * a.kt + h * a.kh) + e);
+    to[i] = reinterpret_cast<UNIT*>(static_cast<ELEM*>(value ? a.vc : a.kc) + (value ? h * a.vch : h * a.kch) + e);
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    if (slot[i] < 0) {
+      to[i] = nullptr;
       continue;
     }
-    using ELEM = typename std::conditional<sizeof(UNIT) == 16, uint16_t, UNIT>::type;
-    const ELEM* from = static_cast<const ELEM*>(value ? a.v : a.k) +
-                       (value ? token * a.vt + h * a.vh : token * a.kt + h * a.kh) + e;
-    x[i] = *reinterpret_cast<const UNIT*>(from);
-    to[i] = reinterpret_cast<UNIT*>(static_cast<ELEM*>(value ? a.vc : a.kc) +
-                                    (value ? block * a.vb + h * a.vch + place * a.vp
-                                           : block * a.kb + h * a.kch + place * a.kp) + e);
+    const uint64_t at = base + 256u * i;
+    const bool value = static_cast<uint32_t>(at - at / per_token * per_token) >= per_part;
+    int64_t block = 0, place = 0;
+    if (slot[i] < static_cast<int64_t>(a.blocks) * a.bs) {
+      if ((slot[i] >> 32) == 0) {
+        block = static_cast<uint32_t>(slot[i]) / static_cast<uint32_t>(a.bs);
+      } else {
+        block = slot[i] / a.bs;
+      }
+      place = slot[i] - block * a.bs;
+    } else {
+      if (a.error_word) atomicOr(a.error_word, Q3S_DECERR_BLOCK_ID);
+      to[i] = nullptr;
+      continue;
+    }
+    to[i] = reinterpret_cast<UNIT*>(reinterpret_cast<ELEM*>(to[i]) + (value ? block * a.vb + place * a.vp : block * a.kb + place * a.kp));
   }
 #pragma unroll
   for (int i = 0; i < U; ++i)

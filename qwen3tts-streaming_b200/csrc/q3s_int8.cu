@@ -28,7 +28,10 @@ bool byte_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int6
 
 template <int ELEM>
 cudaError_t launch_quantize(const q3s::QuantArgs& a, bool vec, cudaStream_t st) {
-  if (vec)
+  // a warp a row once there are warps for every SM's quarter; below that a CTA a row has the shorter chain
+  if (vec && a.M >= 4 * q3s::sm_count() && a.K <= 32 * q3s::QW_KEEP * q3s::Elem<ELEM>::N)
+    q3s::quantize_warps_kernel<ELEM><<<(a.M + q3s::QW_WARPS - 1) / q3s::QW_WARPS, q3s::QW_WARPS * 32, 0, st>>>(a);
+  else if (vec)
     q3s::quantize_rows_kernel<ELEM, true><<<a.M, 128, 0, st>>>(a);
   else
     q3s::quantize_rows_kernel<ELEM, false><<<a.M, 128, 0, st>>>(a);
@@ -69,6 +72,31 @@ cudaError_t launch_gemv(const q3s::Int8Args& a, const q3s::QuantArgs& q, cudaStr
 bool few_rows(int M, int K) { return M <= q3s::GV_MAX_M && static_cast<int64_t>(K) * (M <= 2 ? M : M <= 4 ? 4 : 8) <= q3s::GV_SMEM; }
 
 // -- tensor cores --
+template <int ELEM, int KS>
+cudaError_t launch_split_ks(const q3s::Int8Args& a, const q3s::I8Cut& cut, dim3 grid, int smem, const CUtensorMap& tw,
+                            const CUtensorMap& ta, cudaStream_t st) {
+  auto kern = q3s::int8_split_kernel<ELEM, KS>;
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = q3s::allow_smem(kern, 220 * 1024, done);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = grid;
+  lc.blockDim = dim3(q3s::I8C_NT);
+  lc.dynamicSmemBytes = smem;
+  lc.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 1;
+  at[0].val.clusterDim.y = KS;
+  at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = at;
+  lc.numAttrs = 2;
+  e = cudaLaunchKernelEx(&lc, kern, tw, ta, a, cut);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
 template <int ELEM>
 cudaError_t launch_split(const q3s::Int8Args& a, cudaStream_t st) {
   q3s::I8Cut cut;
@@ -80,36 +108,21 @@ cudaError_t launch_split(const q3s::Int8Args& a, cudaStream_t st) {
   const int ntiles = (a.N + 127) / 128, stage = q3s::I8_TILE + cut.bt * q3s::I8_BK;
   // K is cut until the CTAs are one a SM, or two where two fit (110 KB each), with two chunks each at least
   const int most = 110 * 1024 / stage >= 3 ? 2 : 1;
-  cut.ks = 1;
-  while (cut.ks < 8 && cut.chunks >= 4 * cut.ks && ntiles * mtiles * cut.ks * 2 <= most * q3s::sm_count()) cut.ks *= 2;
-  const bool two = ntiles * mtiles * cut.ks > q3s::sm_count();
-  const int mine = (cut.chunks + cut.ks - 1) / cut.ks;
+  int ks = 1;
+  while (ks < 8 && cut.chunks >= 4 * ks && ntiles * mtiles * ks * 2 <= most * q3s::sm_count()) ks *= 2;
+  const bool two = ntiles * mtiles * ks > q3s::sm_count();
+  const int mine = (cut.chunks + ks - 1) / ks;
   // a ring that also holds the partial sums of the tile
-  const int floor_ = (cut.bt * 512 + stage - 1) / stage;
-  cut.stages = std::max(floor_, std::min({8, mine, (two ? 110 : 196) * 1024 / stage}));
+  const int least = (cut.bt * 512 + stage - 1) / stage;
+  cut.stages = std::max(least, std::min({8, mine, (two ? 110 : 196) * 1024 / stage}));
   const int smem = 1024 + cut.stages * stage;
-  auto kern = q3s::int8_split_kernel<ELEM>;
-  static std::atomic<uint64_t> done{0};
-  cudaError_t e = q3s::allow_smem(kern, 220 * 1024, done);
-  if (e != cudaSuccess) return e;
   CUtensorMap tw, ta;
   if (!byte_map(&tw, a.w, a.N, a.K, a.ldw, 128) || !byte_map(&ta, a.a, a.M, a.K, a.lda, cut.bt)) return cudaErrorInvalidValue;
-  cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(ntiles, cut.ks, mtiles);
-  lc.blockDim = dim3(q3s::I8C_NT);
-  lc.dynamicSmemBytes = smem;
-  lc.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = 1;
-  at[0].val.clusterDim.y = cut.ks;
-  at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  lc.attrs = at;
-  lc.numAttrs = 2;
-  e = cudaLaunchKernelEx(&lc, kern, tw, ta, a, cut);
-  return e != cudaSuccess ? e : cudaGetLastError();
+  const dim3 grid(ntiles, ks, mtiles);
+  if (ks == 1) return launch_split_ks<ELEM, 1>(a, cut, grid, smem, tw, ta, st);
+  if (ks == 2) return launch_split_ks<ELEM, 2>(a, cut, grid, smem, tw, ta, st);
+  if (ks == 4) return launch_split_ks<ELEM, 4>(a, cut, grid, smem, tw, ta, st);
+  return launch_split_ks<ELEM, 8>(a, cut, grid, smem, tw, ta, st);
 }
 
 template <int ELEM>

@@ -29,6 +29,8 @@ struct Elem<Q3S_ELEM_F32> {
   }
   Q3S_DEV static float one(const T* p) { return *p; }
   Q3S_DEV static T narrow(float x) { return x; }
+  Q3S_DEV static uint32_t narrow2(const float* x) { return __float_as_uint(x[0]); }  // 32 bits of output
+  Q3S_DEV static T pick(const uint32_t (&o)[32], int j) { return __uint_as_float(o[j]); }
 };
 template <>
 struct Elem<Q3S_ELEM_BF16> {
@@ -48,6 +50,12 @@ struct Elem<Q3S_ELEM_BF16> {
     asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(x));
     return r;
   }
+  Q3S_DEV static uint32_t narrow2(const float* x) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(x[1]), "f"(x[0]));
+    return r;
+  }
+  Q3S_DEV static T pick(const uint32_t (&o)[32], int j) { return static_cast<T>(o[j / 2] >> (16 * (j % 2))); }
 };
 template <>
 struct Elem<Q3S_ELEM_F16> {
@@ -72,6 +80,12 @@ struct Elem<Q3S_ELEM_F16> {
     asm("cvt.rn.f16.f32 %0, %1;" : "=h"(r) : "f"(x));
     return r;
   }
+  Q3S_DEV static uint32_t narrow2(const float* x) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(x[1]), "f"(x[0]));
+    return r;
+  }
+  Q3S_DEV static T pick(const uint32_t (&o)[32], int j) { return static_cast<T>(o[j / 2] >> (16 * (j % 2))); }
 };
 
 // ---- quantisation -----------------------------------------------------------
@@ -180,6 +194,52 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const QuantArgs a) {
     const QuantScale s = quant_scale(block_absmax<NT>(m, s_red));
     for (int c = t; c < a.K; c += NT) out[c] = static_cast<int8_t>(quant_one(E::one(x + c), s.unit));
     if (t == 0) a.scales[row] = s.scale;
+  }
+}
+
+// Many rows of up to 256 sixteen-byte units: a warp a row, the whole row in
+// registers, all its loads in flight at once and no barrier.
+constexpr int QW_WARPS = 8, QW_KEEP = 8;
+template <int ELEM>
+__global__ void __launch_bounds__(QW_WARPS * 32) quantize_warps_kernel(const QuantArgs a) {
+  using E = Elem<ELEM>;
+  constexpr int N = E::N;
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int lane = static_cast<int>(threadIdx.x) & 31, chunks = a.K / N;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * QW_WARPS + (threadIdx.x >> 5);
+  if (row >= a.M) return;
+  const typename E::T* x = static_cast<const typename E::T*>(a.x) + row * a.ldx;
+  uint4 keep[QW_KEEP];
+#pragma unroll
+  for (int i = 0; i < QW_KEEP; ++i)
+    keep[i] = lane + 32 * i < chunks ? ld_stream16(x + static_cast<int64_t>(lane + 32 * i) * N) : make_uint4(0, 0, 0, 0);
+  float v[N], m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < QW_KEEP; ++i) {
+    E::widen(keep[i], v);
+#pragma unroll
+    for (int j = 0; j < N; ++j) m = absmax(m, v[j]);
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) m = absmax(m, __shfl_xor_sync(FULL, m, d));
+  const QuantScale s = quant_scale(m);
+  if (lane == 0) a.scales[row] = s.scale;
+  int8_t* out = a.values + row * a.ldv;
+#pragma unroll
+  for (int i = 0; i < QW_KEEP; ++i) {
+    if (lane + 32 * i >= chunks) break;
+    E::widen(keep[i], v);
+    uint32_t p[N / 4];
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) {
+      p[j] = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) p[j] |= (static_cast<uint32_t>(quant_one(v[4 * j + b], s.unit)) & 0xffu) << (8 * b);
+    }
+    if constexpr (N == 8)
+      *reinterpret_cast<uint2*>(out + (lane + 32 * i) * N) = make_uint2(p[0], p[1]);
+    else
+      *reinterpret_cast<uint32_t*>(out + (lane + 32 * i) * N) = p[0];
   }
 }
 
@@ -418,12 +478,12 @@ Q3S_DEV int4 ld_cluster16(uint32_t addr) {
 // KS-th group of tokens.  Bound by the latency of that chain (load, products,
 // exchange) and the weights' bytes.
 struct I8Cut {
-  int bt, ks, stages, chunks;  // tokens of a tile, CTAs of a cluster, ring stages, chunks of K
+  int bt, stages, chunks;  // tokens of a tile, ring stages, chunks of K
   int tmem;                    // columns: a power of two >= 32
 };
 constexpr int I8C_NT = 128;
 
-template <int ELEM>
+template <int ELEM, int KS>
 __global__ void __launch_bounds__(I8C_NT)
     int8_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const Int8Args a,
                       const I8Cut cut) {
@@ -438,7 +498,7 @@ __global__ void __launch_bounds__(I8C_NT)
   const int n0 = static_cast<int>(blockIdx.x) * 128, rank = static_cast<int>(cluster_rank());
   const int token0 = static_cast<int>(blockIdx.z) * cut.bt;
   const int stage_bytes = I8_TILE + cut.bt * I8_BK;
-  const int c0 = cut.chunks * rank / cut.ks, count = cut.chunks * (rank + 1) / cut.ks - c0;  // this CTA's chunks, >= 1
+  const int c0 = cut.chunks * rank / KS, count = cut.chunks * (rank + 1) / KS - c0;  // this CTA's chunks, >= 1
   if (t == 0) {
     for (int s = 0; s < cut.stages; ++s) {
       mbar_init(&full[s], 1);
@@ -526,31 +586,42 @@ __global__ void __launch_bounds__(I8C_NT)
       ws[j] = n + j < a.N ? a.w_scales[n + j] : 0.0f;
       bi[j] = a.bias && n + j < a.N ? a.bias[n + j] : 0.0f;
     }
-    for (int tok = rank * 4 + w; tok < cut.bt; tok += cut.ks * 4) {
-      if (token0 + tok >= a.M) break;
-      const uint32_t at = smem_u32(part + tok * 128 + 4 * lane);
-      int4 sum = make_int4(0, 0, 0, 0);
-      for (int k = 0; k < cut.ks; ++k) {
-        const int4 v = ld_cluster16(cluster_addr(at, k));
-        sum.x += v.x;
-        sum.y += v.y;
-        sum.z += v.z;
-        sum.w += v.w;
+    constexpr int T = 3;  // tokens of a warp in flight
+    for (int tok0 = rank * 4 + w; tok0 < cut.bt; tok0 += T * KS * 4) {
+      int4 part_sum[T][KS];
+#pragma unroll
+      for (int i = 0; i < T; ++i) {
+        const int tok = min(tok0 + i * KS * 4, cut.bt - 1);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) part_sum[i][k] = ld_cluster16(cluster_addr(smem_u32(part + tok * 128 + 4 * lane), k));
       }
-      const float as = a.a_scales[token0 + tok];
-      const float v[4] = {int8_out(sum.x, as, ws[0]) + bi[0], int8_out(sum.y, as, ws[1]) + bi[1],
-                          int8_out(sum.z, as, ws[2]) + bi[2], int8_out(sum.w, as, ws[3]) + bi[3]};
-      typename E::T* y = static_cast<typename E::T*>(a.y) + static_cast<int64_t>(token0 + tok) * a.ldy + n;
-      if (a.vec_y && n + 4 <= a.N) {
-        typename E::T o[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = E::narrow(v[j]);
-        if constexpr (sizeof(o) == 8) *reinterpret_cast<uint2*>(y) = *reinterpret_cast<uint2*>(o);
-        else *reinterpret_cast<uint4*>(y) = *reinterpret_cast<uint4*>(o);
-      } else {
+      for (int i = 0; i < T; ++i) {
+        const int tok = tok0 + i * KS * 4;
+        if (tok >= cut.bt || token0 + tok >= a.M) break;
+        int4 sum = part_sum[i][0];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < a.N) y[j] = E::narrow(v[j]);
+        for (int k = 1; k < KS; ++k) {
+          sum.x += part_sum[i][k].x;
+          sum.y += part_sum[i][k].y;
+          sum.z += part_sum[i][k].z;
+          sum.w += part_sum[i][k].w;
+        }
+        const float as = a.a_scales[token0 + tok];
+        const float v[4] = {int8_out(sum.x, as, ws[0]) + bi[0], int8_out(sum.y, as, ws[1]) + bi[1],
+                            int8_out(sum.z, as, ws[2]) + bi[2], int8_out(sum.w, as, ws[3]) + bi[3]};
+        typename E::T* y = static_cast<typename E::T*>(a.y) + static_cast<int64_t>(token0 + tok) * a.ldy + n;
+        if (a.vec_y && n + 4 <= a.N) {
+          typename E::T o[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] = E::narrow(v[j]);
+          if constexpr (sizeof(o) == 8) *reinterpret_cast<uint2*>(y) = *reinterpret_cast<uint2*>(o);
+          else *reinterpret_cast<uint4*>(y) = *reinterpret_cast<uint4*>(o);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < a.N) y[j] = E::narrow(v[j]);
+        }
       }
     }
   }
@@ -573,13 +644,13 @@ __global__ void __launch_bounds__(I8C_NT)
 // halves), because at 8 bits the operands of a one-CTA instruction would take
 // more than the shared memory gives and twice the L2 reads (128 x 128 tiles of
 // one CTA: 200 us for 8192 x 2048 x 8192; 128 x 256: 131 us).  Per CTA: a copy
-// warp, the leading CTA's matrix warp, and four warps that scale and store the
+// warp, the leading CTA's matrix warp, and eight warps that scale and store the
 // previous tile out of the other half of TMEM, through shared memory and TMA
 // stores.
-constexpr int I8P_NT = 192, I8P_STAGES = 5, I8P_N = 256;
+constexpr int I8P_EPI = 8, I8P_NT = (I8P_EPI + 2) * 32, I8P_STAGES = 5, I8P_N = 256;
 constexpr int I8P_STAGE = 2 * I8_TILE;
 constexpr int I8P_OUT = 4096;  // 32 rows of 128 bytes
-constexpr int I8P_SMEM = 1024 + I8P_STAGES * I8P_STAGE + 4 * 2 * I8P_OUT + 4 * I8P_N * 4;
+constexpr int I8P_SMEM = 1024 + I8P_STAGES * I8P_STAGE + I8P_EPI * I8P_OUT + I8P_EPI * I8P_N * 4;
 
 template <int ELEM>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_NT, 1)
@@ -603,12 +674,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_NT, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&ready[b], 1);
-      mbar_init(&drained[b], 8);  // the epilogue warps of both CTAs
+      mbar_init(&drained[b], 2 * I8P_EPI);  // the epilogue warps of both CTAs
     }
     failed = 0;
     fence_mbar_init();
   }
-  if (w == 5) {
+  if (w == I8P_EPI + 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -630,7 +701,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_NT, 1)
     return false;
   };
 
-  if (w == 4) {
+  if (w == I8P_EPI) {
     if (lane == 0) {
       int k = 0;
       bool ok = true;
@@ -652,7 +723,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_NT, 1)
       if (rank == 0)
         for (int i = max(0, k - I8P_STAGES); i < k; ++i) (void)mbar_wait_bounded(&full[i % I8P_STAGES], (i / I8P_STAGES) & 1);
     }
-  } else if (w == 5) {
+  } else if (w == I8P_EPI + 1) {
     if (rank == 0 && lane == 0) {
       constexpr uint32_t idesc = i8_idesc(256, I8P_N);
       int k = 0, i = 0;
@@ -679,53 +750,67 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_NT, 1)
       }
     }
   } else {
-    unsigned char* out = smem + I8P_STAGES * I8P_STAGE + w * 2 * I8P_OUT;
-    float* s_ws = reinterpret_cast<float*>(smem + I8P_STAGES * I8P_STAGE + 4 * 2 * I8P_OUT) + w * I8P_N;
-    int i = 0, sent = 0;
+    // warp w: TMEM lanes (rows) 32 (w % 4) .., columns HALF (w / 4) ..
+    constexpr int HALF = I8P_N / 2;
+    unsigned char* buf = smem + I8P_STAGES * I8P_STAGE + w * I8P_OUT;
+    float* s_ws = reinterpret_cast<float*>(smem + I8P_STAGES * I8P_STAGE + I8P_EPI * I8P_OUT) + w * 2 * HALF;  // scales, bias
+    const int quarter = 32 * (w & 3), half = HALF * (w >> 2);
+    int i = 0;
     for (int tile = pair; tile < tiles; tile += pairs, ++i) {
-      const int b = i & 1, n0 = (tile / mtiles) * I8P_N, row0 = (tile % mtiles) * 256 + 128 * rank + 32 * w, row = row0 + lane;
+      const int b = i & 1, n0 = (tile / mtiles) * I8P_N + half, row0 = (tile % mtiles) * 256 + 128 * rank + quarter, row = row0 + lane;
       const float as = row < a.M ? a.a_scales[row] : 0.0f;
 #pragma unroll
-      for (int j = 0; j < I8P_N / 32; ++j) s_ws[32 * j + lane] = n0 + 32 * j + lane < a.N ? a.w_scales[n0 + 32 * j + lane] : 0.0f;
+      for (int j = 0; j < HALF / 32; ++j) {
+        const int n = n0 + 32 * j + lane;
+        s_ws[32 * j + lane] = n < a.N ? a.w_scales[n] : 0.0f;
+        if (a.bias) s_ws[HALF + 32 * j + lane] = n < a.N ? a.bias[n] : 0.0f;
+      }
       __syncwarp();
       if (!__all_sync(FULL, wait(&ready[b], (i >> 1) & 1))) break;
       tc_fence_after();
 #pragma unroll 1
-      for (int c = 0; c < I8P_N / OC; ++c) {
-        typename E::T o[OC];
+      for (int c = 0; c < HALF / OC; ++c) {
+        uint32_t o[32];  // 128 bytes of the row
 #pragma unroll
         for (int hc = 0; hc < OC / 32; ++hc) {
           float v[32];
-          tmem_ld32(tmem + (static_cast<uint32_t>(32 * w) << 16) + static_cast<uint32_t>(b * I8P_N + OC * c + 32 * hc), v);
+          tmem_ld32(tmem + (static_cast<uint32_t>(quarter) << 16) + static_cast<uint32_t>(b * I8P_N + half + OC * c + 32 * hc), v);
+          const float* ws = s_ws + OC * c + 32 * hc;
+          const float2 as2 = make_float2(as, as);
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
-            const float4 s4 = *reinterpret_cast<const float4*>(s_ws + OC * c + 32 * hc + j);
-            const float ws[4] = {s4.x, s4.y, s4.z, s4.w};
+            const float4 s4 = *reinterpret_cast<const float4*>(ws + j);
+            float2 x0 = make_float2(static_cast<float>(__float_as_int(v[j])), static_cast<float>(__float_as_int(v[j + 1])));
+            float2 x1 = make_float2(static_cast<float>(__float_as_int(v[j + 2])), static_cast<float>(__float_as_int(v[j + 3])));
+            x0 = __fmul2_rn(__fmul2_rn(x0, as2), make_float2(s4.x, s4.y));
+            x1 = __fmul2_rn(__fmul2_rn(x1, as2), make_float2(s4.z, s4.w));
+            v[j] = x0.x, v[j + 1] = x0.y, v[j + 2] = x1.x, v[j + 3] = x1.y;
+          }
+          if (a.bias) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int n = n0 + OC * c + 32 * hc + j + e;
-              float x = int8_out(__float_as_int(v[j + e]), as, ws[e]);
-              if (a.bias && n < a.N) x += __ldg(a.bias + n);
-              o[32 * hc + j + e] = E::narrow(x);
+            for (int j = 0; j < 32; j += 4) {
+              const float4 b4 = *reinterpret_cast<const float4*>(ws + HALF + j);
+              v[j] += b4.x, v[j + 1] += b4.y, v[j + 2] += b4.z, v[j + 3] += b4.w;
             }
           }
+#pragma unroll
+          for (int j = 0; j < 32; j += 4 / static_cast<int>(sizeof(typename E::T)))
+            o[(32 * hc + j) * static_cast<int>(sizeof(typename E::T)) / 4] = E::narrow2(v + j);
         }
         const int n = n0 + OC * c;
-        if (c == I8P_N / OC - 1) {  // the accumulator has been read
+        if (c == HALF / OC - 1) {  // the accumulator has been read
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(cluster_addr(smem_u32(&drained[b]), 0));
         }
         if (n >= a.N || row0 >= a.M) continue;
         if (a.vec_y) {
-          unsigned char* buf = out + (sent & 1) * I8P_OUT;
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the store before last has left the buffer
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last store has left the buffer
           __syncwarp();
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
-            uint4 u;
-            memcpy(&u, o + q * (OC / 8), 16);
-            *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) = u;
+            *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) =
+                make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -733,12 +818,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_NT, 1)
             tma_store_2d(&tm_y, n, row0, smem_u32(buf));
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
-          ++sent;
         } else if (row < a.M) {
           typename E::T* y = static_cast<typename E::T*>(a.y) + row * a.ldy + n;
 #pragma unroll
           for (int j = 0; j < OC; ++j)
-            if (n + j < a.N) y[j] = o[j];
+            if (n + j < a.N) y[j] = E::pick(o, j);
         }
       }
     }
@@ -749,7 +833,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_NT, 1)
   __syncthreads();
   cluster_arrive_release();
   cluster_wait();  // both CTAs are done with each other's barriers, shared memory and TMEM
-  if (w == 5) {
+  if (w == I8P_EPI + 1) {
     tc_fence_after();
     if (failed && rank == 0) {  // products may still be running: their commits (bounded) before the columns go
       if (lane == 0)
