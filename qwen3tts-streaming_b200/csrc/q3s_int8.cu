@@ -100,17 +100,36 @@ cudaError_t launch_split_ks(const q3s::Int8Args& a, const q3s::I8Cut& cut, dim3 
 template <int ELEM>
 cudaError_t launch_split(const q3s::Int8Args& a, cudaStream_t st) {
   q3s::I8Cut cut;
-  const int mtiles = (a.M + 255) / 256;
-  cut.bt = ((a.M + mtiles - 1) / mtiles + 15) / 16 * 16;
+  cut.chunks = (a.K + q3s::I8_BK - 1) / q3s::I8_BK;
+  const int ntiles = (a.N + 127) / 128, sms = q3s::sm_count();
+  // Tile height and K cut: the lowest estimate of the time of a CTA (in clocks:
+  // a start and an end, its operands at 40 bytes a clock, reading its sums out of
+  // TMEM, joining its share of them) times the waves of CTAs.  Two CTAs share a
+  // SM where three stages of each fit.
+  auto stage_of = [](int bt) { return q3s::I8_TILE + bt * q3s::I8_BK; };
+  auto per_sm = [&](int bt) { return 110 * 1024 / stage_of(bt) >= 3 && bt * 512 <= 108 * 1024 ? 2 : 1; };
+  int ks = 1;
+  double best = 0;
+  for (int mt = (a.M + 255) / 256; mt <= (a.M + 31) / 32; ++mt) {
+    const int bt = ((a.M + mt - 1) / mt + 31) / 32 * 32;
+    if ((a.M + bt - 1) / bt != mt) continue;
+    for (int k = 1; k <= 8 && cut.chunks >= k; k *= 2) {
+      const int64_t ctas = static_cast<int64_t>(ntiles) * mt * k;
+      const int wave = ctas > sms ? per_sm(bt) * sms : sms;
+      const double waves = static_cast<double>((ctas + wave - 1) / wave) * (ctas > sms ? per_sm(bt) : 1);
+      const double loads = static_cast<double>((cut.chunks + k - 1) / k) * stage_of(bt) / 40;
+      const double cost = waves * (loads + 6.0 * bt + (k > 1 ? 800 : 0) + bt / (8.0 * k) * (60 + 20 * k)) + 4000;
+      if (best == 0 || cost < best) {
+        best = cost;
+        cut.bt = bt;
+        ks = k;
+      }
+    }
+  }
+  const int mtiles = (a.M + cut.bt - 1) / cut.bt, stage = stage_of(cut.bt);
   cut.tmem = 32;
   while (cut.tmem < cut.bt) cut.tmem *= 2;
-  cut.chunks = (a.K + q3s::I8_BK - 1) / q3s::I8_BK;
-  const int ntiles = (a.N + 127) / 128, stage = q3s::I8_TILE + cut.bt * q3s::I8_BK;
-  // K is cut until the CTAs are one a SM, or two where two fit (110 KB each), with two chunks each at least
-  const int most = 110 * 1024 / stage >= 3 ? 2 : 1;
-  int ks = 1;
-  while (ks < 8 && cut.chunks >= 4 * ks && ntiles * mtiles * ks * 2 <= most * q3s::sm_count()) ks *= 2;
-  const bool two = ntiles * mtiles * ks > q3s::sm_count();
+  const bool two = static_cast<int64_t>(ntiles) * mtiles * ks > sms && per_sm(cut.bt) == 2;
   const int mine = (cut.chunks + ks - 1) / ks;
   // a ring that also holds the partial sums of the tile
   const int least = (cut.bt * 512 + stage - 1) / stage;

@@ -30,7 +30,6 @@ struct Elem<Q3S_ELEM_F32> {
   Q3S_DEV static float one(const T* p) { return *p; }
   Q3S_DEV static T narrow(float x) { return x; }
   Q3S_DEV static uint32_t narrow2(const float* x) { return __float_as_uint(x[0]); }  // 32 bits of output
-  Q3S_DEV static T pick(const uint32_t (&o)[32], int j) { return __uint_as_float(o[j]); }
 };
 template <>
 struct Elem<Q3S_ELEM_BF16> {
@@ -55,7 +54,6 @@ struct Elem<Q3S_ELEM_BF16> {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(x[1]), "f"(x[0]));
     return r;
   }
-  Q3S_DEV static T pick(const uint32_t (&o)[32], int j) { return static_cast<T>(o[j / 2] >> (16 * (j % 2))); }
 };
 template <>
 struct Elem<Q3S_ELEM_F16> {
@@ -85,7 +83,6 @@ struct Elem<Q3S_ELEM_F16> {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(x[1]), "f"(x[0]));
     return r;
   }
-  Q3S_DEV static T pick(const uint32_t (&o)[32], int j) { return static_cast<T>(o[j / 2] >> (16 * (j % 2))); }
 };
 
 // ---- quantisation -----------------------------------------------------------
@@ -471,7 +468,7 @@ Q3S_DEV int4 ld_cluster16(uint32_t addr) {
 }
 
 // Up to a few hundred rows: the weights are the matrix instruction's M (128
-// outputs a CTA), the rows of x its N (BT, a multiple of 16), so that one pass
+// outputs a CTA), the rows of x its N (BT, a multiple of 32), so that one pass
 // over the weights serves all rows of a tile; K is cut over the KS CTAs of a
 // cluster so that all SMs read.  The partial sums (32-bit integers, exact in any
 // order) meet in distributed shared memory: CTA r of a cluster finishes every
@@ -481,7 +478,7 @@ struct I8Cut {
   int bt, stages, chunks;  // tokens of a tile, ring stages, chunks of K
   int tmem;                    // columns: a power of two >= 32
 };
-constexpr int I8C_NT = 128;
+constexpr int I8C_NT = 256;
 
 template <int ELEM, int KS>
 __global__ void __launch_bounds__(I8C_NT)
@@ -561,19 +558,14 @@ __global__ void __launch_bounds__(I8C_NT)
   const bool done = mbar_wait_bounded(&ready, 0);
   if (!done) atomicOr(&failed, 1);
   tc_fence_after();
-  // every product is complete: the ring holds the partial sums now, [token][128 outputs]
+  // every product is complete: the ring holds the partial sums now, [token][128
+  // outputs]; warp w reads TMEM lanes 32 (w % 4) .., every other 32 columns
   int* part = reinterpret_cast<int*>(smem);
-  for (int c = 0; c < cut.bt; c += 16) {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(tmem + (static_cast<uint32_t>(32 * w) << 16) + static_cast<uint32_t>(c))
-        : "memory");
+  for (int c = 32 * (w >> 2); c < cut.bt; c += 64) {
+    float v[32];
+    tmem_ld32(tmem + (static_cast<uint32_t>(32 * (w & 3)) << 16) + static_cast<uint32_t>(c), v);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) part[(c + i) * 128 + t] = static_cast<int>(r[i]);
+    for (int i = 0; i < 32; ++i) part[(c + i) * 128 + (t & 127)] = __float_as_int(v[i]);
   }
   tc_fence_before();
   cluster_arrive_release();
@@ -586,18 +578,18 @@ __global__ void __launch_bounds__(I8C_NT)
       ws[j] = n + j < a.N ? a.w_scales[n + j] : 0.0f;
       bi[j] = a.bias && n + j < a.N ? a.bias[n + j] : 0.0f;
     }
-    constexpr int T = 3;  // tokens of a warp in flight
-    for (int tok0 = rank * 4 + w; tok0 < cut.bt; tok0 += T * KS * 4) {
+    constexpr int T = KS == 8 ? 2 : 4, STEP = KS * (I8C_NT / 32);  // tokens of a warp in flight, and their distance
+    for (int tok0 = rank * (I8C_NT / 32) + w; tok0 < cut.bt && token0 + tok0 < a.M; tok0 += T * STEP) {
       int4 part_sum[T][KS];
 #pragma unroll
       for (int i = 0; i < T; ++i) {
-        const int tok = min(tok0 + i * KS * 4, cut.bt - 1);
+        const int tok = min(tok0 + i * STEP, cut.bt - 1);
 #pragma unroll
         for (int k = 0; k < KS; ++k) part_sum[i][k] = ld_cluster16(cluster_addr(smem_u32(part + tok * 128 + 4 * lane), k));
       }
 #pragma unroll
       for (int i = 0; i < T; ++i) {
-        const int tok = tok0 + i * KS * 4;
+        const int tok = tok0 + i * STEP;
         if (tok >= cut.bt || token0 + tok >= a.M) break;
         int4 sum = part_sum[i][0];
 #pragma unroll
@@ -804,25 +796,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_NT, 1)
           if (lane == 0) mbar_arrive_cluster(cluster_addr(smem_u32(&drained[b]), 0));
         }
         if (n >= a.N || row0 >= a.M) continue;
-        if (a.vec_y) {
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last store has left the buffer
-          __syncwarp();
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last store has left the buffer
+        __syncwarp();
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) =
-                make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
-          }
+        for (int q = 0; q < 8; ++q)
+          *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) =
+              make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+        if (a.vec_y) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
             tma_store_2d(&tm_y, n, row0, smem_u32(buf));
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
-        } else if (row < a.M) {
-          typename E::T* y = static_cast<typename E::T*>(a.y) + row * a.ldy + n;
+        } else {  // rows that do not start on 16 bytes: element by element, a row at a time
+          __syncwarp();
+          typename E::T* y = static_cast<typename E::T*>(a.y) + static_cast<int64_t>(row0) * a.ldy + n;
+          const int rows = min(a.M - row0, 32);
+#pragma unroll 4
+          for (int r = 0; r < rows; ++r, y += a.ldy)
 #pragma unroll
-          for (int j = 0; j < OC; ++j)
-            if (n + j < a.N) y[j] = E::pick(o, j);
+            for (int j = lane; j < OC; j += 32) {
+              const int at = j * static_cast<int>(sizeof(typename E::T));
+              if (n + j < a.N)
+                y[j] = *reinterpret_cast<const typename E::T*>(buf + r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15));
+            }
+          __syncwarp();
         }
       }
     }
