@@ -69,12 +69,12 @@ Layout layout_of(const q3s_prefix_attention_desc* d) {
   const int64_t warps = d->dim == 64 ? (l.nq == 1 ? split_warps<64, 1>() : split_warps<64, 2>())
                                      : (l.nq == 1 ? split_warps<128, 1>() : split_warps<128, 2>());
   // A CTA of the prefix kernel has a SM for itself: this kernel's CTAs that
-  // would be there start when it ends, about that many units (of a good
-  // microsecond) later.
+  // would be there start when it ends, that many units later (a unit takes 1.3
+  // us with 8-row items, 2 us with 16-row ones, and a CTA 3 us to get going).
   const int64_t busy = l.splits ? std::min<int64_t>(static_cast<int64_t>(l.pairs) * d->kv_heads * l.splits, q3s::sm_count()) : 0;
   const int64_t ctas = warps / q3s::SplitTile<64, 1>::WARPS;
   l.early = static_cast<int>(ctas - busy * (ctas / q3s::sm_count()));
-  l.lead = l.splits ? 5 + l.per_split * 3 / 2 : 0;
+  l.lead = l.splits ? (l.nq == 1 ? 8 + 2 * l.per_split : 4 + l.per_split) : 0;
   const int64_t R = 8 * l.nq;
   l.tiles0 = l.splits || d->prefix_length == 0 ? 0 : static_cast<int>((queries + R - 1) / R);
   l.ids = (l.tiles0 + queries / R + d->batch + 1) * d->kv_heads;

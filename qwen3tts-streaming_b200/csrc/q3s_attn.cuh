@@ -501,14 +501,21 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
     {
       // V^T: keys (lane & 7) + 8 (lane >> 4), 16-byte chunk + ((lane >> 3) & 1)
       const int key = (lane & 7) + ((lane >> 4) << 3), cc = (lane >> 3) & 1, x7 = key & 7;
+      constexpr int GROUP = 4 / NQ;  // dims whose products stand between the two that add to one sum
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        uint32_t f[4];
-        ldsm4t(f, va + static_cast<uint32_t>((d / 4) * Tile::SLICE + key * 128 + ((((2 * d) & 7) + cc) ^ x7) * 16));
+      for (int d0 = 0; d0 < D / 16; d0 += GROUP) {
+        uint32_t f[GROUP][4];
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) mma16816<BF16>(o[d][q], f, ph[q][0], ph[q][1]);
+        for (int d = 0; d < GROUP; ++d)
+          ldsm4t(f[d], va + static_cast<uint32_t>(((d0 + d) / 4) * Tile::SLICE + key * 128 + ((((2 * (d0 + d)) & 7) + cc) ^ x7) * 16));
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) mma16816<BF16>(o[d][q], f, pl[q][0], pl[q][1]);
+        for (int d = 0; d < GROUP; ++d)
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) mma16816<BF16>(o[d0 + d][q], f[d], ph[q][0], ph[q][1]);
+#pragma unroll
+        for (int d = 0; d < GROUP; ++d)
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) mma16816<BF16>(o[d0 + d][q], f[d], pl[q][0], pl[q][1]);
       }
     }
     __syncwarp();  // every lane has read the stage

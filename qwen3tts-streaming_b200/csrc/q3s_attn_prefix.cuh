@@ -212,23 +212,57 @@ __global__ void __launch_bounds__(PX_NT, 1)
   const int token0 = pair * 2 * p.per_tile;
   const int tiles = token0 + p.per_tile < a.T ? 2 : 1;  // a last pair may have one tile
 
-  if (t == 0) {
-    mbar_init(q_full, 1);
-    mbar_init(v_clean, 1);
-    for (int s = 0; s < PX_STAGES; ++s) {
-      mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
-      mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], 1);
+  // ---- copies: lane l copies box l of a step (a page, or 128 tokens of one) ----
+  const int rows = min(a.bs, PX_KEYS), pages = PX_KEYS / rows;
+  auto block_of = [&](int j) {  // lane's block of step j; past the cache (it reads as zeros) where there is none
+    const int key = (step0 + j) * PX_KEYS + lane * rows;
+    return j < steps && lane < pages && key < a.L ? a.prefix_blocks[key >> a.bs_log2] : a.blocks;
+  };
+  int bad = 0;
+  auto copy = [&](const CUtensorMap* map, unsigned char* ring, uint64_t* full, int j, int block) {
+    const bool inside = static_cast<unsigned>(block) < static_cast<unsigned>(a.blocks);
+    bad |= !inside && block != a.blocks;
+    const int id = inside ? block : a.blocks, place = ((step0 + j) * PX_KEYS + lane * rows) & (a.bs - 1), s = j % PX_STAGES;
+    if (lane == 0) mbar_expect_tx(&full[s], Tile::KV_BYTES);
+    __syncwarp();
+    if (lane < pages)
+      for (int x = 0; x < HALVES; ++x)
+        tma_load_slice(smem_u32(ring + s * Tile::KV_BYTES + x * PX_KEYS * 128 + lane * rows * 128), map, x, place, h, id, &full[s]);
+  };
+  if (w == 8) {  // the first copies are on their way while TMEM is allocated
+    if (lane < 3) prefetch_map(lane == 0 ? &tm_q : lane == 1 ? &tm_k : &tm_v);
+    int block[PX_STAGES];
+#pragma unroll
+    for (int j = 0; j < PX_STAGES; ++j) block[j] = block_of(j);
+    if (lane == 0) {
+      mbar_init(q_full, 1);
+      mbar_init(v_clean, 1);
+      for (int s = 0; s < PX_STAGES; ++s) {
+        mbar_init(&k_full[s], 1);
+        mbar_init(&k_empty[s], 1);
+        mbar_init(&v_full[s], 1);
+        mbar_init(&v_empty[s], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&s_full[i], 1);
+        mbar_init(&p_half[i], 128);
+        mbar_init(&p_full[i], 128);
+        mbar_init(&o_done[i], 1);
+      }
+      *failed = 0;
+      fence_mbar_init();
+      mbar_expect_tx(q_full, static_cast<uint32_t>(tiles * HALVES * p.per_tile * a.G * 128));
+      for (int i = 0; i < tiles; ++i)
+        for (int x = 0; x < HALVES; ++x)
+          tma_load_3d(smem_u32(s_q + i * Tile::Q_BYTES + x * PX_M * 128), &tm_q, 64 * x, h * a.G, token0 + i * p.per_tile, q_full);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_half[i], 128);
-      mbar_init(&p_full[i], 128);
-      mbar_init(&o_done[i], 1);
-    }
-    *failed = 0;
-    fence_mbar_init();
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < PX_STAGES; ++j)
+      if (j < steps) {
+        copy(&tm_k, s_k, k_full, j, block[j]);
+        copy(&tm_v, s_v, v_full, j, block[j]);
+      }
   }
   if (w == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512)
@@ -250,37 +284,15 @@ __global__ void __launch_bounds__(PX_NT, 1)
   };
 
   if (w == 8) {
-    if (lane < 3) prefetch_map(lane == 0 ? &tm_q : lane == 1 ? &tm_k : &tm_v);
-    // ---- copies: lane l copies box l of a step (a page, or 128 tokens of one) ------------------------------
-    const int rows = min(a.bs, PX_KEYS), pages = PX_KEYS / rows;
-    if (lane == 0) {
-      mbar_expect_tx(q_full, static_cast<uint32_t>(tiles * HALVES * p.per_tile * a.G * 128));
-      for (int i = 0; i < tiles; ++i)
-        for (int x = 0; x < HALVES; ++x)
-          tma_load_3d(smem_u32(s_q + i * Tile::Q_BYTES + x * PX_M * 128), &tm_q, 64 * x, h * a.G, token0 + i * p.per_tile, q_full);
-    }
-    auto block_of = [&](int j) {  // lane's block of step j; past the cache (it reads as zeros) where there is none
-      const int key = (step0 + j) * PX_KEYS + lane * rows;
-      return lane < pages && key < a.L ? a.prefix_blocks[key >> a.bs_log2] : a.blocks;
-    };
-    int next = block_of(0), j = 0, bad = 0;
+    int next = block_of(PX_STAGES), j = min(PX_STAGES, steps);
     for (; j < steps; ++j) {
+      const int block = next;
+      next = block_of(j + 1);
       const int s = j % PX_STAGES;
-      const bool inside = static_cast<unsigned>(next) < static_cast<unsigned>(a.blocks);
-      bad |= !inside && next != a.blocks;
-      const int id = inside ? next : a.blocks, place = ((step0 + j) * PX_KEYS + lane * rows) & (a.bs - 1);
-      if (j + 1 < steps) next = block_of(j + 1);
-      auto copy = [&](const CUtensorMap* map, unsigned char* ring, uint64_t* full, uint64_t* empty) {
-        if (j >= PX_STAGES && !__all_sync(FULL, wait(&empty[s], ((j / PX_STAGES) - 1) & 1))) return false;
-        if (lane == 0) mbar_expect_tx(&full[s], Tile::KV_BYTES);
-        __syncwarp();
-        if (lane < pages)
-          for (int x = 0; x < HALVES; ++x)
-            tma_load_slice(smem_u32(ring + s * Tile::KV_BYTES + x * PX_KEYS * 128 + lane * rows * 128), map, x, place, h, id, &full[s]);
-        return true;
-      };
-      if (!copy(&tm_k, s_k, k_full, k_empty)) break;
-      if (!copy(&tm_v, s_v, v_full, v_empty)) break;
+      if (!__all_sync(FULL, wait(&k_empty[s], ((j / PX_STAGES) - 1) & 1))) break;
+      copy(&tm_k, s_k, k_full, j, block);
+      if (!__all_sync(FULL, wait(&v_empty[s], ((j / PX_STAGES) - 1) & 1))) break;
+      copy(&tm_v, s_v, v_full, j, block);
     }
     if (bad && a.error_word) atomicOr(a.error_word, Q3S_DECERR_BLOCK_ID);
     const int valid = a.L - (step0 + steps - 1) * PX_KEYS;  // keys of the last step
@@ -435,37 +447,33 @@ __global__ void __launch_bounds__(PX_NT, 1)
       if (ok) ok = __all_sync(FULL, wait(&o_done[i], (steps - 1) & 1));
       if (ok) {
         tc_fence_after();
-        // O through shared memory, so that a row's stores are whole lines: tile
-        // 0's rows in the K ring, whose last readers came before this tile's last
-        // product, tile 1's in the V ring; a warp stages and stores its own 32
-        // rows (16-byte chunk c of row r at c ^ (r & 7))
-        unsigned char* stage = (i == 0 ? s_k : s_v) + (w & 3) * (32 * D * 4);
+        // O through shared memory: a thread writes its row there (16 bytes of
+        // padding a row keep that free of bank conflicts) and copies it out in one
+        // piece.  Tile 0's rows take the place of tile 1's queries and of K, whose
+        // last readers came before this tile's last product; tile 1's what follows.
+        constexpr int PITCH = D * 4 + 16;
+        static_assert(2 * PX_M * PITCH + 1024 <= Tile::Q_BYTES + 2 * PX_STAGES * Tile::KV_BYTES, "room for both tiles");
+        static_assert(PX_M * PITCH <= Tile::Q_BYTES + PX_STAGES * Tile::KV_BYTES, "tile 0 leaves V alone");
+        unsigned char* stage = s_q + Tile::Q_BYTES + i * PX_M * PITCH + row * PITCH;
 #pragma unroll 1
         for (int k = 0; k < D / 32; ++k) {
           float v[32];
           tmem_ld32(to + static_cast<uint32_t>(32 * k), v);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            *reinterpret_cast<float4*>(stage + lane * D * 4 + (((8 * k + e) ^ (lane & 7)) << 4)) =
-                make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+            *reinterpret_cast<float4*>(stage + (8 * k + e) * 16) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
         }
-        __syncwarp();
-        auto at = [&](int r) {  // query row r of the tile, in the part's rows (-1: there is none)
-          const int token = token0 + i * p.per_tile + r / a.G;
-          return r < p.per_tile * a.G && token < a.T
-                     ? (static_cast<int64_t>(split) * a.T + token) * a.Hq + h * a.G + r % a.G
-                     : static_cast<int64_t>(-1);
-        };
-        const int64_t mine = at(row);
-        if (mine >= 0) a.pre_ml[mine] = make_float2(m, l);
-        constexpr int LANES = D / 4, ROWS = 32 / LANES;  // lanes of a row, rows at a time
-#pragma unroll 4
-        for (int r0 = 0; r0 < 32; r0 += ROWS) {
-          const int r = r0 + lane / LANES, c = lane % LANES;
-          const int64_t to_row = __shfl_sync(FULL, mine, r);
-          const float4 v = *reinterpret_cast<const float4*>(stage + r * D * 4 + ((c ^ (r & 7)) << 4));
-          if (to_row >= 0) *reinterpret_cast<float4*>(a.pre_o + to_row * D + c * 4) = v;
+        const int token = token0 + i * p.per_tile + row / a.G;
+        if (row < p.per_tile * a.G && token < a.T) {  // there is such a query row
+          const int64_t at = (static_cast<int64_t>(split) * a.T + token) * a.Hq + h * a.G + row % a.G;
+          fence_proxy_async_smem();
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.pre_o + at * D), "r"(smem_u32(stage)),
+                       "r"(D * 4)
+                       : "memory");
+          a.pre_ml[at] = make_float2(m, l);
         }
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       }
     }
   }

@@ -63,8 +63,8 @@ def cache_tables(context_lengths: torch.Tensor, new_lengths: torch.Tensor, block
     gets slot -1 for its tokens; ``error_word`` says why.  ``max_tokens`` sizes
     the slot map: entries past the last token are -1 (positions 0), so a
     captured graph can keep one size."""
-    return CacheTables(*_op("cache_tables")(context_lengths, new_lengths, block_table, free_blocks, free_state,
-                                            block_size, max_tokens, released))
+    return tuple.__new__(CacheTables, _op("cache_tables")(context_lengths, new_lengths, block_table, free_blocks,
+                                                          free_state, block_size, max_tokens, released))
 
 
 def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
