@@ -169,6 +169,19 @@ cudaError_t launch_split(const q3s::AttnArgs& a, bool beside, cudaStream_t st) {
   return q3s::launch_maybe_pdl(split, dim3(q3s::sm_count() * Tile::PER_SM), dim3(Tile::NT), Tile::SMEM, st, beside, tk, tv, a);
 }
 
+// A warp a row.  It requests four parts at a time; eight where an item is cut
+// into more (few items over all the warps, or many parts of the prefix), which
+// takes more registers and so fewer warps at once (61 rows with some 20 parts:
+// 13.7 us with four against .. us; 256 rows with six: the same).
+template <int D, bool BF16, int NQ>
+cudaError_t launch_join(const q3s::AttnArgs& a, const Layout& l, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(a.T) * a.Hq + 3) / 4));
+  const int64_t items = static_cast<int64_t>(std::max(std::min(a.B, a.T), 1)) * a.H;
+  const bool many = l.splits > 8 || split_warps<D, NQ>() / items > 6;
+  return many ? q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, NQ, 8>, grid, dim3(128), 0, st, true, a)
+              : q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, NQ, 4>, grid, dim3(128), 0, st, true, a);
+}
+
 template <int D, bool BF16>
 cudaError_t launch_prefix(const q3s::AttnArgs& a, const Layout& l, cudaStream_t st) {
   auto prefix = q3s::attn_prefix_kernel<D, BF16>;
@@ -193,9 +206,7 @@ cudaError_t launch(const q3s::AttnArgs& a, const Layout& l, cudaStream_t st) {
   // beside the prefix kernel where there is one: neither reads what the other writes
   e = l.nq == 1 ? launch_split<D, BF16, 1>(a, l.splits > 0, st) : launch_split<D, BF16, 2>(a, l.splits > 0, st);
   if (e != cudaSuccess) return e;
-  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(a.T) * a.Hq + 3) / 4));  // a warp a row
-  return l.nq == 1 ? q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, 1>, grid, dim3(128), 0, st, true, a)
-                   : q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, 2>, grid, dim3(128), 0, st, true, a);
+  return l.nq == 1 ? launch_join<D, BF16, 1>(a, l, st) : launch_join<D, BF16, 2>(a, l, st);
 }
 
 }  // namespace

@@ -564,15 +564,13 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
 }
 
 // Joins the parts of each query row (m, l, o as above) and writes out and lse.
-// One warp a row of [T * q_heads]; a lane holds D / 32 of its values and, for up
-// to 32 parts at a time, one part's m and l.  A token's batch row is found in
+// One warp a row of [T * q_heads]; a lane holds D / 32 of its values.  A token's batch row is found in
 // query_offsets by bisection, before the grid waits for the parts; tokens past
-// the last row see nothing.  Bound by latency: the record of the row's own
-// parts, then their sums; the prefix parts' sums are requested before the record
-// has arrived.
-template <int D, bool BF16, int NQ>
-__global__ void __launch_bounds__(128, 5) attn_join_kernel(const AttnArgs a) {
-  constexpr int E = D / 32, R = 8 * NQ, AHEAD = 8;
+// the last row see nothing.  Bound by latency, of the record of the row's own
+// parts and of the sums, and by fetching its own instructions: kept short.
+template <int D, bool BF16, int NQ, int AHEAD>
+__global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
+  constexpr int E = D / 32, R = 8 * NQ;
   const int lane = static_cast<int>(threadIdx.x) & 31;
   const int64_t out_row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   const int token = static_cast<int>(out_row / a.Hq), head = static_cast<int>(out_row - static_cast<int64_t>(token) * a.Hq);
@@ -595,102 +593,58 @@ __global__ void __launch_bounds__(128, 5) attn_join_kernel(const AttnArgs a) {
   if (token >= a.T) return;
   {
     const int row = live ? (token - x.t0) * a.G + gq : 0;  // of the batch row's n * G
-    // two runs of parts, the prefix's and the row's own: part i of a run is
-    // query row `at + i * step` of `o` and `ml`
-    const float* o0 = a.part_o;
-    const float2* ml0 = a.part_ml;
-    int64_t at0 = 0, step0 = R, at1 = 0;
-    int n0 = 0, n1 = 0;
     int2 own = make_int2(0, 0);
     if (x.units) {
       const int64_t id = attn_first_id<R>(a, b + 1, x) + static_cast<int64_t>(h) * x.tiles + row / R;
       if (id < a.ids) own = a.items[id];
     }
-    if (live && a.tiles0) {
-      const int r = token * a.G + gq;
-      const int2 it = a.items[static_cast<int64_t>(h) * a.tiles0 + r / R];
-      at0 = static_cast<int64_t>(it.x) * R + r % R;
-      n0 = it.x >= 0 && it.y > 0 && static_cast<int64_t>(it.x) + it.y <= a.slots ? it.y : 0;
-    } else if (live && a.splits) {
-      o0 = a.pre_o;
-      ml0 = a.pre_ml;
-      at0 = out_row;
-      step0 = static_cast<int64_t>(a.T) * a.Hq;
-      n0 = a.splits;
-    }
-    float y[AHEAD][E], z[2][E];  // sums of the first parts of each run
-    auto fetch = [&](const float* src, float (&v)[E]) {
-      if constexpr (E == 4) {
-        const float4 f = *reinterpret_cast<const float4*>(src);
-        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-      } else {
-        const float2 f = *reinterpret_cast<const float2*>(src);
-        v[0] = f.x, v[1] = f.y;
-      }
-    };
-    const float* src0 = o0 + at0 * D + lane * E;
-#pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
-      if (j < n0) fetch(src0 + j * step0 * D, y[j]);
-    n1 = own.x >= 0 && own.y > 0 && static_cast<int64_t>(own.x) + own.y <= a.slots ? own.y : 0;
-    at1 = static_cast<int64_t>(own.x) * R + row % R;
-    const float* src1 = a.part_o + at1 * D + lane * E;
-    const int parts = n0 + n1;
     float acc[E], m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-      const int k = min(parts - i0, 32), k0 = min(max(n0 - i0, 0), k);  // parts of this round, and of the prefix's run
-      float2 ml = make_float2(-INFINITY, 0.0f);
-      if (lane < k) {
-        const int i = i0 + lane;
-        ml = i < n0 ? ml0[at0 + i * step0] : a.part_ml[at1 + (i - n0) * static_cast<int64_t>(R)];
-      }
-      if (i0 == 0) {
+    // n parts: query row `at + i * step` of `o` and `ml`, in order, AHEAD of them requested at a time
+    auto join = [&](const float* o, const float2* ml, int64_t at, int64_t step, int n) {
+      const float* src = o + at * D + lane * E;
+      const float2* sml = ml + at;
+      for (int i = 0; i < n; i += AHEAD) {
+        float y[AHEAD][E];
+        float2 p[AHEAD];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (j < n1 && n0 + j < k) fetch(src1 + j * (R * D), z[j]);
-      }
-      float top = ml.x;
-#pragma unroll
-      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, d));
-      const float nm = fmaxf(m, top);
-      const float base = nm == -INFINITY ? 0.0f : nm;
-      const float c = ex2(m - base), wt = ex2(ml.x - base);
-      m = nm;
-      float lw = wt * ml.y;
-#pragma unroll
-      for (int d = 16; d; d >>= 1) lw += __shfl_xor_sync(FULL, lw, d);
-      l = l * c + lw;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] *= c;
-      auto add = [&](const float (&v)[E], int i) {
-        const float wi = __shfl_sync(FULL, wt, i);
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += wi * v[e];
-      };
-      auto run = [&](const float* src, int64_t stride, int i1, int i2) {  // parts i1 .. i2 - 1 of the round
-        float v[E];
-#pragma unroll 4
-        for (int i = i1; i < i2; ++i, src += stride) {
-          fetch(src, v);
-          add(v, i);
+        for (int k = 0; k < AHEAD; ++k) {
+          p[k] = make_float2(-INFINITY, 0.0f);
+          if (i + k < n) {
+            p[k] = *sml;
+            if constexpr (E == 4) {
+              const float4 f = *reinterpret_cast<const float4*>(src);
+              y[k][0] = f.x, y[k][1] = f.y, y[k][2] = f.z, y[k][3] = f.w;
+            } else {
+              const float2 f = *reinterpret_cast<const float2*>(src);
+              y[k][0] = f.x, y[k][1] = f.y;
+            }
+          }
+          src += step * D;
+          sml += step;
         }
-      };
-      if (i0 == 0) {
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j)
-          if (j < k0) add(y[j], j);
+        for (int k = 0; k < AHEAD; ++k) {
+          if (i + k >= n) break;
+          const float nm = fmaxf(m, p[k].x), base = nm == -INFINITY ? 0.0f : nm;
+          const float c = ex2(m - base), wt = ex2(p[k].x - base);
+          m = nm;
+          l = l * c + wt * p[k].y;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (k0 + j < k) add(z[j], k0 + j);
-        run(src0 + AHEAD * step0 * D, step0 * D, AHEAD, k0);
-        run(src1 + 2 * (R * D), R * D, k0 + 2, k);
-      } else {
-        run(src0 + i0 * step0 * D, step0 * D, 0, k0);
-        run(src1 + static_cast<int64_t>(i0 + k0 - n0) * (R * D), R * D, k0, k);
+          for (int e = 0; e < E; ++e) acc[e] = acc[e] * c + wt * y[k][e];
+        }
       }
+    };
+    auto parts = [&](int2 it) { return it.x >= 0 && it.y > 0 && static_cast<int64_t>(it.x) + it.y <= a.slots ? it.y : 0; };
+    if (live && a.tiles0) {
+      const int r = token * a.G + gq;
+      const int2 it = a.items[static_cast<int64_t>(h) * a.tiles0 + r / R];
+      join(a.part_o, a.part_ml, static_cast<int64_t>(it.x) * R + r % R, R, parts(it));
+    } else if (live && a.splits) {
+      join(a.pre_o, a.pre_ml, out_row, static_cast<int64_t>(a.T) * a.Hq, a.splits);
     }
+    join(a.part_o, a.part_ml, static_cast<int64_t>(own.x) * R + row % R, R, parts(own));
     const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;  // a NaN stays one
     uint16_t* dst = static_cast<uint16_t*>(a.out) + token * a.ot + head * a.oh + lane * E;
     if constexpr (E == 4)
