@@ -74,7 +74,7 @@ Layout layout_of(const q3s_prefix_attention_desc* d) {
   const int64_t busy = l.splits ? std::min<int64_t>(static_cast<int64_t>(l.pairs) * d->kv_heads * l.splits, q3s::sm_count()) : 0;
   const int64_t ctas = warps / q3s::SplitTile<64, 1>::WARPS;
   l.early = static_cast<int>(ctas - busy * (ctas / q3s::sm_count()));
-  l.lead = l.splits ? (l.nq == 1 ? 8 + 2 * l.per_split : 4 + l.per_split) : 0;
+  l.lead = l.splits ? (l.nq == 1 ? 8 + l.per_split * 17 / 10 : 4 + l.per_split) : 0;
   const int64_t R = 8 * l.nq;
   l.tiles0 = l.splits || d->prefix_length == 0 ? 0 : static_cast<int>((queries + R - 1) / R);
   l.ids = (l.tiles0 + queries / R + d->batch + 1) * d->kv_heads;
@@ -169,17 +169,16 @@ cudaError_t launch_split(const q3s::AttnArgs& a, bool beside, cudaStream_t st) {
   return q3s::launch_maybe_pdl(split, dim3(q3s::sm_count() * Tile::PER_SM), dim3(Tile::NT), Tile::SMEM, st, beside, tk, tv, a);
 }
 
-// A warp a row.  It requests four parts at a time; eight where an item is cut
-// into more (few items over all the warps, or many parts of the prefix), which
-// takes more registers and so fewer warps at once (61 rows with some 20 parts:
-// 13.7 us with four against .. us; 256 rows with six: the same).
+// A warp a row, or four where an item is cut into many parts (few items over
+// all the warps, or many parts of the prefix).
 template <int D, bool BF16, int NQ>
 cudaError_t launch_join(const q3s::AttnArgs& a, const Layout& l, cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(a.T) * a.Hq + 3) / 4));
+  const int64_t rows = static_cast<int64_t>(a.T) * a.Hq;
   const int64_t items = static_cast<int64_t>(std::max(std::min(a.B, a.T), 1)) * a.H;
-  const bool many = l.splits > 8 || split_warps<D, NQ>() / items > 6;
-  return many ? q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, NQ, 8>, grid, dim3(128), 0, st, true, a)
-              : q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, NQ, 4>, grid, dim3(128), 0, st, true, a);
+  return l.splits > 12 || split_warps<D, NQ>() / items > 6
+             ? q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, NQ, true>, dim3(static_cast<unsigned>(rows)), dim3(128), 0, st, true, a)
+             : q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, NQ, false>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0,
+                                     st, true, a);
 }
 
 template <int D, bool BF16>

@@ -568,11 +568,14 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
 // query_offsets by bisection, before the grid waits for the parts; tokens past
 // the last row see nothing.  Bound by latency, of the record of the row's own
 // parts and of the sums, and by fetching its own instructions: kept short.
-template <int D, bool BF16, int NQ, int AHEAD>
+//
+// TEAM: the four warps of a CTA share a row, each every fourth part, and meet in
+// shared memory.
+template <int D, bool BF16, int NQ, bool TEAM>
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
-  constexpr int E = D / 32, R = 8 * NQ;
-  const int lane = static_cast<int>(threadIdx.x) & 31;
-  const int64_t out_row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  constexpr int E = D / 32, R = 8 * NQ, AHEAD = 4, STRIDE = TEAM ? 4 : 1;
+  const int lane = static_cast<int>(threadIdx.x) & 31, w = static_cast<int>(threadIdx.x) >> 5;
+  const int64_t out_row = TEAM ? static_cast<int64_t>(blockIdx.x) : static_cast<int64_t>(blockIdx.x) * 4 + w;
   const int token = static_cast<int>(out_row / a.Hq), head = static_cast<int>(out_row - static_cast<int64_t>(token) * a.Hq);
   const int h = head / a.G, gq = head - h * a.G;
   AttnRow x;
@@ -603,6 +606,11 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
     // n parts: query row `at + i * step` of `o` and `ml`, in order, AHEAD of them requested at a time
     auto join = [&](const float* o, const float2* ml, int64_t at, int64_t step, int n) {
+      if constexpr (TEAM) {  // this warp's
+        at += w * step;
+        step *= STRIDE;
+        n = (n - w + STRIDE - 1) / STRIDE;
+      }
       const float* src = o + at * D + lane * E;
       const float2* sml = ml + at;
       for (int i = 0; i < n; i += AHEAD) {
@@ -645,6 +653,25 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
       join(a.pre_o, a.pre_ml, out_row, static_cast<int64_t>(a.T) * a.Hq, a.splits);
     }
     join(a.part_o, a.part_ml, static_cast<int64_t>(own.x) * R + row % R, R, parts(own));
+    if constexpr (TEAM) {
+      __shared__ float s_acc[3][32][E + 1], s_ml[3][2];
+      if (w) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) s_acc[w - 1][lane][e] = acc[e];
+        if (lane == 0) s_ml[w - 1][0] = m, s_ml[w - 1][1] = l;
+      }
+      __syncthreads();
+      if (w) return;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        const float nm = fmaxf(m, s_ml[k][0]), base = nm == -INFINITY ? 0.0f : nm;
+        const float c = ex2(m - base), wt = ex2(s_ml[k][0] - base);
+        m = nm;
+        l = l * c + wt * s_ml[k][1];
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = acc[e] * c + wt * s_acc[k][lane][e];
+      }
+    }
     const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;  // a NaN stays one
     uint16_t* dst = static_cast<uint16_t*>(a.out) + token * a.ot + head * a.oh + lane * E;
     if constexpr (E == 4)
