@@ -158,7 +158,7 @@ bool cache_maps(const q3s::AttnArgs& a, int dim, bool bf16, int tokens, int slic
 }
 
 template <int D, bool BF16, int NQ>
-cudaError_t launch_split(const q3s::AttnArgs& a, bool beside, cudaStream_t st) {
+cudaError_t launch_split(const q3s::AttnArgs& a, cudaStream_t st) {
   using Tile = q3s::SplitTile<D, NQ>;
   auto split = q3s::attn_split_kernel<D, BF16, NQ>;
   static std::atomic<uint64_t> done{0};
@@ -166,7 +166,7 @@ cudaError_t launch_split(const q3s::AttnArgs& a, bool beside, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   CUtensorMap tk, tv;
   if (!cache_maps(a, D, BF16, q3s::AT_KEYS, D / 64, &tk, &tv)) return cudaErrorInvalidValue;
-  return q3s::launch_maybe_pdl(split, dim3(q3s::sm_count() * Tile::PER_SM), dim3(Tile::NT), Tile::SMEM, st, beside, tk, tv, a);
+  return q3s::launch_maybe_pdl(split, dim3(q3s::sm_count() * Tile::PER_SM), dim3(Tile::NT), Tile::SMEM, st, true, tk, tv, a);
 }
 
 // A warp a row, or four where an item is cut into many parts (few items over
@@ -195,7 +195,7 @@ cudaError_t launch_prefix(const q3s::AttnArgs& a, const Layout& l, cudaStream_t 
   p.per_tile = l.per_tile;
   p.steps = l.steps;
   p.per_split = l.per_split;
-  return q3s::launch_maybe_pdl(prefix, dim3(l.pairs, a.H, l.splits), dim3(q3s::PX_NT), smem, st, false, tq, tk, tv, p);
+  return q3s::launch_maybe_pdl(prefix, dim3(l.pairs, a.H, l.splits), dim3(q3s::PX_NT), smem, st, true, tq, tk, tv, p);
 }
 
 template <int D, bool BF16>
@@ -203,7 +203,7 @@ cudaError_t launch(const q3s::AttnArgs& a, const Layout& l, cudaStream_t st) {
   cudaError_t e = l.splits ? launch_prefix<D, BF16>(a, l, st) : cudaSuccess;
   if (e != cudaSuccess) return e;
   // beside the prefix kernel where there is one: neither reads what the other writes
-  e = l.nq == 1 ? launch_split<D, BF16, 1>(a, l.splits > 0, st) : launch_split<D, BF16, 2>(a, l.splits > 0, st);
+  e = l.nq == 1 ? launch_split<D, BF16, 1>(a, st) : launch_split<D, BF16, 2>(a, st);
   if (e != cudaSuccess) return e;
   return l.nq == 1 ? launch_join<D, BF16, 1>(a, l, st) : launch_join<D, BF16, 2>(a, l, st);
 }

@@ -18,6 +18,7 @@
 #include "q3s_decode.h"
 #include "q3s_device.cuh"
 #include "q3s_head.cuh"
+#include "q3s_pdl.cuh"
 
 namespace q3s {
 
@@ -263,7 +264,6 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
   __shared__ AttnRow s_rows[AT_NT];  // the rows, where there are no more than threads
   __shared__ __align__(8) uint64_t s_full[BARS], s_empty[BARS];
   const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
-  asm volatile("griddepcontrol.launch_dependents;");
   if (t == 0) {
     prefetch_map(&tm_k);
     prefetch_map(&tm_v);
@@ -273,6 +273,8 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
     }
     fence_mbar_init();
   }
+  if (!a.splits) grid_wait();  // else the prefix kernel, launched before this one, has waited for what both read
+  grid_release();
 
   // ---- the work list: thread t sums rows [t * per, (t + 1) * per) ------------
   const int rows = a.B + 1, per = (rows + AT_NT - 1) / AT_NT;
@@ -375,7 +377,7 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
     for (int i = max(0, fetched - AT_STAGES); i < fetched; ++i)
       (void)mbar_wait_bounded(&full[i % AT_STAGES], (i / AT_STAGES) & 1);
     __syncwarp();
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // as below
+    grid_wait();  // as below
     return;
   }
 
@@ -560,7 +562,7 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
   if (!ok && lane == 0 && a.error_word) atomicOr(a.error_word, Q3S_DECERR_WAIT);  // a copy did not arrive
   // this grid starts beside the prefix kernel's: it does not end before that
   // one, so that the join, which waits for this grid, has both
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  grid_wait();
 }
 
 // Joins the parts of each query row (m, l, o as above) and writes out and lse.
@@ -592,7 +594,8 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
     live = token >= x.t0 && token < x.t0 + x.n;
     if (!live) x.units = 0;
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  grid_wait();
+  grid_release();
   if (token >= a.T) return;
   {
     const int row = live ? (token - x.t0) * a.G + gq : 0;  // of the batch row's n * G

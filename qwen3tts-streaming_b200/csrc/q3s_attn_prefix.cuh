@@ -205,8 +205,6 @@ __global__ void __launch_bounds__(PX_NT, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_clean + 1);
   int* failed = reinterpret_cast<int*>(tmem_slot + 1);
   const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
-  asm volatile("griddepcontrol.launch_dependents;");
-
   const int pair = static_cast<int>(blockIdx.x), h = static_cast<int>(blockIdx.y), split = static_cast<int>(blockIdx.z);
   const int step0 = split * p.per_split, steps = min(p.per_split, p.steps - step0);  // >= 1
   const int token0 = pair * 2 * p.per_tile;
@@ -229,6 +227,8 @@ __global__ void __launch_bounds__(PX_NT, 1)
       for (int x = 0; x < HALVES; ++x)
         tma_load_slice(smem_u32(ring + s * Tile::KV_BYTES + x * PX_KEYS * 128 + lane * rows * 128), map, x, place, h, id, &full[s]);
   };
+  grid_wait();
+  grid_release();  // the key-split kernel
   if (w == 8) {  // the first copies are on their way while TMEM is allocated
     if (lane < 3) prefetch_map(lane == 0 ? &tm_q : lane == 1 ? &tm_k : &tm_v);
     int block[PX_STAGES];

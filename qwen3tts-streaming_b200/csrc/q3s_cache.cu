@@ -9,6 +9,7 @@
 #include "q3s_args.cuh"
 #include "q3s_decode.h"
 #include "q3s_device.cuh"
+#include "q3s_pdl.cuh"
 
 namespace q3s {
 
@@ -64,6 +65,8 @@ __global__ void __launch_bounds__(NT) cache_tables_kernel(const TablesArgs a) {
   const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
   const int cta = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
   const int chunk = (a.max_tokens + ctas - 1) / ctas;
+  grid_wait();
+  grid_release();
   const uint32_t tok0 = static_cast<uint32_t>(min(static_cast<int64_t>(cta) * chunk, static_cast<int64_t>(a.max_tokens)));
   const uint32_t tok1 = min(tok0 + static_cast<uint32_t>(chunk), static_cast<uint32_t>(a.max_tokens));
   const int head = min(max(a.free_state[0], 0), a.ring - 1);
@@ -239,6 +242,8 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
   const int t = static_cast<int>(threadIdx.x), per = max(256 / a.units, 1);  // tokens of a group
   const int row = t / a.units;
   const int64_t token0 = static_cast<int64_t>(blockIdx.x) * per * U + row, limit = static_cast<int64_t>(a.blocks) * a.bs;
+  grid_wait();
+  grid_release();
   if (row >= per) return;
   for (int part = static_cast<int>(blockIdx.y); part < 2 * a.H; part += static_cast<int>(gridDim.y)) {
     const bool value = part >= a.H;
@@ -280,10 +285,8 @@ cudaError_t launch_append(const AppendArgs& a, cudaStream_t st) {
   auto tiles = [&](int u) { return static_cast<unsigned>((static_cast<int64_t>(a.T) + static_cast<int64_t>(per) * u - 1) / (static_cast<int64_t>(per) * u)); };
   // four groups a CTA once that leaves CTAs for every SM; below, one, for more of them
   if (static_cast<int64_t>(tiles(4)) * parts >= 4 * sm_count())
-    cache_append_kernel<UNIT, 4><<<dim3(tiles(4), parts), 256, 0, st>>>(a);
-  else
-    cache_append_kernel<UNIT, 1><<<dim3(tiles(1), parts), 256, 0, st>>>(a);
-  return cudaGetLastError();
+    return launch_maybe_pdl(cache_append_kernel<UNIT, 4>, dim3(tiles(4), parts), dim3(256), 0, st, true, a);
+  return launch_maybe_pdl(cache_append_kernel<UNIT, 1>, dim3(tiles(1), parts), dim3(256), 0, st, true, a);
 }
 
 }  // namespace q3s
@@ -340,13 +343,11 @@ extern "C" q3s_status q3s_cache_tables(const q3s_cache_tables_desc* d, void* str
   auto ctas = [&](int nt) {
     return std::max(1, std::min(sms, std::max(static_cast<int>((static_cast<int64_t>(a.max_tokens) + nt - 1) / nt), (a.B + 31) / 32)));
   };
-  if (a.B <= 128 && a.max_tokens <= 1024)
-    q3s::cache_tables_kernel<128, 1><<<ctas(128), 128, 0, st>>>(a);
-  else if (a.B <= 1024)
-    q3s::cache_tables_kernel<1024, 1><<<ctas(1024), 1024, 0, st>>>(a);
-  else
-    q3s::cache_tables_kernel<1024, 2><<<ctas(1024), 1024, 0, st>>>(a);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e =
+      a.B <= 128 && a.max_tokens <= 1024
+          ? q3s::launch_maybe_pdl(q3s::cache_tables_kernel<128, 1>, dim3(ctas(128)), dim3(128), 0, st, true, a)
+      : a.B <= 1024 ? q3s::launch_maybe_pdl(q3s::cache_tables_kernel<1024, 1>, dim3(ctas(1024)), dim3(1024), 0, st, true, a)
+                    : q3s::launch_maybe_pdl(q3s::cache_tables_kernel<1024, 2>, dim3(ctas(1024)), dim3(1024), 0, st, true, a);
   if (e != cudaSuccess) return report(Q3S_ERR_CUDA, "q3s_cache_tables: launch failed: %s", cudaGetErrorString(e));
   return report(Q3S_OK, "");
 }

@@ -30,12 +30,10 @@ template <int ELEM>
 cudaError_t launch_quantize(const q3s::QuantArgs& a, bool vec, cudaStream_t st) {
   // a warp a row once there are warps for every SM's quarter; below that a CTA a row has the shorter chain
   if (vec && a.M >= 4 * q3s::sm_count() && a.K <= 32 * q3s::QW_KEEP * q3s::Elem<ELEM>::N)
-    q3s::quantize_warps_kernel<ELEM><<<(a.M + q3s::QW_WARPS - 1) / q3s::QW_WARPS, q3s::QW_WARPS * 32, 0, st>>>(a);
-  else if (vec)
-    q3s::quantize_rows_kernel<ELEM, true><<<a.M, 128, 0, st>>>(a);
-  else
-    q3s::quantize_rows_kernel<ELEM, false><<<a.M, 128, 0, st>>>(a);
-  return cudaGetLastError();
+    return q3s::launch_maybe_pdl(q3s::quantize_warps_kernel<ELEM>, dim3((a.M + q3s::QW_WARPS - 1) / q3s::QW_WARPS),
+                                 dim3(q3s::QW_WARPS * 32), 0, st, true, a);
+  return vec ? q3s::launch_maybe_pdl(q3s::quantize_rows_kernel<ELEM, true>, dim3(a.M), dim3(128), 0, st, true, a)
+             : q3s::launch_maybe_pdl(q3s::quantize_rows_kernel<ELEM, false>, dim3(a.M), dim3(128), 0, st, true, a);
 }
 
 // -- few rows --
@@ -49,8 +47,7 @@ cudaError_t launch_gemv_rw(const q3s::Int8Args& a, const q3s::QuantArgs& q, cuda
     if (e != cudaSuccess) return e;
   }
   const int per = q3s::GV_WARPS * RW;
-  kern<<<(a.N + per - 1) / per, q3s::GV_NT, smem, st>>>(a, q);
-  return cudaGetLastError();
+  return q3s::launch_maybe_pdl(kern, dim3((a.N + per - 1) / per), dim3(q3s::GV_NT), smem, st, true, a, q);
 }
 template <bool QUANT, int ELEM, int MB>
 cudaError_t launch_gemv_mb(const q3s::Int8Args& a, const q3s::QuantArgs& q, cudaStream_t st) {
@@ -208,6 +205,7 @@ q3s_status quant_args(const q3s_quantize_rows_desc* d, const char* who, q3s::Qua
   a->values = d->values;
   a->ldv = d->values_row_stride;
   a->scales = d->scales;
+  a->release = false;
   const int n = d->elem == Q3S_ELEM_F32 ? 4 : 8;  // elements in 16 bytes
   *vec = a->K % n == 0 && q3s::aligned16(a->x) && reinterpret_cast<uintptr_t>(a->values) % n == 0 &&
          (a->M == 1 || (a->ldx % n == 0 && a->ldv % n == 0));
@@ -309,6 +307,7 @@ extern "C" q3s_status q3s_int8_linear(const q3s_quantize_rows_desc* q, const q3s
                        : d->elem == Q3S_ELEM_BF16 ? launch_gemv<true, Q3S_ELEM_BF16>(a, qa, st)
                                                   : launch_gemv<true, Q3S_ELEM_F16>(a, qa, st),
                        who);
+  qa.release = true;
   const cudaError_t e = quantize(qa, q->elem, vec, st);
   if (e != cudaSuccess) return cuda_status(e, who);
   return cuda_status(matmul(a, d->elem, st), who);

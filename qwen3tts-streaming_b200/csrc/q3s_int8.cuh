@@ -10,6 +10,7 @@
 #include "q3s_decode.h"
 #include "q3s_device.cuh"
 #include "q3s_head.cuh"
+#include "q3s_pdl.cuh"
 
 namespace q3s {
 
@@ -114,6 +115,10 @@ struct QuantArgs {
   int8_t* values;
   int64_t ldv;
   float* scales;
+  // Whether the next grid may start early.  Only where that is the product of
+  // these rows: a grid that reads weights before it waits for its predecessor
+  // must not find them being written here.
+  bool release;
 };
 
 // Block-wide maximum over NT threads (NaN if any thread's is).
@@ -139,7 +144,8 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const QuantArgs a) {
   constexpr int NT = 128, KEEP = 4, N = E::N;
   __shared__ float s_red[NT / 32];
   const int t = static_cast<int>(threadIdx.x);
-  asm volatile("griddepcontrol.launch_dependents;");
+  grid_wait();
+  if (a.release) grid_release();
   const int64_t row = blockIdx.x;
   const typename E::T* x = static_cast<const typename E::T*>(a.x) + row * a.ldx;
   int8_t* out = a.values + row * a.ldv;
@@ -201,7 +207,8 @@ template <int ELEM>
 __global__ void __launch_bounds__(QW_WARPS * 32) quantize_warps_kernel(const QuantArgs a) {
   using E = Elem<ELEM>;
   constexpr int N = E::N;
-  asm volatile("griddepcontrol.launch_dependents;");
+  grid_wait();
+  if (a.release) grid_release();
   const int lane = static_cast<int>(threadIdx.x) & 31, chunks = a.K / N;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * QW_WARPS + (threadIdx.x >> 5);
   if (row >= a.M) return;
@@ -292,6 +299,8 @@ __global__ void __launch_bounds__(GV_NT) int8_gemv_kernel(const Int8Args a, cons
       const int k = 512 * c + 16 * lane;
       first[r][c] = n0 + r < a.N && k < a.K ? ld_stream16(a.w + (n0 + r) * a.ldw + k) : make_uint4(0, 0, 0, 0);
     }
+  grid_wait();  // the weights do not depend on the kernel before (QuantArgs::release)
+  grid_release();
   if constexpr (QUANT) {
     constexpr int GROUP = GV_NT / MB, KEEP = 4;  // threads of a row; 16-byte loads that stay in registers
     const int m = t / GROUP, i = t % GROUP, chunks = a.K / E::N;
@@ -516,13 +525,13 @@ __global__ void __launch_bounds__(I8C_NT)
   const uint32_t tmem = tmem_slot;
   if (t == 0) {
     auto load_w = [&](int c) { tma_load_2d(smem_u32(smem + (c % cut.stages) * stage_bytes), &tm_w, (c0 + c) * I8_BK, n0, &full[c % cut.stages]); };
-    // the weights do not depend on the kernel before: they are on their way while it ends
+    // the weights do not depend on the kernel before (QuantArgs::release): they are on their way while it ends
     const int ahead = min(count, cut.stages);
     for (int c = 0; c < ahead; ++c) {
       mbar_expect_tx(&full[c], stage_bytes);
       load_w(c);
     }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    grid_wait();
     for (int c = 0; c < count; ++c) {
       const int s = c % cut.stages;
       if (c >= ahead) {
@@ -554,7 +563,8 @@ __global__ void __launch_bounds__(I8C_NT)
     umma_commit(&ready);
   }
   __syncwarp();
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  grid_wait();
+  grid_release();
   const bool done = mbar_wait_bounded(&ready, 0);
   if (!done) atomicOr(&failed, 1);
   tc_fence_after();
@@ -682,7 +692,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_NT, 1)
   cluster_wait();  // the pair's barriers are initialised and its TMEM is allocated
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the quantised rows, when this grid is launched behind them
+  grid_wait();  // the quantised rows, when this grid is launched behind them
+  grid_release();
 
   // a wait that gives up marks the CTA; every role then stops at its next wait
   auto wait = [&](uint64_t* bar, uint32_t parity) {

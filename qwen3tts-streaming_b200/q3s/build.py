@@ -27,7 +27,7 @@ TORCH_DECODE_SRC = CSRC / "q3s_torch_decode.cpp"
 SOURCES = [CSRC / "q3s_sampler.cu", CSRC / "q3s_warp.cu", CSRC / "q3s_head.cu", CSRC / "q3s_lean.cu",
            CSRC / "q3s_cache.cu", CSRC / "q3s_attn.cu", CSRC / "q3s_int8.cu"]
 DEPS = SOURCES + [CSRC / "q3s_args.cuh", CSRC / "q3s_device.cuh", CSRC / "q3s_warp.cuh", CSRC / "q3s_philox.cuh", CSRC / "q3s_step.cuh", CSRC / "q3s_head.cuh", CSRC / "q3s_lean.cuh", CSRC / "q3s_cp.cuh", CSRC / "q3s_core.cuh",
-                  CSRC / "q3s_attn.cuh", CSRC / "q3s_attn_prefix.cuh", CSRC / "q3s_int8.cuh", CSRC / "q3s_tma.cuh",
+                  CSRC / "q3s_attn.cuh", CSRC / "q3s_attn_prefix.cuh", CSRC / "q3s_int8.cuh", CSRC / "q3s_tma.cuh", CSRC / "q3s_pdl.cuh",
                   INCLUDE / "q3s_sampler.h", INCLUDE / "q3s_decode.h"]
 
 NVCC_FLAGS = [

@@ -515,3 +515,20 @@ def test_example_decode_step(dev):
         ended = (drawn[:-1, r] == 7).nonzero()
         start = int(ended[-1]) + 1 if len(ended) else 0
         assert int(lengths[r]) == 30 - start
+
+
+def test_products_wait_for_weights_made_just_before(dev):
+    """Weights quantised by the kernel right before the product (and rows made right before them)."""
+    g = torch.Generator(device=dev).manual_seed(0)
+    x = torch.randn(300, 4096, device=dev, generator=g).bfloat16()
+    for rows in (1, 8, 40, 300):
+        for _ in range(5):
+            w = torch.randn(3000, 4096, device=dev, generator=g)
+            torch.cuda.synchronize()
+            v, s = q3s.quantize_rows(w)
+            y = q3s.int8_linear(x[:rows], v, s)
+            v.fill_(1)
+            torch.cuda.synchronize()
+            v2, s2 = q3s.quantize_rows(w)
+            torch.cuda.synchronize()
+            assert torch.equal(y, q3s.int8_linear(x[:rows], v2, s2))
