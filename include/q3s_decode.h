@@ -35,7 +35,7 @@ extern "C" {
 #define Q3S_DECERR_TABLE 2     /* a row outgrew its block table: it got no blocks */
 #define Q3S_DECERR_POOL 4      /* the free ring ran out: this row and later ones that need blocks got none */
 #define Q3S_DECERR_TOKENS 8    /* more new tokens than max_tokens: the rest have no slot */
-#define Q3S_DECERR_BLOCK_ID 16 /* a block id or slot outside the cache: skipped */
+#define Q3S_DECERR_BLOCK_ID 16 /* a block id or slot outside the cache: its tokens read as zeros / are not stored */
 #define Q3S_DECERR_WAIT 32     /* a bounded device wait gave up */
 
 /* Element types of the operators' tensors. */
@@ -178,7 +178,7 @@ q3s_status q3s_quantize_rows(const q3s_quantize_rows_desc* desc, void* stream);
 typedef struct q3s_int8_matmul_desc {
   uint32_t struct_size;        /* = sizeof(q3s_int8_matmul_desc) */
   int32_t rows;                /* M >= 0 */
-  int32_t inputs;              /* K: a positive multiple of 16, <= 131072 */
+  int32_t inputs;              /* K: a positive multiple of 16, <= 131056 (so that no sum reaches 2^31) */
   int32_t outputs;             /* N >= 1 */
   int32_t elem;                /* q3s_elem of y */
   int32_t reserved0;

@@ -231,8 +231,8 @@ q3s_status matmul_args(const q3s_int8_matmul_desc* d, const char* who, q3s::Int8
                   static_cast<unsigned>(sizeof(q3s_int8_matmul_desc)));
   if (d->rows < 0 || d->outputs < 1)
     return report(Q3S_ERR_INVALID_ARGUMENT, "%s: rows must not be negative and outputs must be positive", who);
-  if (d->inputs < 16 || d->inputs % 16 || d->inputs > 131072)
-    return report(Q3S_ERR_INVALID_ARGUMENT, "%s: inputs %d is not a multiple of 16 in [16, 131072]", who, d->inputs);
+  if (d->inputs < 16 || d->inputs % 16 || d->inputs > 131056)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "%s: inputs %d is not a multiple of 16 in [16, 131056]", who, d->inputs);
   if (!known_elem(d->elem)) return report(Q3S_ERR_INVALID_ARGUMENT, "%s: unknown elem %d", who, d->elem);
   if (d->rows == 0) return report(Q3S_OK, "");
   if (!d->a || !d->a_scales || !d->w || !d->w_scales || !d->y)
