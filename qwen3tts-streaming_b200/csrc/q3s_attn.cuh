@@ -203,6 +203,58 @@ struct SplitTile {
   static constexpr int SMEM = 1024 + WARPS * STAGES * 2 * BYTES;
 };
 
+// A part again, key by key, with what a query does not see left out instead of
+// taken times p = 0: there an infinity or NaN in V would reach the queries of
+// the part that do not see it.  Only for parts whose queries see different keys
+// and whose sums are not finite; one warp, queries in turn, D / 32 dims a lane.
+template <int D, bool BF16, int R>
+Q3S_DEV void attn_part_by_key(const AttnArgs& a, const AttnRow& x, int r, int h, int tile, int first_u, int last_u,
+                              int64_t slot, int lane) {
+  constexpr int E = D / 32;
+  auto dims = [&](const void* at, int64_t offset, float (&y)[E]) {
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(at) + offset + lane * E);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 f = unpack2<BF16>(p[e / 2]);
+      y[e] = f.x, y[e + 1] = f.y;
+    }
+  };
+  const int rows = min(R, x.n * a.G - tile * R);
+#pragma unroll 1
+  for (int i = 0; i < rows; ++i) {
+    const int row = tile * R + i, token = row / a.G;
+    float q[E], acc[E], m = -INFINITY, l = 0.0f;
+    dims(a.q, static_cast<int64_t>(x.t0 + token) * a.qt + (static_cast<int64_t>(h) * a.G + row % a.G) * a.qh, q);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+    const int end = min((last_u + 1) * AT_KEYS, x.len - x.n + token + 1);
+#pragma unroll 1
+    for (int j = first_u * AT_KEYS; j < end; ++j) {
+      const int id = a.table[(r - 1) * a.table_stride + (j >> a.bs_log2)], place = j & (a.bs - 1);
+      float k[E], v[E], s = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) k[e] = v[e] = 0.0f;
+      if (static_cast<unsigned>(id) < static_cast<unsigned>(a.blocks)) {
+        dims(a.k, id * a.kb + h * a.kh + place * a.kp, k);
+        dims(a.v, id * a.vb + h * a.vh + place * a.vp, v);
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) s = fmaf(q[e], k[e], s);
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) s += __shfl_xor_sync(FULL, s, d);
+      s *= a.scale_log2;
+      const float nm = fmaxf(m, s), base = nm == -INFINITY ? 0.0f : nm, c = ex2(m - base), p = ex2(s - base);
+      m = nm;
+      l = l * c + p;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = acc[e] * c + p * v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) a.part_o[slot * (R * D) + i * D + lane * E + e] = acc[e];
+    if (lane == 0) a.part_ml[slot * R + i] = make_float2(m, l);
+  }
+}
+
 // How the unit list is cut into the warps' ranges.  The CTAs that find a SM
 // free start at once, the others when the prefix kernel leaves theirs: warps of
 // the first `early` CTAs take `lead` units more.
@@ -242,7 +294,8 @@ Q3S_DEV AttnCut attn_cut(const AttnArgs& a, long long all, long long ctas, long 
 // 128-byte swizzle), because issuing a unit's copies takes a third as long as
 // computing it.  What lies
 // past the end of a row's last unit is cleared in V (so that nothing that lies
-// there, NaN included, reaches the products) and masked in the scores.  Both
+// there, NaN included, reaches the products) and masked in the scores; a key that some of an
+// item's queries see and others do not is masked for those, and counts for nothing (attn_part_by_key).  Both
 // products have the keys' side as the matrix instruction's M (m16n8k16):
 // S^T = K Q^T, O^T += V^T P^T, with N = 8 query rows, so one query a row and its
 // group of heads waste little of it.  p is carried as the sum of two 16-bit
@@ -539,6 +592,7 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
           a.items[id] = make_int2(static_cast<int>(slot), parts);
         }
         float* po = a.part_o + slot * (R * D);
+        float size = 0.0f;  // NaN if one of the sums is not finite
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -552,10 +606,15 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
               for (int i = 0; i < D / 16; ++i) {
                 po[row * D + 16 * i + g] = o[i][q][e];
                 po[row * D + 16 * i + g + 8] = o[i][q][2 + e];
+                size = fmaf(o[i][q][e], 0.0f, fmaf(o[i][q][2 + e], 0.0f, size));
               }
               if (g == 0) a.part_ml[slot * R + row] = make_float2(m[q][e], x);
             }
           }
+        if (wx.causal && wx.n > 1 && __any_sync(FULL, size != 0.0f)) {
+          __syncwarp();  // its writes come after those above
+          attn_part_by_key<D, BF16, R>(a, wx, wr, wh, wt, first_u, wu, slot, lane);
+        }
       }
     }
   }

@@ -265,6 +265,26 @@ def check_attention(c, out, lse):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,group,n,length", [(64, 2, 3, 19), (128, 4, 9, 40), (64, 1, 20, 20), (128, 1, 33, 33)])
+def test_attention_odd_values_reach_only_who_sees_them(dev, dtype, dim, group, n, length):
+    """NaN and infinities in V of the step's own tokens: a query before them is
+    as if they were finite; one that sees them has them, in their dims."""
+    c = make_attention(dev, n=[n, 2], lengths=[length, 5], prefix=7, q_heads=2 * group, kv_heads=2, dim=dim,
+                       block=16, dtype=dtype, poison=False)
+    clean = dict(c, v=c["v"].clone())
+    table = c["table"].cpu()
+    for back, x in ((1, float("nan")), (2, float("inf"))):  # the row's last token and the one before it
+        j = length - back
+        c["v"][int(table[0, j // 16]), :, j % 16, 3::5] = x
+    out, lse = run_attention(c)
+    hit = torch.zeros(dim, dtype=torch.bool)
+    hit[3::5] = True
+    assert bool(torch.isposinf(out[n - 2][..., hit]).all()) and bool(torch.isnan(out[n - 1][..., hit]).all())
+    out[n - 2:n, :, 3::5] = run_attention(clean)[0][n - 2:n, :, 3::5]  # checked above
+    check_attention(clean, out, lse)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("q_heads,kv_heads,dim,block", [(16, 8, 128, 16), (8, 1, 64, 32), (3, 3, 128, 64), (32, 2, 64, 128),
                                                         (10, 2, 128, 16)])
 @pytest.mark.parametrize("prefix,lengths", [
