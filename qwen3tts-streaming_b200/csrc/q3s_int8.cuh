@@ -273,7 +273,7 @@ Q3S_DEV float int8_out(int sum, float a_scale, float w_scale) {
 
 constexpr int GV_NT = 256, GV_WARPS = GV_NT / 32;
 constexpr int GV_MAX_M = 8;
-constexpr int GV_SMEM = 96 * 1024;  // most bytes of activations
+constexpr int GV_SMEM = 24 * 1024;  // most bytes of activations
 
 // M <= MB <= 8 rows: the product is bound by reading the weights once, and at
 // these sizes by latency.  A warp owns RW outputs and reads their weight rows

@@ -481,6 +481,22 @@ def test_int8_matmul(dev, M, K, N, dtype):
         assert y.dtype == dtype and bool(((y.double() - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("M,K", [(8, 3056), (8, 3088), (8, 6144), (4, 6144), (3, 6160), (2, 12288), (1, 24576), (1, 24592),
+                                 (2, 24576), (1, 49152)])
+def test_int8_few_rows_of_many_inputs(dev, M, K):
+    """On both sides of the size up to which few rows are one launch, and where their bytes are 48 KB."""
+    g = torch.Generator().manual_seed(M + K)
+    x = torch.randn(M, K, generator=g)
+    w = torch.randint(-128, 128, (19, K), generator=g, dtype=torch.int8)
+    ws = torch.rand(19, generator=g) + 0.5
+    values, scales = (torch.from_numpy(y).double() for y in R.quantize_rows(x.numpy()))
+    want = (values @ w.double().t()) * scales[:, None] * ws.double()
+    y = q3s.int8_linear(x.to(dev), w.to(dev), ws.to(dev))
+    z = q3s.int8_matmul(*q3s.quantize_rows(x.to(dev)), w.to(dev), ws.to(dev), dtype=torch.float32)
+    assert bool(((y.cpu().double() - want).abs() <= (ROUNDOFF[torch.float32] + 2.0 ** -22) * want.abs()).all())
+    assert torch.equal(y, z)
+
+
 def test_int8_matmul_largest_sums_and_strides(dev):
     """The longest K at full scale and operands that are slices."""
     K = 131056
