@@ -55,15 +55,21 @@ void plan_prefix(const q3s_prefix_attention_desc* d, Layout* l) {
 Layout layout_of(const q3s_prefix_attention_desc* d) {
   Layout l;
   const int64_t G = d->q_heads / d->kv_heads, queries = static_cast<int64_t>(d->tokens) * G;
-  // The prefix kernel's tiles are 128 query rows: with fewer than
-  // 64 of them, or fewer than 64 keys, the key-split kernel takes
-  // the prefix as one more row.  A scale that is not positive turns the order
-  // of the scores around, which the prefix kernel's running maximum does not
-  // follow.
+  // With few queries or keys the key-split kernel takes the prefix as one more
+  // row: that costs it about queries * keys, the prefix kernel about the square
+  // root of the keys (more of them are cut into more parts).  So the rule is on
+  // queries^2 * keys.  Key-split against prefix kernel, 8 heads of 128 and 100
+  // own tokens: 32 queries x 2048 keys (2.1e6) 14.2 against 15.0 us, 32 x 8192
+  // (8.4e6) 23.0 against 20.4, 48 x 2048 (4.7e6) 16.7 against 15.6, 128 x 128
+  // (2.1e6) 12.1 against 12.5, 96 x 512 (4.7e6) 14.4 against 12.5, 256 x 8192
+  // 112 against 31.  A scale that is not positive turns the order of the scores
+  // around, which the prefix kernel's running maximum does not follow.
   l.splits = 0;
-  if (queries >= 64 && d->prefix_length >= 64 && d->scale > 0.0f) plan_prefix(d, &l);
+  if (queries * queries >= 4000000 / std::max(d->prefix_length, 1) && d->prefix_length >= 64 && d->scale > 0.0f) plan_prefix(d, &l);
   // An item of the key-split kernel holds the query rows of an average row of
-  // the batch (an item reads its keys once), in tiles of 8 or 16.
+  // the batch (an item reads its keys once), in tiles of 8 or 16.  8 against 16,
+  // 60 rows of 2000 keys: 8 query rows 85 against 93 us, 10 query rows 160
+  // against 95; 16 rows of 1000 keys: 13.4 against 17.7 and 19.0 against 18.1.
   const int64_t mean = (queries + std::max(d->batch, 1) - 1) / std::max(d->batch, 1);
   l.nq = mean <= 8 ? 1 : 2;
   const int64_t warps = d->dim == 64 ? (l.nq == 1 ? split_warps<64, 1>() : split_warps<64, 2>())
@@ -170,12 +176,14 @@ cudaError_t launch_split(const q3s::AttnArgs& a, cudaStream_t st) {
 }
 
 // A warp a row, or four where an item is cut into many parts (few items over
-// all the warps, or many parts of the prefix).
+// all the warps, or many parts of the prefix).  One against four, 8 heads, rows
+// of 2000 keys: 1 row 14.0 against 10.1 us, 24 rows 40.5 against 38.6, 48 rows
+// 71.1 against 72.6; 64 rows, 2 heads, a prefix of 30000 in 32 parts: 34.2 against 32.1.
 template <int D, bool BF16, int NQ>
 cudaError_t launch_join(const q3s::AttnArgs& a, const Layout& l, cudaStream_t st) {
   const int64_t rows = static_cast<int64_t>(a.T) * a.Hq;
   const int64_t items = static_cast<int64_t>(std::max(std::min(a.B, a.T), 1)) * a.H;
-  return l.splits > 12 || split_warps<D, NQ>() / items > 6
+  return l.splits > 12 || split_warps<D, NQ>() / items >= 4
              ? q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, NQ, true>, dim3(static_cast<unsigned>(rows)), dim3(128), 0, st, true, a)
              : q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, NQ, false>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0,
                                      st, true, a);
