@@ -117,8 +117,10 @@ q3s_status q3s_cache_append(const q3s_cache_append_desc* desc, void* stream);
  * key/value head h / (q_heads / kv_heads).
  *   out = softmax(scale * q . k) v,   lse = log sum exp(scale * q . k)
  * with 0 and -inf for a query that sees nothing.  Softmax statistics and sums
- * are 32-bit; probabilities are rounded to the cache's type for the product
- * with v, as the tensor cores take them. */
+ * are 32-bit.  For the product with v, as the tensor cores take it,
+ * probabilities over the prefix of a large batch are rounded to the cache's
+ * type, the others held as the sum of two such values.  A key that a query does
+ * not see has no part in its result, whatever k and v hold there. */
 typedef struct q3s_prefix_attention_desc {
   uint32_t struct_size;        /* = sizeof(q3s_prefix_attention_desc) */
   int32_t batch;               /* B, 0..Q3S_MAX_CACHE_ROWS */

@@ -304,8 +304,15 @@ Q3S_DEV AttnCut attn_cut(const AttnArgs& a, long long all, long long ctas, long 
 //
 // With one query a row this is bound by reading the cache (2 * G useful
 // operations a byte), as long as a warp's dependent chain of a unit stays below
-// the time that its 8 KB take.  The tcgen05 form, whose M is 128, would be
-// nearly empty; many queries on a long prefix are the other kernel's.
+// the time that its 8 KB take: 61 rows of 6000 keys of 2 x 64 (117 MB) in 31.4 us
+// with the join, 3.7 TB/s, 96 rows of 500 behind a prefix of 1500 (130 MB) in 32.8.
+// With 16-row items the chain (two products of every score, in order) is the
+// longer of the two: 40 rows of 1 to 9 queries x 4 heads take 52 us of which the
+// bytes are 16.  Query rows as the instruction's M instead, with keys as N, took
+// 34 us for the 96 rows before the join; copies by lanes (cp.async) in place of TMA
+// 1100 clocks for 32 keys; four 2 KB copies a unit in place of two of a
+// 5-dimensional map 900 clocks to issue.  The tcgen05 form, whose M is
+// 128, would be nearly empty; many queries on a long prefix are the other kernel's.
 template <int D, bool BF16, int NQ>
 __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM)
     attn_split_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -628,7 +635,9 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
 // One warp a row of [T * q_heads]; a lane holds D / 32 of its values.  A token's batch row is found in
 // query_offsets by bisection, before the grid waits for the parts; tokens past
 // the last row see nothing.  Bound by latency, of the record of the row's own
-// parts and of the sums, and by fetching its own instructions: kept short.
+// parts and of the sums, and by fetching its own instructions: kept short (with the weights of
+// up to 32 parts computed before the sums it took 8.8 us, and 256 rows of 32 heads
+// 99 us in all against 93).
 //
 // TEAM: the four warps of a CTA share a row, each every fourth part, and meet in
 // shared memory.

@@ -178,7 +178,13 @@ Q3S_DEV float max3(float a, float b, float c) {
 // Keys past the end: whole boxes read as zeros (an out-of-range block
 // coordinate), the rest of the last one is cleared in V and masked in S.
 // Bound by the exponentials (16 a clock and SM: 1024 clocks for 128 x 128
-// scores) and, equally, by the two products (1024 clocks at the tensor peak).
+// scores) and, equally, by the two products (1024 clocks at the tensor peak):
+// 256 rows of 4 x 8 heads on 16000 keys of 128 (67 GFLOP, 41 us at the peak of a
+// large product) take 79 us, 54% of the tensor pipe.  Some of the exponentials as
+// polynomials made it slower (90 to 95 us with the rest of the operator, 88.7
+// without): the two products in the shape 128 x 128 x 16 are near what they
+// reach.  One tile a CTA where that fills more SMs was no faster either: from 2.5
+// us less to 8 more, as the key-split kernel beside it loses those SMs.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(PX_NT, 1)
     attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
