@@ -23,6 +23,7 @@
 namespace q3s {
 
 constexpr int AT_KEYS = 16;    // keys of a unit (one pipeline stage of a warp); a block is a multiple of it
+constexpr float AT_SLACK = 8.0f;  // log2 units that a running maximum may lag behind: p up to 256
 constexpr int AT_MIN_UNITS = 3;  // fewest units a warp takes before another one is used
 
 struct AttnArgs {
@@ -508,45 +509,49 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
       }
     }
     const bool cut = j0 + AT_KEYS - 1 > low;
-    float c[NQ][2], base[NQ][2];
-    bool moved = false;
+    // a lane looks at its own scores only; what rises above the maximum by more than the slack moves it
+    float top[NQ][2];
+    bool rise = false;
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
-      float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[0][q][e] = (s[0][q][e] + s[1][q][e]) * a.scale_log2;
         if (cut && j0 + g + 8 * (e >> 1) > lim[q][e & 1]) s[0][q][e] = -INFINITY;
-        top[e & 1] = fmaxf(top[e & 1], s[0][q][e]);
-      }
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1) {
-        top[0] = fmaxf(top[0], __shfl_xor_sync(FULL, top[0], d));
-        top[1] = fmaxf(top[1], __shfl_xor_sync(FULL, top[1], d));
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float nm = fmaxf(m[q][e], top[e]);
-        base[q][e] = nm == -INFINITY ? 0.0f : nm;
-        moved |= nm != m[q][e];
-        c[q][e] = ex2(m[q][e] - base[q][e]);  // 0 for the item's first unit (m = -inf)
-        m[q][e] = nm;
+        top[q][e] = fmaxf(s[0][q][e], s[0][q][2 + e]);
+        rise |= top[q][e] > m[q][e] + AT_SLACK;
       }
     }
-    if (__any_sync(FULL, moved)) {
+    if (__any_sync(FULL, rise)) {
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
-        l[q][0] *= c[q][0];
-        l[q][1] *= c[q][1];
+        float c[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) top[q][e] = fmaxf(top[q][e], __shfl_xor_sync(FULL, top[q][e], d));
+          const float nm = fmaxf(m[q][e], top[q][e]);
+          c[e] = ex2(m[q][e] - (nm == -INFINITY ? 0.0f : nm));  // 0 for the item's first unit (m = -inf)
+          m[q][e] = nm;
+          l[q][e] *= c[e];
+        }
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
-          o[i][q][0] *= c[q][0];
-          o[i][q][1] *= c[q][1];
-          o[i][q][2] *= c[q][0];
-          o[i][q][3] *= c[q][1];
+          o[i][q][0] *= c[0];
+          o[i][q][1] *= c[1];
+          o[i][q][2] *= c[0];
+          o[i][q][3] *= c[1];
         }
       }
     }
+    float base[NQ][2];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) base[q][e] = m[q][e] == -INFINITY ? 0.0f : m[q][e];
     uint32_t ph[NQ][2], pl[NQ][2];  // p^T, upper and lower part: the B operand
 #pragma unroll
     for (int q = 0; q < NQ; ++q)
