@@ -13,11 +13,7 @@
 namespace {
 
 // Computing warps of the key-split kernel's grid.
-template <int D, int NQ>
-int split_warps() {
-  using Tile = q3s::SplitTile<D, NQ>;
-  return q3s::sm_count() * Tile::PER_SM * Tile::WARPS;
-}
+int split_warps() { return q3s::sm_count() * q3s::SplitTile<128, 1>::PER_SM * q3s::SplitTile<128, 1>::WARPS; }
 
 struct Layout {
   int64_t items, part_o, part_ml, pre_o, pre_ml, bytes;  // byte offsets
@@ -72,8 +68,7 @@ Layout layout_of(const q3s_prefix_attention_desc* d) {
   // against 95; 16 rows of 1000 keys: 13.4 against 17.7 and 19.0 against 18.1.
   const int64_t mean = (queries + std::max(d->batch, 1) - 1) / std::max(d->batch, 1);
   l.nq = mean <= 8 ? 1 : 2;
-  const int64_t warps = d->dim == 64 ? (l.nq == 1 ? split_warps<64, 1>() : split_warps<64, 2>())
-                                     : (l.nq == 1 ? split_warps<128, 1>() : split_warps<128, 2>());
+  const int64_t warps = split_warps();
   // A CTA of the prefix kernel has a SM for itself: this kernel's CTAs that
   // would be there start when it ends, that many units later (a unit takes 1.3
   // us with 8-row items, 2 us with 16-row ones, and a CTA 3 us to get going).
@@ -171,7 +166,7 @@ cudaError_t launch_split(const q3s::AttnArgs& a, cudaStream_t st) {
   const cudaError_t e = q3s::allow_smem(split, Tile::SMEM, done);
   if (e != cudaSuccess) return e;
   CUtensorMap tk, tv;
-  if (!cache_maps(a, D, BF16, q3s::AT_KEYS, D / 64, &tk, &tv)) return cudaErrorInvalidValue;
+  if (!cache_maps(a, D, BF16, Tile::KEYS, D / 64, &tk, &tv)) return cudaErrorInvalidValue;
   return q3s::launch_maybe_pdl(split, dim3(q3s::sm_count() * Tile::PER_SM), dim3(Tile::NT), Tile::SMEM, st, true, tk, tv, a);
 }
 
@@ -179,13 +174,13 @@ cudaError_t launch_split(const q3s::AttnArgs& a, cudaStream_t st) {
 // all the warps, or many parts of the prefix).  One against four, 8 heads, rows
 // of 2000 keys: 1 row 14.0 against 10.1 us, 24 rows 40.5 against 38.6, 48 rows
 // 71.1 against 72.6; 64 rows, 2 heads, a prefix of 30000 in 32 parts: 34.2 against 32.1.
-template <int D, bool BF16, int NQ>
+template <int D, bool BF16, int R>
 cudaError_t launch_join(const q3s::AttnArgs& a, const Layout& l, cudaStream_t st) {
   const int64_t rows = static_cast<int64_t>(a.T) * a.Hq;
   const int64_t items = static_cast<int64_t>(std::max(std::min(a.B, a.T), 1)) * a.H;
-  return l.splits > 12 || split_warps<D, NQ>() / items >= 4
-             ? q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, NQ, true>, dim3(static_cast<unsigned>(rows)), dim3(128), 0, st, true, a)
-             : q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, NQ, false>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0,
+  return l.splits > 12 || split_warps() / items >= 4
+             ? q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, R, true>, dim3(static_cast<unsigned>(rows)), dim3(128), 0, st, true, a)
+             : q3s::launch_maybe_pdl(q3s::attn_join_kernel<D, BF16, R, false>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0,
                                      st, true, a);
 }
 
@@ -213,7 +208,7 @@ cudaError_t launch(const q3s::AttnArgs& a, const Layout& l, cudaStream_t st) {
   // beside the prefix kernel where there is one: neither reads what the other writes
   e = l.nq == 1 ? launch_split<D, BF16, 1>(a, st) : launch_split<D, BF16, 2>(a, st);
   if (e != cudaSuccess) return e;
-  return l.nq == 1 ? launch_join<D, BF16, 1>(a, l, st) : launch_join<D, BF16, 2>(a, l, st);
+  return l.nq == 1 ? launch_join<D, BF16, 8>(a, l, st) : launch_join<D, BF16, 16>(a, l, st);
 }
 
 }  // namespace

@@ -22,7 +22,9 @@
 
 namespace q3s {
 
-constexpr int AT_KEYS = 16;    // keys of a unit (one pipeline stage of a warp); a block is a multiple of it
+// Keys of a unit (one pipeline stage): 4 KB of K and of V, taken 16 at a time.
+template <int D>
+constexpr int AT_KEYS = D == 64 ? 32 : 16;
 constexpr float AT_SLACK = 8.0f;  // log2 units that a running maximum may lag behind: p up to 256
 constexpr int AT_MIN_UNITS = 3;  // fewest units a warp takes before another one is used
 
@@ -60,7 +62,7 @@ struct AttnRow {
   int t0, n, len, causal;  // first token, tokens, keys; 1: token i sees keys j <= len - n + i
   int units, tiles;
 };
-template <int R>
+template <int R, int KEYS>
 Q3S_DEV AttnRow attn_row(const AttnArgs& a, int r) {
   AttnRow x;
   if (r == 0) {
@@ -75,7 +77,7 @@ Q3S_DEV AttnRow attn_row(const AttnArgs& a, int r) {
     x.len = static_cast<int>(min(static_cast<int64_t>(max(len, 0)), static_cast<int64_t>(a.max_blocks) * a.bs));
     x.causal = 1;
   }
-  x.units = x.n > 0 ? (x.len + AT_KEYS - 1) / AT_KEYS : 0;
+  x.units = x.n > 0 ? (x.len + KEYS - 1) / KEYS : 0;
   x.tiles = x.units ? (x.n * a.G + R - 1) / R : 0;
   return x;
 }
@@ -192,14 +194,18 @@ Q3S_DEV bool attn_next(const AttnArgs& a, AttnPos& p, const Rows& row_at) {
 }
 
 // Shapes of the key-split kernel: four computing warps (and one that copies)
-// with rings of three units; two CTAs a SM at dim 128, four or three at 64.
+// with rings of three units, two CTAs a SM.  At dim 64 a unit is 32 keys, because
+// a copy costs the same whatever its size: with 16 (four CTAs a SM) 61 rows of 4000
+// keys of 2 heads took 37.4 us against 28.8, and 40 rows of 16 x 4 queries on 1000
+// keys of 8 heads 85 against 57.
 template <int D, int NQ>
 struct SplitTile {
   static constexpr int WARPS = 4, STAGES = 3;
-  static constexpr int PER_SM = D == 128 ? 2 : 5 - NQ;
+  static constexpr int PER_SM = 2;
+  static constexpr int KEYS = AT_KEYS<D>;
   static constexpr int NT = (WARPS + 1) * 32;
   static constexpr int HALVES = D / 64;                 // 128-byte slices of a key
-  static constexpr int SLICE = AT_KEYS * 128;           // bytes of a unit's keys in one slice
+  static constexpr int SLICE = KEYS * 128;              // bytes of a unit's keys in one slice
   static constexpr int BYTES = HALVES * SLICE;          // a unit's keys (or values)
   static constexpr int SMEM = 1024 + WARPS * STAGES * 2 * BYTES;
 };
@@ -211,7 +217,7 @@ struct SplitTile {
 template <int D, bool BF16, int R>
 Q3S_DEV void attn_part_by_key(const AttnArgs& a, const AttnRow& x, int r, int h, int tile, int first_u, int last_u,
                               int64_t slot, int lane) {
-  constexpr int E = D / 32;
+  constexpr int E = D / 32, KEYS = AT_KEYS<D>;
   auto dims = [&](const void* at, int64_t offset, float (&y)[E]) {
     const uint32_t* p = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(at) + offset + lane * E);
 #pragma unroll
@@ -228,9 +234,9 @@ Q3S_DEV void attn_part_by_key(const AttnArgs& a, const AttnRow& x, int r, int h,
     dims(a.q, static_cast<int64_t>(x.t0 + token) * a.qt + (static_cast<int64_t>(h) * a.G + row % a.G) * a.qh, q);
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-    const int end = min((last_u + 1) * AT_KEYS, x.len - x.n + token + 1);
+    const int end = min((last_u + 1) * KEYS, x.len - x.n + token + 1);
 #pragma unroll 1
-    for (int j = first_u * AT_KEYS; j < end; ++j) {
+    for (int j = first_u * KEYS; j < end; ++j) {
       const int id = a.table[(r - 1) * a.table_stride + (j >> a.bs_log2)], place = j & (a.bs - 1);
       float k[E], v[E], s = 0.0f;
 #pragma unroll
@@ -320,6 +326,7 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
                       const AttnArgs a) {
   using Tile = SplitTile<D, NQ>;
   constexpr int R = 8 * NQ, AT_WARPS = Tile::WARPS, AT_NT = Tile::NT, AT_STAGES = Tile::STAGES, BARS = AT_WARPS * AT_STAGES;
+  constexpr int KEYS = Tile::KEYS;
   extern __shared__ __align__(1024) unsigned char at_smem[];
   __shared__ long long s_units[AT_NT + 1];
   __shared__ AttnRow s_rows[AT_NT];  // the rows, where there are no more than threads
@@ -344,7 +351,7 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
   for (int i = 0; i < per; ++i) {
     const int r = t * per + i;
     if (r >= rows) break;
-    const AttnRow x = attn_row<R>(a, r);
+    const AttnRow x = attn_row<R, KEYS>(a, r);
     mu += static_cast<long long>(x.units) * x.tiles * a.H;
     if (r > 0) bad |= a.lengths[r - 1] != x.len || a.offsets[r - 1] != x.t0 || a.offsets[r] != x.t0 + x.n;
     if (per == 1) s_rows[t] = x;
@@ -376,7 +383,7 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
   const long long u0 = cuts.start(gw);
   const int total = mine < AT_WARPS ? static_cast<int>(cuts.start(gw + 1) - u0) : 0;
 
-  auto row_at = [&](int r) { return per == 1 ? s_rows[r] : attn_row<R>(a, r); };
+  auto row_at = [&](int r) { return per == 1 ? s_rows[r] : attn_row<R, KEYS>(a, r); };
   AttnPos p;
   p.r = p.h = p.tile = p.u = 0;
   if (total > 0) {
@@ -407,12 +414,23 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
 
   if (w == AT_WARPS) {
     // ---- copies: lane l for warp l -----------------------------------------------
-    auto block_of = [&](const AttnPos& q) {  // its cache block, as the table has it
-      const int j = (q.u * AT_KEYS) >> a.bs_log2;
+    auto block_of = [&](const AttnPos& q, int key) {  // the cache block of a unit's key, as the table has it
+      const int j = (q.u * KEYS + key) >> a.bs_log2;
       return q.r == 0 ? a.prefix_blocks[j] : a.table[(q.r - 1) * a.table_stride + j];
     };
-    int next_id = total > 0 ? block_of(p) : 0, fetched = 0, idle = 0;
+    // a unit of more keys than a block has is two blocks, the second where it holds some of the row
+    const bool halves = KEYS > 16 && a.bs < KEYS;
+    auto second = [&](const AttnPos& q) { return halves && q.u * KEYS + 16 < q.x.len; };
+    int next_id = total > 0 ? block_of(p, 0) : 0, next_second = total > 0 && second(p) ? block_of(p, 16) : 0;
+    int fetched = 0, idle = 0;
     bool bad_block = false;
+    auto copy = [&](uint32_t dst, int id, int place, uint64_t* bar) {
+      const bool inside = static_cast<unsigned>(id) < static_cast<unsigned>(a.blocks);
+      bad_block |= !inside;
+      if (!inside) id = a.blocks;  // past the cache: reads as zeros
+      tma_load_block(dst, &tm_k, place, p.h, id, bar);
+      tma_load_block(dst + Tile::BYTES, &tm_v, place, p.h, id, bar);
+    };
     while (fetched < total) {
       const int s = fetched % AT_STAGES;
       if (fetched >= AT_STAGES && !mbar_test(&empty[s], ((fetched / AT_STAGES) - 1) & 1)) {
@@ -421,16 +439,14 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
       }
       idle = 0;
       const uint32_t dst = smem_u32(ring + s * 2 * Tile::BYTES);
-      const bool inside = static_cast<unsigned>(next_id) < static_cast<unsigned>(a.blocks);
-      bad_block |= !inside;
-      const int id = inside ? next_id : a.blocks;  // past the cache: reads as zeros
-      const int place = (p.u * AT_KEYS) & (a.bs - 1);
-      mbar_expect_tx(&full[s], 2 * Tile::BYTES);
-      tma_load_block(dst, &tm_k, place, p.h, id, &full[s]);
-      tma_load_block(dst + Tile::BYTES, &tm_v, place, p.h, id, &full[s]);
+      const bool two = second(p);
+      mbar_expect_tx(&full[s], halves && !two ? Tile::BYTES : 2 * Tile::BYTES);
+      copy(dst, next_id, (p.u * KEYS) & (a.bs - 1), &full[s]);
+      if (two) copy(dst + 16 * 128, next_second, 0, &full[s]);
       if (++fetched < total) {
         attn_next(a, p, row_at);
-        next_id = block_of(p);  // not looked at before the next round: its latency is not waited for
+        if (second(p)) next_second = block_of(p, 16);
+        next_id = block_of(p, 0);  // not looked at before the next round: its latency is not waited for
       }
     }
     if (bad_block && a.error_word) atomicOr(a.error_word, Q3S_DECERR_BLOCK_ID);
@@ -481,108 +497,113 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
     ok = __shfl_sync(FULL, ok, 0);
     if (!ok) break;
     unsigned char* kt = ring + st * 2 * Tile::BYTES;
-    const int j0 = p.u * AT_KEYS, valid = p.x.len - j0;
-    if (valid < AT_KEYS) {  // clear V past the end
-      for (int c = lane; c < (AT_KEYS - valid) * 8; c += 32)
+    const int unit0 = p.u * KEYS, valid = p.x.len - unit0;
+    if (valid < KEYS) {  // clear V past the end
+      for (int c = lane; c < (KEYS - valid) * 8; c += 32)
 #pragma unroll
         for (int x = 0; x < Tile::HALVES; ++x)
           *reinterpret_cast<uint4*>(kt + Tile::BYTES + x * Tile::SLICE + valid * 128 + c * 16) = make_uint4(0, 0, 0, 0);
       fence_proxy_async_smem();  // the next copy into this stage comes after
       __syncwarp();
     }
-    const uint32_t ka = smem_u32(kt), va = ka + Tile::BYTES;
+#pragma unroll
+    for (int part = 0; part < KEYS / 16; ++part) {
+      if (part && valid <= 16 * part) break;
+      const int j0 = unit0 + 16 * part;
+      const uint32_t ka = smem_u32(kt) + part * 16 * 128, va = ka + Tile::BYTES;
 
-    float s[2][NQ][4];  // two chains of sums, over every other 16 dims
+      float s[2][NQ][4];  // two chains of sums, over every other 16 dims
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) s[i][q][0] = s[i][q][1] = s[i][q][2] = s[i][q][3] = 0.0f;
-    {
-      // the four 8x8 matrices: keys (lane & 7) + 8 ((lane >> 3) & 1), 16-byte chunk + (lane >> 4)
-      const int key = (lane & 7) + (((lane >> 3) & 1) << 3), cc = lane >> 4, x7 = key & 7;
+        for (int q = 0; q < NQ; ++q) s[i][q][0] = s[i][q][1] = s[i][q][2] = s[i][q][3] = 0.0f;
+      {
+        // the four 8x8 matrices: keys (lane & 7) + 8 ((lane >> 3) & 1), 16-byte chunk + (lane >> 4)
+        const int key = (lane & 7) + (((lane >> 3) & 1) << 3), cc = lane >> 4, x7 = key & 7;
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        uint32_t f[4];
-        ldsm4(f, ka + static_cast<uint32_t>((k / 4) * Tile::SLICE + key * 128 + ((((2 * k) & 7) + cc) ^ x7) * 16));
+        for (int k = 0; k < D / 16; ++k) {
+          uint32_t f[4];
+          ldsm4(f, ka + static_cast<uint32_t>((k / 4) * Tile::SLICE + key * 128 + ((((2 * k) & 7) + cc) ^ x7) * 16));
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) mma16816<BF16>(s[k & 1][q], f, qf[q][k][0], qf[q][k][1]);
+          for (int q = 0; q < NQ; ++q) mma16816<BF16>(s[k & 1][q], f, qf[q][k][0], qf[q][k][1]);
+        }
       }
-    }
-    const bool cut = j0 + AT_KEYS - 1 > low;
-    // a lane looks at its own scores only; what rises above the maximum by more than the slack moves it
-    float top[NQ][2];
-    bool rise = false;
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[0][q][e] = (s[0][q][e] + s[1][q][e]) * a.scale_log2;
-        if (cut && j0 + g + 8 * (e >> 1) > lim[q][e & 1]) s[0][q][e] = -INFINITY;
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        top[q][e] = fmaxf(s[0][q][e], s[0][q][2 + e]);
-        rise |= top[q][e] > m[q][e] + AT_SLACK;
-      }
-    }
-    if (__any_sync(FULL, rise)) {
+      const bool cut = j0 + 15 > low;
+      // a lane looks at its own scores only; what rises above the maximum by more than the slack moves it
+      float top[NQ][2];
+      bool rise = false;
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
-        float c[2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[0][q][e] = (s[0][q][e] + s[1][q][e]) * a.scale_log2;
+          if (cut && j0 + g + 8 * (e >> 1) > lim[q][e & 1]) s[0][q][e] = -INFINITY;
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) top[q][e] = fmaxf(top[q][e], __shfl_xor_sync(FULL, top[q][e], d));
-          const float nm = fmaxf(m[q][e], top[q][e]);
-          c[e] = ex2(m[q][e] - (nm == -INFINITY ? 0.0f : nm));  // 0 for the item's first unit (m = -inf)
-          m[q][e] = nm;
-          l[q][e] *= c[e];
-        }
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          o[i][q][0] *= c[0];
-          o[i][q][1] *= c[1];
-          o[i][q][2] *= c[0];
-          o[i][q][3] *= c[1];
+          top[q][e] = fmaxf(s[0][q][e], s[0][q][2 + e]);
+          rise |= top[q][e] > m[q][e] + AT_SLACK;
         }
       }
-    }
-    float base[NQ][2];
+      if (__any_sync(FULL, rise)) {
 #pragma unroll
-    for (int q = 0; q < NQ; ++q)
+        for (int q = 0; q < NQ; ++q) {
+          float c[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) base[q][e] = m[q][e] == -INFINITY ? 0.0f : m[q][e];
-    uint32_t ph[NQ][2], pl[NQ][2];  // p^T, upper and lower part: the B operand
+          for (int e = 0; e < 2; ++e) {
 #pragma unroll
-    for (int q = 0; q < NQ; ++q)
+            for (int d = 4; d < 32; d <<= 1) top[q][e] = fmaxf(top[q][e], __shfl_xor_sync(FULL, top[q][e], d));
+            const float nm = fmaxf(m[q][e], top[q][e]);
+            c[e] = ex2(m[q][e] - (nm == -INFINITY ? 0.0f : nm));  // 0 for the item's first unit (m = -inf)
+            m[q][e] = nm;
+            l[q][e] *= c[e];
+          }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float p0 = ex2(s[0][q][2 * e] - base[q][0]), p1 = ex2(s[0][q][2 * e + 1] - base[q][1]);
-        l[q][0] += p0;
-        l[q][1] += p1;
-        const uint32_t hi = pack2<BF16>(p0, p1);
-        const float2 back = unpack2<BF16>(hi);
-        ph[q][e] = transpose8(hi);
-        pl[q][e] = transpose8(pack2<BF16>(p0 - back.x, p1 - back.y));
+          for (int i = 0; i < D / 16; ++i) {
+            o[i][q][0] *= c[0];
+            o[i][q][1] *= c[1];
+            o[i][q][2] *= c[0];
+            o[i][q][3] *= c[1];
+          }
+        }
       }
-    {
-      // V^T: keys (lane & 7) + 8 (lane >> 4), 16-byte chunk + ((lane >> 3) & 1)
-      const int key = (lane & 7) + ((lane >> 4) << 3), cc = (lane >> 3) & 1, x7 = key & 7;
-      constexpr int GROUP = 4 / NQ;  // dims whose products stand between the two that add to one sum
+      float base[NQ][2];
 #pragma unroll
-      for (int d0 = 0; d0 < D / 16; d0 += GROUP) {
-        uint32_t f[GROUP][4];
+      for (int q = 0; q < NQ; ++q)
 #pragma unroll
-        for (int d = 0; d < GROUP; ++d)
-          ldsm4t(f[d], va + static_cast<uint32_t>(((d0 + d) / 4) * Tile::SLICE + key * 128 + ((((2 * (d0 + d)) & 7) + cc) ^ x7) * 16));
+        for (int e = 0; e < 2; ++e) base[q][e] = m[q][e] == -INFINITY ? 0.0f : m[q][e];
+      uint32_t ph[NQ][2], pl[NQ][2];  // p^T, upper and lower part: the B operand
 #pragma unroll
-        for (int d = 0; d < GROUP; ++d)
+      for (int q = 0; q < NQ; ++q)
 #pragma unroll
-          for (int q = 0; q < NQ; ++q) mma16816<BF16>(o[d0 + d][q], f[d], ph[q][0], ph[q][1]);
+        for (int e = 0; e < 2; ++e) {
+          const float p0 = ex2(s[0][q][2 * e] - base[q][0]), p1 = ex2(s[0][q][2 * e + 1] - base[q][1]);
+          l[q][0] += p0;
+          l[q][1] += p1;
+          const uint32_t hi = pack2<BF16>(p0, p1);
+          const float2 back = unpack2<BF16>(hi);
+          ph[q][e] = transpose8(hi);
+          pl[q][e] = transpose8(pack2<BF16>(p0 - back.x, p1 - back.y));
+        }
+      {
+        // V^T: keys (lane & 7) + 8 (lane >> 4), 16-byte chunk + ((lane >> 3) & 1)
+        const int key = (lane & 7) + ((lane >> 4) << 3), cc = (lane >> 3) & 1, x7 = key & 7;
+        constexpr int GROUP = 4 / NQ;  // dims whose products stand between the two that add to one sum
 #pragma unroll
-        for (int d = 0; d < GROUP; ++d)
+        for (int d0 = 0; d0 < D / 16; d0 += GROUP) {
+          uint32_t f[GROUP][4];
 #pragma unroll
-          for (int q = 0; q < NQ; ++q) mma16816<BF16>(o[d0 + d][q], f[d], pl[q][0], pl[q][1]);
+          for (int d = 0; d < GROUP; ++d)
+            ldsm4t(f[d], va + static_cast<uint32_t>(((d0 + d) / 4) * Tile::SLICE + key * 128 + ((((2 * (d0 + d)) & 7) + cc) ^ x7) * 16));
+#pragma unroll
+          for (int d = 0; d < GROUP; ++d)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) mma16816<BF16>(o[d0 + d][q], f[d], ph[q][0], ph[q][1]);
+#pragma unroll
+          for (int d = 0; d < GROUP; ++d)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) mma16816<BF16>(o[d0 + d][q], f[d], pl[q][0], pl[q][1]);
+        }
       }
     }
     __syncwarp();  // every lane has read the stage
@@ -646,9 +667,9 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
 //
 // TEAM: the four warps of a CTA share a row, each every fourth part, and meet in
 // shared memory.
-template <int D, bool BF16, int NQ, bool TEAM>
+template <int D, bool BF16, int R, bool TEAM>
 __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
-  constexpr int E = D / 32, R = 8 * NQ, AHEAD = 4, STRIDE = TEAM ? 4 : 1;
+  constexpr int E = D / 32, AHEAD = 4, STRIDE = TEAM ? 4 : 1;
   const int lane = static_cast<int>(threadIdx.x) & 31, w = static_cast<int>(threadIdx.x) >> 5;
   const int64_t out_row = TEAM ? static_cast<int64_t>(blockIdx.x) : static_cast<int64_t>(blockIdx.x) * 4 + w;
   const int token = static_cast<int>(out_row / a.Hq), head = static_cast<int>(out_row - static_cast<int64_t>(token) * a.Hq);
@@ -663,7 +684,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
       const int m = (b + r) >> 1;
       if (a.offsets[m] <= token) b = m; else r = m;
     }
-    x = attn_row<R>(a, b + 1);
+    x = attn_row<R, AT_KEYS<D>>(a, b + 1);
     live = token >= x.t0 && token < x.t0 + x.n;
     if (!live) x.units = 0;
   }
