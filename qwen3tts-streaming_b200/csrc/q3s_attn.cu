@@ -71,11 +71,14 @@ Layout layout_of(const q3s_prefix_attention_desc* d) {
   const int64_t warps = split_warps();
   // A CTA of the prefix kernel has a SM for itself: this kernel's CTAs that
   // would be there start when it ends, that many units later (a unit takes 1.3
-  // us with 8-row items, 2 us with 16-row ones, and a CTA 3 us to get going).
+  // us with 8-row items, 2 us with 16-row ones, and a CTA 3 us to get going).  With
+  // 4, 8, 12 and 16 for the constant of 8-row items 96 rows take 35.0, 33.1, 32.8
+  // and 32.9 us, 256 rows behind 16000 keys 90.0, 90.2, 88.3 and 90.1; with 0, 4 and 8
+  // for that of 16-row ones 40 ragged rows 51.9, 51.7 and 52.3.
   const int64_t busy = l.splits ? std::min<int64_t>(static_cast<int64_t>(l.pairs) * d->kv_heads * l.splits, q3s::sm_count()) : 0;
   const int64_t ctas = warps / q3s::SplitTile<64, 1>::WARPS;
   l.early = static_cast<int>(ctas - busy * (ctas / q3s::sm_count()));
-  l.lead = l.splits ? (l.nq == 1 ? 8 + l.per_split * 17 / 10 : 4 + l.per_split) : 0;
+  l.lead = l.splits ? (l.nq == 1 ? 12 + l.per_split * 17 / 10 : 4 + l.per_split) : 0;
   const int64_t R = 8 * l.nq;
   l.tiles0 = l.splits || d->prefix_length == 0 ? 0 : static_cast<int>((queries + R - 1) / R);
   l.ids = (l.tiles0 + queries / R + d->batch + 1) * d->kv_heads;
