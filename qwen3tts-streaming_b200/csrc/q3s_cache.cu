@@ -235,19 +235,21 @@ struct AppendArgs {
 // block, so a CTA's stores are one run of memory.  With whole tokens a CTA
 // instead (all heads, short runs 16 blocks' strides apart) 12289 tokens of
 // 8 x 128 took 25 us against 20.6.  The data and the slots are requested side by
-// side.  12289 tokens in shuffled blocks, from cold: 21.7 us, 4.5 TB/s (a plain
-// copy's 6.5 TB/s would take 15.1); 8 tokens: 1.6 us.
+// side.  The heads of the same tokens are neighbours in the grid (22.0
+// us for 12289 tokens in shuffled blocks with the tokens there, and three CTAs a
+// SM; four 20.0; both 19.3: 5.1 TB/s, where a plain copy's 6.5 TB/s would take
+// 15.1); 8 tokens: 1.6 us.
 template <typename UNIT, int U>
-__global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256, 4) cache_append_kernel(const AppendArgs a) {
   using ELEM = typename std::conditional<sizeof(UNIT) == 16, uint16_t, UNIT>::type;
   constexpr int E = sizeof(UNIT) / sizeof(ELEM);
   const int t = static_cast<int>(threadIdx.x), per = max(256 / a.units, 1);  // tokens of a group
   const int row = t / a.units;
-  const int64_t token0 = static_cast<int64_t>(blockIdx.x) * per * U + row, limit = static_cast<int64_t>(a.blocks) * a.bs;
+  const int64_t token0 = static_cast<int64_t>(blockIdx.y) * per * U + row, limit = static_cast<int64_t>(a.blocks) * a.bs;
   grid_wait();
   grid_release();
   if (row >= per) return;
-  for (int part = static_cast<int>(blockIdx.y); part < 2 * a.H; part += static_cast<int>(gridDim.y)) {
+  for (int part = static_cast<int>(blockIdx.x); part < 2 * a.H; part += static_cast<int>(gridDim.x)) {
     const bool value = part >= a.H;
     const int64_t h = value ? part - a.H : part;
     const ELEM* from = static_cast<const ELEM*>(value ? a.v : a.k) + h * (value ? a.vh : a.kh);
@@ -287,10 +289,24 @@ cudaError_t launch_append(const AppendArgs& a, cudaStream_t st) {
   auto tiles = [&](int u) { return static_cast<unsigned>((static_cast<int64_t>(a.T) + static_cast<int64_t>(per) * u - 1) / (static_cast<int64_t>(per) * u)); };
   // Four groups a CTA once those CTAs are about one a SM; below, one, for more of
   // them.  One against four, 8 heads of 128: 256 tokens 2.1 against 2.3 us, 512
-  // tokens 2.6 against 2.3, 2048 tokens 6.0 against 4.2, 12289 tokens 29 against 16.
-  if (static_cast<int64_t>(tiles(4)) * parts * 4 >= 3 * sm_count())
-    return launch_maybe_pdl(cache_append_kernel<UNIT, 4>, dim3(tiles(4), parts), dim3(256), 0, st, true, a);
-  return launch_maybe_pdl(cache_append_kernel<UNIT, 1>, dim3(tiles(1), parts), dim3(256), 0, st, true, a);
+  // tokens 2.6 against 2.3, 2048 tokens 6.0 against 4.2, 12289 tokens 29 against 16
+  // (with the tokens first in the grid).
+  if (static_cast<int64_t>(tiles(4)) * parts * 4 < 3 * sm_count())
+    return launch_maybe_pdl(cache_append_kernel<UNIT, 1>, dim3(parts, tiles(1)), dim3(256), 0, st, true, a);
+  // a grid has 65535 rows of CTAs: millions of tokens take several
+  const int64_t most = static_cast<int64_t>(65535) * per * 4;
+  cudaError_t e = cudaSuccess;
+  for (int64_t t0 = 0; t0 < a.T && e == cudaSuccess; t0 += most) {
+    AppendArgs b = a;
+    constexpr int64_t size = sizeof(uint16_t);  // of an element, as the strides count them
+    b.T = static_cast<int>(std::min(most, a.T - t0));
+    b.k = static_cast<const unsigned char*>(a.k) + t0 * a.kt * size;
+    b.v = static_cast<const unsigned char*>(a.v) + t0 * a.vt * size;
+    b.slots = a.slots + t0;
+    e = launch_maybe_pdl(cache_append_kernel<UNIT, 4>, dim3(parts, static_cast<unsigned>((b.T + per * 4 - 1) / (per * 4))), dim3(256), 0,
+                         st, true, b);
+  }
+  return e;
 }
 
 }  // namespace q3s

@@ -206,6 +206,19 @@ def test_append_slot_outside_the_cache_is_skipped_and_reported(dev):
     q3s.cache_append(k[:0], k[:0], cache, cache, torch.zeros(0, dtype=torch.int64, device=dev))
 
 
+def test_append_more_tokens_than_one_grid_takes(dev):
+    """Rows of 257 elements, one token a group: 262140 tokens fill a grid."""
+    T = 262140 + 77
+    k = torch.randint(-1000, 1000, (T, 1, 257), dtype=torch.int16, device=dev).view(torch.bfloat16)
+    v = torch.randint(-1000, 1000, (T, 1, 257), dtype=torch.int16, device=dev).view(torch.bfloat16)
+    kc = torch.zeros(T // 7 + 1, 1, 7, 257, dtype=torch.bfloat16, device=dev)
+    vc = torch.zeros_like(kc)
+    slots = torch.arange(T, device=dev).flip(0)
+    q3s.cache_append(k, v, kc, vc, slots)
+    for x, c in ((k, kc), (v, vc)):
+        assert torch.equal(c.view(torch.int16).reshape(-1, 257)[:T].flip(0), x.view(torch.int16).reshape(T, 257))
+
+
 # ---- attention ------------------------------------------------------------------
 
 def make_attention(dev, *, n, lengths, prefix, q_heads, kv_heads, dim, block, dtype, seed=0, layout="heads", spread=1.0,
