@@ -203,8 +203,9 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const QuantArgs a) {
 
 // Many rows of up to 256 sixteen-byte units: a warp a row, the whole row in
 // registers, all its loads in flight at once and no barrier.  8192 rows of 2048
-// (50 MB): 11.9 us from cold, 4.2 TB/s.
-constexpr int QW_WARPS = 8, QW_KEEP = 8;
+// (50 MB): 11.9 us from cold, 4.2 TB/s.  Four warps a CTA: with eight 4096 rows of
+// 2048 took 4.6 us against 4.4; more CTAs a SM spill (5.4).
+constexpr int QW_WARPS = 4, QW_KEEP = 8;
 template <int ELEM>
 __global__ void __launch_bounds__(QW_WARPS * 32) quantize_warps_kernel(const QuantArgs a) {
   using E = Elem<ELEM>;
