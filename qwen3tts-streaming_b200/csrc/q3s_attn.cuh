@@ -289,7 +289,7 @@ Q3S_DEV AttnCut attn_cut(const AttnArgs& a, long long all, long long ctas, long 
   return c;
 }
 
-// The key-split kernel.  The keys of every item are cut into units of 16; all
+// The key-split kernel.  The keys of every item are cut into units of 4 KB; all
 // units of the batch form one list, cut into contiguous ranges, one a warp, so
 // that rows of any lengths load the GPU evenly with no more than one part per
 // item plus one per warp.  Each CTA derives the list from the device's lengths
@@ -311,11 +311,17 @@ Q3S_DEV AttnCut attn_cut(const AttnArgs& a, long long all, long long ctas, long 
 //
 // With one query a row this is bound by reading the cache (2 * G useful
 // operations a byte), as long as a warp's dependent chain of a unit stays below
-// the time that its 8 KB take: 61 rows of 6000 keys of 2 x 64 (117 MB) in 31.4 us
-// with the join, 3.7 TB/s, 96 rows of 500 behind a prefix of 1500 (130 MB) in 32.8.
-// With 16-row items the chain (two products of every score, in order) is the
-// longer of the two: 40 rows of 1 to 9 queries x 4 heads take 52 us of which the
-// bytes are 16.  Query rows as the instruction's M instead, with keys as N, took
+// the time that its 8 KB take: 6.8 TB/s while it streams (96 rows, from 4000 to 8000
+// keys), 61 rows of 6000 keys of 2 x 64 (117 MB) in 29.5 us with the start and the
+// join, 96 rows of 500 behind a prefix of 1500 (130 MB) in 32.6.  With 16-row items
+// the chain weighs as much, and several tiles copy the same keys: 40 rows of 1 to 9
+// queries x 4 heads take 51.5 us, 45 with the products taken out, of which the bytes
+// are 16; two warps sharing the copies of 32 rows took 344 in place of 417 us at 40
+// rows of 5 x 4 queries on 8000 keys and 57 here.
+//
+// The running maximum may lag by 8, as in the prefix kernel, so that a unit
+// mostly needs neither the maximum over the lanes nor O rescaled (52.4 to 51.5 us
+// for the 40 rows).  Query rows as the instruction's M instead, with keys as N, took
 // 34 us for the 96 rows before the join; copies by lanes (cp.async) in place of TMA
 // 1100 clocks for 32 keys; four 2 KB copies a unit in place of two of a
 // 5-dimensional map 900 clocks to issue.  The tcgen05 form, whose M is
