@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstring>
 
 #include "q3s_attn.cuh"
@@ -26,8 +27,13 @@ struct Layout {
 
 // Parts that the prefix kernel cuts the keys into.  A part costs its steps of
 // 128 keys plus about three for its start and end; the CTAs of all parts run
-// in waves of one a SM; and each part writes and the join reads fp32 sums of
-// all queries.  The number with the lowest estimate is taken.
+// in waves of one a SM; each part writes and the join reads fp32 sums of all
+// queries; and the SMs that the CTAs hold are time that the key-split kernel
+// beside them does not have, which weighs more where that one has 16-row items
+// (without the term 40 ragged rows took 6 parts and 51.6 us, with it 3 and 43.9;
+// 96 rows 6 and 32.6, 4 and 31.8; at the full weight 32 rows with short caches
+// behind 2048 keys took 18.1 us in place of 15.2).  The number with the lowest
+// estimate is taken.
 void plan_prefix(const q3s_prefix_attention_desc* d, Layout* l) {
   const int G = d->q_heads / d->kv_heads;
   l->per_tile = q3s::PX_M / G;
@@ -39,7 +45,8 @@ void plan_prefix(const q3s_prefix_attention_desc* d, Layout* l) {
   for (int s = 1; s <= l->steps && s <= 64; ++s) {
     const int per = (l->steps + s - 1) / s, parts = (l->steps + per - 1) / per;
     if (parts != s) continue;
-    const double cost = static_cast<double>((items * s + sms - 1) / sms) * (per + 3) * step_us + s * part_us;
+    const double part = (per + 3) * step_us, held = static_cast<double>(items * s) / sms;
+    const double cost = (std::ceil(held) + (l->nq == 1 ? 0.4 : 1.0) * held) * part + s * part_us;
     if (l->splits == 0 || cost < best) {
       best = cost;
       l->splits = s;
@@ -51,6 +58,12 @@ void plan_prefix(const q3s_prefix_attention_desc* d, Layout* l) {
 Layout layout_of(const q3s_prefix_attention_desc* d) {
   Layout l;
   const int64_t G = d->q_heads / d->kv_heads, queries = static_cast<int64_t>(d->tokens) * G;
+  // An item of the key-split kernel holds the query rows of an average row of
+  // the batch (an item reads its keys once), in tiles of 8 or 16.  8 against 16,
+  // 60 rows of 2000 keys: 8 query rows 85 against 93 us, 10 query rows 160
+  // against 95; 16 rows of 1000 keys: 13.4 against 17.7 and 19.0 against 18.1.
+  const int64_t mean = (queries + std::max(d->batch, 1) - 1) / std::max(d->batch, 1);
+  l.nq = mean <= 8 ? 1 : 2;
   // With few queries or keys the key-split kernel takes the prefix as one more
   // row: that costs it about queries * keys, the prefix kernel about the square
   // root of the keys (more of them are cut into more parts).  So the rule is on
@@ -62,23 +75,17 @@ Layout layout_of(const q3s_prefix_attention_desc* d) {
   // around, which the prefix kernel's running maximum does not follow.
   l.splits = 0;
   if (queries * queries >= 4000000 / std::max(d->prefix_length, 1) && d->prefix_length >= 64 && d->scale > 0.0f) plan_prefix(d, &l);
-  // An item of the key-split kernel holds the query rows of an average row of
-  // the batch (an item reads its keys once), in tiles of 8 or 16.  8 against 16,
-  // 60 rows of 2000 keys: 8 query rows 85 against 93 us, 10 query rows 160
-  // against 95; 16 rows of 1000 keys: 13.4 against 17.7 and 19.0 against 18.1.
-  const int64_t mean = (queries + std::max(d->batch, 1) - 1) / std::max(d->batch, 1);
-  l.nq = mean <= 8 ? 1 : 2;
   const int64_t warps = split_warps();
   // A CTA of the prefix kernel has a SM for itself: this kernel's CTAs that
   // would be there start when it ends, that many units later (a unit takes 1.3
   // us with 8-row items, 2 us with 16-row ones, and a CTA 3 us to get going).  With
   // 4, 8, 12 and 16 for the constant of 8-row items 96 rows take 35.0, 33.1, 32.8
-  // and 32.9 us, 256 rows behind 16000 keys 90.0, 90.2, 88.3 and 90.1; with 0, 4 and 8
-  // for that of 16-row ones 40 ragged rows 51.9, 51.7 and 52.3.
+  // and 32.9 us, 256 rows behind 16000 keys 90.0, 90.2, 88.3 and 90.1; with 4, 8 and 12
+  // for that of 16-row ones 40 ragged rows 45.3, 43.9 and 46.8.
   const int64_t busy = l.splits ? std::min<int64_t>(static_cast<int64_t>(l.pairs) * d->kv_heads * l.splits, q3s::sm_count()) : 0;
   const int64_t ctas = warps / q3s::SplitTile<64, 1>::WARPS;
   l.early = static_cast<int>(ctas - busy * (ctas / q3s::sm_count()));
-  l.lead = l.splits ? (l.nq == 1 ? 12 + l.per_split * 17 / 10 : 4 + l.per_split) : 0;
+  l.lead = l.splits ? (l.nq == 1 ? 12 + l.per_split * 17 / 10 : 8 + l.per_split) : 0;
   const int64_t R = 8 * l.nq;
   l.tiles0 = l.splits || d->prefix_length == 0 ? 0 : static_cast<int>((queries + R - 1) / R);
   l.ids = (l.tiles0 + queries / R + d->batch + 1) * d->kv_heads;
