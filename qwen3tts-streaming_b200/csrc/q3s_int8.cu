@@ -216,7 +216,6 @@ q3s_status quant_args(const q3s_quantize_rows_desc* d, const char* who, q3s::Qua
   a->values = d->values;
   a->ldv = d->values_row_stride;
   a->scales = d->scales;
-  a->release = false;
   const int n = d->elem == Q3S_ELEM_F32 ? 4 : 8;  // elements in 16 bytes
   *vec = a->K % n == 0 && q3s::aligned16(a->x) && reinterpret_cast<uintptr_t>(a->values) % n == 0 &&
          (a->M == 1 || (a->ldx % n == 0 && a->ldv % n == 0));
@@ -318,7 +317,6 @@ extern "C" q3s_status q3s_int8_linear(const q3s_quantize_rows_desc* q, const q3s
                        : d->elem == Q3S_ELEM_BF16 ? launch_gemv<true, Q3S_ELEM_BF16>(a, qa, st)
                                                   : launch_gemv<true, Q3S_ELEM_F16>(a, qa, st),
                        who);
-  qa.release = true;
   const cudaError_t e = quantize(qa, q->elem, vec, st);
   if (e != cudaSuccess) return cuda_status(e, who);
   return cuda_status(matmul(a, d->elem, st), who);

@@ -115,10 +115,6 @@ struct QuantArgs {
   int8_t* values;
   int64_t ldv;
   float* scales;
-  // Whether the next grid may start early.  Only where that is the product of
-  // these rows: a grid that reads weights before it waits for its predecessor
-  // must not find them being written here.
-  bool release;
 };
 
 // Block-wide maximum over NT threads (NaN if any thread's is).
@@ -146,7 +142,7 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const QuantArgs a) {
   __shared__ float s_red[NT / 32];
   const int t = static_cast<int>(threadIdx.x);
   grid_wait();
-  if (a.release) grid_release();
+  grid_release();
   const int64_t row = blockIdx.x;
   const typename E::T* x = static_cast<const typename E::T*>(a.x) + row * a.ldx;
   int8_t* out = a.values + row * a.ldv;
@@ -211,7 +207,7 @@ __global__ void __launch_bounds__(QW_WARPS * 32) quantize_warps_kernel(const Qua
   using E = Elem<ELEM>;
   constexpr int N = E::N;
   grid_wait();
-  if (a.release) grid_release();
+  grid_release();
   const int lane = static_cast<int>(threadIdx.x) & 31, chunks = a.K / N;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * QW_WARPS + (threadIdx.x >> 5);
   if (row >= a.M) return;
@@ -280,7 +276,8 @@ constexpr int GV_SMEM = 24 * 1024;  // most bytes of activations
 
 // M <= MB <= 8 rows: the product is bound by reading the weights once, and at
 // these sizes by latency.  A warp owns RW outputs and reads their weight rows
-// 512 bytes at a time, the first rounds of all of them before anything else; the
+// 512 bytes at a time, the first rounds of all of them before anything else
+// (after the grid's wait: the weights may come from the kernel before); the
 // activations sit in shared memory as bytes; sums are reduced over the warp by
 // one integer instruction each.  QUANT: the rows of x are quantised here, by
 // every CTA for itself (they are few), with the weights already on their way,
@@ -295,6 +292,8 @@ __global__ void __launch_bounds__(GV_NT) int8_gemv_kernel(const Int8Args a, cons
   const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
   const int n0 = (static_cast<int>(blockIdx.x) * GV_WARPS + w) * RW;
   const int rounds = (a.K + 511) / 512;
+  grid_wait();
+  grid_release();
   uint4 first[RW][AHEAD];
 #pragma unroll
   for (int r = 0; r < RW; ++r)
@@ -303,8 +302,6 @@ __global__ void __launch_bounds__(GV_NT) int8_gemv_kernel(const Int8Args a, cons
       const int k = 512 * c + 16 * lane;
       first[r][c] = n0 + r < a.N && k < a.K ? ld_stream16(a.w + (n0 + r) * a.ldw + k) : make_uint4(0, 0, 0, 0);
     }
-  grid_wait();  // the weights do not depend on the kernel before (QuantArgs::release)
-  grid_release();
   if constexpr (QUANT) {
     constexpr int GROUP = GV_NT / MB, KEEP = 4;  // threads of a row; 16-byte loads that stay in registers
     const int m = t / GROUP, i = t % GROUP, chunks = a.K / E::N;
@@ -529,25 +526,17 @@ __global__ void __launch_bounds__(I8C_NT)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   if (t == 0) {
-    auto load_w = [&](int c) { tma_load_2d(smem_u32(smem + (c % cut.stages) * stage_bytes), &tm_w, (c0 + c) * I8_BK, n0, &full[c % cut.stages]); };
-    // the weights do not depend on the kernel before (QuantArgs::release): they are on their way while it ends
-    const int ahead = min(count, cut.stages);
-    for (int c = 0; c < ahead; ++c) {
-      mbar_expect_tx(&full[c], stage_bytes);
-      load_w(c);
-    }
-    grid_wait();
+    grid_wait();  // rows and weights may both come from the kernel before
     for (int c = 0; c < count; ++c) {
       const int s = c % cut.stages;
-      if (c >= ahead) {
-        if (!mbar_wait_bounded(&empty[s], ((c / cut.stages) - 1) & 1)) {
-          atomicOr(&failed, 1);
-          break;
-        }
-        mbar_expect_tx(&full[s], stage_bytes);
-        load_w(c);
+      if (c >= cut.stages && !mbar_wait_bounded(&empty[s], ((c / cut.stages) - 1) & 1)) {
+        atomicOr(&failed, 1);
+        break;
       }
-      tma_load_2d(smem_u32(smem + s * stage_bytes + I8_TILE), &tm_a, (c0 + c) * I8_BK, token0, &full[s]);
+      const uint32_t dst = smem_u32(smem + s * stage_bytes);
+      mbar_expect_tx(&full[s], stage_bytes);
+      tma_load_2d(dst, &tm_w, (c0 + c) * I8_BK, n0, &full[s]);
+      tma_load_2d(dst + I8_TILE, &tm_a, (c0 + c) * I8_BK, token0, &full[s]);
     }
   } else if (t == 32) {
     const uint32_t idesc = i8_idesc(128, cut.bt);
