@@ -20,7 +20,8 @@ struct PrefixTile {
   static constexpr int HALVES = D / 64;                   // 64-element (128-byte) slices of a row
   static constexpr int Q_BYTES = PX_M * D * 2;
   static constexpr int KV_BYTES = PX_KEYS * D * 2;
-  static constexpr int SMEM = 1024 + 2 * Q_BYTES + 2 * PX_STAGES * KV_BYTES + 256;
+  static constexpr int USED = 1024 + 2 * Q_BYTES + 2 * PX_STAGES * KV_BYTES + 256;
+  static constexpr int SMEM = USED > TMEM_ALL_SMEM ? USED : TMEM_ALL_SMEM;  // all of the tensor memory
 };
 
 struct PrefixArgs {

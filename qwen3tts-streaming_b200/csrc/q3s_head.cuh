@@ -67,6 +67,18 @@ constexpr int HEAD_SMEM_LIMIT = 227 * 1024;     // per CTA
 // still computes and starts on the logits the moment the head's grid is done.
 constexpr int HEAD_SMEM_SHARED = 192 * 1024;
 
+// Tensor memory.  A SM has 512 columns; an allocation waits, without a limit,
+// until other CTAs of the SM free theirs.  A CTA of a cluster holds its columns
+// while it waits for the cluster's other CTAs, so if clusters of two grids (on
+// two streams) could fill each other's columns, two of them could wait for each
+// other for good.  So no CTAs that fit a SM together (228 KB of shared memory)
+// need more than 512 columns: a kernel that takes all of them asks for at least
+// TMEM_ALL_SMEM of dynamic shared memory, one that takes some for TMEM_PART_SMEM;
+// what the latter hold there besides (their partial sums) keeps several of them
+// within 512 columns.
+constexpr int TMEM_ALL_SMEM = 200 * 1024, TMEM_PART_SMEM = 32 * 1024;
+static_assert(TMEM_ALL_SMEM + TMEM_PART_SMEM > 228 * 1024, "not on one SM");
+
 // One configuration: KS CTAs per cluster (one K slice each, 4 or 8) and a
 // vocabulary tile of BN entries (the MMA's N).
 template <int KS, int BN>
@@ -91,6 +103,7 @@ struct HeadTile {
   static_assert(STAGES >= 2 && STAGING_BYTES <= RING_BYTES, "ring");
   static_assert(SLOT_BYTES % 16 == 0, "bulk copy sizes");
   static_assert(SMEM_BYTES <= HEAD_SMEM_LIMIT, "shared memory");
+  static_assert(SMEM_BYTES >= TMEM_PART_SMEM, "shared memory of a kernel that takes tensor memory");
 };
 
 struct HeadArgs {

@@ -73,16 +73,16 @@ bool few_rows(int M, int K) { return M <= q3s::GV_MAX_M && static_cast<int64_t>(
 
 // -- tensor cores --
 template <int ELEM, int KS>
-cudaError_t launch_split_ks(const q3s::Int8Args& a, const q3s::I8Cut& cut, dim3 grid, int smem, const CUtensorMap& tw,
-                            const CUtensorMap& ta, cudaStream_t st) {
+cudaError_t launch_split_ks(const q3s::Int8Args& a, const q3s::I8Cut& cut, const CUtensorMap& tw, const CUtensorMap& ta,
+                            cudaStream_t st) {
   auto kern = q3s::int8_split_kernel<ELEM, KS>;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = q3s::allow_smem(kern, 220 * 1024, done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t lc = {};
-  lc.gridDim = grid;
+  lc.gridDim = dim3((a.N + 127) / 128, KS, (a.M + cut.bt - 1) / cut.bt);
   lc.blockDim = dim3(q3s::I8C_NT);
-  lc.dynamicSmemBytes = smem;
+  lc.dynamicSmemBytes = cut.smem;
   lc.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -99,54 +99,13 @@ cudaError_t launch_split_ks(const q3s::Int8Args& a, const q3s::I8Cut& cut, dim3 
 
 template <int ELEM>
 cudaError_t launch_split(const q3s::Int8Args& a, cudaStream_t st) {
-  q3s::I8Cut cut;
-  cut.chunks = (a.K + q3s::I8_BK - 1) / q3s::I8_BK;
-  const int ntiles = (a.N + 127) / 128, sms = q3s::sm_count();
-  // Tile height and K cut: the lowest estimate of the time in clocks.  A CTA loads
-  // its operands (168 bytes a clock of a SM, shared by the CTAs there), reads its
-  // sums out of TMEM and joins its share of the cluster's; two CTAs share a SM
-  // where three stages of each fit, and overlap all but a little of the latter.
-  // The constants are fitted to 400 timings over 26 shapes from 12 x 2048 x 5000
-  // to 8000 x 512 x 100, on which the choice is 3% slower than the best in the
-  // mean and 12% at most.
-  auto stage_of = [](int bt) { return q3s::I8_TILE + bt * q3s::I8_BK; };
-  auto per_sm = [&](int bt) { return 110 * 1024 / stage_of(bt) >= 3 && bt * 512 <= 108 * 1024 ? 2 : 1; };
-  const double cluster_clocks[4] = {0, 50, 730, 2350};  // of 1, 2, 4, 8 CTAs
-  int ks = 1;
-  double best = 0;
-  for (int mt = (a.M + 255) / 256; mt <= (a.M + 31) / 32; ++mt) {
-    const int bt = ((a.M + mt - 1) / mt + 31) / 32 * 32;
-    if ((a.M + bt - 1) / bt != mt) continue;
-    for (int e = 0; e < 4 && cut.chunks >= (1 << e); ++e) {
-      const int k = 1 << e;
-      const double ctas = static_cast<double>(ntiles) * mt * k;
-      const double waves = std::ceil(ctas / (per_sm(bt) * sms)), share = waves > 1 ? per_sm(bt) : std::max(1.0, ctas / sms);
-      const double loads = static_cast<double>((cut.chunks + k - 1) / k) * stage_of(bt) / 168;
-      const double sums = 2.6 * bt + cluster_clocks[e] + 24.0 * bt / k;
-      const double cost = waves * (loads * share + sums * (1 + 0.06 * (share - 1)));
-      if (best == 0 || cost < best) {
-        best = cost;
-        cut.bt = bt;
-        ks = k;
-      }
-    }
-  }
-  const int mtiles = (a.M + cut.bt - 1) / cut.bt, stage = stage_of(cut.bt);
-  cut.tmem = 32;
-  while (cut.tmem < cut.bt) cut.tmem *= 2;
-  const bool two = static_cast<int64_t>(ntiles) * mtiles * ks > sms && per_sm(cut.bt) == 2;
-  const int mine = (cut.chunks + ks - 1) / ks;
-  // a ring that also holds the partial sums of the tile
-  const int least = (cut.bt * 512 + stage - 1) / stage;
-  cut.stages = std::max(least, std::min({8, mine, (two ? 110 : 196) * 1024 / stage}));
-  const int smem = 1024 + cut.stages * stage;
+  const q3s::I8Cut cut = q3s::int8_cut(a.M, a.N, a.K, q3s::sm_count());
   CUtensorMap tw, ta;
   if (!byte_map(&tw, a.w, a.N, a.K, a.ldw, 128) || !byte_map(&ta, a.a, a.M, a.K, a.lda, cut.bt)) return cudaErrorInvalidValue;
-  const dim3 grid(ntiles, ks, mtiles);
-  if (ks == 1) return launch_split_ks<ELEM, 1>(a, cut, grid, smem, tw, ta, st);
-  if (ks == 2) return launch_split_ks<ELEM, 2>(a, cut, grid, smem, tw, ta, st);
-  if (ks == 4) return launch_split_ks<ELEM, 4>(a, cut, grid, smem, tw, ta, st);
-  return launch_split_ks<ELEM, 8>(a, cut, grid, smem, tw, ta, st);
+  if (cut.ks == 1) return launch_split_ks<ELEM, 1>(a, cut, tw, ta, st);
+  if (cut.ks == 2) return launch_split_ks<ELEM, 2>(a, cut, tw, ta, st);
+  if (cut.ks == 4) return launch_split_ks<ELEM, 4>(a, cut, tw, ta, st);
+  return launch_split_ks<ELEM, 8>(a, cut, tw, ta, st);
 }
 
 template <int ELEM>

@@ -1,6 +1,7 @@
 """What the decode step's operators promise about order, resources and reports,
 as far as it can be checked without a GPU."""
 import re
+import subprocess
 from pathlib import Path
 
 import pytest
@@ -29,3 +30,52 @@ def test_8_bit_kernels_read_no_operand_before_they_wait(kernel):
     body = kernel_bodies("q3s_int8.cuh")[kernel]
     before = body[:body.index("grid_wait()")]
     assert not re.search(r"ld_stream16|tma_load|reinterpret_cast<const|a_scales|w_scales|bias", before), before
+
+
+TENSOR_MEMORY_PROGRAM = r"""
+#include <cstdio>
+#include <set>
+#include <utility>
+#include "q3s_attn_prefix.cuh"
+#include "q3s_int8.cuh"
+int main() {
+  std::set<std::pair<int, int>> cuts;  // the cluster product's shared memory and columns, over its range of shapes
+  for (int M : {1, 2, 9, 16, 31, 32, 33, 64, 65, 96, 97, 128, 129, 160, 161, 192, 200, 224, 225, 256, 257, 300, 400, 513, 1000, 3000, 9400})
+    for (int N : {1, 128, 257, 1000, 2048, 5000, 9000, 18000})
+      for (int K : {16, 128, 144, 256, 272, 512, 528, 1024, 2048, 4096, 6144, 16384, 131056}) {
+        const q3s::I8Cut c = q3s::int8_cut(M, N, K, 148);
+        cuts.insert({c.smem, c.tmem});
+      }
+  for (const auto& c : cuts) printf("split %d %d\n", c.first, c.second);
+  printf("pair %d 512\n", q3s::I8P_SMEM);
+  printf("prefix %d 512\nprefix %d 512\n", q3s::PrefixTile<64>::SMEM, q3s::PrefixTile<128>::SMEM);
+  printf("head %d %d\n", q3s::HeadTile<4, 64>::SMEM_BYTES, q3s::HeadTile<4, 64>::TMEM_COLS);
+  printf("head %d %d\n", q3s::HeadTile<4, 96>::SMEM_BYTES, q3s::HeadTile<4, 96>::TMEM_COLS);
+  printf("head %d %d\n", q3s::HeadTile<4, 128>::SMEM_BYTES, q3s::HeadTile<4, 128>::TMEM_COLS);
+  printf("head %d %d\n", q3s::HeadTile<8, 128>::SMEM_BYTES, q3s::HeadTile<8, 128>::TMEM_COLS);
+  printf("head %d %d\n", q3s::HeadTile<8, 192>::SMEM_BYTES, q3s::HeadTile<8, 192>::TMEM_COLS);
+}
+"""
+
+
+def test_kernels_on_one_multiprocessor_never_wait_for_each_others_tensor_memory(tmp_path):
+    """CTAs that fit a SM together, by shared memory alone (228 KB, 1 KB of it reserved a CTA), need 512 columns at most:
+    a CTA of a cluster that waited for another grid's columns could wait for good."""
+    from q3s import build
+
+    src, exe = tmp_path / "columns.cu", tmp_path / "columns"
+    src.write_text(TENSOR_MEMORY_PROGRAM)
+    subprocess.run([build.nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", f"-I{CSRC}", f"-I{build.INCLUDE}",
+                    "-o", str(exe), str(src)], check=True, capture_output=True)
+    lines = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split("\n")
+    kinds = {}
+    for kind, smem, columns in (ln.split() for ln in lines if ln):
+        kinds.setdefault(int(columns), []).append((int(smem), kind))
+    assert sum(len(v) for v in kinds.values()) > 20
+    unit = 128  # shared memory is handed out in pieces of this size
+    room = 228 * 1024 // unit
+    need = {c: (min(v)[0] + 1024) // unit for c, v in kinds.items()}  # a kernel's least shared memory decides
+    most = [0] * (room + 1)  # columns that CTAs within so much shared memory can ask for
+    for x in range(room + 1):
+        most[x] = max([0] + [most[x - n] + c for c, n in need.items() if n <= x])
+    assert most[room] <= 512, (most[room], {c: min(v) for c, v in kinds.items()})
