@@ -119,7 +119,9 @@ q3s_status q3s_cache_append(const q3s_cache_append_desc* desc, void* stream);
  * with 0 and -inf for a query that sees nothing.  Softmax statistics and sums
  * are 32-bit.  For the product with v, as the tensor cores take it,
  * probabilities over the prefix of a large batch are rounded to the cache's
- * type, the others held as the sum of two such values.  A key that a query does
+ * type (and divided by the sum of what was rounded: with U its unit roundoff,
+ * that moves out by U sum p |v - out| at most), the others held as the sum of
+ * two such values.  A key that a query does
  * not see has no part in its result, whatever k and v hold there. */
 typedef struct q3s_prefix_attention_desc {
   uint32_t struct_size;        /* = sizeof(q3s_prefix_attention_desc) */

@@ -172,9 +172,14 @@ Q3S_DEV float max3(float a, float b, float c) {
 //
 // The running maximum is allowed to lag by 8 (p up to 256, sums in fp32), so
 // O is rescaled only when a score rises above that: the first step sets it,
-// later ones almost never.  l sums the unrounded p.  Rounding p to 16 bits is
-// what the product takes; the prefix of a large batch has many keys, over
-// which it averages out (the other kernel, for few keys, holds p in two).
+// later ones almost never.  The product takes p rounded to 16 bits.  l sums the
+// unrounded p, for the log-sum-exp and the join, and a second sum the rounded
+// ones: O is divided by that one (times l) at the end, so that a rounding moves
+// the result by p |v - out|, not p |v|: next to nothing where one key carries the
+// row, and over many keys it averages out (the other kernel, for few keys, holds
+// p in two parts).  With U the type's unit roundoff the result is off by
+// U |out| + U sum p |v - out|.  The second sum costs three instructions a pair of
+// keys (the 256 rows below 92 us in place of 88; in one chain 93).
 //
 // Keys past the end: whole boxes read as zeros (an out-of-range block
 // coordinate), the rest of the last one is cleared in V and masked in S.
@@ -386,7 +391,7 @@ __global__ void __launch_bounds__(PX_NT, 1)
     if (i < tiles) {
       const uint32_t lanes = static_cast<uint32_t>((w & 3) * 32) << 16;
       const uint32_t ts = tmem + lanes + static_cast<uint32_t>(128 * i), to = tmem + lanes + static_cast<uint32_t>(256 + 128 * i);
-      float m = -INFINITY, l = 0.0f;
+      float m = -INFINITY, l = 0.0f, lr = 0.0f;  // lr: of the rounded p
       bool ok = true;
       for (int j = 0; j < steps; ++j) {
         ok = __all_sync(FULL, wait(&s_full[i], j & 1));
@@ -415,6 +420,7 @@ __global__ void __launch_bounds__(PX_NT, 1)
           const float nm = rise ? top : m;
           const float c = rise ? ex2(m - nm) : 1.0f;  // 0 from -inf
           l *= c;
+          lr *= c;
           m = nm;
           if (j > 0) {
             ok = __all_sync(FULL, wait(&o_done[i], (j - 1) & 1));
@@ -433,7 +439,7 @@ __global__ void __launch_bounds__(PX_NT, 1)
         }
         const float base = m == -INFINITY ? 0.0f : m;
         const float2 sc = make_float2(a.scale_log2, a.scale_log2), nb = make_float2(-base, -base);
-        float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
+        float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0, rounded0 = sum0, rounded1 = sum0;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t pk[32];
@@ -444,12 +450,15 @@ __global__ void __launch_bounds__(PX_NT, 1)
             e.y = ex2(e.y);
             if (c & 1) sum1 = __fadd2_rn(sum1, e); else sum0 = __fadd2_rn(sum0, e);
             pk[c] = pack2<BF16>(e.x, e.y);
+            const float2 r2 = unpack2<BF16>(pk[c]);
+            if (c & 1) rounded1 = __fadd2_rn(rounded1, r2); else rounded0 = __fadd2_rn(rounded0, r2);
           }
           tmem_st32(ts + static_cast<uint32_t>(32 * half), pk);
           tc_fence_before();
           mbar_arrive(half ? &p_full[i] : &p_half[i]);
         }
         l += (sum0.x + sum1.x) + (sum0.y + sum1.y);
+        lr += (rounded0.x + rounded1.x) + (rounded0.y + rounded1.y);
       }
       if (ok) ok = __all_sync(FULL, wait(&o_done[i], (steps - 1) & 1));
       if (ok) {
@@ -462,13 +471,14 @@ __global__ void __launch_bounds__(PX_NT, 1)
         static_assert(2 * PX_M * PITCH + 1024 <= Tile::Q_BYTES + 2 * PX_STAGES * Tile::KV_BYTES, "room for both tiles");
         static_assert(PX_M * PITCH <= Tile::Q_BYTES + PX_STAGES * Tile::KV_BYTES, "tile 0 leaves V alone");
         unsigned char* stage = s_q + Tile::Q_BYTES + i * PX_M * PITCH + row * PITCH;
+        const float even = lr > 0.0f ? l / lr : 1.0f;
 #pragma unroll 1
         for (int k = 0; k < D / 32; ++k) {
           float v[32];
           tmem_ld32(to + static_cast<uint32_t>(32 * k), v);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            *reinterpret_cast<float4*>(stage + (8 * k + e) * 16) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+            *reinterpret_cast<float4*>(stage + (8 * k + e) * 16) = make_float4(v[4 * e] * even, v[4 * e + 1] * even, v[4 * e + 2] * even, v[4 * e + 3] * even);
         }
         const int token = token0 + i * p.per_tile + row / a.G;
         if (row < p.per_tile * a.G && token < a.T) {  // there is such a query row

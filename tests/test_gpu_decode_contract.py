@@ -3,6 +3,7 @@ on the GPU, against plain forms in Python integers and float64."""
 import pytest
 import torch
 
+import decode_reference as R
 import q3s
 
 pytestmark = pytest.mark.gpu
@@ -50,3 +51,45 @@ def test_weight_written_by_another_kernel_right_before(dev, rows):
         y = q3s.int8_matmul(a, s[:rows], w, s, dtype=torch.float32)
         want, tol = exact_product(a, s[:rows], fresh, s)
         assert bool(((y.double() - want).abs() <= tol).all())
+
+
+# ---- attention: one key carries a query ------------------------------------------
+
+@pytest.mark.parametrize("dim,dtype", [(128, torch.bfloat16), (64, torch.bfloat16), (128, torch.float16), (64, torch.float16)])
+def test_attention_one_key_carries_the_prefix(dev, dtype, dim):
+    """A key far above all others, met after the running maximum was set 2^7 to 2^8 below it.
+
+    With U the type's unit roundoff, probabilities rounded to that type and divided by their own sum move the result by U
+    sum p |v - out| at most (to first order; U^2 mass for the rest), its own rounding by U |out|, ex2 and the 32-bit sums
+    by less than 2^-16 of sum p |v|, and in f16 each of the keys' probabilities, subnormal below 2^-14, by 2^-25."""
+    rows, heads, kv_heads, keys, block = 64, 8, 2, 4096, 16
+    g = torch.Generator().manual_seed(dim)
+    scale = dim ** -0.5
+    blocks = keys // block + rows
+    k = torch.zeros(blocks, kv_heads, block, dim)
+    v = torch.randn(blocks, kv_heads, block, dim, generator=g)
+    # scores, in units of log 2, along the first dimension: q is 1 to 8/7 there, times what makes 7 of a key's 1
+    unit = 7 * 0.6931471805599453 / scale
+    k[..., 0] = -4.0  # the others: 2^-28
+    first = k[:keys // block].transpose(1, 2).reshape(keys, kv_heads, dim)
+    first[::128, :, 0] = 0.0  # one of each 128 keys sets the running maximum to 0
+    first[7 * 128 + 77, :, 0] = 1.0  # and this one is above it
+    k[:keys // block] = first.reshape(keys // block, block, kv_heads, dim).transpose(1, 2)
+    q = torch.zeros(rows, heads, dim)
+    q[..., 0] = unit * (1 + torch.rand(rows, heads, generator=g) / 7.2)
+    q, k, v = (x.to(dtype) for x in (q, k, v))
+    table = torch.arange(keys // block, blocks, dtype=torch.int32)[:, None]
+    offsets = torch.arange(rows + 1, dtype=torch.int32)
+    shared, lengths = torch.arange(keys // block, dtype=torch.int32), torch.ones(rows, dtype=torch.int32)
+    out, lse = q3s.prefix_attention(q.to(dev), k.to(dev), v.to(dev), offsets.to(dev), table.to(dev), lengths.to(dev),
+                                    prefix_blocks=shared.to(dev), prefix_length=keys, scale=scale, return_lse=True)
+    want, want_lse, mass = R.prefix_attention(q, k, v, offsets, table, lengths, shared, keys, scale)
+    # sum p |v - out|: the key that carries the query, and the rest (whose p sum to 1 - p of it)
+    top = v.double()[(7 * 128 + 77) // block, :, (7 * 128 + 77) % block].repeat_interleave(heads // kv_heads, 0)
+    p = torch.exp(scale * q.double()[..., 0] * 1.0 - want_lse)[..., None]
+    away = p * (top - want).abs() + (mass - p * top.abs()).clamp(min=0) + (1 - p) * want.abs()
+    U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
+    tol = U * want.abs() + U * away + (U * U + 2.0 ** -16) * mass + (keys * 2.0 ** -25 * 5 if dtype == torch.float16 else 0)
+    d = (out.cpu().double() - want).abs()
+    assert bool((d <= tol).all()), f"worst {float((d / tol).max())} of the tolerance"
+    assert bool(((lse.cpu().double() - want_lse).abs() <= 2.0 ** -16 * (1 + want_lse.abs())).all())
