@@ -122,7 +122,9 @@ q3s_status q3s_cache_append(const q3s_cache_append_desc* desc, void* stream);
  * type (and divided by the sum of what was rounded: with U its unit roundoff,
  * that moves out by U sum p |v - out| at most), the others held as the sum of
  * two such values.  A key that a query does
- * not see has no part in its result, whatever k and v hold there. */
+ * not see has no part in its result, whatever k and v hold there; an infinity
+ * in v of one that it sees makes out that infinity (NaN where the key's
+ * probability underflows). */
 typedef struct q3s_prefix_attention_desc {
   uint32_t struct_size;        /* = sizeof(q3s_prefix_attention_desc) */
   int32_t batch;               /* B, 0..Q3S_MAX_CACHE_ROWS */

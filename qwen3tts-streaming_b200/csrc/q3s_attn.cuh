@@ -210,13 +210,15 @@ struct SplitTile {
   static constexpr int SMEM = 1024 + WARPS * STAGES * 2 * BYTES;
 };
 
-// A part again, key by key, with what a query does not see left out instead of
-// taken times p = 0: there an infinity or NaN in V would reach the queries of
-// the part that do not see it.  Only for parts whose queries see different keys
-// and whose sums are not finite; one warp, queries in turn, D / 32 dims a lane.
+// A part again, key by key, with p in one piece and what a query does not see
+// left out instead of taken times p = 0: there an infinity or NaN in V would
+// reach the queries of the part that do not see it, and an infinity times the
+// lower piece of p would be NaN for those that do.  Only for the queries in
+// `which`, whose sums are not finite though their scores are; one warp, queries
+// in turn, D / 32 dims a lane.
 template <int D, bool BF16, int R>
 Q3S_DEV void attn_part_by_key(const AttnArgs& a, const AttnRow& x, int r, int h, int tile, int first_u, int last_u,
-                              int64_t slot, int lane) {
+                              int64_t slot, uint32_t which, int lane) {
   constexpr int E = D / 32, KEYS = AT_KEYS<D>;
   auto dims = [&](const void* at, int64_t offset, float (&y)[E]) {
     const uint32_t* p = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(at) + offset + lane * E);
@@ -226,18 +228,18 @@ Q3S_DEV void attn_part_by_key(const AttnArgs& a, const AttnRow& x, int r, int h,
       y[e] = f.x, y[e + 1] = f.y;
     }
   };
-  const int rows = min(R, x.n * a.G - tile * R);
+  const int32_t* blocks = r == 0 ? a.prefix_blocks : a.table + (r - 1) * a.table_stride;
 #pragma unroll 1
-  for (int i = 0; i < rows; ++i) {
-    const int row = tile * R + i, token = row / a.G;
+  for (; which; which &= which - 1) {
+    const int i = __ffs(which) - 1, row = tile * R + i, token = row / a.G;
     float q[E], acc[E], m = -INFINITY, l = 0.0f;
     dims(a.q, static_cast<int64_t>(x.t0 + token) * a.qt + (static_cast<int64_t>(h) * a.G + row % a.G) * a.qh, q);
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-    const int end = min((last_u + 1) * KEYS, x.len - x.n + token + 1);
+    const int end = min((last_u + 1) * KEYS, x.causal ? x.len - x.n + token + 1 : x.len);
 #pragma unroll 1
     for (int j = first_u * KEYS; j < end; ++j) {
-      const int id = a.table[(r - 1) * a.table_stride + (j >> a.bs_log2)], place = j & (a.bs - 1);
+      const int id = blocks[j >> a.bs_log2], place = j & (a.bs - 1);
       float k[E], v[E], s = 0.0f;
 #pragma unroll
       for (int e = 0; e < E; ++e) k[e] = v[e] = 0.0f;
@@ -302,7 +304,8 @@ Q3S_DEV AttnCut attn_cut(const AttnArgs& a, long long all, long long ctas, long 
 // computing it.  What lies
 // past the end of a row's last unit is cleared in V (so that nothing that lies
 // there, NaN included, reaches the products) and masked in the scores; a key that some of an
-// item's queries see and others do not is masked for those, and counts for nothing (attn_part_by_key).  Both
+// item's queries see and others do not is masked for those, and counts for nothing; where V is not finite,
+// attn_part_by_key takes the part again.  Both
 // products have the keys' side as the matrix instruction's M (m16n8k16):
 // S^T = K Q^T, O^T += V^T P^T, with N = 8 query rows, so one query a row and its
 // group of heads waste little of it.  p is carried as the sum of two 16-bit
@@ -631,7 +634,7 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
           a.items[id] = make_int2(static_cast<int>(slot), parts);
         }
         float* po = a.part_o + slot * (R * D);
-        float size = 0.0f;  // NaN if one of the sums is not finite
+        uint32_t odd = 0;  // query rows whose sums are not finite, though the sum of their p is
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -640,6 +643,8 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(FULL, x, d);
             const int row = 8 * q + 2 * tq + e;
+            float size = x * 0.0f;  // 0, and NaN once something is not finite
+            const bool known = size == 0.0f;
             if (row < M) {
 #pragma unroll
               for (int i = 0; i < D / 16; ++i) {
@@ -649,10 +654,14 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
               }
               if (g == 0) a.part_ml[slot * R + row] = make_float2(m[q][e], x);
             }
+            const uint32_t lanes = __ballot_sync(FULL, row < M && known && size != 0.0f);
+#pragma unroll
+            for (int d = 0; d < 4; ++d)  // lanes d, d + 4, .. hold row 8 q + 2 d + e
+              if (lanes & (0x11111111u << d)) odd |= 1u << (8 * q + 2 * d + e);
           }
-        if (wx.causal && wx.n > 1 && __any_sync(FULL, size != 0.0f)) {
+        if (odd) {
           __syncwarp();  // its writes come after those above
-          attn_part_by_key<D, BF16, R>(a, wx, wr, wh, wt, first_u, wu, slot, lane);
+          attn_part_by_key<D, BF16, R>(a, wx, wr, wh, wt, first_u, wu, slot, odd, lane);
         }
       }
     }

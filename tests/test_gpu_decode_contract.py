@@ -93,3 +93,37 @@ def test_attention_one_key_carries_the_prefix(dev, dtype, dim):
     d = (out.cpu().double() - want).abs()
     assert bool((d <= tol).all()), f"worst {float((d / tol).max())} of the tolerance"
     assert bool(((lse.cpu().double() - want_lse).abs() <= 2.0 ** -16 * (1 + want_lse.abs())).all())
+
+
+# ---- attention: infinities in V -----------------------------------------------------
+
+@pytest.mark.parametrize("dim,dtype", [(128, torch.bfloat16), (64, torch.float16)])
+@pytest.mark.parametrize("rows,prefix", [(1, 0), (3, 40), (100, 600)])
+@pytest.mark.parametrize("n", [1, 2])
+def test_attention_infinity_that_a_query_sees(dev, dim, dtype, rows, prefix, n):
+    """+inf in one dim of V and -inf in another, of a row's first own key or of a key of the prefix, taken by either kernel:
+    the queries that see it have that infinity there, and nothing else changes."""
+    heads, kv_heads, own, block = 4, 2, 21, 16
+    g = torch.Generator(device=dev).manual_seed(rows + n)
+    shared = -(-prefix // block)
+    blocks = shared + 2 * rows
+    k, v = (torch.randn(blocks, kv_heads, block, dim, device=dev, generator=g).to(dtype) for _ in range(2))
+    q = torch.randn(rows * n, heads, dim, device=dev, generator=g).to(dtype)
+    i32 = dict(dtype=torch.int32, device=dev)
+    table = torch.arange(shared, blocks, **i32).view(rows, 2)
+    args = dict(prefix_blocks=torch.arange(shared, **i32), prefix_length=prefix, return_lse=True)
+    rest = (torch.arange(0, rows * n + 1, n, **i32), table, torch.full((rows,), own, **i32))
+    out, lse = q3s.prefix_attention(q, k, v, *rest, **args)
+    for block_of, place, hit in [(int(table[0, 0]), 0, slice(0, n))] + ([(prefix // 2 // block, prefix // 2 % block, slice(None))] if prefix else []):
+        w = v.clone()
+        w[block_of, :, place, 5] = float("inf")
+        w[block_of, :, place, 40] = -float("inf")
+        odd, odd_lse = q3s.prefix_attention(q, k, w, *rest, **args)
+        want = out.clone()
+        want[hit, :, 5] = float("inf")
+        want[hit, :, 40] = -float("inf")
+        finite = torch.isfinite(want)
+        assert torch.equal(odd[~finite], want[~finite])
+        # what is taken again key by key has its sums in another order and p in one piece: two roundings of the type apart
+        assert bool(((odd - want)[finite].abs().double() <= 2.0 ** (-7 if dtype == torch.bfloat16 else -10) * want[finite].abs().double() + 1e-3).all())
+        assert bool(((odd_lse - lse).abs() <= 2.0 ** -15 * (1 + lse.abs())).all())
