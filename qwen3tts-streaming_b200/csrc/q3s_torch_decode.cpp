@@ -10,8 +10,8 @@
 //   prefix_attention(q, k_cache, v_cache, query_offsets, block_table, lengths, prefix_blocks=None, prefix_length=0,
 //                    scale=None, error_word!=None) -> (out, lse)
 //   quantize_rows(x) -> (values, scales)
-//   int8_matmul(values, scales, weight, weight_scales, dtype, bias=None) -> y
-//   int8_linear(x, weight, weight_scales, bias=None) -> (y, values, scales)
+//   int8_matmul(values, scales, weight, weight_scales, dtype, bias=None, error_word!=None) -> y
+//   int8_linear(x, weight, weight_scales, bias=None, error_word!=None) -> (y, values, scales)
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -295,7 +295,7 @@ std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {
 }
 
 q3s_int8_matmul_desc matmul_desc(const Tensor& a, const Tensor& a_scales, const Tensor& w, const Tensor& w_scales,
-                                 const OptTensor& bias, const Tensor& y) {
+                                 const OptTensor& bias, const OptTensor& error_word, const Tensor& y) {
   const int64_t M = a.size(0), K = a.size(1), N = w.size(0);
   need(w, a, at::kChar, 2, "weight");
   TORCH_CHECK(w.size(1) == K && w.stride(1) == 1, "q3s: weight must be [N, ", K, "] with unit column stride, got ", w.sizes());
@@ -320,24 +320,25 @@ q3s_int8_matmul_desc matmul_desc(const Tensor& a, const Tensor& a_scales, const 
   }
   d.y = y.data_ptr();
   d.y_row_stride = N;
+  d.error_word = error_of(error_word, a);
   return d;
 }
 
 Tensor int8_matmul(const Tensor& values, const Tensor& scales, const Tensor& weight, const Tensor& weight_scales,
-                   at::ScalarType dtype, const OptTensor& bias) {
+                   at::ScalarType dtype, const OptTensor& bias, OptTensor error_word) {
   need_cuda(values, "values");
   c10::cuda::CUDAGuard guard(values.device());
   need(values, values, at::kChar, 2, "values");
   TORCH_CHECK(values.size(1) <= 1 || values.stride(1) == 1, "q3s: values must have unit column stride");
   TORCH_CHECK(weight.dim() == 2, "q3s: weight must be [N, K], got ", weight.sizes());
   Tensor y = make({values.size(0), weight.size(0)}, dtype, values);
-  const q3s_int8_matmul_desc d = matmul_desc(values, scales, weight, weight_scales, bias, y);
+  const q3s_int8_matmul_desc d = matmul_desc(values, scales, weight, weight_scales, bias, error_word, y);
   check_status(q3s_int8_matmul(&d, stream_of(values)), "q3s_int8_matmul");
   return y;
 }
 
 std::tuple<Tensor, Tensor, Tensor> int8_linear(const Tensor& x, const Tensor& weight, const Tensor& weight_scales,
-                                               const OptTensor& bias) {
+                                               const OptTensor& bias, OptTensor error_word) {
   const Tensor r = rows_of(x);
   c10::cuda::CUDAGuard guard(r.device());
   TORCH_CHECK(weight.dim() == 2, "q3s: weight must be [N, K], got ", weight.sizes());
@@ -347,7 +348,7 @@ std::tuple<Tensor, Tensor, Tensor> int8_linear(const Tensor& x, const Tensor& we
   Tensor values = part(arena, 0, {M, K}, at::kChar), scales = part(arena, at_scales, {M}, at::kFloat);
   Tensor y = make({M, N}, r.scalar_type(), r);
   const q3s_quantize_rows_desc q = quantize_desc(r, values, scales);
-  const q3s_int8_matmul_desc d = matmul_desc(values, scales, weight, weight_scales, bias, y);
+  const q3s_int8_matmul_desc d = matmul_desc(values, scales, weight, weight_scales, bias, error_word, y);
   check_status(q3s_int8_linear(&q, &d, stream_of(r)), "q3s_int8_linear");
   if (x.dim() == 2) return {y, values, scales};
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
@@ -375,11 +376,11 @@ std::tuple<Tensor, Tensor> quantize_rows_meta(const Tensor& x) {
           at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat))};
 }
 Tensor int8_matmul_meta(const Tensor& values, const Tensor&, const Tensor& weight, const Tensor&, at::ScalarType dtype,
-                        const OptTensor&) {
+                        const OptTensor&, OptTensor) {
   return at::empty({values.size(0), weight.size(0)}, values.options().dtype(dtype));
 }
 std::tuple<Tensor, Tensor, Tensor> int8_linear_meta(const Tensor& x, const Tensor& weight, const Tensor&,
-                                                    const OptTensor&) {
+                                                    const OptTensor&, OptTensor) {
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = weight.size(0);
   const auto q = quantize_rows_meta(x);
@@ -399,8 +400,9 @@ TORCH_LIBRARY_FRAGMENT(q3s, m) {
         "Tensor(a!)? error_word=None) -> (Tensor, Tensor)");
   m.def("quantize_rows(Tensor x) -> (Tensor, Tensor)");
   m.def("int8_matmul(Tensor values, Tensor scales, Tensor weight, Tensor weight_scales, ScalarType dtype, "
-        "Tensor? bias=None) -> Tensor");
-  m.def("int8_linear(Tensor x, Tensor weight, Tensor weight_scales, Tensor? bias=None) -> (Tensor, Tensor, Tensor)");
+        "Tensor? bias=None, Tensor(a!)? error_word=None) -> Tensor");
+  m.def("int8_linear(Tensor x, Tensor weight, Tensor weight_scales, Tensor? bias=None, Tensor(a!)? error_word=None) -> "
+        "(Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(q3s, CUDA, m) {

@@ -108,34 +108,39 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def int8_matmul(values: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, *,
-                dtype: torch.dtype = torch.bfloat16, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+                dtype: torch.dtype = torch.bfloat16, bias: Optional[torch.Tensor] = None,
+                error_word: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``(values @ weight^T) * scales[:, None] * weight_scales (+ bias)``:
     int8 [M, K] and [N, K] (K a multiple of 16), exact 32-bit sums, fp32
-    scales and bias, one rounding to ``dtype``."""
-    return _op("int8_matmul")(values, scales, weight, weight_scales, dtype, bias)
+    scales and bias, one rounding to ``dtype``.  ``error_word`` (int32 [1]) gets
+    ``DECERR_WAIT`` if a device wait gave up, which leaves the result
+    incomplete."""
+    return _op("int8_matmul")(values, scales, weight, weight_scales, dtype, bias, error_word)
 
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, *,
-                bias: Optional[torch.Tensor] = None, return_quantized: bool = False):
+                bias: Optional[torch.Tensor] = None, return_quantized: bool = False,
+                error_word: Optional[torch.Tensor] = None):
     """``quantize_rows(x)`` times an int8 weight [N, K] with a scale per
     output: y [..., N] in x's type.  ``return_quantized`` also returns the
     values and scales of x, for another product of the same activations
-    (``int8_matmul``)."""
-    y, values, scales = _op("int8_linear")(x, weight, weight_scales, bias)
+    (``int8_matmul``); ``error_word`` as there."""
+    y, values, scales = _op("int8_linear")(x, weight, weight_scales, bias, error_word)
     return (y, values, scales) if return_quantized else y
 
 
 class Int8Linear:
     """A Linear whose weight is held as int8 with a scale per output channel,
     quantised once from ``weight`` [N, K] (``nn.Linear.weight``; K a multiple
-    of 16)."""
+    of 16).  ``error_word`` collects ``DECERR_*`` bits of its calls."""
 
     def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
         self.weight, self.scales = quantize_rows(weight)
         self.bias = None if bias is None else bias.float().contiguous()
+        self.error_word = torch.zeros(1, dtype=torch.int32, device=self.weight.device)
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
-        return int8_linear(x, self.weight, self.scales, bias=self.bias)
+        return int8_linear(x, self.weight, self.scales, bias=self.bias, error_word=self.error_word)
 
 
 class PagedCache:

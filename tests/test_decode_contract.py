@@ -79,3 +79,14 @@ def test_kernels_on_one_multiprocessor_never_wait_for_each_others_tensor_memory(
     for x in range(room + 1):
         most[x] = max([0] + [most[x - n] + c for c, n in need.items() if n <= x])
     assert most[room] <= 512, (most[room], {c: min(v) for c, v in kinds.items()})
+
+
+def test_every_operator_with_device_waits_takes_an_error_word():
+    import q3s
+
+    q3s.load_torch_ops()
+    import torch
+
+    for name in ("cache_append", "prefix_attention", "int8_matmul", "int8_linear"):
+        arg = {a.name: a for a in getattr(torch.ops.q3s, name).default._schema.arguments}["error_word"]
+        assert arg.alias_info is not None and arg.alias_info.is_write and arg.default_value is None

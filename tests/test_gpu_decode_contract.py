@@ -1,5 +1,8 @@
 """What the decode step's operators promise about order, odd values and reports,
 on the GPU, against plain forms in Python integers and float64."""
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -127,3 +130,58 @@ def test_attention_infinity_that_a_query_sees(dev, dim, dtype, rows, prefix, n):
         # what is taken again key by key has its sums in another order and p in one piece: two roundings of the type apart
         assert bool(((odd - want)[finite].abs().double() <= 2.0 ** (-7 if dtype == torch.bfloat16 else -10) * want[finite].abs().double() + 1e-3).all())
         assert bool(((odd_lse - lse).abs() <= 2.0 ** -15 * (1 + lse.abs())).all())
+
+
+# ---- reports -------------------------------------------------------------------------
+
+# stands in front of the library's 8-bit products and keeps the error word that they are given
+SHIM = r"""
+#include "q3s_decode.h"
+extern "C" {
+const void* seen = 0;
+q3s_status q3s_int8_matmul(const q3s_int8_matmul_desc* d, void*) { seen = d->error_word; return Q3S_OK; }
+q3s_status q3s_int8_linear(const q3s_quantize_rows_desc*, const q3s_int8_matmul_desc* d, void*) { seen = d->error_word; return Q3S_OK; }
+}
+"""
+SHIM_CALLER = r"""
+import ctypes, sys
+shim = ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)
+sys.path.insert(0, sys.argv[2])
+import torch, q3s
+seen = ctypes.c_void_p.in_dll(shim, "seen")
+dev = torch.device("cuda:0")
+w, s = torch.ones(32, 64, dtype=torch.int8, device=dev), torch.ones(32, device=dev)
+x, err = torch.ones(3, 64, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+q3s.int8_matmul(w[:3], s[:3], w, s, error_word=err)
+assert seen.value == err.data_ptr(), "int8_matmul"
+q3s.int8_matmul(w[:3], s[:3], w, s)
+assert seen.value is None
+q3s.int8_linear(x, w, s, error_word=err)
+assert seen.value == err.data_ptr(), "int8_linear"
+linear = q3s.Int8Linear(torch.randn(32, 64, device=dev))
+linear(x)
+assert seen.value == linear.error_word.data_ptr() and int(linear.error_word) == 0, "Int8Linear"
+"""
+
+
+def test_error_words_of_8_bit_products_reach_the_library(dev, tmp_path):
+    from q3s import build
+
+    src, lib = tmp_path / "shim.cpp", tmp_path / "shim.so"
+    src.write_text(SHIM)
+    subprocess.run([build.system_cxx(), "-shared", "-fPIC", f"-I{build.INCLUDE}", "-o", str(lib), str(src)], check=True)
+    done = subprocess.run([sys.executable, "-c", SHIM_CALLER, str(lib), str(build.PKG_DIR.parent)], capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr
+
+
+def test_error_word_of_a_product_is_checked_and_left_alone(dev):
+    w, s = torch.ones(32, 64, dtype=torch.int8, device=dev), torch.ones(32, device=dev)
+    err = torch.zeros(1, dtype=torch.int32, device=dev)
+    for rows in (1, 20):
+        y = q3s.int8_linear(torch.ones(rows, 64, device=dev), w, s, error_word=err)
+        assert int(err) == 0 and bool((y == 64.0).all())
+    for bad in (err.long(), err.cpu(), torch.zeros(2, dtype=torch.int32, device=dev)):
+        with pytest.raises(RuntimeError, match="error_word"):
+            q3s.int8_linear(torch.ones(1, 64, device=dev), w, s, error_word=bad)
+        with pytest.raises(RuntimeError, match="error_word"):
+            q3s.int8_matmul(w[:3], s[:3], w, s, error_word=bad)
