@@ -94,8 +94,9 @@ def main(rows=48, steps=20, voice_tokens=200, max_tokens_per_row=256, seed=0):
             history.reset_rows(done)
             guard.reset_rows(done)
         drawn.append(ids)
-    if int(t.error_word):
-        raise RuntimeError(f"cache tables reported {int(t.error_word)}")
+    words = [t.error_word, cache.error_word] + [p.error_word for x in layers for p in (x.qkv, x.out, x.up, x.down)]
+    if int(torch.stack(words).max()):
+        raise RuntimeError(f"the decode operators reported {[int(w) for w in words]}")
     return torch.stack(drawn), cache.lengths
 
 

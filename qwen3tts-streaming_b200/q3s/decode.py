@@ -150,7 +150,9 @@ class PagedCache:
     ``blocks`` blocks of ``block_size`` tokens; the first ``prefix_blocks`` of
     them are set aside for a prefix that all rows share (``prefix``), the rest
     are the ring that rows draw from.  ``step`` leaves the row lengths, the
-    ring and the step's tables on the device and reads nothing back."""
+    ring and the step's tables on the device and reads nothing back.
+    ``tables.error_word`` reports on the step, ``error_word`` collects the
+    ``DECERR_*`` bits of ``append`` and ``attend``."""
 
     def __init__(self, batch: int, blocks: int, *, layers: int, kv_heads: int, dim: int, block_size: int = 16,
                  max_blocks: int, prefix_blocks: int = 0, dtype: torch.dtype = torch.bfloat16,
@@ -170,6 +172,7 @@ class PagedCache:
         self.ring_state = torch.tensor([0, blocks - prefix_blocks], **i32)
         self.table = torch.full((batch, max_blocks), -1, **i32)
         self.lengths = torch.zeros(batch, **i32)
+        self.error_word = torch.zeros(1, **i32)
         self.tables: Optional[CacheTables] = None
 
     def write_prefix(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
@@ -178,7 +181,7 @@ class PagedCache:
             raise ValueError(f"a prefix of {k.shape[0]} tokens in {self.prefix.numel()} blocks of {self.block_size}")
         self.prefix_length = k.shape[0]
         # the prefix's blocks are the cache's first ones, in order: token p has slot p
-        cache_append(k, v, self.k[layer], self.v[layer], torch.arange(k.shape[0], device=k.device))
+        cache_append(k, v, self.k[layer], self.v[layer], torch.arange(k.shape[0], device=k.device), error_word=self.error_word)
 
     def step(self, new_lengths: torch.Tensor, max_tokens: int, released: Optional[torch.Tensor] = None) -> CacheTables:
         """Start a step that adds ``new_lengths`` tokens to the rows."""
@@ -189,9 +192,10 @@ class PagedCache:
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """Store this step's keys and values of one layer ([max_tokens, kv_heads, dim])."""
-        cache_append(k, v, self.k[layer], self.v[layer], self.tables.slot_map)
+        cache_append(k, v, self.k[layer], self.v[layer], self.tables.slot_map, error_word=self.error_word)
 
     def attend(self, layer: int, q: torch.Tensor, **kw):
         """This step's queries of one layer ([max_tokens, q_heads, dim]) over prefix and rows."""
         return prefix_attention(q, self.k[layer], self.v[layer], self.tables.query_offsets, self.table, self.lengths,
-                                prefix_blocks=self.prefix, prefix_length=self.prefix_length, **kw)
+                                prefix_blocks=self.prefix, prefix_length=self.prefix_length,
+                                **{"error_word": self.error_word, **kw})

@@ -185,3 +185,27 @@ def test_error_word_of_a_product_is_checked_and_left_alone(dev):
             q3s.int8_linear(torch.ones(1, 64, device=dev), w, s, error_word=bad)
         with pytest.raises(RuntimeError, match="error_word"):
             q3s.int8_matmul(w[:3], s[:3], w, s, error_word=bad)
+
+
+def test_paged_cache_collects_reports(dev):
+    def fresh():
+        cache = q3s.PagedCache(2, 8, layers=1, kv_heads=1, dim=64, max_blocks=3, device=dev)
+        cache.step(torch.ones(2, dtype=torch.int32, device=dev), max_tokens=2)
+        return cache
+
+    x = torch.ones(2, 1, 64, dtype=torch.bfloat16, device=dev)
+    cache = fresh()
+    cache.append(0, x, x)
+    cache.attend(0, x)
+    assert int(cache.error_word) == 0 and int(cache.tables.error_word) == 0
+    cache.table[1, 0] = 10 ** 6
+    cache.attend(0, x)
+    assert int(cache.error_word) == q3s.decode.DECERR_BLOCK_ID
+    own = torch.zeros(1, dtype=torch.int32, device=dev)
+    cache.error_word.zero_()
+    cache.attend(0, x, error_word=own)
+    assert int(own) == q3s.decode.DECERR_BLOCK_ID and int(cache.error_word) == 0
+    cache = fresh()
+    cache.tables.slot_map[0] = 8 * 16
+    cache.append(0, x, x)
+    assert int(cache.error_word) == q3s.decode.DECERR_BLOCK_ID
