@@ -68,17 +68,6 @@ int32_t i32(int64_t x, const char* name) {
 Tensor make(at::IntArrayRef sizes, at::ScalarType dt, const Tensor& ref) {
   return at::detail::empty_cuda(sizes, dt, ref.device(), c10::nullopt);
 }
-// A tensor of its own over part of `base`'s memory (which stays alive with it): the outputs of a call that always come
-// together share one allocation.  `byte` is a multiple of the element size.
-Tensor part(const Tensor& base, int64_t byte, at::IntArrayRef sizes, at::ScalarType dt) {
-  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA),
-                                                      c10::scalarTypeToTypeMeta(dt));
-  t.unsafeGetTensorImpl()->set_storage_offset(byte / static_cast<int64_t>(c10::elementSize(dt)));
-  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-  return t;
-}
-int64_t round16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
-
 // Two tensors that a call reads and writes must not share memory.
 void apart(const Tensor& out, const Tensor& in, const char* what) {
   TORCH_CHECK(!out.is_alias_of(in) || out.data_ptr() != in.data_ptr(), "q3s: ", what, " must not be the same tensor");
@@ -122,12 +111,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> cache_tables(
   d.ring_size = i32(free_blocks.size(0), "free_blocks");
   d.free_state = free_state.data_ptr<int32_t>();
   d.max_tokens = i32(max_tokens, "max_tokens");
-  const int64_t at_slots = 0, at_positions = at_slots + round16(8 * max_tokens), at_offsets = at_positions + round16(4 * max_tokens),
-                at_lengths = at_offsets + round16(4 * (B + 1)), at_state = at_lengths + round16(4 * B), all = at_state + 32;
-  const Tensor arena = make({all}, at::kByte, context);
-  Tensor slots = part(arena, at_slots, {max_tokens}, at::kLong), positions = part(arena, at_positions, {max_tokens}, at::kInt);
-  Tensor offsets = part(arena, at_offsets, {B + 1}, at::kInt), lengths = part(arena, at_lengths, {B}, at::kInt);
-  Tensor state = part(arena, at_state, {2}, at::kInt), error = part(arena, at_state + 16, {1}, at::kInt);
+  Tensor slots = make({max_tokens}, at::kLong, context), positions = make({max_tokens}, at::kInt, context);
+  Tensor offsets = make({B + 1}, at::kInt, context), lengths = make({B}, at::kInt, context);
+  Tensor state = make({2}, at::kInt, context), error = make({1}, at::kInt, context);
   d.query_offsets = offsets.data_ptr<int32_t>();
   d.slot_map = slots.data_ptr<int64_t>();
   d.positions = positions.data_ptr<int32_t>();
@@ -343,10 +329,7 @@ std::tuple<Tensor, Tensor, Tensor> int8_linear(const Tensor& x, const Tensor& we
   c10::cuda::CUDAGuard guard(r.device());
   TORCH_CHECK(weight.dim() == 2, "q3s: weight must be [N, K], got ", weight.sizes());
   const int64_t M = r.size(0), K = r.size(1), N = weight.size(0);
-  const int64_t at_scales = round16(M * K);
-  const Tensor arena = make({at_scales + 4 * M}, at::kByte, r);
-  Tensor values = part(arena, 0, {M, K}, at::kChar), scales = part(arena, at_scales, {M}, at::kFloat);
-  Tensor y = make({M, N}, r.scalar_type(), r);
+  Tensor values = make({M, K}, at::kChar, r), scales = make({M}, at::kFloat, r), y = make({M, N}, r.scalar_type(), r);
   const q3s_quantize_rows_desc q = quantize_desc(r, values, scales);
   const q3s_int8_matmul_desc d = matmul_desc(values, scales, weight, weight_scales, bias, error_word, y);
   check_status(q3s_int8_linear(&q, &d, stream_of(r)), "q3s_int8_linear");

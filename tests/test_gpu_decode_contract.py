@@ -209,3 +209,22 @@ def test_paged_cache_collects_reports(dev):
     cache.tables.slot_map[0] = 8 * 16
     cache.append(0, x, x)
     assert int(cache.error_word) == q3s.decode.DECERR_BLOCK_ID
+
+
+# ---- outputs ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows", [1, 5, 300])
+def test_outputs_are_tensors_of_their_own(dev, rows):
+    """No two outputs of a call share memory, as their schemas say (an output that is kept keeps nothing else)."""
+    from torch._subclasses.schema_check_mode import SchemaCheckMode
+
+    i32 = dict(dtype=torch.int32, device=dev)
+    ring, state = torch.arange(rows, **i32), torch.tensor([0, rows], **i32)
+    x = torch.ones(rows, 64, device=dev)
+    with SchemaCheckMode():
+        t = q3s.cache_tables(torch.zeros(rows, **i32), torch.ones(rows, **i32), torch.zeros(rows, 2, **i32), ring, state,
+                             block_size=16, max_tokens=rows)
+        y = q3s.int8_linear(x, torch.ones(32, 64, dtype=torch.int8, device=dev), torch.ones(32, device=dev), return_quantized=True)
+    for outs in (t, y):
+        assert len({o.untyped_storage().data_ptr() for o in outs}) == len(outs)
+        assert all(o.untyped_storage().nbytes() == o.numel() * o.element_size() for o in outs)
