@@ -34,7 +34,7 @@ extern "C" {
 #define Q3S_DECERR_LENGTHS 1   /* a negative length, or offsets that do not ascend (treated as 0 / cut) */
 #define Q3S_DECERR_TABLE 2     /* a row outgrew its block table: it got no blocks */
 #define Q3S_DECERR_POOL 4      /* the free ring ran out: this row and later ones that need blocks got none */
-#define Q3S_DECERR_TOKENS 8    /* more new tokens than max_tokens: the rest have no slot */
+#define Q3S_DECERR_TOKENS 8    /* more new tokens than max_tokens: the rest have no slot (Q3S_TABLES_WHOLE_ROWS) */
 #define Q3S_DECERR_BLOCK_ID 16 /* a block id or slot outside the cache: its tokens read as zeros / are not stored */
 #define Q3S_DECERR_WAIT 32     /* a bounded device wait gave up */
 
@@ -43,6 +43,12 @@ typedef enum q3s_elem { Q3S_ELEM_F32 = 0, Q3S_ELEM_BF16 = 1, Q3S_ELEM_F16 = 2 } 
 
 #define Q3S_MAX_CACHE_ROWS 65536
 #define Q3S_MAX_QUERY_GROUP 16 /* query heads per key/value head */
+
+/* q3s_cache_tables_desc.flags: a row whose new tokens end past max_tokens is
+ * refused whole, like one that does not fit its table.  Without it such a row
+ * is granted, and its length counts tokens that have no slot: a caller that
+ * goes on from those lengths would read places that nothing was written to. */
+#define Q3S_TABLES_WHOLE_ROWS 1u
 
 /* Block tables, slot map and positions of one step, from the rows' lengths.
  *
@@ -78,6 +84,8 @@ typedef struct q3s_cache_tables_desc {
   int32_t* error_word;            /* optional, written (not OR-ed) */
   int32_t ring_size;              /* blocks that the ring can hold, >= 1 */
   int32_t max_tokens;             /* >= 0 */
+  uint32_t flags;                 /* Q3S_TABLES_*; a struct_size that ends before this field means 0 */
+  uint32_t reserved0;
 } q3s_cache_tables_desc;
 
 q3s_status q3s_cache_tables(const q3s_cache_tables_desc* desc, void* stream);

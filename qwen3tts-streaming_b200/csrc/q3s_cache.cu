@@ -1,6 +1,7 @@
 // q3s_cache.cu -- the paged key/value cache's bookkeeping (q3s_cache_tables)
 // and append (q3s_cache_append).
 #include <cuda_runtime.h>
+#include <stddef.h>
 #include <stdint.h>
 
 #include <algorithm>
@@ -28,6 +29,7 @@ struct TablesArgs {
   int64_t* slots;
   int32_t* positions;
   int32_t* error_word;
+  bool whole_rows;  // rows that end past max_tokens are refused
 };
 
 constexpr uint32_t SAT = 0x7fffffffu;
@@ -138,8 +140,10 @@ __global__ void __launch_bounds__(NT) cache_tables_kernel(const TablesArgs a) {
       const Sums at = before;
       before = before + mine[i];
       const uint32_t need = mine[i].need;
-      const bool granted = fits[i] && (need == 0 || before.need <= static_cast<uint32_t>(count));
-      if (!granted && fits[i]) bad |= Q3S_DECERR_POOL;
+      // past the last slot: then so are the tokens of every later row, so the sums of needs that count are those before
+      const bool past = a.whole_rows && mine[i].tokens && static_cast<int64_t>(at.tokens) + mine[i].tokens > a.max_tokens;
+      const bool granted = fits[i] && !past && (need == 0 || before.need <= static_cast<uint32_t>(count));
+      if (!granted && fits[i] && !past) bad |= Q3S_DECERR_POOL;
       if (granted && need) taken = max(taken, before.need);
       s_off[k] = at.tokens;
       s_context[k] = context[i];
@@ -314,9 +318,11 @@ cudaError_t launch_append(const AppendArgs& a, cudaStream_t st) {
 extern "C" q3s_status q3s_cache_tables(const q3s_cache_tables_desc* d, void* stream) {
   using q3s::report;
   if (!d) return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_tables: desc is NULL");
-  if (d->struct_size != sizeof(q3s_cache_tables_desc))
+  if (d->struct_size != sizeof(q3s_cache_tables_desc) && d->struct_size != offsetof(q3s_cache_tables_desc, flags))
     return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_tables: struct_size %u != %u (ABI mismatch)", d->struct_size,
                   static_cast<unsigned>(sizeof(q3s_cache_tables_desc)));
+  const uint32_t flags = d->struct_size == sizeof(q3s_cache_tables_desc) ? d->flags : 0u;
+  if (flags & ~Q3S_TABLES_WHOLE_ROWS) return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_tables: unknown flags %#x", flags);
   if (d->batch < 0 || d->batch > Q3S_MAX_CACHE_ROWS)
     return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_tables: batch %d is not in [0, %d]", d->batch, Q3S_MAX_CACHE_ROWS);
   if (d->block_size < 1 || d->max_blocks < 1 || d->ring_size < 1 || d->max_tokens < 0)
@@ -357,6 +363,7 @@ extern "C" q3s_status q3s_cache_tables(const q3s_cache_tables_desc* d, void* str
   a.slots = d->slot_map;
   a.positions = d->positions;
   a.error_word = d->error_word;
+  a.whole_rows = (flags & Q3S_TABLES_WHOLE_ROWS) != 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   // CTAs: one per NT tokens or per 32 rows (their entries), up to one per SM.
   // Threads and rows a thread, so that the rows are one scan.  Small against

@@ -5,7 +5,7 @@
 // raises before anything is launched.
 //
 //   cache_tables(context_lengths, new_lengths, block_table!, free_blocks!, free_state, block_size, max_tokens,
-//                released=None) -> (query_offsets, slot_map, positions, lengths, free_state, error_word)
+//                released=None, whole_rows=False) -> (query_offsets, slot_map, positions, lengths, free_state, error_word)
 //   cache_append(k, v, k_cache!, v_cache!, slot_map, error_word!=None) -> ()
 //   prefix_attention(q, k_cache, v_cache, query_offsets, block_table, lengths, prefix_blocks=None, prefix_length=0,
 //                    scale=None, error_word!=None) -> (out, lse)
@@ -75,7 +75,7 @@ void apart(const Tensor& out, const Tensor& in, const char* what) {
 
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> cache_tables(
     const Tensor& context, const Tensor& fresh, Tensor block_table, Tensor free_blocks, const Tensor& free_state,
-    int64_t block_size, int64_t max_tokens, const OptTensor& released) {
+    int64_t block_size, int64_t max_tokens, const OptTensor& released, bool whole_rows) {
   need_cuda(context, "context_lengths");
   c10::cuda::CUDAGuard guard(context.device());
   need(context, context, at::kInt, 1, "context_lengths");
@@ -111,6 +111,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> cache_tables(
   d.ring_size = i32(free_blocks.size(0), "free_blocks");
   d.free_state = free_state.data_ptr<int32_t>();
   d.max_tokens = i32(max_tokens, "max_tokens");
+  d.flags = whole_rows ? Q3S_TABLES_WHOLE_ROWS : 0;
   Tensor slots = make({max_tokens}, at::kLong, context), positions = make({max_tokens}, at::kInt, context);
   Tensor offsets = make({B + 1}, at::kInt, context), lengths = make({B}, at::kInt, context);
   Tensor state = make({2}, at::kInt, context), error = make({1}, at::kInt, context);
@@ -342,7 +343,7 @@ std::tuple<Tensor, Tensor, Tensor> int8_linear(const Tensor& x, const Tensor& we
 // ---- Meta kernels: shapes and dtypes only ------------------------------------
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> cache_tables_meta(const Tensor& context, const Tensor&,
                                                                              Tensor, Tensor, const Tensor&, int64_t,
-                                                                             int64_t max_tokens, const OptTensor&) {
+                                                                             int64_t max_tokens, const OptTensor&, bool) {
   const auto o = context.options();
   const int64_t B = context.size(0);
   return {at::empty({B + 1}, o), at::empty({max_tokens}, o.dtype(at::kLong)), at::empty({max_tokens}, o),
@@ -374,8 +375,8 @@ std::tuple<Tensor, Tensor, Tensor> int8_linear_meta(const Tensor& x, const Tenso
 
 TORCH_LIBRARY_FRAGMENT(q3s, m) {
   m.def("cache_tables(Tensor context_lengths, Tensor new_lengths, Tensor(a!) block_table, Tensor(b!) free_blocks, "
-        "Tensor free_state, int block_size, int max_tokens, Tensor? released=None) -> (Tensor, Tensor, Tensor, "
-        "Tensor, Tensor, Tensor)");
+        "Tensor free_state, int block_size, int max_tokens, Tensor? released=None, bool whole_rows=False) -> (Tensor, "
+        "Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("cache_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slot_map, "
         "Tensor(c!)? error_word=None) -> ()");
   m.def("prefix_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor query_offsets, Tensor block_table, "

@@ -168,6 +168,7 @@ class HeadDesc(C.Structure):
 # the decode step's operators (include/q3s_decode.h)
 ELEM_F32, ELEM_BF16, ELEM_F16 = 0, 1, 2
 MAX_CACHE_ROWS, MAX_QUERY_GROUP = 65536, 16
+TABLES_WHOLE_ROWS = 1
 
 
 class CacheTablesDesc(C.Structure):
@@ -191,6 +192,8 @@ class CacheTablesDesc(C.Structure):
         ("error_word", _p),
         ("ring_size", C.c_int32),
         ("max_tokens", C.c_int32),
+        ("flags", C.c_uint32),
+        ("reserved0", C.c_uint32),
     ]
 
 

@@ -51,7 +51,7 @@ class CacheTables(NamedTuple):
 
 def cache_tables(context_lengths: torch.Tensor, new_lengths: torch.Tensor, block_table: torch.Tensor,
                  free_blocks: torch.Tensor, free_state: torch.Tensor, *, block_size: int, max_tokens: int,
-                 released: Optional[torch.Tensor] = None) -> CacheTables:
+                 released: Optional[torch.Tensor] = None, whole_rows: bool = False) -> CacheTables:
     """Give every row the blocks that its new tokens need, and number the
     tokens' slots, in one launch from the lengths on the GPU.
 
@@ -62,9 +62,12 @@ def cache_tables(context_lengths: torch.Tensor, new_lengths: torch.Tensor, block
     more.  A row that its table or the ring cannot serve keeps its length and
     gets slot -1 for its tokens; ``error_word`` says why.  ``max_tokens`` sizes
     the slot map: entries past the last token are -1 (positions 0), so a
-    captured graph can keep one size."""
+    captured graph can keep one size.  With ``whole_rows`` a row whose new
+    tokens end past it is refused like one that its table cannot serve; without,
+    ``lengths`` counts all of its tokens, and a caller that sees
+    ``DECERR_TOKENS`` must not go on from them."""
     return tuple.__new__(CacheTables, _op("cache_tables")(context_lengths, new_lengths, block_table, free_blocks,
-                                                          free_state, block_size, max_tokens, released))
+                                                          free_state, block_size, max_tokens, released, whole_rows))
 
 
 def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -184,9 +187,12 @@ class PagedCache:
         cache_append(k, v, self.k[layer], self.v[layer], torch.arange(k.shape[0], device=k.device), error_word=self.error_word)
 
     def step(self, new_lengths: torch.Tensor, max_tokens: int, released: Optional[torch.Tensor] = None) -> CacheTables:
-        """Start a step that adds ``new_lengths`` tokens to the rows."""
+        """Start a step that adds ``new_lengths`` tokens to the rows.  A row
+        that its table or the ring cannot serve, or whose tokens end past
+        ``max_tokens``, is refused: it keeps its length and its new tokens get
+        slot -1; ``error_word`` of the result says why."""
         t = cache_tables(self.lengths, new_lengths, self.table, self.ring, self.ring_state,
-                         block_size=self.block_size, max_tokens=max_tokens, released=released)
+                         block_size=self.block_size, max_tokens=max_tokens, released=released, whole_rows=True)
         self.lengths, self.ring_state, self.tables = t.lengths, t.free_state, t
         return t
 

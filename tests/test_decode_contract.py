@@ -90,3 +90,17 @@ def test_every_operator_with_device_waits_takes_an_error_word():
     for name in ("cache_append", "prefix_attention", "int8_matmul", "int8_linear"):
         arg = {a.name: a for a in getattr(torch.ops.q3s, name).default._schema.arguments}["error_word"]
         assert arg.alias_info is not None and arg.alias_info.is_write and arg.default_value is None
+
+
+def test_cache_tables_descriptor_of_before_the_flags_is_taken():
+    import ctypes as C
+
+    from q3s import _lib
+    from test_decode_host import GOOD
+
+    lib, (cls, good) = _lib.load(), GOOD["q3s_cache_tables"]
+    old = cls.flags.offset
+    for size, kw, message in ((old, dict(flags=77), "ring_size"), (C.sizeof(cls), dict(flags=2), "flags"), (old + 4, {}, "struct_size"),
+                              (C.sizeof(cls), dict(flags=_lib.TABLES_WHOLE_ROWS), "ring_size")):
+        d = cls(**{**good, "struct_size": size, "ring_size": 0, **kw})
+        assert lib.q3s_cache_tables(C.byref(d), None) == _lib.ERR_INVALID_ARGUMENT and message in _lib.last_error()

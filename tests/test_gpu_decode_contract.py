@@ -3,6 +3,7 @@ on the GPU, against plain forms in Python integers and float64."""
 import subprocess
 import sys
 
+import numpy as np
 import pytest
 import torch
 
@@ -228,3 +229,67 @@ def test_outputs_are_tensors_of_their_own(dev, rows):
     for outs in (t, y):
         assert len({o.untyped_storage().data_ptr() for o in outs}) == len(outs)
         assert all(o.untyped_storage().nbytes() == o.numel() * o.element_size() for o in outs)
+
+
+# ---- tables: more tokens than a step has slots for ----------------------------------------
+
+@pytest.mark.parametrize("rows,cap", [(3, 2), (200, 1000), (1500, 300), (40, 0)])
+def test_tables_refuse_whole_rows_past_the_last_slot(dev, rows, cap):
+    """Rows up to the one whose tokens end past the cap are served as in a step without the others; those keep their length."""
+    rng = np.random.RandomState(rows)
+    block, width = 16, 12
+    context, new = rng.randint(0, 100, rows), rng.randint(0, 30, rows)
+    if rows == 3:
+        new[:] = 1
+    gone = rng.rand(rows) < 0.1
+    held = R.ceil_div(context, block)
+    ids = rng.permutation(int(held.sum()) + 5 * rows)
+    table = np.full((rows, width), -1)
+    table[np.arange(width)[None, :] < held[:, None]] = ids[: int(held.sum())]
+    ring = np.concatenate([ids[int(held.sum()):], np.full(int(held.sum()), -1)])
+    state = [0, len(ids) - int(held.sum())]
+    kept = np.where(np.cumsum(new) <= cap, new, 0)
+    want = R.cache_tables(context.tolist(), kept.tolist(), table.tolist(), ring.tolist(), state, block_size=block, max_tokens=cap,
+                          released=gone.tolist())
+    i32 = dict(dtype=torch.int32, device=dev)
+    on_gpu = [torch.as_tensor(x, **i32) for x in (context, new, table, ring, state)]
+    t = q3s.cache_tables(*on_gpu, block_size=block, max_tokens=cap, released=torch.as_tensor(gone, device=dev), whole_rows=True)
+    for name in ("lengths", "free_state", "slot_map"):
+        np.testing.assert_array_equal(getattr(t, name).cpu().numpy(), want[name], err_msg=name)
+    np.testing.assert_array_equal(on_gpu[2].cpu().numpy(), want["table"])
+    np.testing.assert_array_equal(on_gpu[3].cpu().numpy(), want["ring"])
+    np.testing.assert_array_equal(t.query_offsets.cpu().numpy(), np.concatenate([[0], np.cumsum(new)]))
+    assert int(t.error_word) == q3s.decode.DECERR_TOKENS
+    n = int(kept.sum())
+    np.testing.assert_array_equal(t.positions.cpu().numpy()[:n], want["positions"][:n])
+
+
+def test_paged_cache_after_a_step_with_too_many_tokens(dev):
+    """The row that a step had no room for is as before it; the next steps read what was stored, and nothing else."""
+    rows, heads, dim, block = 3, 2, 64, 16
+    g = torch.Generator(device=dev).manual_seed(0)
+    cache = q3s.PagedCache(rows, 9, layers=1, kv_heads=heads, dim=dim, max_blocks=3, device=dev)
+    cache.k.fill_(float("nan"))
+    cache.v.fill_(float("nan"))
+    stored = [torch.zeros(0, heads, dim, dtype=torch.bfloat16, device=dev) for _ in range(rows)]
+    for new, cap, served in (([2, 1, 1], 4, [2, 1, 1]), ([1, 2, 1], 2, [1, 0, 0]), ([17, 1, 1], 19, [17, 1, 1]), ([1, 1, 0], 2, [1, 1, 0])):
+        t = cache.step(torch.tensor(new, dtype=torch.int32, device=dev), max_tokens=cap)
+        assert int(t.error_word) == (0 if new == served else q3s.decode.DECERR_TOKENS)
+        x = torch.randn(cap, heads, dim, device=dev, generator=g).bfloat16()
+        cache.append(0, x, x)
+        at = 0
+        for b in range(rows):
+            stored[b] = torch.cat([stored[b], x[at:at + served[b]]])
+            at += new[b]
+        assert cache.lengths.tolist() == [len(s) for s in stored]
+        out = cache.attend(0, x)
+        at = 0
+        for b in range(rows):
+            for i in range(served[b]):
+                keys = stored[b][: len(stored[b]) - served[b] + i + 1].double()
+                p = (torch.einsum("hd,jhd->hj", x[at + i].double(), keys) * dim ** -0.5).softmax(1)
+                want = torch.einsum("hj,jhd->hd", p, keys)
+                mass = torch.einsum("hj,jhd->hd", p, keys.abs())
+                # out's rounding, and 2^-16 for p in two parts, ex2 and the sums
+                assert bool(((out[at + i].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -15 * mass).all())
+            at += new[b]
