@@ -122,7 +122,9 @@ q3s_status q3s_cache_append(const q3s_cache_append_desc* desc, void* stream);
  * prefix (blocks prefix_blocks[]), and query i of row b the row's own tokens
  * j <= lengths[b] - n_b + i (blocks block_table[b, :]; lengths count the
  * step's own tokens, which are already in the cache).  Query head h reads
- * key/value head h / (q_heads / kv_heads).
+ * key/value head h / (q_heads / kv_heads).  A row that q3s_cache_tables refused
+ * has queries but not their keys: with the step's slot_map they see nothing
+ * (without, they would be taken for the row's last stored tokens).
  *   out = softmax(scale * q . k) v,   lse = log sum exp(scale * q . k)
  * with 0 and -inf for a query that sees nothing.  Softmax statistics and sums
  * are 32-bit.  For the product with v, as the tensor cores take it,
@@ -163,6 +165,7 @@ typedef struct q3s_prefix_attention_desc {
   void* workspace;              /* q3s_prefix_attention_workspace() bytes, 16-byte aligned; needs no initial value */
   int64_t workspace_bytes;
   int32_t* error_word;          /* optional, OR-ed */
+  const int64_t* slot_map;      /* optional [T]: a query whose slot is negative sees nothing (a struct_size that ends before this field: none) */
 } q3s_prefix_attention_desc;
 
 /* Workspace bytes for a descriptor's sizes (its pointers are not read). */

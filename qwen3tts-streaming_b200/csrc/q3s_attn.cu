@@ -1,6 +1,7 @@
 // q3s_attn.cu -- host side of q3s_prefix_attention.
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <stddef.h>
 
 #include <algorithm>
 #include <atomic>
@@ -109,7 +110,7 @@ Layout layout_of(const q3s_prefix_attention_desc* d) {
 q3s_status check_sizes(const q3s_prefix_attention_desc* d) {
   using q3s::report;
   if (!d) return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_prefix_attention: desc is NULL");
-  if (d->struct_size != sizeof(q3s_prefix_attention_desc))
+  if (d->struct_size != sizeof(q3s_prefix_attention_desc) && d->struct_size != offsetof(q3s_prefix_attention_desc, slot_map))
     return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_prefix_attention: struct_size %u != %u (ABI mismatch)", d->struct_size,
                   static_cast<unsigned>(sizeof(q3s_prefix_attention_desc)));
   if (d->batch < 0 || d->batch > Q3S_MAX_CACHE_ROWS || d->tokens < 0)
@@ -292,6 +293,7 @@ extern "C" q3s_status q3s_prefix_attention(const q3s_prefix_attention_desc* d, v
   a.oh = d->out_head_stride;
   a.lse = d->lse;
   a.error_word = d->error_word;
+  a.slot_map = d->struct_size == sizeof(q3s_prefix_attention_desc) ? d->slot_map : nullptr;
   unsigned char* ws = static_cast<unsigned char*>(d->workspace);
   a.items = reinterpret_cast<int2*>(ws + l.items);
   a.part_o = reinterpret_cast<float*>(ws + l.part_o);

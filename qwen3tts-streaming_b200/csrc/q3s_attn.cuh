@@ -46,6 +46,7 @@ struct AttnArgs {
   int64_t ot, oh;
   float* lse;
   int32_t* error_word;
+  const int64_t* slot_map;  // or null
   // workspace
   int2* items;       // [ids] {first slot, slots} of an item's parts
   float* part_o;     // [slots][R][D]
@@ -675,7 +676,7 @@ __global__ void __launch_bounds__(SplitTile<D, NQ>::NT, SplitTile<D, NQ>::PER_SM
 // Joins the parts of each query row (m, l, o as above) and writes out and lse.
 // One warp a row of [T * q_heads]; a lane holds D / 32 of its values.  A token's batch row is found in
 // query_offsets by bisection, before the grid waits for the parts; tokens past
-// the last row see nothing.  Bound by latency, of the record of the row's own
+// the last row, and those of a refused row (slot_map), see nothing.  Bound by latency, of the record of the row's own
 // parts and of the sums, and by fetching its own instructions: kept short (with the weights of
 // up to 32 parts computed before the sums it took 8.8 us, and 256 rows of 32 heads
 // 99 us in all against 93).
@@ -700,7 +701,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
       if (a.offsets[m] <= token) b = m; else r = m;
     }
     x = attn_row<R, AT_KEYS<D>>(a, b + 1);
-    live = token >= x.t0 && token < x.t0 + x.n;
+    live = token >= x.t0 && token < x.t0 + x.n && (!a.slot_map || a.slot_map[token] >= 0);
     if (!live) x.units = 0;
   }
   grid_wait();

@@ -8,7 +8,7 @@
 //                released=None, whole_rows=False) -> (query_offsets, slot_map, positions, lengths, free_state, error_word)
 //   cache_append(k, v, k_cache!, v_cache!, slot_map, error_word!=None) -> ()
 //   prefix_attention(q, k_cache, v_cache, query_offsets, block_table, lengths, prefix_blocks=None, prefix_length=0,
-//                    scale=None, error_word!=None) -> (out, lse)
+//                    scale=None, error_word!=None, slot_map=None) -> (out, lse)
 //   quantize_rows(x) -> (values, scales)
 //   int8_matmul(values, scales, weight, weight_scales, dtype, bias=None, error_word!=None) -> y
 //   int8_linear(x, weight, weight_scales, bias=None, error_word!=None) -> (y, values, scales)
@@ -178,7 +178,7 @@ std::tuple<Tensor, Tensor> prefix_attention(const Tensor& q, const Tensor& k_cac
                                             const Tensor& query_offsets, const Tensor& block_table,
                                             const Tensor& lengths, const OptTensor& prefix_blocks,
                                             int64_t prefix_length, c10::optional<double> scale,
-                                            OptTensor error_word) {
+                                            OptTensor error_word, const OptTensor& slot_map) {
   need_cuda(q, "q");
   c10::cuda::CUDAGuard guard(q.device());
   need(q, q, q.scalar_type(), 3, "q");
@@ -238,6 +238,10 @@ std::tuple<Tensor, Tensor> prefix_attention(const Tensor& q, const Tensor& k_cac
   d.out_head_stride = q.size(2);
   d.lse = lse.data_ptr<float>();
   d.error_word = error_of(error_word, q);
+  if (slot_map.has_value()) {
+    need_vector(*slot_map, q, at::kLong, T, "slot_map");
+    d.slot_map = slot_map->data_ptr<int64_t>();
+  }
   int64_t bytes = 0;
   check_status(q3s_prefix_attention_workspace(&d, &bytes), "q3s_prefix_attention");
   const Tensor ws = make({bytes}, at::kByte, q);
@@ -352,7 +356,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> cache_tables_meta(con
 void cache_append_meta(const Tensor&, const Tensor&, Tensor, Tensor, const Tensor&, OptTensor) {}
 std::tuple<Tensor, Tensor> prefix_attention_meta(const Tensor& q, const Tensor&, const Tensor&, const Tensor&,
                                                  const Tensor&, const Tensor&, const OptTensor&, int64_t,
-                                                 c10::optional<double>, OptTensor) {
+                                                 c10::optional<double>, OptTensor, const OptTensor&) {
   return {at::empty(q.sizes(), q.options()), at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat))};
 }
 std::tuple<Tensor, Tensor> quantize_rows_meta(const Tensor& x) {
@@ -381,7 +385,7 @@ TORCH_LIBRARY_FRAGMENT(q3s, m) {
         "Tensor(c!)? error_word=None) -> ()");
   m.def("prefix_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor query_offsets, Tensor block_table, "
         "Tensor lengths, Tensor? prefix_blocks=None, int prefix_length=0, float? scale=None, "
-        "Tensor(a!)? error_word=None) -> (Tensor, Tensor)");
+        "Tensor(a!)? error_word=None, Tensor? slot_map=None) -> (Tensor, Tensor)");
   m.def("quantize_rows(Tensor x) -> (Tensor, Tensor)");
   m.def("int8_matmul(Tensor values, Tensor scales, Tensor weight, Tensor weight_scales, ScalarType dtype, "
         "Tensor? bias=None, Tensor(a!)? error_word=None) -> Tensor");

@@ -263,6 +263,7 @@ class PrefixAttentionDesc(C.Structure):
         ("workspace", _p),
         ("workspace_bytes", C.c_int64),
         ("error_word", _p),
+        ("slot_map", _p),
     ]
 
 

@@ -3,11 +3,11 @@ tables and append, attention over a shared prefix, and 8-bit projections.
 
 A step runs them in this order, from device lengths alone (no host read)::
 
-    t = q3s.cache_tables(lengths, new, table, ring, ring_state, block_size=16, max_tokens=T)
+    t = q3s.cache_tables(lengths, new, table, ring, ring_state, block_size=16, max_tokens=T, whole_rows=True)
     # for every layer:
     q3s.cache_append(k, v, k_cache, v_cache, t.slot_map)
     out = q3s.prefix_attention(q, k_cache, v_cache, t.query_offsets, table, t.lengths,
-                               prefix_blocks=voice_blocks, prefix_length=voice_tokens)
+                               prefix_blocks=voice_blocks, prefix_length=voice_tokens, slot_map=t.slot_map)
     hidden = projection(out)                 # q3s.Int8Linear
     # then the codec head, the sampler and the epilogue (q3s.head_sample, q3s.StepGuard)
 
@@ -83,7 +83,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                      block_table: torch.Tensor, lengths: torch.Tensor, *,
                      prefix_blocks: Optional[torch.Tensor] = None, prefix_length: int = 0,
                      scale: Optional[float] = None, return_lse: bool = False,
-                     error_word: Optional[torch.Tensor] = None):
+                     error_word: Optional[torch.Tensor] = None, slot_map: Optional[torch.Tensor] = None):
     """Attention of a batch whose rows share a prefix, which is read and
     computed once for all of them.
 
@@ -95,9 +95,12 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     1 / sqrt(dim).  Returns ``out`` like ``q``, and with ``return_lse`` the
     log-sum-exp of the scaled scores (fp32 [T, q_heads]), with which the
     result joins others over further keys.  A query that sees nothing gets 0
-    and -inf."""
+    and -inf; so does one whose entry in ``slot_map`` (int64 [T], the step's) is
+    negative: a row that ``cache_tables`` refused has queries, but their keys
+    were not stored, and without the slot map the row's older tokens would be
+    taken for them."""
     out, lse = _op("prefix_attention")(q, k_cache, v_cache, query_offsets, block_table, lengths, prefix_blocks,
-                                       prefix_length, scale, error_word)
+                                       prefix_length, scale, error_word, slot_map)
     return (out, lse) if return_lse else out
 
 
@@ -201,7 +204,11 @@ class PagedCache:
         cache_append(k, v, self.k[layer], self.v[layer], self.tables.slot_map, error_word=self.error_word)
 
     def attend(self, layer: int, q: torch.Tensor, **kw):
-        """This step's queries of one layer ([max_tokens, q_heads, dim]) over prefix and rows."""
+        """This step's queries of one layer ([max_tokens, q_heads, dim]) over
+        prefix and rows; those of a refused row get 0 (and a log-sum-exp of -inf)."""
+        slots = self.tables.slot_map
+        if q.shape[0] != slots.shape[0]:  # queries past the step's tokens have no slot
+            slots = torch.nn.functional.pad(slots, (0, q.shape[0] - slots.shape[0]), value=-1)
         return prefix_attention(q, self.k[layer], self.v[layer], self.tables.query_offsets, self.table, self.lengths,
                                 prefix_blocks=self.prefix, prefix_length=self.prefix_length,
-                                **{"error_word": self.error_word, **kw})
+                                **{"error_word": self.error_word, "slot_map": slots, **kw})

@@ -104,3 +104,15 @@ def test_cache_tables_descriptor_of_before_the_flags_is_taken():
                               (C.sizeof(cls), dict(flags=_lib.TABLES_WHOLE_ROWS), "ring_size")):
         d = cls(**{**good, "struct_size": size, "ring_size": 0, **kw})
         assert lib.q3s_cache_tables(C.byref(d), None) == _lib.ERR_INVALID_ARGUMENT and message in _lib.last_error()
+
+
+def test_attention_descriptor_of_before_the_slot_map_is_taken():
+    import ctypes as C
+
+    from q3s import _lib
+    from test_decode_host import GOOD
+
+    lib, (cls, good) = _lib.load(), GOOD["q3s_prefix_attention"]
+    n = C.c_int64()
+    for size, status in ((cls.slot_map.offset, _lib.OK), (C.sizeof(cls), _lib.OK), (cls.slot_map.offset - 8, _lib.ERR_INVALID_ARGUMENT)):
+        assert lib.q3s_prefix_attention_workspace(C.byref(cls(**{**good, "struct_size": size})), C.byref(n)) == status

@@ -293,3 +293,57 @@ def test_paged_cache_after_a_step_with_too_many_tokens(dev):
                 # out's rounding, and 2^-16 for p in two parts, ex2 and the sums
                 assert bool(((out[at + i].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -15 * mass).all())
             at += new[b]
+
+
+# ---- attention of refused rows ---------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,prefix", [(6, 0), (6, 40), (120, 400)])
+@pytest.mark.parametrize("why", ["table", "ring", "slots"])
+def test_refused_rows_attend_to_nothing(dev, rows, prefix, why):
+    """Queries of a row that got no slots: 0 and -inf, in place of what the row's older tokens would give; the others' are as
+    without those rows."""
+    heads, dim, block, n = 2, 64, 16, 3
+    g = torch.Generator(device=dev).manual_seed(rows)
+    shared = -(-prefix // block)
+    spare = {"ring": 2 * rows - 2, "table": 3 * rows, "slots": 3 * rows}[why]
+    cache = q3s.PagedCache(rows, shared + spare, layers=1, kv_heads=heads, dim=dim, max_blocks=2 if why == "table" else 3,
+                           prefix_blocks=shared, device=dev)
+
+    def draw(tokens, h=heads):
+        return torch.randn(tokens, h, dim, device=dev, generator=g).bfloat16()
+
+    if prefix:
+        cache.write_prefix(0, draw(prefix), draw(prefix))
+    first = torch.full((rows,), 15, dtype=torch.int32, device=dev)
+    first[rows // 2] = 30 if why == "table" else 15
+    total = int(first.sum())
+    cache.step(first, max_tokens=total)
+    cache.append(0, draw(total), draw(total))
+    before = cache.lengths.clone()
+    cap = n * rows - (2 if why == "slots" else 0)
+    t = cache.step(torch.full((rows,), n, dtype=torch.int32, device=dev), max_tokens=cap)
+    refused = {"table": [rows // 2], "ring": [rows - 2, rows - 1], "slots": [rows - 1]}[why]
+    assert int(t.error_word) == {"table": 2, "ring": 4, "slots": 8}[why]
+    served = torch.ones(rows, dtype=torch.bool, device=dev)
+    served[refused] = False
+    assert torch.equal(cache.lengths, before + n * served)
+    x = draw(cap)
+    cache.append(0, x, x)
+    q = draw(cap, 2 * heads)
+    out, lse = cache.attend(0, q, return_lse=True)
+    token = served.repeat_interleave(n)[:cap]
+    assert not bool(out[~token].any()) and bool((lse[~token] == -float("inf")).all())
+    plain, plain_lse = cache.attend(0, q, return_lse=True, slot_map=None)
+    assert torch.equal(out[token], plain[token]) and torch.equal(lse[token], plain_lse[token])
+    assert bool(plain[~token].any())
+    more, more_lse = cache.attend(0, torch.cat([q, q[:5]]), return_lse=True)
+    assert torch.equal(more[:cap], out) and not bool(more[cap:].any()) and bool((more_lse[cap:] == -float("inf")).all())
+
+
+def test_attention_slot_map_is_checked(dev):
+    q = torch.zeros(2, 2, 64, dtype=torch.bfloat16, device=dev)
+    c = torch.zeros(2, 2, 16, 64, dtype=torch.bfloat16, device=dev)
+    i32 = dict(dtype=torch.int32, device=dev)
+    for bad in (torch.zeros(3, dtype=torch.int64, device=dev), torch.zeros(2, **i32), torch.zeros(2, dtype=torch.int64)):
+        with pytest.raises(RuntimeError, match="slot_map"):
+            q3s.prefix_attention(q, c, c, torch.arange(3, **i32), torch.zeros(2, 1, **i32), torch.ones(2, **i32), slot_map=bad)
