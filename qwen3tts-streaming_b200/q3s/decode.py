@@ -196,7 +196,9 @@ class PagedCache:
         slot -1; ``error_word`` of the result says why."""
         t = cache_tables(self.lengths, new_lengths, self.table, self.ring, self.ring_state,
                          block_size=self.block_size, max_tokens=max_tokens, released=released, whole_rows=True)
-        self.lengths, self.ring_state, self.tables = t.lengths, t.free_state, t
+        self.lengths.copy_(t.lengths)  # in place: a captured step goes on from what the last replay left
+        self.ring_state.copy_(t.free_state)
+        self.tables = t
         return t
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:

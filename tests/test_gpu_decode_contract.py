@@ -347,3 +347,44 @@ def test_attention_slot_map_is_checked(dev):
     for bad in (torch.zeros(3, dtype=torch.int64, device=dev), torch.zeros(2, **i32), torch.zeros(2, dtype=torch.int64)):
         with pytest.raises(RuntimeError, match="slot_map"):
             q3s.prefix_attention(q, c, c, torch.arange(3, **i32), torch.zeros(2, 1, **i32), torch.ones(2, **i32), slot_map=bad)
+
+
+# ---- a step of PagedCache in a graph -------------------------------------------------------
+
+def test_paged_cache_step_in_a_cuda_graph(dev):
+    """A captured step advances the cache at each replay, as a step that is called does."""
+    rows, heads, dim, block, steps = 5, 2, 64, 16, 40
+    g = torch.Generator(device=dev).manual_seed(0)
+    new = torch.randint(0, 3, (steps, rows), device=dev, generator=g, dtype=torch.int32)
+    gone = torch.rand(steps, rows, device=dev, generator=g) < 0.1
+    x = torch.randn(steps, 2 * rows, heads, dim, device=dev, generator=g).bfloat16()
+
+    def fresh():
+        return q3s.PagedCache(rows, 31, layers=1, kv_heads=heads, dim=dim, block_size=block, max_blocks=6, device=dev)
+
+    def step(cache, n, r, y):
+        t = cache.step(n, max_tokens=2 * rows, released=r)
+        cache.append(0, y, y)
+        return cache.attend(0, y), t
+
+    called = fresh()
+    want = []
+    for i in range(steps):
+        out, t = step(called, new[i], gone[i], x[i])
+        want.append((out, t.lengths.clone(), t.slot_map.clone(), t.error_word.clone()))
+    cache = fresh()
+    n, r, y = new[0].clone(), gone[0].clone(), x[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out, t = step(cache, n, r, y)
+    for i in range(steps):
+        n.copy_(new[i])
+        r.copy_(gone[i])
+        y.copy_(x[i])
+        graph.replay()
+        for got, ref in zip((out, t.lengths, t.slot_map, t.error_word), want[i]):
+            assert torch.equal(got, ref), i
+        assert torch.equal(cache.lengths, t.lengths)
+    assert torch.equal(cache.k, called.k) and torch.equal(cache.table, called.table) and torch.equal(cache.ring, called.ring)
