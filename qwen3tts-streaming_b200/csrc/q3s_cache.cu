@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(NT) cache_tables_kernel(const TablesArgs a) {
   __shared__ Sums s_warp[WARPS];
   const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
   const int cta = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
-  const int chunk = (a.max_tokens + ctas - 1) / ctas;
+  const int chunk = static_cast<int>((static_cast<int64_t>(a.max_tokens) + ctas - 1) / ctas);
   grid_wait();
   grid_release();
   const uint32_t tok0 = static_cast<uint32_t>(min(static_cast<int64_t>(cta) * chunk, static_cast<int64_t>(a.max_tokens)));

@@ -388,3 +388,14 @@ def test_paged_cache_step_in_a_cuda_graph(dev):
             assert torch.equal(got, ref), i
         assert torch.equal(cache.lengths, t.lengths)
     assert torch.equal(cache.k, called.k) and torch.equal(cache.table, called.table) and torch.equal(cache.ring, called.ring)
+
+
+def test_tables_with_the_largest_slot_map(dev):
+    """2^31 - 1 places (26 GB): the CTAs' shares of them are counted in more than 32 bits."""
+    most = 2 ** 31 - 1
+    i32 = dict(dtype=torch.int32, device=dev)
+    t = q3s.cache_tables(torch.tensor([5, 0], **i32), torch.tensor([2, 1], **i32), torch.tensor([[3, -1], [-1, -1]], **i32),
+                         torch.tensor([7, 8], **i32), torch.tensor([0, 2], **i32), block_size=16, max_tokens=most)
+    assert t.slot_map[:3].tolist() == [53, 54, 112] and t.positions[:3].tolist() == [5, 6, 0] and int(t.error_word) == 0
+    assert int(t.slot_map[3:].amax()) == int(t.slot_map[3:].amin()) == -1
+    assert int(t.positions[3:].amax()) == int(t.positions[3:].amin()) == 0
