@@ -191,8 +191,10 @@ typedef struct q3s_quantize_rows_desc {
 q3s_status q3s_quantize_rows(const q3s_quantize_rows_desc* desc, void* stream);
 
 /* y[m, n] = (sum_k a[m, k] * w[n, k]) * a_scales[m] * w_scales[n] (+ bias[n]):
- * 8-bit integers, exact 32-bit sums, one rounding to y's type.  Any operand,
- * the weight too, may be what the call before on the stream writes. */
+ * 8-bit integers and exact 32-bit sums; the sum's conversion, the two products
+ * and the bias are fp32 operations (four roundings of 2^-24, which for fp32 y are
+ * the whole error), then y is rounded to its type.  Any operand, the weight too,
+ * may be what the call before on the stream writes. */
 typedef struct q3s_int8_matmul_desc {
   uint32_t struct_size;        /* = sizeof(q3s_int8_matmul_desc) */
   int32_t rows;                /* M >= 0 */

@@ -69,10 +69,10 @@ Layout layout_of(const q3s_prefix_attention_desc* d) {
   // row: that costs it about queries * keys, the prefix kernel about the square
   // root of the keys (more of them are cut into more parts).  So the rule is on
   // queries^2 * keys.  Key-split against prefix kernel, 8 heads of 128 and 100
-  // own tokens: 32 queries x 2048 keys (2.1e6) 14.2 against 15.0 us, 32 x 8192
-  // (8.4e6) 23.0 against 20.4, 48 x 2048 (4.7e6) 16.7 against 15.6, 128 x 128
-  // (2.1e6) 12.1 against 12.5, 96 x 512 (4.7e6) 14.4 against 12.5, 256 x 8192
-  // 112 against 31.  A scale that is not positive turns the order of the scores
+  // own tokens: 32 queries x 2048 keys (2.1e6) 14.0 against 15.2 us, 32 x 8192
+  // (8.4e6) 22.6 against 20.9, 48 x 2048 (4.7e6) 15.0 against 15.6, 64 x 2048
+  // (8.4e6) 16.8 against 15.6, 128 x 128 (2.1e6) 11.4 to 12.2 against 12.5 to 13.4,
+  // 96 x 512 (4.7e6) 14.4 against 13.0, 256 x 8192 106 to 110 against 28 to 32.  A scale that is not positive turns the order of the scores
   // around, which the prefix kernel's running maximum does not follow.
   l.splits = 0;
   if (queries * queries >= 4000000 / std::max(d->prefix_length, 1) && d->prefix_length >= 64 && d->scale > 0.0f) plan_prefix(d, &l);

@@ -317,9 +317,9 @@ Q3S_DEV AttnCut attn_cut(const AttnArgs& a, long long all, long long ctas, long 
 // operations a byte), as long as a warp's dependent chain of a unit stays below
 // the time that its 8 KB take: 6.8 TB/s while it streams (96 rows, from 4000 to 8000
 // keys), 61 rows of 6000 keys of 2 x 64 (117 MB) in 29.5 us with the start and the
-// join, 96 rows of 500 behind a prefix of 1500 (130 MB) in 31.8.  With 16-row items
+// join, 96 rows of 500 behind a prefix of 1500 (130 MB) in 32.4.  With 16-row items
 // the chain weighs as much, and several tiles copy the same keys: 40 rows of 1 to 9
-// queries x 4 heads behind a prefix of 2049 take 43.9 us, of which the bytes are 16;
+// queries x 4 heads behind a prefix of 2049 take 44.4 us, of which the bytes are 16;
 // taking the products out saved 7.  Two warps sharing the copies of 32 rows took 344
 // in place of 417 us at 40 rows of 5 x 4 queries on 8000 keys, and 5 more here.
 //

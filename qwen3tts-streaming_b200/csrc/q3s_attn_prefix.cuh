@@ -186,7 +186,8 @@ Q3S_DEV float max3(float a, float b, float c) {
 // Bound by the exponentials (16 a clock and SM: 1024 clocks for 128 x 128
 // scores) and, equally, by the two products (1024 clocks at the tensor peak):
 // 256 rows of 4 x 8 heads on 16000 keys of 128 (67 GFLOP, 41 us at the peak of a
-// large product) take 79 us, 54% of the tensor pipe.  Some of the exponentials as
+// large product) take 79 us, 54% of the tensor pipe (the whole operator 92 us in a burst and
+// 107 in seconds of it, at the power limit and 1.66 GHz).  Some of the exponentials as
 // polynomials made it slower (90 to 95 us with the rest of the operator, 88.7
 // without): the two products in the shape 128 x 128 x 16 are near what they
 // reach.  One tile a CTA where that fills more SMs was no faster either: from 2.5

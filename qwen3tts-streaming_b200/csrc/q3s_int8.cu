@@ -30,8 +30,8 @@ bool byte_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int6
 template <int ELEM>
 cudaError_t launch_quantize(const q3s::QuantArgs& a, bool vec, cudaStream_t st) {
   // A warp a row once there are 8 rows a SM; below that a CTA a row has the
-  // shorter chain.  CTA against warp: 592 rows of 2048 1.95 against 2.31 us, 1184
-  // rows 2.52 against 2.36 (of 64: 2.14 against 1.69), 4096 rows 5.42 against 4.56.
+  // shorter chain.  CTA against warp: 592 rows of 2048 1.9 against 2.1 us, 1184
+  // rows 2.5 against 2.3 (of 64: 2.1 against 1.7), 4096 rows 5.6 against 4.4.
   if (vec && a.M >= 8 * q3s::sm_count() && a.K <= 32 * q3s::QW_KEEP * q3s::Elem<ELEM>::N)
     return q3s::launch_maybe_pdl(q3s::quantize_warps_kernel<ELEM>, dim3((a.M + q3s::QW_WARPS - 1) / q3s::QW_WARPS),
                                  dim3(q3s::QW_WARPS * 32), 0, st, true, a);
@@ -50,8 +50,8 @@ cudaError_t launch_gemv_rw(const q3s::Int8Args& a, const q3s::QuantArgs& q, cuda
 template <bool QUANT, int ELEM, int MB>
 cudaError_t launch_gemv_mb(const q3s::Int8Args& a, const q3s::QuantArgs& q, cudaStream_t st) {
   // Outputs of a warp: the fewest with which the CTAs are one a SM.  One against
-  // two, 1 row: 1184 outputs 2.3 against 2.5 us, 2048 outputs 2.9 against 2.5; two
-  // against four, 8 rows: 2048 outputs 4.6 against 5.4, 8000 outputs 10.1 against 7.7.
+  // two, 1 row: 1184 outputs 2.3 against 2.5 us, 2048 outputs 2.7 against 2.5; two
+  // against four, 8 rows: 2048 outputs 4.6 against 5.4, 8000 outputs 10.2 against 7.6.
   const int warps = q3s::sm_count() * q3s::GV_WARPS;
   if (a.N <= warps) return launch_gemv_rw<QUANT, ELEM, MB, 1>(a, q, st);
   if (a.N <= 2 * warps) return launch_gemv_rw<QUANT, ELEM, MB, 2>(a, q, st);
@@ -66,9 +66,9 @@ cudaError_t launch_gemv(const q3s::Int8Args& a, const q3s::QuantArgs& q, cudaStr
 }
 // The vector kernel up to 8 rows of 24 KB in all: every CTA quantises all of
 // them.  Vector kernel against tensor cores with the quantisation: 1 row of 2048,
-// 2048 outputs 2.5 against 7.3 us; 8 rows of 2048, 8000 outputs 7.6 against 8.2,
-// of 4096 13.0 against 11.3; 4 rows of 6144, 8000 outputs 11.9 against 14.2, of
-// 8192 16.7 against 12.5.
+// 2048 outputs 2.5 against 7.2 us; 8 rows of 2048, 8000 outputs 7.6 against 7.6,
+// of 4096 13.0 against 10.7; 4 rows of 6144, 8000 outputs 11.9 against 14.2, of
+// 8192 16.7 against 13.8.
 bool few_rows(int M, int K) { return M <= q3s::GV_MAX_M && static_cast<int64_t>(K) * (M <= 2 ? M : M <= 4 ? 4 : 8) <= q3s::GV_SMEM; }
 
 // -- tensor cores --

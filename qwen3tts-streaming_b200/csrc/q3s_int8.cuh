@@ -689,8 +689,9 @@ __global__ void __launch_bounds__(I8C_NT)
 // halves), because at 8 bits the operands of a one-CTA instruction would take
 // more than the shared memory gives and twice the L2 reads (128 x 128 tiles of
 // one CTA: 200 us for 8192 x 2048 x 8192; 128 x 256: 131 us; this: 98 us, 2.8
-// POP/s, 72% of the tensor pipe).  Bound by the products at the power limit, and
-// at small K by the epilogue (79 us without one; 140 with 4-byte stores from
+// POP/s, 72% of the tensor pipe; bursts of a few ms, 115 us in seconds of them,
+// where the power limit takes the SMs to 1.47 GHz).  Bound by the products at the
+// power limit, and at small K by the epilogue (79 us without one; 140 with 4-byte stores from
 // registers, where a sixth stage changed nothing).  Per CTA: a copy warp, the
 // leading CTA's matrix warp, and eight warps that scale and store the previous
 // tile out of the other half of TMEM, through shared memory and TMA stores.

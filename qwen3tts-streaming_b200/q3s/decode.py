@@ -118,8 +118,8 @@ def int8_matmul(values: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor
                 error_word: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``(values @ weight^T) * scales[:, None] * weight_scales (+ bias)``:
     int8 [M, K] and [N, K] (K a multiple of 16), exact 32-bit sums, fp32
-    scales and bias, one rounding to ``dtype``.  ``error_word`` (int32 [1]) gets
-    ``DECERR_WAIT`` if a device wait gave up, which leaves the result
+    scales, bias and arithmetic after them, rounded to ``dtype`` at the end.
+    ``error_word`` (int32 [1]) gets ``DECERR_WAIT`` if a device wait gave up, which leaves the result
     incomplete."""
     return _op("int8_matmul")(values, scales, weight, weight_scales, dtype, bias, error_word)
 
