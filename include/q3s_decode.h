@@ -1,7 +1,9 @@
 /*
  * q3s_decode.h -- C ABI of the decode step's operators beside the sampler
  * (B200, sm_100a): the paged key/value cache's bookkeeping and append, the
- * attention that reads it, and the 8-bit projections.  Same library and
+ * attention that reads it, the 8-bit projections, and what a step of several
+ * tokens a row needs besides (rotary positions, attention of chunks, drafts
+ * verified, rows cut back).  Same library and
  * conventions as q3s_sampler.h: every pointer in a descriptor is a DEVICE
  * pointer; calls are asynchronous on `stream`, never allocate and never
  * synchronise; arguments are checked on the host before any CUDA call (a bad
@@ -37,6 +39,7 @@ extern "C" {
 #define Q3S_DECERR_TOKENS 8    /* more new tokens than max_tokens: the rest have no slot (Q3S_TABLES_WHOLE_ROWS) */
 #define Q3S_DECERR_BLOCK_ID 16 /* a block id or slot outside the cache: its tokens read as zeros / are not stored */
 #define Q3S_DECERR_WAIT 32     /* a bounded device wait gave up */
+#define Q3S_DECERR_VALUES 64   /* a row stopped at a draft outside the vocabulary (refused), or at logits without a distribution */
 
 /* Element types of the operators' tensors. */
 typedef enum q3s_elem { Q3S_ELEM_F32 = 0, Q3S_ELEM_BF16 = 1, Q3S_ELEM_F16 = 2 } q3s_elem;
@@ -221,8 +224,135 @@ q3s_status q3s_int8_matmul(const q3s_int8_matmul_desc* desc, void* stream);
  * type).  One launch for a few rows, two otherwise. */
 q3s_status q3s_int8_linear(const q3s_quantize_rows_desc* quantize, const q3s_int8_matmul_desc* product, void* stream);
 
+/* Rotary positions, and with caches the append of what was turned.
+ *
+ * Pair i of `pairs` turns by angle = positions[axis(i), t] * inv_freq[i]:
+ *   (x1, x2) -> (x1 c - x2 s, x1 s + x2 c),  c = scale cos, s = scale sin,
+ * x1, x2 being elements i and i + pairs of a head, or with Q3S_ROTARY_ADJACENT
+ * 2i and 2i + 1; elements from 2 * pairs on are copied.  axis(i): the first
+ * sections[0] pairs turn with axis 0, the next sections[1] with axis 1, ...; or
+ * with Q3S_ROTARY_INTERLEAVED i % axes where i < axes * sections[i % axes], else
+ * 0 (each section then fits its axis's places).  The angle is the product in 64
+ * bits, reduced there to an eighth of a turn; cos, sin and the two products are 32-bit (each
+ * result a product and a fused multiply-add), rounded once to the type.
+ *
+ * With k_cache, k is turned like q and stored with v at slot_map, as
+ * q3s_cache_append does; q may have no heads then.  Without, kv_heads is 0. */
+#define Q3S_ROTARY_ADJACENT 1u
+#define Q3S_ROTARY_INTERLEAVED 2u
+#define Q3S_MAX_ROTARY_AXES 4
+
+typedef struct q3s_rotary_desc {
+  uint32_t struct_size;         /* = sizeof(q3s_rotary_desc) */
+  int32_t tokens;               /* T >= 0 */
+  int32_t q_heads;              /* >= 0 */
+  int32_t kv_heads;             /* >= 0; 0: nothing is appended */
+  int32_t dim;
+  int32_t pairs;                /* 1..dim / 2 */
+  int32_t axes;                 /* 1..Q3S_MAX_ROTARY_AXES */
+  int32_t sections[Q3S_MAX_ROTARY_AXES]; /* pairs of each axis, adding up to `pairs` */
+  uint32_t flags;               /* Q3S_ROTARY_* */
+  float scale;                  /* of cos and sin (1, or a scaled rotary's attention factor) */
+  int32_t elem;                 /* q3s_elem of q, k, v, out and the caches */
+  int32_t block_size;
+  int32_t blocks;
+  const int32_t* positions;     /* [axes, T] */
+  int64_t position_stride;      /* elements between axes (0: all the same) */
+  const float* inv_freq;        /* [pairs] */
+  const void* q;                /* [T, q_heads, dim], strides below (elements), unit last stride */
+  int64_t q_token_stride, q_head_stride;
+  void* out;                    /* [T, q_heads, dim]; may be q itself with the same strides */
+  int64_t out_token_stride, out_head_stride;
+  const void* k;                /* [T, kv_heads, dim] */
+  const void* v;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  const int64_t* slot_map;      /* [T]; < 0 = not stored */
+  void* k_cache;                /* [blocks, kv_heads, block_size, dim], strides below (elements) */
+  void* v_cache;
+  int64_t k_block_stride, k_cache_head_stride, k_place_stride;
+  int64_t v_block_stride, v_cache_head_stride, v_place_stride;
+  int32_t* error_word;          /* optional, OR-ed: Q3S_DECERR_BLOCK_ID */
+} q3s_rotary_desc;
+
+q3s_status q3s_rotary(const q3s_rotary_desc* desc, void* stream);
+
+/* Drafted tokens verified against the target's probabilities.
+ *
+ * Row b's tokens of the step are [query_offsets[b], query_offsets[b+1]), n of
+ * them: one that is settled and n - 1 drafts.  With p_t = softmax(logits[t] /
+ * temperature) (temperature below 2^-100 or NaN: all of it at the lowest index
+ * of the largest logit), logits[t] predicting token t + 1, and q_t the
+ * distribution that token t was drawn from (draft_probs[t]; without them all of
+ * it at ids[t]), drafts are taken in order while
+ *   uniforms[t] * q_t(ids[t]) < p_{t-1}(ids[t]).
+ * At the first that is not, at token t, the row draws from max(p_{t-1} - q_t, 0)
+ * (from p_{t-1} where that is 0 everywhere), after its last draft from the last
+ * p: the lowest index whose cumulative sum is above u * total, u being
+ * the uniform of the row's first token.  So the tokens have the distribution
+ * that the target alone gives them.
+ *
+ * Decisions are those of 64-bit arithmetic: probabilities are taken in 32 bits
+ * with a bound on their error, and again in 64 where a comparison is within it;
+ * what a draw is made from is summed in 64 bits.
+ *
+ * A place whose logits hold a NaN, or whose largest is not finite, has no
+ * distribution: a draft there is refused and the draw is the lowest index of the
+ * largest logit that is not a NaN (0 where all are NaN or -infinity);
+ * Q3S_DECERR_VALUES if the row stops there.  (Temperatures are finite.) */
+typedef struct q3s_verify_drafts_desc {
+  uint32_t struct_size;         /* = sizeof(q3s_verify_drafts_desc) */
+  int32_t batch;                /* B, 0..Q3S_MAX_CACHE_ROWS */
+  int32_t tokens;               /* T >= 0 */
+  int32_t vocab;                /* V, 1..Q3S_MAX_VERIFY_VOCAB */
+  int32_t elem;                 /* q3s_elem of logits */
+  float temperature_default;    /* where temperature is NULL */
+  const void* logits;           /* [T, logits_row_stride] */
+  int64_t logits_row_stride;    /* elements, >= V */
+  const int64_t* ids;           /* [T] the step's input tokens */
+  const int32_t* query_offsets; /* [B+1] */
+  const float* uniforms;        /* [T] in [0, 1) */
+  const float* draft_probs;     /* optional [T, draft_row_stride]; not read for a row's first token */
+  int64_t draft_row_stride;     /* elements, >= V */
+  const float* temperature;     /* optional [B] */
+  const int64_t* slot_map;      /* optional [T]: a row with a token without a slot (negative) is left out, like an idle one */
+  int64_t* tokens_out;          /* [T] from each row's first place on: its accepted drafts, then what it drew; -1 behind that and past the last row */
+  int32_t* accepted;            /* [B] drafts accepted; 0 for a row without tokens */
+  int32_t* rejected;            /* [B] drafts not accepted; 0 for a row without tokens */
+  int64_t* next_ids;            /* [B] what the row drew; -1 for a row without tokens */
+  int32_t* error_word;          /* optional, OR-ed */
+} q3s_verify_drafts_desc;
+#define Q3S_MAX_VERIFY_VOCAB (1 << 24)
+
+q3s_status q3s_verify_drafts(const q3s_verify_drafts_desc* desc, void* stream);
+
+/* Rows cut back: row b gives up the last removed[b] of its lengths[b] tokens.
+ * Its blocks past ceil(what is left / block_size) go to the back of the free
+ * ring, in row order, as those of released rows do in q3s_cache_tables;
+ * block_table is only read. */
+typedef struct q3s_cache_trim_desc {
+  uint32_t struct_size;         /* = sizeof(q3s_cache_trim_desc) */
+  int32_t batch;                /* B, 0..Q3S_MAX_CACHE_ROWS */
+  int32_t block_size;           /* tokens per block, >= 1 */
+  int32_t max_blocks;           /* columns of block_table */
+  const int32_t* lengths;       /* [B] */
+  const int32_t* removed;       /* [B]; outside [0, lengths[b]]: cut to it, Q3S_DECERR_LENGTHS */
+  const int32_t* block_table;   /* [B, block_table_stride] */
+  int64_t block_table_stride;   /* elements, >= max_blocks */
+  int32_t* free_blocks;         /* [ring_size] ring of free block ids, updated */
+  const int32_t* free_state;    /* [2]: first entry, number of entries */
+  int32_t* free_state_out;      /* [2], not overlapping any input */
+  int32_t* lengths_out;         /* [B], not overlapping any input */
+  int32_t* error_word;          /* optional, written (not OR-ed): LENGTHS; POOL: more blocks than the ring has room for */
+  int32_t ring_size;            /* blocks that the ring can hold, >= 1 */
+  uint32_t reserved0;
+} q3s_cache_trim_desc;
+
+q3s_status q3s_cache_trim(const q3s_cache_trim_desc* desc, void* stream);
+
 /* sizeof() of the descriptors above as compiled (which: 0 = cache_tables,
- * 1 = cache_append, 2 = prefix_attention, 3 = quantize_rows, 4 = int8_matmul). */
+ * 1 = cache_append, 2 = prefix_attention, 3 = quantize_rows, 4 = int8_matmul,
+ * 5 = rotary, 6 = verify_drafts, 7 = cache_trim). */
 uint32_t q3s_decode_desc_size(int32_t which);
 
 #ifdef __cplusplus

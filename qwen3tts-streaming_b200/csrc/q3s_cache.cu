@@ -1,5 +1,5 @@
-// q3s_cache.cu -- the paged key/value cache's bookkeeping (q3s_cache_tables)
-// and append (q3s_cache_append).
+// q3s_cache.cu -- the paged key/value cache's bookkeeping (q3s_cache_tables,
+// q3s_cache_trim) and append (q3s_cache_append).
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -221,6 +221,98 @@ __global__ void __launch_bounds__(NT) cache_tables_kernel(const TablesArgs a) {
   }
 }
 
+struct TrimArgs {
+  int B, bs, max_blocks, ring;
+  const int32_t* lengths;
+  const int32_t* removed;
+  const int32_t* table;
+  int64_t table_stride;
+  int32_t* free_blocks;
+  const int32_t* free_state;
+  int32_t* free_state_out;
+  int32_t* lengths_out;
+  int32_t* error_word;
+};
+
+// Rows cut back.  As above, one launch without a wait between CTAs: where a
+// row's blocks go is a prefix sum of the blocks that the rows before it give up,
+// so every CTA scans all rows by itself and writes the rows r with
+// r % gridDim.x == c.  Nothing that another CTA reads is written (the ring is
+// only written, lengths and ring state have separate outputs).  A row's entries
+// are copied by its lane where there are up to two, by the warp otherwise.  Bound by launch and latency.
+template <int NT>
+__global__ void __launch_bounds__(NT) cache_trim_kernel(const TrimArgs a) {
+  constexpr int WARPS = NT / 32;
+  __shared__ uint32_t s_warp[2][WARPS];
+  const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
+  const int cta = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
+  grid_wait();
+  grid_release();
+  const int head = min(max(a.free_state[0], 0), a.ring - 1);
+  const int count = min(max(a.free_state[1], 0), a.ring);
+  const int64_t room = static_cast<int64_t>(a.max_blocks) * a.bs;
+  int bad = 0;
+  uint32_t carry = 0;
+  for (int row0 = 0, phase = 0; row0 < a.B; row0 += NT, phase ^= 1) {
+    const int row = row0 + t;
+    const bool in = row < a.B;
+    const int length = in ? a.lengths[row] : 0, gone = in ? a.removed[row] : 0;
+    const int had = static_cast<int>(min(static_cast<int64_t>(max(length, 0)), room)), cut = min(max(gone, 0), had);
+    if (had != length || cut != gone) bad |= Q3S_DECERR_LENGTHS;
+    const int kept = had - cut;
+    const int first = static_cast<int>((static_cast<int64_t>(kept) + a.bs - 1) / a.bs);
+    const int back = static_cast<int>((static_cast<int64_t>(had) + a.bs - 1) / a.bs) - first;
+    uint32_t up = static_cast<uint32_t>(back);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t o = __shfl_up_sync(FULL, up, d);
+      if (lane >= d) up = sat_add(up, o);
+    }
+    if (lane == 31) s_warp[phase][w] = up;
+    __syncthreads();  // one a tile: the next tile writes the other half
+    uint32_t before = __shfl_up_sync(FULL, up, 1);
+    if (lane == 0) before = 0;
+    {
+      uint32_t x = lane < WARPS ? s_warp[phase][lane] : 0u;
+#pragma unroll
+      for (int d = 1; d < WARPS; d <<= 1) {
+        const uint32_t o = __shfl_up_sync(FULL, x, d);
+        if (lane >= d) x = sat_add(x, o);
+      }
+      const uint32_t base = __shfl_sync(FULL, x, max(w - 1, 0));
+      before = sat_add(carry, sat_add(w ? base : 0u, before));
+      carry = sat_add(carry, __shfl_sync(FULL, x, WARPS - 1));
+    }
+    const bool here = in && row % ctas == cta;
+    if (here) a.lengths_out[row] = kept;
+    // entry j of the ring behind its last one, unless it is full
+    auto give = [&](uint32_t rank, int32_t id) {
+      const uint64_t at = static_cast<uint64_t>(count) + rank;
+      if (at < static_cast<uint64_t>(a.ring)) a.free_blocks[(static_cast<uint64_t>(head) + at) % static_cast<uint32_t>(a.ring)] = id;
+    };
+    if (here && back <= 2)
+      for (int j = 0; j < back; ++j) give(sat_add(before, j), a.table[row * a.table_stride + first + j]);
+    unsigned longer = __ballot_sync(FULL, here && back > 2);
+    while (longer) {
+      const int src = __ffs(longer) - 1;
+      longer &= longer - 1;
+      const int r = __shfl_sync(FULL, row, src), n = __shfl_sync(FULL, back, src), f = __shfl_sync(FULL, first, src);
+      const uint32_t behind = __shfl_sync(FULL, before, src);
+      const int32_t* entries = a.table + r * a.table_stride + f;
+      for (int j = lane; j < n; j += 32) give(sat_add(behind, j), entries[j]);
+    }
+  }
+  if (cta == 0) {
+    const int any = __syncthreads_or(bad);
+    if (t == 0) {
+      const uint64_t held = static_cast<uint64_t>(count) + carry;
+      a.free_state_out[0] = head;
+      a.free_state_out[1] = static_cast<int>(min(held, static_cast<uint64_t>(a.ring)));
+      if (a.error_word) *a.error_word = (any ? Q3S_DECERR_LENGTHS : 0) | (held > static_cast<uint64_t>(a.ring) ? Q3S_DECERR_POOL : 0);
+    }
+  }
+}
+
 struct AppendArgs {
   int T, H, bs, blocks;
   int units;  // units of one head's row: dim / 8 (of 16 bytes) or dim (single elements)
@@ -383,6 +475,51 @@ extern "C" q3s_status q3s_cache_tables(const q3s_cache_tables_desc* d, void* str
   return report(Q3S_OK, "");
 }
 
+extern "C" q3s_status q3s_cache_trim(const q3s_cache_trim_desc* d, void* stream) {
+  using q3s::report;
+  if (!d) return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_trim: desc is NULL");
+  if (d->struct_size != sizeof(q3s_cache_trim_desc))
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_trim: struct_size %u != %u (ABI mismatch)", d->struct_size,
+                  static_cast<unsigned>(sizeof(q3s_cache_trim_desc)));
+  if (d->batch < 0 || d->batch > Q3S_MAX_CACHE_ROWS)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_trim: batch %d is not in [0, %d]", d->batch, Q3S_MAX_CACHE_ROWS);
+  if (d->block_size < 1 || d->max_blocks < 1 || d->ring_size < 1)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_trim: block_size, max_blocks and ring_size must be positive");
+  if (static_cast<int64_t>(d->max_blocks) * d->block_size > 0x7fffffffll)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_trim: a table of %d blocks of %d tokens passes 31 bits", d->max_blocks,
+                  d->block_size);
+  if (!d->free_blocks || !d->free_state || !d->free_state_out)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_trim: free_blocks, free_state and free_state_out are required");
+  if (d->batch > 0 && (!d->lengths || !d->removed || !d->block_table || !d->lengths_out))
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_trim: lengths, removed, block_table and lengths_out are required");
+  if (d->batch > 1 && d->block_table_stride < d->max_blocks)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_trim: block_table_stride is below max_blocks");
+  if (d->lengths_out && (d->lengths_out == d->lengths || d->lengths_out == d->removed))
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_trim: lengths_out must not be an input");
+  if (d->free_state_out == d->free_state)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_trim: free_state_out must not be free_state");
+  q3s::TrimArgs a;
+  a.B = d->batch;
+  a.bs = d->block_size;
+  a.max_blocks = d->max_blocks;
+  a.ring = d->ring_size;
+  a.lengths = d->lengths;
+  a.removed = d->removed;
+  a.table = d->block_table;
+  a.table_stride = d->block_table_stride;
+  a.free_blocks = d->free_blocks;
+  a.free_state = d->free_state;
+  a.free_state_out = d->free_state_out;
+  a.lengths_out = d->lengths_out;
+  a.error_word = d->error_word;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const unsigned ctas = static_cast<unsigned>(std::max(1, std::min(q3s::sm_count(), (a.B + 31) / 32)));
+  const cudaError_t e = a.B <= 128 ? q3s::launch_maybe_pdl(q3s::cache_trim_kernel<128>, dim3(ctas), dim3(128), 0, st, true, a)
+                                   : q3s::launch_maybe_pdl(q3s::cache_trim_kernel<1024>, dim3(ctas), dim3(1024), 0, st, true, a);
+  if (e != cudaSuccess) return report(Q3S_ERR_CUDA, "q3s_cache_trim: launch failed: %s", cudaGetErrorString(e));
+  return report(Q3S_OK, "");
+}
+
 extern "C" q3s_status q3s_cache_append(const q3s_cache_append_desc* d, void* stream) {
   using q3s::report;
   if (!d) return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_cache_append: desc is NULL");
@@ -439,6 +576,9 @@ extern "C" uint32_t q3s_decode_desc_size(int32_t which) {
     case 2: return sizeof(q3s_prefix_attention_desc);
     case 3: return sizeof(q3s_quantize_rows_desc);
     case 4: return sizeof(q3s_int8_matmul_desc);
+    case 5: return sizeof(q3s_rotary_desc);
+    case 6: return sizeof(q3s_verify_drafts_desc);
+    case 7: return sizeof(q3s_cache_trim_desc);
   }
   return 0;
 }

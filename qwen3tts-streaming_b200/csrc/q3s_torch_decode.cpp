@@ -12,6 +12,12 @@
 //   quantize_rows(x) -> (values, scales)
 //   int8_matmul(values, scales, weight, weight_scales, dtype, bias=None, error_word!=None) -> y
 //   int8_linear(x, weight, weight_scales, bias=None, error_word!=None) -> (y, values, scales)
+//   rotary(x, positions, inv_freq, sections, interleaved=False, adjacent=False, scale=1.0) -> y
+//   rotary_append(q, k, v, positions, inv_freq, k_cache!, v_cache!, slot_map, sections, interleaved=False,
+//                 adjacent=False, scale=1.0, error_word!=None) -> q
+//   verify_drafts(logits, ids, query_offsets, uniforms, draft_probs=None, temperature=None, temperature_default=1.0,
+//                 slot_map=None, error_word!=None) -> (tokens, accepted, rejected, next_ids)
+//   cache_trim(lengths, removed, block_table, free_blocks!, free_state, block_size) -> (lengths, free_state, error_word)
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -344,6 +350,189 @@ std::tuple<Tensor, Tensor, Tensor> int8_linear(const Tensor& x, const Tensor& we
   return {y.view(shape), values.view(x.sizes()), scales.view(x.sizes().slice(0, x.dim() - 1))};
 }
 
+// What the two rotary operators share: positions [T] or [axes, T], frequencies, sections.
+q3s_rotary_desc rotary_desc(const Tensor& ref, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections,
+                            bool interleaved, bool adjacent, double scale) {
+  q3s_rotary_desc d;
+  std::memset(&d, 0, sizeof(d));
+  d.struct_size = sizeof(d);
+  d.tokens = i32(ref.size(0), "tokens");
+  d.dim = i32(ref.size(2), "dim");
+  d.elem = elem_of(ref, "q");
+  need_vector(inv_freq, ref, at::kFloat, inv_freq.dim() == 1 ? inv_freq.size(0) : 0, "inv_freq");
+  d.pairs = i32(inv_freq.size(0), "inv_freq");
+  const int64_t axes = sections.empty() ? 1 : static_cast<int64_t>(sections.size());
+  TORCH_CHECK(axes <= Q3S_MAX_ROTARY_AXES, "q3s: ", axes, " sections are more than ", Q3S_MAX_ROTARY_AXES);
+  d.axes = static_cast<int32_t>(axes);
+  for (int64_t i = 0; i < axes; ++i) d.sections[i] = sections.empty() ? d.pairs : i32(sections[i], "a section");
+  need(positions, ref, at::kInt, positions.dim() == 2 ? 2 : 1, "positions");
+  TORCH_CHECK(positions.size(-1) == ref.size(0) && (positions.dim() == 1 || positions.size(0) == axes),
+              "q3s: positions must be [", axes, ", ", ref.size(0), "] or [", ref.size(0), "], got ", positions.sizes());
+  TORCH_CHECK(positions.size(-1) <= 1 || positions.stride(-1) == 1, "q3s: positions must have unit token stride");
+  d.positions = positions.data_ptr<int32_t>();
+  d.position_stride = positions.dim() == 2 ? positions.stride(0) : 0;  // [T]: every axis the same
+  d.inv_freq = inv_freq.data_ptr<float>();
+  d.flags = (interleaved ? Q3S_ROTARY_INTERLEAVED : 0u) | (adjacent ? Q3S_ROTARY_ADJACENT : 0u);
+  d.scale = static_cast<float>(scale);
+  return d;
+}
+Tensor rotary_queries(q3s_rotary_desc& d, const Tensor& q) {
+  TORCH_CHECK(q.size(2) <= 1 || q.stride(2) == 1, "q3s: q must have unit last stride");
+  Tensor out = make(q.sizes(), q.scalar_type(), q);
+  d.q_heads = i32(q.size(1), "q_heads");
+  d.q = q.data_ptr();
+  d.q_token_stride = q.stride(0);
+  d.q_head_stride = q.stride(1);
+  d.out = out.data_ptr();
+  d.out_token_stride = q.size(1) * q.size(2);
+  d.out_head_stride = q.size(2);
+  return out;
+}
+
+Tensor rotary(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, at::IntArrayRef sections, bool interleaved,
+              bool adjacent, double scale) {
+  need_cuda(x, "x");
+  c10::cuda::CUDAGuard guard(x.device());
+  need(x, x, x.scalar_type(), 3, "x");
+  q3s_rotary_desc d = rotary_desc(x, positions, inv_freq, sections, interleaved, adjacent, scale);
+  Tensor out = rotary_queries(d, x);
+  check_status(q3s_rotary(&d, stream_of(x)), "q3s_rotary");
+  return out;
+}
+
+Tensor rotary_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& positions, const Tensor& inv_freq,
+                     Tensor k_cache, Tensor v_cache, const Tensor& slot_map, at::IntArrayRef sections, bool interleaved,
+                     bool adjacent, double scale, OptTensor error_word) {
+  need_cuda(q, "q");
+  c10::cuda::CUDAGuard guard(q.device());
+  need(q, q, q.scalar_type(), 3, "q");
+  need(k, q, q.scalar_type(), 3, "k");
+  need(v, q, q.scalar_type(), 3, "v");
+  need_cache(k_cache, q, "k_cache");
+  need_cache(v_cache, q, "v_cache");
+  TORCH_CHECK(k.sizes() == v.sizes() && k_cache.sizes() == v_cache.sizes() && k_cache.size(1) == k.size(1) &&
+                  k_cache.size(3) == k.size(2) && k.size(0) == q.size(0) && k.size(2) == q.size(2),
+              "q3s: q, k and v must be [T, heads, dim] and the caches [blocks, kv_heads, block_size, dim], got ", q.sizes(),
+              k.sizes(), v.sizes(), k_cache.sizes(), v_cache.sizes());
+  TORCH_CHECK((k.size(2) <= 1 || k.stride(2) == 1) && (v.size(2) <= 1 || v.stride(2) == 1),
+              "q3s: k and v must have unit last stride");
+  need_vector(slot_map, q, at::kLong, q.size(0), "slot_map");
+  q3s_rotary_desc d = rotary_desc(q, positions, inv_freq, sections, interleaved, adjacent, scale);
+  d.kv_heads = i32(k.size(1), "kv_heads");
+  d.block_size = i32(k_cache.size(2), "block_size");
+  d.blocks = i32(k_cache.size(0), "blocks");
+  d.k = k.data_ptr();
+  d.v = v.data_ptr();
+  d.k_token_stride = k.stride(0);
+  d.k_head_stride = k.stride(1);
+  d.v_token_stride = v.stride(0);
+  d.v_head_stride = v.stride(1);
+  d.slot_map = slot_map.data_ptr<int64_t>();
+  d.k_cache = k_cache.data_ptr();
+  d.v_cache = v_cache.data_ptr();
+  d.k_block_stride = k_cache.stride(0);
+  d.k_cache_head_stride = k_cache.stride(1);
+  d.k_place_stride = k_cache.stride(2);
+  d.v_block_stride = v_cache.stride(0);
+  d.v_cache_head_stride = v_cache.stride(1);
+  d.v_place_stride = v_cache.stride(2);
+  d.error_word = error_of(error_word, q);
+  Tensor out = rotary_queries(d, q);
+  check_status(q3s_rotary(&d, stream_of(q)), "q3s_rotary");
+  return out;
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> verify_drafts(const Tensor& logits, const Tensor& ids, const Tensor& query_offsets,
+                                                         const Tensor& uniforms, const OptTensor& draft_probs,
+                                                         const OptTensor& temperature, double temperature_default,
+                                                         const OptTensor& slot_map, OptTensor error_word) {
+  need_cuda(logits, "logits");
+  c10::cuda::CUDAGuard guard(logits.device());
+  need(logits, logits, logits.scalar_type(), 2, "logits");
+  const int64_t T = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(V >= 1 && (V == 1 || logits.stride(1) == 1), "q3s: logits must be [T, V] with unit column stride, got ", logits.sizes());
+  need_vector(ids, logits, at::kLong, T, "ids");
+  need(query_offsets, logits, at::kInt, 1, "query_offsets");
+  TORCH_CHECK(query_offsets.size(0) >= 1, "q3s: query_offsets must have an entry for every row and one more");
+  const int64_t B = query_offsets.size(0) - 1;
+  need_vector(query_offsets, logits, at::kInt, B + 1, "query_offsets");
+  need_vector(uniforms, logits, at::kFloat, T, "uniforms");
+  q3s_verify_drafts_desc d;
+  std::memset(&d, 0, sizeof(d));
+  d.struct_size = sizeof(d);
+  d.batch = i32(B, "batch");
+  d.tokens = i32(T, "tokens");
+  d.vocab = i32(V, "vocab");
+  d.elem = elem_of(logits, "logits");
+  d.logits = logits.data_ptr();
+  d.logits_row_stride = T > 1 ? logits.stride(0) : V;
+  d.ids = ids.data_ptr<int64_t>();
+  d.query_offsets = query_offsets.data_ptr<int32_t>();
+  d.uniforms = uniforms.data_ptr<float>();
+  if (draft_probs.has_value()) {
+    need(*draft_probs, logits, at::kFloat, 2, "draft_probs");
+    TORCH_CHECK(draft_probs->size(0) == T && draft_probs->size(1) == V && (V == 1 || draft_probs->stride(1) == 1),
+                "q3s: draft_probs must be [", T, ", ", V, "] with unit column stride, got ", draft_probs->sizes());
+    d.draft_probs = draft_probs->data_ptr<float>();
+    d.draft_row_stride = T > 1 ? draft_probs->stride(0) : V;
+  }
+  if (temperature.has_value()) {
+    need_vector(*temperature, logits, at::kFloat, B, "temperature");
+    d.temperature = temperature->data_ptr<float>();
+  }
+  d.temperature_default = static_cast<float>(temperature_default);
+  if (slot_map.has_value()) {
+    need_vector(*slot_map, logits, at::kLong, T, "slot_map");
+    d.slot_map = slot_map->data_ptr<int64_t>();
+  }
+  d.error_word = error_of(error_word, logits);
+  Tensor tokens = make({T}, at::kLong, logits), accepted = make({B}, at::kInt, logits);
+  Tensor rejected = make({B}, at::kInt, logits), next = make({B}, at::kLong, logits);
+  d.tokens_out = tokens.data_ptr<int64_t>();
+  d.accepted = accepted.data_ptr<int32_t>();
+  d.rejected = rejected.data_ptr<int32_t>();
+  d.next_ids = next.data_ptr<int64_t>();
+  check_status(q3s_verify_drafts(&d, stream_of(logits)), "q3s_verify_drafts");
+  return {tokens, accepted, rejected, next};
+}
+
+std::tuple<Tensor, Tensor, Tensor> cache_trim(const Tensor& lengths, const Tensor& removed, const Tensor& block_table,
+                                              Tensor free_blocks, const Tensor& free_state, int64_t block_size) {
+  need_cuda(lengths, "lengths");
+  c10::cuda::CUDAGuard guard(lengths.device());
+  need(lengths, lengths, at::kInt, 1, "lengths");
+  const int64_t B = lengths.size(0);
+  need_vector(lengths, lengths, at::kInt, B, "lengths");
+  need_vector(removed, lengths, at::kInt, B, "removed");
+  need(block_table, lengths, at::kInt, 2, "block_table");
+  TORCH_CHECK(block_table.size(0) == B && (block_table.size(1) <= 1 || block_table.stride(1) == 1),
+              "q3s: block_table must be [", B, ", max_blocks] with unit column stride, got ", block_table.sizes());
+  need(free_blocks, lengths, at::kInt, 1, "free_blocks");
+  need_vector(free_blocks, lengths, at::kInt, free_blocks.size(0), "free_blocks");
+  need_vector(free_state, lengths, at::kInt, 2, "free_state");
+  apart(free_blocks, block_table, "block_table and free_blocks");
+  q3s_cache_trim_desc d;
+  std::memset(&d, 0, sizeof(d));
+  d.struct_size = sizeof(d);
+  d.batch = i32(B, "batch");
+  d.block_size = i32(block_size, "block_size");
+  d.max_blocks = i32(block_table.size(1), "max_blocks");
+  d.lengths = lengths.data_ptr<int32_t>();
+  d.removed = removed.data_ptr<int32_t>();
+  d.block_table = block_table.data_ptr<int32_t>();
+  d.block_table_stride = B > 1 ? block_table.stride(0) : block_table.size(1);
+  TORCH_CHECK(d.block_table_stride >= block_table.size(1), "q3s: rows of block_table overlap");
+  d.free_blocks = free_blocks.data_ptr<int32_t>();
+  d.ring_size = i32(free_blocks.size(0), "free_blocks");
+  d.free_state = free_state.data_ptr<int32_t>();
+  Tensor left = make({B}, at::kInt, lengths), state = make({2}, at::kInt, lengths), error = make({1}, at::kInt, lengths);
+  d.lengths_out = left.data_ptr<int32_t>();
+  d.free_state_out = state.data_ptr<int32_t>();
+  d.error_word = error.data_ptr<int32_t>();
+  check_status(q3s_cache_trim(&d, stream_of(lengths)), "q3s_cache_trim");
+  return {left, state, error};
+}
+
 // ---- Meta kernels: shapes and dtypes only ------------------------------------
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> cache_tables_meta(const Tensor& context, const Tensor&,
                                                                              Tensor, Tensor, const Tensor&, int64_t,
@@ -375,6 +564,26 @@ std::tuple<Tensor, Tensor, Tensor> int8_linear_meta(const Tensor& x, const Tenso
   return {at::empty(shape, x.options()), std::get<0>(q), std::get<1>(q)};
 }
 
+Tensor rotary_meta(const Tensor& x, const Tensor&, const Tensor&, at::IntArrayRef, bool, bool, double) {
+  return at::empty(x.sizes(), x.options());
+}
+Tensor rotary_append_meta(const Tensor& q, const Tensor&, const Tensor&, const Tensor&, const Tensor&, Tensor, Tensor,
+                          const Tensor&, at::IntArrayRef, bool, bool, double, OptTensor) {
+  return at::empty(q.sizes(), q.options());
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor> verify_drafts_meta(const Tensor&, const Tensor& ids, const Tensor& offsets,
+                                                              const Tensor&, const OptTensor&, const OptTensor&, double,
+                                                              const OptTensor&, OptTensor) {
+  const int64_t B = offsets.size(0) - 1;
+  return {at::empty(ids.sizes(), ids.options()), at::empty({B}, offsets.options()), at::empty({B}, offsets.options()),
+          at::empty({B}, ids.options())};
+}
+std::tuple<Tensor, Tensor, Tensor> cache_trim_meta(const Tensor& lengths, const Tensor&, const Tensor&, Tensor, const Tensor&,
+                                                   int64_t) {
+  const auto o = lengths.options();
+  return {at::empty(lengths.sizes(), o), at::empty({2}, o), at::empty({1}, o)};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(q3s, m) {
@@ -391,6 +600,16 @@ TORCH_LIBRARY_FRAGMENT(q3s, m) {
         "Tensor? bias=None, Tensor(a!)? error_word=None) -> Tensor");
   m.def("int8_linear(Tensor x, Tensor weight, Tensor weight_scales, Tensor? bias=None, Tensor(a!)? error_word=None) -> "
         "(Tensor, Tensor, Tensor)");
+  m.def("rotary(Tensor x, Tensor positions, Tensor inv_freq, int[] sections, bool interleaved=False, bool adjacent=False, "
+        "float scale=1.0) -> Tensor");
+  m.def("rotary_append(Tensor q, Tensor k, Tensor v, Tensor positions, Tensor inv_freq, Tensor(a!) k_cache, "
+        "Tensor(b!) v_cache, Tensor slot_map, int[] sections, bool interleaved=False, bool adjacent=False, "
+        "float scale=1.0, Tensor(c!)? error_word=None) -> Tensor");
+  m.def("verify_drafts(Tensor logits, Tensor ids, Tensor query_offsets, Tensor uniforms, Tensor? draft_probs=None, "
+        "Tensor? temperature=None, float temperature_default=1.0, Tensor? slot_map=None, Tensor(a!)? error_word=None) -> "
+        "(Tensor, Tensor, Tensor, Tensor)");
+  m.def("cache_trim(Tensor lengths, Tensor removed, Tensor block_table, Tensor(a!) free_blocks, Tensor free_state, "
+        "int block_size) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(q3s, CUDA, m) {
@@ -400,6 +619,10 @@ TORCH_LIBRARY_IMPL(q3s, CUDA, m) {
   m.impl("quantize_rows", &quantize_rows);
   m.impl("int8_matmul", &int8_matmul);
   m.impl("int8_linear", &int8_linear);
+  m.impl("rotary", &rotary);
+  m.impl("rotary_append", &rotary_append);
+  m.impl("verify_drafts", &verify_drafts);
+  m.impl("cache_trim", &cache_trim);
 }
 
 TORCH_LIBRARY_IMPL(q3s, Meta, m) {
@@ -409,4 +632,8 @@ TORCH_LIBRARY_IMPL(q3s, Meta, m) {
   m.impl("quantize_rows", &quantize_rows_meta);
   m.impl("int8_matmul", &int8_matmul_meta);
   m.impl("int8_linear", &int8_linear_meta);
+  m.impl("rotary", &rotary_meta);
+  m.impl("rotary_append", &rotary_append_meta);
+  m.impl("verify_drafts", &verify_drafts_meta);
+  m.impl("cache_trim", &cache_trim_meta);
 }

@@ -1,0 +1,512 @@
+// q3s_verify.cu -- drafted tokens verified against the target's probabilities
+// (q3s_verify_drafts).
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "q3s_args.cuh"
+#include "q3s_decode.h"
+#include "q3s_device.cuh"
+#include "q3s_pdl.cuh"
+
+namespace q3s {
+
+namespace cg = cooperative_groups;
+
+struct VerifyArgs {
+  int B, T, V;
+  int slice;   // entries of the vocabulary that a CTA of a row's cluster takes
+  int places;  // places that a CTA looks at together: a power of two, 1..VF_WARPS
+  float temperature_default;
+  const void* logits;
+  int64_t logits_stride;
+  const int64_t* ids;
+  const int32_t* offsets;
+  const float* uniforms;
+  const float* probs;  // or null
+  int64_t probs_stride;
+  const float* temperature;  // or null
+  const int64_t* slot_map;   // or null
+  int64_t* tokens_out;
+  int32_t* accepted;
+  int32_t* rejected;
+  int64_t* next_ids;
+  int32_t* error_word;
+};
+
+constexpr int VF_NT = 512, VF_WARPS = VF_NT / 32;
+constexpr int VF_MAX_CLUSTER = 8;
+// Relative error that a 32-bit probability may have, besides its distance (in
+// log2 units) from the largest one times VF_GAP.  An exponential is off by 2^-22
+// (its instruction) and by the rounding of its argument, 2^-24 ln 2 times its
+// distance from k; averaged over the distribution that distance is at most its
+// entropy and one, so at most 25 (V up to 2^24): 1.0e-6.  c = log2(e) /
+// temperature is off by 2^-23, the same for all entries, which counts times the
+// distance between the draft's logit and the average one: again at most 24 * 2^-23 ln 2
+// = 2.0e-6, or the draft's own distance (VF_GAP).  Sums of eight add 3 * 2^-24, everything
+// after them is 64-bit.  In all 3.4e-6, below 2^-18.
+constexpr double VF_BOUND = 1.0 / (1 << 18), VF_GAP = 1.0 / (1 << 22);
+
+// Beyond this |x c| its rounding is too coarse for the 32-bit sum to say anything.
+constexpr float VF_LARGE = 1048576.0f;
+
+// sum_v 2^(x_v c - k) over some entries, k an integer above their largest
+// x c (however large that is: no term overflows), with the largest logit and its
+// lowest index.  A NaN among the entries makes the sum one; nothing else does
+// where the largest logit is finite.
+struct VerifyStat {
+  double sum;
+  float k, best;
+  int index;
+};
+
+// 2^d for an integer d <= 0 (0 below -1000), exactly.
+Q3S_DEV double pow2_int(float d) { return d < -1000.0f ? 0.0 : __hiloint2double((1023 + static_cast<int>(d)) << 20, 0); }
+
+Q3S_DEV VerifyStat verify_join(const VerifyStat& a, const VerifyStat& b) {
+  VerifyStat r;
+  r.k = fmaxf(a.k, b.k);
+  // -inf: nothing there, or only entries that have no probability (sum 0)
+  r.sum = a.sum * (a.k == r.k ? 1.0 : pow2_int(a.k - r.k)) + b.sum * (b.k == r.k ? 1.0 : pow2_int(b.k - r.k));
+  const bool first = a.best > b.best || (a.best == b.best && a.index < b.index);
+  r.best = first ? a.best : b.best;
+  r.index = first ? a.index : b.index;
+  return r;
+}
+Q3S_DEV VerifyStat verify_shfl_xor(const VerifyStat& a, int d) {
+  return {__shfl_xor_sync(FULL, a.sum, d), __shfl_xor_sync(FULL, a.k, d), __shfl_xor_sync(FULL, a.best, d),
+          __shfl_xor_sync(FULL, a.index, d)};
+}
+// Whether the logits have a distribution.
+Q3S_DEV bool verify_defined(const VerifyStat& s) { return s.sum == s.sum && fabsf(s.best) < INFINITY; }
+Q3S_DEV float vf_ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// N neighbouring entries, the first at index v.
+template <int N>
+Q3S_DEV void verify_take(VerifyStat& s, const float (&x)[N], int v, float c) {
+  float top = x[0];
+#pragma unroll
+  for (int e = 1; e < N; ++e) top = fmaxf(top, x[e]);
+  if (top > s.best) {
+    s.best = top;
+    int at = N - 1;
+#pragma unroll
+    for (int e = N - 2; e >= 0; --e) at = x[e] == top ? e : at;
+    s.index = v + at;
+    const float y = top * c, k = ceilf(fmaf(fabsf(y), 2.384185791015625e-07f, y));  // 2^-22: above the rounding of y
+    if (k > s.k) {
+      s.sum = s.k == -INFINITY ? 0.0 : s.sum * pow2_int(fmaxf(s.k - k, -2000.0f));
+      s.k = k;
+    }
+  }
+  const float k = s.k == -INFINITY ? 0.0f : s.k;
+  float e[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = vf_ex2(fmaf(x[i], c, -k));
+#pragma unroll
+  for (int w = 1; w < N; w *= 2)
+#pragma unroll
+    for (int i = 0; i + w < N; i += 2 * w) e[i] += e[i + w];
+  s.sum += static_cast<double>(e[0]);  // a NaN among the entries stays one
+}
+
+template <typename T>
+struct VerifyVec;
+template <>
+struct VerifyVec<float> {
+  static constexpr int N = 4;
+  Q3S_DEV static void load(const float* p, float (&x)[4]) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+  }
+};
+template <>
+struct VerifyVec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  Q3S_DEV static void load(const __nv_bfloat16* p, float (&x)[8]) {
+    const uint4 f = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+};
+template <>
+struct VerifyVec<__half> {
+  static constexpr int N = 8;
+  Q3S_DEV static void load(const __half* p, float (&x)[8]) {
+    const uint4 f = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = h.x, x[2 * i + 1] = h.y;
+    }
+  }
+};
+
+// One row's shared state of a CTA.
+struct VerifyShared {
+  VerifyStat warp[VF_WARPS];
+  VerifyStat part[VF_WARPS][VF_MAX_CLUSTER];  // [place][CTA of the cluster], written by that CTA
+  double sums[VF_MAX_CLUSTER * VF_WARPS];     // a pass's sums, CTA by CTA and warp by warp
+  VerifyStat stat;                            // of the place that is being decided
+  int verdict, place, winner;
+  double before, aim;
+  int refused;
+};
+
+// A cluster a row; its CTAs cut the vocabulary into slices.
+//
+// First pass, in 32 bits: groups of the CTA's warps take `places` of the row's places at once,
+// a running maximum and sum each.  The partial results meet in every CTA's shared memory, and
+// every CTA decides for itself, in the same order, which drafts hold; a comparison within the bound of the 32-bit sum's error is
+// decided again from a 64-bit sum.  Then the place where the row stops is drawn from: each warp sums its
+// neighbouring entries in 64 bits, the sums meet, and the one warp whose entries reach u * total looks for the entry.
+template <typename T>
+__global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
+  __shared__ VerifyShared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
+  const int b = static_cast<int>(blockIdx.x) / ctas;
+  auto sync = [&]() {
+    if (ctas > 1) cluster.sync(); else __syncthreads();
+  };
+  grid_wait();
+  grid_release();
+
+  // ---- the row's tokens ----
+  int t0 = 0, n = 0;
+  if (b < a.B) {
+    const int o0 = a.offsets[b], o1 = a.offsets[b + 1];
+    t0 = min(max(o0, 0), a.T);
+    const int end = min(max(o1, t0), a.T);
+    n = end - t0;
+    if ((t0 != o0 || end != o1) && t == 0 && rank == 0 && a.error_word) atomicOr(a.error_word, Q3S_DECERR_LENGTHS);
+  }
+  if (t == 0) sh.refused = 0;
+  __syncthreads();
+  if (rank == 0 && b >= a.B - 1) {  // places past the last row
+    const int last = a.B ? t0 + n : 0;
+    for (int i = last + t; i < a.T; i += VF_NT) a.tokens_out[i] = -1;
+  }
+  if (a.slot_map) {
+    bool without = false;
+    for (int i = t; i < n; i += VF_NT) without |= a.slot_map[t0 + i] < 0;
+    if (without) sh.refused = 1;  // every writer writes 1
+    __syncthreads();
+  }
+  if (n == 0 || sh.refused) {  // the same in all CTAs of the cluster
+    if (rank == 0) {
+      for (int i = t; i < n; i += VF_NT) a.tokens_out[t0 + i] = -1;
+      if (t == 0 && b < a.B) {
+        a.accepted[b] = 0;
+        a.rejected[b] = 0;
+        a.next_ids[b] = -1;
+      }
+    }
+    return;
+  }
+  const float heat = a.temperature ? a.temperature[b] : a.temperature_default;
+  const bool greedy = !(heat >= 7.888609052210118e-31f);  // 2^-100
+  const float c = greedy ? 1.0f : 1.4426950408889634f / heat;
+  const double c64 = greedy ? 1.0 : 1.4426950408889634074 / static_cast<double>(heat);
+  const int v0 = min(rank * a.slice, a.V), v1 = min(v0 + a.slice, a.V);
+  const T* logits = static_cast<const T*>(a.logits);
+
+  // ---- 64-bit passes over one place: each warp's neighbouring entries ----
+  const int share = ((v1 - v0 + VF_WARPS - 1) / VF_WARPS + 31) & ~31;
+  const int w0 = min(v0 + w * share, v1), w1 = min(w0 + share, v1);
+  // e(v) = 2^((x_v - largest) log2(e) / temperature)
+  auto weight = [&](const T* x, int v, double best) { return exp2((static_cast<double>(static_cast<float>(x[v])) - best) * c64); };
+  // f summed over the vocabulary: the warps' sums meet in every CTA
+  auto sum_all = [&](auto f) {
+    double s = 0.0;
+    for (int v = w0 + lane; v < w1; v += 32) s += f(v);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(FULL, s, d);
+    sync();  // the sums of the pass before have been read
+    for (int r = lane; r < ctas; r += 32) cluster.map_shared_rank(&sh, r)->sums[rank * VF_WARPS + w] = s;
+    sync();
+    double total = 0.0;
+    for (int i = 0; i < ctas * VF_WARPS; i += 32) {
+      double x = i + lane < ctas * VF_WARPS ? sh.sums[i + lane] : 0.0;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(FULL, x, d);
+      total += x;
+    }
+    return total;
+  };
+
+  // ---- which drafts hold ----
+  int place = 0;  // where the row stops
+  const int group = VF_WARPS / a.places;
+  for (int first = 0;; first += a.places) {
+    const int mine = first + w / group;
+    VerifyStat s = {0.0, -INFINITY, -INFINITY, 0x7fffffff};
+    if (mine < n) {
+      constexpr int N = VerifyVec<T>::N;
+      const T* x = logits + (t0 + mine) * a.logits_stride;
+      const int lanes = group * 32, l = (w % group) * 32 + lane;
+      // single entries up to the first 16-byte boundary, vectors, single entries
+      const int head = static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(x + v0) & 15)) & 15) / sizeof(T));
+      const int vec0 = min(v0 + head, v1), vecs = (v1 - vec0) / N;
+      if (l < vec0 - v0) {
+        const float one[1] = {static_cast<float>(x[v0 + l])};
+        verify_take<1>(s, one, v0 + l, c);
+      }
+#pragma unroll 4
+      for (int i = l; i < vecs; i += lanes) {
+        float y[N];
+        VerifyVec<T>::load(x + vec0 + i * N, y);
+        verify_take<N>(s, y, vec0 + i * N, c);
+      }
+      const int rest = vec0 + vecs * N + l;
+      if (rest < v1) {
+        const float one[1] = {static_cast<float>(x[rest])};
+        verify_take<1>(s, one, rest, c);
+      }
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) s = verify_join(s, verify_shfl_xor(s, d));
+    if (lane == 0) sh.warp[w] = s;
+    sync();  // and the parts of the turn before have been read
+    if (t < a.places) {
+      VerifyStat p = sh.warp[t * group];
+      for (int i = 1; i < group; ++i) p = verify_join(p, sh.warp[t * group + i]);
+      for (int r = 0; r < ctas; ++r) cluster.map_shared_rank(&sh, r)->part[t][rank] = p;
+    }
+    sync();
+    int from = 0;  // places of this turn that are decided
+    bool stop = false;
+    while (!stop) {
+      if (w == 0) {
+        const int i = first + lane;
+        const bool live = lane < a.places && i < n;
+        VerifyStat p = {0.0, -INFINITY, -INFINITY, 0x7fffffff};
+        int verdict = 1;  // 0: the row stops here, 1: the draft holds, 2: too close
+        if (live) {
+          p = sh.part[lane][0];
+          for (int r = 1; r < ctas; ++r) p = verify_join(p, sh.part[lane][r]);
+          verdict = 0;
+          if (i + 1 < n && verify_defined(p)) {
+            const int64_t d = a.ids[t0 + i + 1];
+            if (d >= 0 && d < a.V) {
+              const double q = a.probs ? static_cast<double>(a.probs[(t0 + i + 1) * a.probs_stride + d]) : 1.0;
+              const double aim = static_cast<double>(a.uniforms[t0 + i + 1]) * q;
+              if (greedy) {
+                verdict = aim < (d == p.index ? 1.0 : 0.0);
+              } else {
+                const float x = static_cast<float>(logits[(t0 + i) * a.logits_stride + d]);
+                const double y = static_cast<double>(x) * static_cast<double>(c) - static_cast<double>(p.k);
+                const double left = aim * p.sum, right = exp2(y);
+                const double error = (VF_BOUND - VF_GAP * fmin(y, 0.0)) * (left + right);
+                verdict = !(p.sum > 0.0) || fabsf(p.k) > VF_LARGE ? 2
+                          : !(right > 0.0)                        ? 0
+                          : fabs(left - right) <= error           ? 2
+                                                                  : left < right;
+              }
+            }
+          }
+        }
+        const unsigned open = __ballot_sync(FULL, live && verdict != 1 && lane >= from);
+        const int at = open ? __ffs(open) - 1 : 0;
+        if (open && lane == at) {
+          sh.place = at;
+          sh.verdict = verdict;
+          sh.stat = p;
+        }
+        if (!open && lane == 0) sh.verdict = 1;
+      }
+      __syncthreads();
+      const int verdict = sh.verdict, at = sh.place;
+      if (verdict == 1) break;  // all drafts of this turn hold
+      place = first + at;
+      if (verdict == 0) {
+        stop = true;
+      } else {
+        const T* x = logits + (t0 + place) * a.logits_stride;
+        const double best = static_cast<double>(sh.stat.best);
+        const double total = sum_all([&](int v) { return weight(x, v, best); });
+        const int64_t d = a.ids[t0 + place + 1];
+        const double q = a.probs ? static_cast<double>(a.probs[(t0 + place + 1) * a.probs_stride + d]) : 1.0;
+        stop = !(static_cast<double>(a.uniforms[t0 + place + 1]) * q * total < weight(x, static_cast<int>(d), best));
+        from = at + 1;
+      }
+      __syncthreads();  // before warp 0 writes the next verdict
+    }
+    if (stop) break;
+  }
+
+  // ---- the draw ----
+  const VerifyStat stat = sh.stat;
+  const bool bad = !verify_defined(stat);
+  const T* x = logits + (t0 + place) * a.logits_stride;
+  const int64_t draft = place + 1 < n ? a.ids[t0 + place + 1] : -1;
+  if (rank == 0) {
+    for (int i = t; i < n; i += VF_NT)
+      if (i != place) a.tokens_out[t0 + i] = i < place ? a.ids[t0 + i + 1] : -1;
+    if (t == 0) {
+      a.accepted[b] = place;
+      a.rejected[b] = n - 1 - place;
+      const bool outside = place + 1 < n && (draft < 0 || draft >= a.V);
+      if ((bad || outside) && a.error_word) atomicOr(a.error_word, Q3S_DECERR_VALUES);
+    }
+  }
+  auto finish = [&](int id) {
+    a.next_ids[b] = id;
+    a.tokens_out[t0 + place] = id;
+  };
+  if (bad || greedy) {
+    if (rank == 0 && t == 0) finish(stat.index == 0x7fffffff ? 0 : stat.index);
+    return;
+  }
+  const double best = static_cast<double>(stat.best);
+  const float* q = a.probs && place + 1 < n ? a.probs + (t0 + place + 1) * a.probs_stride : nullptr;
+  double mass = 0.0;  // sum of e: q is taken times it
+  if (q) mass = sum_all([&](int v) { return weight(x, v, best); });
+  int mode = q ? 2 : place + 1 < n && draft >= 0 && draft < a.V ? 1 : 0;  // what p loses: q, the draft, nothing
+  auto left = [&](int v) {
+    const double e = weight(x, v, best);
+    return mode == 2 ? fmax(e - static_cast<double>(q[v]) * mass, 0.0) : mode == 1 && v == static_cast<int>(draft) ? 0.0 : e;
+  };
+  double total = sum_all(left);
+  if (!(total > 0.0)) {  // nothing is left: from p
+    mode = 0;
+    total = sum_all(left);
+  }
+  if (w == 0) {  // the warp (of all CTAs') whose entries reach u * total: its number, and the sum before it
+    const double aim = static_cast<double>(a.uniforms[t0]) * total;
+    const int warps = ctas * VF_WARPS;
+    double carry = 0.0, before = 0.0;
+    int winner = -1, last = 0;  // last: the last warp with a sum
+    for (int i = 0; i < warps; i += 32) {
+      const double s = i + lane < warps ? sh.sums[i + lane] : 0.0;
+      double up = s;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const double o = __shfl_up_sync(FULL, up, d);
+        if (lane >= d) up += o;
+      }
+      const double at = carry + up;
+      const double prior = __shfl_up_sync(FULL, at, 1);
+      const unsigned over = __ballot_sync(FULL, s > 0.0 && at > aim), some = __ballot_sync(FULL, s > 0.0);
+      if (winner < 0 && over) {
+        const int src = __ffs(over) - 1;
+        winner = i + src;
+        before = src ? __shfl_sync(FULL, prior, src) : carry;
+      }
+      if (some) last = i + 31 - __clz(some);
+      carry = __shfl_sync(FULL, at, 31);
+    }
+    if (lane == 0) {
+      sh.winner = winner < 0 ? last : winner;
+      sh.before = before;
+      sh.aim = winner < 0 ? INFINITY : aim;  // rounding left the aim at or above the sum: the last entry that has any
+    }
+  }
+  __syncthreads();
+  if (sh.winner == rank * VF_WARPS + w) {
+    double carry = sh.before;
+    const double aim = sh.aim;
+    int id = -1, last = v0;
+    for (int v = w0; v < w1 && id < 0; v += 32) {
+      const double s = v + lane < w1 ? left(v + lane) : 0.0;
+      double up = s;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const double o = __shfl_up_sync(FULL, up, d);
+        if (lane >= d) up += o;
+      }
+      const unsigned over = __ballot_sync(FULL, s > 0.0 && carry + up > aim), some = __ballot_sync(FULL, s > 0.0);
+      if (over) id = v + __ffs(over) - 1;
+      if (some) last = v + 31 - __clz(some);
+      carry += __shfl_sync(FULL, up, 31);
+    }
+    if (lane == 0) finish(id < 0 ? last : id);
+  }
+}
+
+template <typename T>
+cudaError_t launch_verify(const VerifyArgs& a, int ctas, cudaStream_t st) {
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3(static_cast<unsigned>(std::max(a.B, 1)) * ctas);
+  lc.blockDim = dim3(VF_NT);
+  lc.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = static_cast<unsigned>(ctas);
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  lc.attrs = at;
+  lc.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&lc, verify_kernel<T>, a);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+}  // namespace q3s
+
+extern "C" q3s_status q3s_verify_drafts(const q3s_verify_drafts_desc* d, void* stream) {
+  using q3s::report;
+  if (!d) return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_verify_drafts: desc is NULL");
+  if (d->struct_size != sizeof(q3s_verify_drafts_desc))
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_verify_drafts: struct_size %u != %u (ABI mismatch)", d->struct_size,
+                  static_cast<unsigned>(sizeof(q3s_verify_drafts_desc)));
+  if (d->batch < 0 || d->batch > Q3S_MAX_CACHE_ROWS || d->tokens < 0)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_verify_drafts: batch %d is not in [0, %d] or tokens %d is negative", d->batch,
+                  Q3S_MAX_CACHE_ROWS, d->tokens);
+  if (d->vocab < 1 || d->vocab > Q3S_MAX_VERIFY_VOCAB)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_verify_drafts: vocab %d is not in [1, %d]", d->vocab, Q3S_MAX_VERIFY_VOCAB);
+  if (d->elem != Q3S_ELEM_F32 && d->elem != Q3S_ELEM_BF16 && d->elem != Q3S_ELEM_F16)
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_verify_drafts: unknown elem %d", d->elem);
+  if (!d->query_offsets) return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_verify_drafts: query_offsets is required");
+  if (d->batch > 0 && (!d->accepted || !d->rejected || !d->next_ids))
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_verify_drafts: accepted, rejected and next_ids are required");
+  if (d->tokens > 0 && (!d->logits || !d->ids || !d->uniforms || !d->tokens_out))
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_verify_drafts: logits, ids, uniforms and tokens_out are required");
+  if (d->tokens > 1 && (d->logits_row_stride < d->vocab || (d->draft_probs && d->draft_row_stride < d->vocab)))
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_verify_drafts: row strides are below vocab");
+  if (d->tokens_out == d->ids && d->ids) return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_verify_drafts: tokens_out must not be ids");
+  if (d->batch == 0 && d->tokens == 0) return report(Q3S_OK, "");
+  q3s::VerifyArgs a;
+  a.B = d->batch;
+  a.T = d->tokens;
+  a.V = d->vocab;
+  a.temperature_default = d->temperature_default;
+  a.logits = d->logits;
+  a.logits_stride = d->logits_row_stride;
+  a.ids = d->ids;
+  a.offsets = d->query_offsets;
+  a.uniforms = d->uniforms;
+  a.probs = d->draft_probs;
+  a.probs_stride = d->draft_row_stride;
+  a.temperature = d->temperature;
+  a.slot_map = d->slot_map;
+  a.tokens_out = d->tokens_out;
+  a.accepted = d->accepted;
+  a.rejected = d->rejected;
+  a.next_ids = d->next_ids;
+  a.error_word = d->error_word;
+  int ctas = 1;
+  while (ctas < q3s::VF_MAX_CLUSTER && static_cast<int64_t>(ctas) * 8192 < a.V) ctas *= 2;
+  a.slice = ((a.V + ctas - 1) / ctas + 31) & ~31;
+  // as many places at once as a row of the batch has on average
+  const int mean = (a.T + std::max(a.B, 1) - 1) / std::max(a.B, 1);
+  a.places = 1;
+  while (a.places < std::min(mean, q3s::VF_WARPS)) a.places *= 2;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = d->elem == Q3S_ELEM_F32    ? q3s::launch_verify<float>(a, ctas, st)
+                        : d->elem == Q3S_ELEM_BF16 ? q3s::launch_verify<__nv_bfloat16>(a, ctas, st)
+                                                   : q3s::launch_verify<__half>(a, ctas, st);
+  if (e != cudaSuccess) return report(Q3S_ERR_CUDA, "q3s_verify_drafts: launch failed: %s", cudaGetErrorString(e));
+  return report(Q3S_OK, "");
+}

@@ -6,14 +6,21 @@ itself runs only in the sm_100a kernels of ``libq3s_sampler.so``.
 from . import _lib
 from .decode import (
     CacheTables,
+    CacheTrim,
     Int8Linear,
     PagedCache,
+    Rotary,
+    VerifiedDrafts,
     cache_append,
     cache_tables,
+    cache_trim,
     int8_linear,
     int8_matmul,
     prefix_attention,
     quantize_rows,
+    rotary,
+    rotary_append,
+    verify_drafts,
 )
 from .step import RowHistory, StepGuard, step_update
 from .ops import (
@@ -36,14 +43,21 @@ from .ops import (
 
 __all__ = [
     "CacheTables",
+    "CacheTrim",
     "Int8Linear",
     "PagedCache",
+    "Rotary",
+    "VerifiedDrafts",
     "cache_append",
     "cache_tables",
+    "cache_trim",
     "int8_linear",
     "int8_matmul",
     "prefix_attention",
     "quantize_rows",
+    "rotary",
+    "rotary_append",
+    "verify_drafts",
     "CodecSampler",
     "CpFramePlan",
     "HeadPlan",

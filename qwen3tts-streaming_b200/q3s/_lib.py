@@ -169,6 +169,8 @@ class HeadDesc(C.Structure):
 ELEM_F32, ELEM_BF16, ELEM_F16 = 0, 1, 2
 MAX_CACHE_ROWS, MAX_QUERY_GROUP = 65536, 16
 TABLES_WHOLE_ROWS = 1
+ROTARY_ADJACENT, ROTARY_INTERLEAVED, MAX_ROTARY_AXES = 1, 2, 4
+MAX_VERIFY_VOCAB = 1 << 24
 
 
 class CacheTablesDesc(C.Structure):
@@ -302,7 +304,96 @@ class Int8MatmulDesc(C.Structure):
     ]
 
 
-DECODE_DESCS = (CacheTablesDesc, CacheAppendDesc, PrefixAttentionDesc, QuantizeRowsDesc, Int8MatmulDesc)
+class RotaryDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("tokens", C.c_int32),
+        ("q_heads", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("dim", C.c_int32),
+        ("pairs", C.c_int32),
+        ("axes", C.c_int32),
+        ("sections", C.c_int32 * MAX_ROTARY_AXES),
+        ("flags", C.c_uint32),
+        ("scale", C.c_float),
+        ("elem", C.c_int32),
+        ("block_size", C.c_int32),
+        ("blocks", C.c_int32),
+        ("positions", _p),
+        ("position_stride", C.c_int64),
+        ("inv_freq", _p),
+        ("q", _p),
+        ("q_token_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("out", _p),
+        ("out_token_stride", C.c_int64),
+        ("out_head_stride", C.c_int64),
+        ("k", _p),
+        ("v", _p),
+        ("k_token_stride", C.c_int64),
+        ("k_head_stride", C.c_int64),
+        ("v_token_stride", C.c_int64),
+        ("v_head_stride", C.c_int64),
+        ("slot_map", _p),
+        ("k_cache", _p),
+        ("v_cache", _p),
+        ("k_block_stride", C.c_int64),
+        ("k_cache_head_stride", C.c_int64),
+        ("k_place_stride", C.c_int64),
+        ("v_block_stride", C.c_int64),
+        ("v_cache_head_stride", C.c_int64),
+        ("v_place_stride", C.c_int64),
+        ("error_word", _p),
+    ]
+
+
+class VerifyDraftsDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("batch", C.c_int32),
+        ("tokens", C.c_int32),
+        ("vocab", C.c_int32),
+        ("elem", C.c_int32),
+        ("temperature_default", C.c_float),
+        ("logits", _p),
+        ("logits_row_stride", C.c_int64),
+        ("ids", _p),
+        ("query_offsets", _p),
+        ("uniforms", _p),
+        ("draft_probs", _p),
+        ("draft_row_stride", C.c_int64),
+        ("temperature", _p),
+        ("slot_map", _p),
+        ("tokens_out", _p),
+        ("accepted", _p),
+        ("rejected", _p),
+        ("next_ids", _p),
+        ("error_word", _p),
+    ]
+
+
+class CacheTrimDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("batch", C.c_int32),
+        ("block_size", C.c_int32),
+        ("max_blocks", C.c_int32),
+        ("lengths", _p),
+        ("removed", _p),
+        ("block_table", _p),
+        ("block_table_stride", C.c_int64),
+        ("free_blocks", _p),
+        ("free_state", _p),
+        ("free_state_out", _p),
+        ("lengths_out", _p),
+        ("error_word", _p),
+        ("ring_size", C.c_int32),
+        ("reserved0", C.c_uint32),
+    ]
+
+
+DECODE_DESCS = (CacheTablesDesc, CacheAppendDesc, PrefixAttentionDesc, QuantizeRowsDesc, Int8MatmulDesc,
+                RotaryDesc, VerifyDraftsDesc, CacheTrimDesc)
 # every symbol include/q3s_decode.h declares
 DECODE_EXPORTS = (
     "q3s_cache_tables",
@@ -312,6 +403,9 @@ DECODE_EXPORTS = (
     "q3s_quantize_rows",
     "q3s_int8_matmul",
     "q3s_int8_linear",
+    "q3s_rotary",
+    "q3s_verify_drafts",
+    "q3s_cache_trim",
     "q3s_decode_desc_size",
 )
 
@@ -368,7 +462,7 @@ def load(path: str | Path | None = None) -> C.CDLL:
         lib.q3s_head_sample.argtypes = [C.POINTER(HeadDesc), _p]
         lib.q3s_head_sample.restype = C.c_int
         for name, st in zip(("q3s_cache_tables", "q3s_cache_append", "q3s_prefix_attention", "q3s_quantize_rows",
-                             "q3s_int8_matmul"), DECODE_DESCS):
+                             "q3s_int8_matmul", "q3s_rotary", "q3s_verify_drafts", "q3s_cache_trim"), DECODE_DESCS):
             getattr(lib, name).argtypes = [C.POINTER(st), _p]
             getattr(lib, name).restype = C.c_int
         lib.q3s_int8_linear.argtypes = [C.POINTER(QuantizeRowsDesc), C.POINTER(Int8MatmulDesc), _p]

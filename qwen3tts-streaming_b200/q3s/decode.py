@@ -18,7 +18,7 @@ the C ABI of ``include/q3s_decode.h``.  There is no CPU fallback.
 """
 from __future__ import annotations
 
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Sequence, Union
 
 import torch
 
@@ -26,6 +26,7 @@ from . import torch_ops
 
 #: bits of the error words (include/q3s_decode.h)
 DECERR_LENGTHS, DECERR_TABLE, DECERR_POOL, DECERR_TOKENS, DECERR_BLOCK_ID, DECERR_WAIT = 1, 2, 4, 8, 16, 32
+DECERR_VALUES = 64
 
 _bound: dict = {}
 
@@ -102,6 +103,116 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     out, lse = _op("prefix_attention")(q, k_cache, v_cache, query_offsets, block_table, lengths, prefix_blocks,
                                        prefix_length, scale, error_word, slot_map)
     return (out, lse) if return_lse else out
+
+
+class CacheTrim(NamedTuple):
+    """What ``cache_trim`` leaves (device tensors)."""
+
+    lengths: torch.Tensor     # int32 [B]: tokens that stay in the cache
+    free_state: torch.Tensor  # int32 [2]: the ring's first entry and number of entries
+    error_word: torch.Tensor  # int32 [1]: DECERR_* bits
+
+
+def cache_trim(lengths: torch.Tensor, removed: torch.Tensor, block_table: torch.Tensor, free_blocks: torch.Tensor,
+               free_state: torch.Tensor, *, block_size: int) -> CacheTrim:
+    """Take the last ``removed[b]`` tokens of every row back out of the cache,
+    in one launch: the blocks that a row no longer needs go to the back of the
+    ring ``free_blocks`` (updated in place) in row order.  ``block_table`` is
+    only read: entries past a row's blocks mean nothing.  ``removed`` outside
+    [0, lengths[b]] is cut to it (``DECERR_LENGTHS``)."""
+    return tuple.__new__(CacheTrim, _op("cache_trim")(lengths, removed, block_table, free_blocks, free_state, block_size))
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, sections: Optional[Sequence[int]] = None,
+           interleaved: bool = False, adjacent: bool = False, scale: float = 1.0) -> torch.Tensor:
+    """Rotary positions of ``x`` [T, heads, dim] (bf16, f16 or fp32, any
+    strides with unit last one): a new tensor in which pair i of every head is
+    turned by ``positions[axis(i)][t] * inv_freq[i]``.
+
+    ``inv_freq`` fp32 [P] turns the first 2 P dims (2 P <= dim; the others are
+    copied), as pairs (i, i + P), or (2 i, 2 i + 1) with ``adjacent``.
+    ``positions`` int32 [T], or [axes, T] for several axes (time, height, width),
+    whose pairs ``sections`` counts (``sum(sections) == P``): the first
+    sections[0] pairs turn with axis 0 and so on, or with ``interleaved`` pair i
+    with axis i % axes while i < axes * sections[i % axes], else with axis 0.
+    The angle is exact to 64 bits, far positions included; cos and sin are
+    multiplied by ``scale``."""
+    return _op("rotary")(x, positions, inv_freq, sections or (), interleaved, adjacent, scale)
+
+
+def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                  k_cache: torch.Tensor, v_cache: torch.Tensor, slot_map: torch.Tensor, *,
+                  sections: Optional[Sequence[int]] = None, interleaved: bool = False, adjacent: bool = False,
+                  scale: float = 1.0, error_word: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``rotary`` of the step's queries and keys and ``cache_append`` of the
+    turned keys and the values, in one launch that reads and writes each once.
+    Returns the queries."""
+    return _op("rotary_append")(q, k, v, positions, inv_freq, k_cache, v_cache, slot_map, sections or (), interleaved,
+                                adjacent, scale, error_word)
+
+
+class Rotary:
+    """Rotary positions of one model: frequencies base^(-i / P) of P pairs
+    (``pairs``, by default dim / 2) and how the pairs lie.  ``inv_freq`` may be given
+    instead of ``base`` (scaled variants), with their factor as ``scale``."""
+
+    def __init__(self, dim: int, *, base: float = 10000.0, pairs: Optional[int] = None,
+                 sections: Optional[Sequence[int]] = None, interleaved: bool = False, adjacent: bool = False,
+                 scale: float = 1.0, inv_freq: Optional[torch.Tensor] = None, device: Optional[torch.device] = None):
+        pairs = dim // 2 if pairs is None else pairs
+        if not 1 <= pairs <= dim // 2:
+            raise ValueError(f"{pairs} pairs of {dim} elements")
+        if inv_freq is None:
+            inv_freq = (float(base) ** (-torch.arange(pairs, dtype=torch.float64) / pairs)).float()
+        elif inv_freq.shape != (pairs,):
+            raise ValueError(f"inv_freq of shape {tuple(inv_freq.shape)} for {pairs} pairs")
+        if sections is not None and sum(sections) != pairs:
+            raise ValueError(f"sections {list(sections)} of {pairs} pairs")
+        self.inv_freq = inv_freq.float().contiguous().to(device if device is not None else "cuda")
+        self.how = dict(sections=None if sections is None else tuple(sections), interleaved=interleaved, adjacent=adjacent, scale=scale)
+
+    def __call__(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+        return rotary(x, positions, self.inv_freq, **self.how)
+
+    def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tensor,
+               v_cache: torch.Tensor, slot_map: torch.Tensor, *, error_word: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return rotary_append(q, k, v, positions, self.inv_freq, k_cache, v_cache, slot_map, error_word=error_word, **self.how)
+
+
+class VerifiedDrafts(NamedTuple):
+    """What ``verify_drafts`` decides (device tensors)."""
+
+    tokens: torch.Tensor    # int64 [T]: from each row's first place on its accepted drafts, then what it drew; -1 elsewhere
+    accepted: torch.Tensor  # int32 [B]: drafts accepted
+    rejected: torch.Tensor  # int32 [B]: drafts not accepted (their tokens are in the cache: cache_trim takes them out)
+    next_ids: torch.Tensor  # int64 [B]: what the row drew, its next settled token; -1 for a row without tokens
+
+
+def verify_drafts(logits: torch.Tensor, ids: torch.Tensor, query_offsets: torch.Tensor, uniforms: torch.Tensor, *,
+                  draft_probs: Optional[torch.Tensor] = None, temperature: Union[float, torch.Tensor] = 1.0,
+                  slot_map: Optional[torch.Tensor] = None, error_word: Optional[torch.Tensor] = None) -> VerifiedDrafts:
+    """Speculative sampling's decision, from given random numbers: which
+    drafted tokens of a step hold against the target's probabilities, and what
+    every row draws behind them, so that the tokens are distributed as the
+    target's alone.
+
+    Row b's tokens are [query_offsets[b], query_offsets[b+1]) of the step: one
+    that is settled, then drafts.  ``logits`` [T, V] (bf16, f16 or fp32) are the
+    target's for the token after each; ``ids`` int64 [T] the tokens;
+    ``draft_probs`` fp32 [T, V] the distributions that they were drawn from
+    (without: each was certain, as from a lookup); ``uniforms`` fp32 [T] in
+    [0, 1).  With p = softmax(logits / temperature), a draft d at token t holds
+    if ``uniforms[t] * draft_probs[t, d] < p[t - 1, d]``; behind the last that
+    does the row draws from max(p - draft_probs, 0), or from p after all of them,
+    by the inverse of the cumulative sum at the uniform of the row's first token.
+    ``temperature`` is a number or fp32 [B]; 0 is greedy (ties: the lowest
+    index).  Logits of -inf (what top-k or a mask left out) have no probability.
+    A row with a negative entry in ``slot_map`` (refused by ``cache_tables``) is
+    treated like one without tokens.  ``error_word``: ``DECERR_VALUES``,
+    ``DECERR_LENGTHS``."""
+    heat = (temperature, 1.0) if isinstance(temperature, torch.Tensor) else (None, temperature)
+    return tuple.__new__(VerifiedDrafts, _op("verify_drafts")(logits, ids, query_offsets, uniforms, draft_probs, *heat, slot_map,
+                                                              error_word))
 
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

@@ -1,0 +1,121 @@
+"""Plain forms of the operators for steps of several tokens a row, in Python
+integers and float64 on the CPU, written from their definitions
+(include/q3s_decode.h)."""
+import math
+
+import numpy as np
+import torch
+
+
+def ceil_div(a, b):
+    return -(-a // b)
+
+
+def rotary_axes(pairs, sections, interleaved):
+    """The axis of every pair."""
+    if not sections:
+        return [0] * pairs
+    if interleaved:
+        n = len(sections)
+        return [i % n if i < n * sections[i % n] else 0 for i in range(pairs)]
+    return [a for a, m in enumerate(sections) for _ in range(m)]
+
+
+def rotary(x, positions, inv_freq, sections=(), interleaved=False, adjacent=False, scale=1.0):
+    """(y, size, angle) in float64: y, and per element |x1| + |x2| of its pair and the angle it turned by (0 where copied)."""
+    x = x.double().cpu()
+    T, _, D = x.shape
+    P = inv_freq.numel()
+    positions = positions.cpu().reshape(-1, T)
+    axis = rotary_axes(P, sections, interleaved)
+    y, size, angle = x.clone(), torch.zeros_like(x), torch.zeros_like(x)
+    for i in range(P):
+        a, b = (2 * i, 2 * i + 1) if adjacent else (i, i + P)
+        # the angle as an exact product of integers and dyadic fractions, then reduced with Python's own floats
+        turn = torch.tensor([int(p) * float(inv_freq[i]) for p in positions[axis[i] % len(positions)]], dtype=torch.float64)
+        c, s = scale * turn.cos()[:, None], scale * turn.sin()[:, None]
+        y[..., a], y[..., b] = x[..., a] * c - x[..., b] * s, x[..., a] * s + x[..., b] * c
+        for e in (a, b):
+            size[..., e] = (x[..., a].abs() + x[..., b].abs()) * abs(scale)
+            angle[..., e] = turn.abs()[:, None]
+    return y, size, angle
+
+
+def cache_trim(lengths, removed, table, ring, state, *, block_size):
+    table, ring = [list(r) for r in table], list(ring)
+    room, (head, count), error, out = len(table[0]) * block_size if table else 0, state, 0, []
+    for b, (n, gone) in enumerate(zip(lengths, removed)):
+        had = min(max(n, 0), room)
+        cut = min(max(gone, 0), had)
+        error |= had != n or cut != gone
+        for j in range(ceil_div(had - cut, block_size), ceil_div(had, block_size)):
+            if count < len(ring):
+                ring[(head + count) % len(ring)] = table[b][j]
+            count += 1
+        out.append(had - cut)
+    if count > len(ring):
+        error |= 4
+    return dict(lengths=out, ring=ring, free_state=[head, min(count, len(ring))], error_word=[int(error)])
+
+
+def verify_drafts(logits, ids, offsets, uniforms, probs=None, temperature=None, slot_map=None):
+    """Lists; logits fp32 and probs fp32 numpy [T, V], temperature one number a row."""
+    T, V = logits.shape
+    B = len(offsets) - 1
+    tokens, accepted, rejected, fresh, error = [-1] * T, [0] * B, [0] * B, [-1] * B, 0
+
+    def target(t, heat):
+        """(p, argmax); p None: no distribution"""
+        x = logits[t].astype(np.float64)
+        kept = np.where(np.isnan(x), -np.inf, x)
+        best = int(np.argmax(kept))
+        if np.isnan(x).any() or not np.isfinite(kept[best]):
+            return None, best
+        if not heat >= 2.0 ** -100:
+            p = np.zeros(V)
+            p[best] = 1
+            return p, best
+        p = np.exp((x - x[best]) / float(heat))
+        return p / math.fsum(p), best
+
+    for b in range(B):
+        t, end = offsets[b], offsets[b + 1]
+        if t == end or (slot_map is not None and min(slot_map[t:end]) < 0):
+            continue
+        start, outside = t, False
+        while True:
+            p, best = target(t, temperature[b])
+            if t + 1 == end:
+                rest = p
+                break
+            d = ids[t + 1]
+            outside = not 0 <= d < V
+            q = None
+            if not outside:
+                q = probs[t + 1].astype(np.float64) if probs is not None else np.eye(1, V, d)[0]
+                if p is not None and float(uniforms[t + 1]) * q[d] < p[d]:
+                    tokens[t] = d
+                    t += 1
+                    continue
+            rest = p
+            if p is not None:
+                if probs is not None:
+                    q = probs[t + 1].astype(np.float64)
+                if q is not None:
+                    with np.errstate(invalid="ignore"):
+                        rest = np.fmax(p - q, 0)
+                    if not rest.any():
+                        rest = p
+            break
+        if p is None:
+            tokens[t] = best
+        elif not temperature[b] >= 2.0 ** -100:
+            tokens[t] = best
+        else:
+            edges = np.cumsum(rest)
+            over = np.flatnonzero(edges > float(uniforms[start]) * edges[-1])
+            tokens[t] = int(over[0]) if over.size else int(np.flatnonzero(rest)[-1])
+        if p is None or outside:
+            error |= 64
+        accepted[b], rejected[b], fresh[b] = t - start, end - 1 - t, tokens[t]
+    return dict(tokens=tokens, accepted=accepted, rejected=rejected, next_ids=fresh, error=error)
