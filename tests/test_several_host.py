@@ -154,8 +154,9 @@ def test_reference_verification_by_hand():
     assert got["tokens"] == [1, 2, 1] and got["accepted"] == [2] and got["rejected"] == [0] and got["next_ids"] == [1]
     got = R.verify_drafts(logits, [0, 1, 2], [0, 3], [0.6, 0.51, 0.99], q, [1.0])
     assert got["tokens"] == [0, -1, -1] and got["accepted"] == [0] and got["rejected"] == [2] and got["next_ids"] == [0]
-    got = R.verify_drafts(logits, [0, 1, 2], [0, 3], [0.6, 0.3, 0.9], None, [1.0])  # certain drafts: held below p
-    assert got["tokens"][0] == 2 and got["rejected"] == [2]
+    # a certain draft holds below p = 1/4; what is left, (1/2, 0, 1/4), reaches 0.6 * 3/4 = 0.45 with its first entry
+    got = R.verify_drafts(logits, [0, 1, 2], [0, 3], [0.6, 0.3, 0.9], None, [1.0])
+    assert got["tokens"] == [0, -1, -1] and got["rejected"] == [2]
 
 
 def test_verified_tokens_have_the_targets_distribution():
