@@ -277,6 +277,58 @@ typedef struct q3s_rotary_desc {
 
 q3s_status q3s_rotary(const q3s_rotary_desc* desc, void* stream);
 
+/* Attention of every row's chunk of new tokens, over a shared prefix and its own pages.
+ *
+ * The keys of row b are the prefix's tokens, at positions 0..prefix_length - 1,
+ * and its own lengths[b] tokens behind them.  Query i of its n (tokens
+ * [query_offsets[b], query_offsets[b+1])) stands at position
+ *   p = prefix_length + lengths[b] - n + i
+ * and sees the keys at positions (p - window, p], all up to p where window is 0.
+ * Otherwise as q3s_prefix_attention: the same result without a window, computed
+ * by a kernel whose tiles are 128 query rows of one row of the batch and not 16,
+ * for chunks from some tens of query rows on.  Probabilities are rounded to the cache's type for the product
+ * with v, as described there for the prefix of a large batch. */
+#define Q3S_MAX_CHUNK_GROUP 128 /* query heads per key/value head */
+
+typedef struct q3s_chunk_attention_desc {
+  uint32_t struct_size;        /* = sizeof(q3s_chunk_attention_desc) */
+  int32_t batch;               /* B, 0..Q3S_MAX_CACHE_ROWS */
+  int32_t tokens;              /* T >= 0: queries in the packed batch */
+  int32_t q_heads;
+  int32_t kv_heads;            /* divides q_heads, q_heads / kv_heads <= Q3S_MAX_CHUNK_GROUP */
+  int32_t dim;                 /* 64 or 128 */
+  int32_t block_size;          /* 16, 32, 64 or 128 */
+  int32_t blocks;              /* blocks in the cache */
+  int32_t elem;                /* Q3S_ELEM_BF16 or Q3S_ELEM_F16: q, caches and out */
+  int32_t max_blocks;          /* columns of block_table */
+  int32_t prefix_length;       /* >= 0 */
+  int32_t window;              /* >= 0; 0: none */
+  float scale;                 /* > 0 */
+  int32_t reserved0;
+  const void* q;               /* [T, q_heads, dim], 16-byte aligned rows */
+  int64_t q_token_stride, q_head_stride;
+  const void* k_cache;         /* [blocks, kv_heads, block_size, dim]: strides multiples of 8 elements, base 16-byte aligned */
+  const void* v_cache;
+  int64_t k_block_stride, k_head_stride, k_place_stride;
+  int64_t v_block_stride, v_head_stride, v_place_stride;
+  const int32_t* query_offsets; /* [B+1] */
+  const int32_t* block_table;   /* [B, block_table_stride] */
+  int64_t block_table_stride;
+  const int32_t* lengths;       /* [B] */
+  const int32_t* prefix_blocks; /* [ceil(prefix_length / block_size)]; may be NULL when prefix_length is 0 */
+  void* out;                    /* [T, q_heads, dim], 16-byte aligned rows */
+  int64_t out_token_stride, out_head_stride;
+  float* lse;                   /* optional [T, q_heads] */
+  void* workspace;              /* q3s_chunk_attention_workspace() bytes, 16-byte aligned; needs no initial value */
+  int64_t workspace_bytes;
+  int32_t* error_word;          /* optional, OR-ed */
+  const int64_t* slot_map;      /* optional [T]: a query whose slot is negative sees nothing */
+} q3s_chunk_attention_desc;
+
+/* Workspace bytes for a descriptor's sizes (its pointers are not read). */
+q3s_status q3s_chunk_attention_workspace(const q3s_chunk_attention_desc* desc, int64_t* bytes);
+q3s_status q3s_chunk_attention(const q3s_chunk_attention_desc* desc, void* stream);
+
 /* Drafted tokens verified against the target's probabilities.
  *
  * Row b's tokens of the step are [query_offsets[b], query_offsets[b+1]), n of
@@ -352,7 +404,7 @@ q3s_status q3s_cache_trim(const q3s_cache_trim_desc* desc, void* stream);
 
 /* sizeof() of the descriptors above as compiled (which: 0 = cache_tables,
  * 1 = cache_append, 2 = prefix_attention, 3 = quantize_rows, 4 = int8_matmul,
- * 5 = rotary, 6 = verify_drafts, 7 = cache_trim). */
+ * 5 = rotary, 6 = verify_drafts, 7 = cache_trim, 8 = chunk_attention). */
 uint32_t q3s_decode_desc_size(int32_t which);
 
 #ifdef __cplusplus

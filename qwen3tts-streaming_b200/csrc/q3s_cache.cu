@@ -579,6 +579,7 @@ extern "C" uint32_t q3s_decode_desc_size(int32_t which) {
     case 5: return sizeof(q3s_rotary_desc);
     case 6: return sizeof(q3s_verify_drafts_desc);
     case 7: return sizeof(q3s_cache_trim_desc);
+    case 8: return sizeof(q3s_chunk_attention_desc);
   }
   return 0;
 }

@@ -15,6 +15,8 @@
 //   rotary(x, positions, inv_freq, sections, interleaved=False, adjacent=False, scale=1.0) -> y
 //   rotary_append(q, k, v, positions, inv_freq, k_cache!, v_cache!, slot_map, sections, interleaved=False,
 //                 adjacent=False, scale=1.0, error_word!=None) -> q
+//   chunk_attention(q, k_cache, v_cache, query_offsets, block_table, lengths, prefix_blocks=None, prefix_length=0,
+//                   window=0, scale=None, error_word!=None, slot_map=None) -> (out, lse)
 //   verify_drafts(logits, ids, query_offsets, uniforms, draft_probs=None, temperature=None, temperature_default=1.0,
 //                 slot_map=None, error_word!=None) -> (tokens, accepted, rejected, next_ids)
 //   cache_trim(lengths, removed, block_table, free_blocks!, free_state, block_size) -> (lengths, free_state, error_word)
@@ -442,6 +444,84 @@ Tensor rotary_append(const Tensor& q, const Tensor& k, const Tensor& v, const Te
   return out;
 }
 
+std::tuple<Tensor, Tensor> chunk_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+                                           const Tensor& query_offsets, const Tensor& block_table,
+                                           const Tensor& lengths, const OptTensor& prefix_blocks,
+                                           int64_t prefix_length, int64_t window, c10::optional<double> scale,
+                                           OptTensor error_word, const OptTensor& slot_map) {
+  need_cuda(q, "q");
+  c10::cuda::CUDAGuard guard(q.device());
+  need(q, q, q.scalar_type(), 3, "q");
+  need_cache(k_cache, q, "k_cache");
+  need_cache(v_cache, q, "v_cache");
+  TORCH_CHECK(q.stride(2) == 1 || q.size(2) <= 1, "q3s: q must have unit last stride");
+  TORCH_CHECK(k_cache.sizes() == v_cache.sizes() && k_cache.size(3) == q.size(2),
+              "q3s: the caches must be [blocks, kv_heads, block_size, ", q.size(2), "], got ", k_cache.sizes(), " and ",
+              v_cache.sizes());
+  need(lengths, q, at::kInt, 1, "lengths");
+  const int64_t B = lengths.size(0), T = q.size(0);
+  need_vector(lengths, q, at::kInt, B, "lengths");
+  need_vector(query_offsets, q, at::kInt, B + 1, "query_offsets");
+  need(block_table, q, at::kInt, 2, "block_table");
+  TORCH_CHECK(block_table.size(0) == B && (block_table.size(1) <= 1 || block_table.stride(1) == 1),
+              "q3s: block_table must be [", B, ", max_blocks] with unit column stride, got ", block_table.sizes());
+  q3s_chunk_attention_desc d;
+  std::memset(&d, 0, sizeof(d));
+  d.struct_size = sizeof(d);
+  d.batch = i32(B, "batch");
+  d.tokens = i32(T, "tokens");
+  d.q_heads = i32(q.size(1), "q_heads");
+  d.kv_heads = i32(k_cache.size(1), "kv_heads");
+  d.dim = i32(q.size(2), "dim");
+  d.block_size = i32(k_cache.size(2), "block_size");
+  d.blocks = i32(k_cache.size(0), "blocks");
+  d.elem = elem_of(q, "q");
+  d.max_blocks = i32(block_table.size(1), "max_blocks");
+  d.prefix_length = i32(prefix_length, "prefix_length");
+  d.window = i32(window, "window");
+  if (prefix_length > 0) {
+    TORCH_CHECK(prefix_blocks.has_value(), "q3s: a prefix needs prefix_blocks");
+    need(*prefix_blocks, q, at::kInt, 1, "prefix_blocks");
+    need_vector(*prefix_blocks, q, at::kInt, prefix_blocks->size(0), "prefix_blocks");
+    TORCH_CHECK(prefix_blocks->size(0) * k_cache.size(2) >= prefix_length, "q3s: prefix_blocks holds ",
+                prefix_blocks->size(0), " blocks of ", k_cache.size(2), " for a prefix of ", prefix_length);
+    d.prefix_blocks = prefix_blocks->data_ptr<int32_t>();
+  }
+  d.scale = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(2))));
+  d.q = q.data_ptr();
+  d.q_token_stride = T > 1 ? q.stride(0) : q.size(1) * q.size(2);
+  d.q_head_stride = q.stride(1);
+  d.k_cache = k_cache.data_ptr();
+  d.v_cache = v_cache.data_ptr();
+  d.k_block_stride = k_cache.stride(0);
+  d.k_head_stride = k_cache.stride(1);
+  d.k_place_stride = k_cache.stride(2);
+  d.v_block_stride = v_cache.stride(0);
+  d.v_head_stride = v_cache.stride(1);
+  d.v_place_stride = v_cache.stride(2);
+  d.query_offsets = query_offsets.data_ptr<int32_t>();
+  d.block_table = block_table.data_ptr<int32_t>();
+  d.block_table_stride = B > 1 ? block_table.stride(0) : block_table.size(1);
+  d.lengths = lengths.data_ptr<int32_t>();
+  Tensor out = make({T, q.size(1), q.size(2)}, q.scalar_type(), q), lse = make({T, q.size(1)}, at::kFloat, q);
+  d.out = out.data_ptr();
+  d.out_token_stride = q.size(1) * q.size(2);
+  d.out_head_stride = q.size(2);
+  d.lse = lse.data_ptr<float>();
+  d.error_word = error_of(error_word, q);
+  if (slot_map.has_value()) {
+    need_vector(*slot_map, q, at::kLong, T, "slot_map");
+    d.slot_map = slot_map->data_ptr<int64_t>();
+  }
+  int64_t bytes = 0;
+  check_status(q3s_chunk_attention_workspace(&d, &bytes), "q3s_chunk_attention");
+  const Tensor ws = make({bytes}, at::kByte, q);
+  d.workspace = ws.data_ptr();
+  d.workspace_bytes = bytes;
+  check_status(q3s_chunk_attention(&d, stream_of(q)), "q3s_chunk_attention");
+  return {out, lse};
+}
+
 std::tuple<Tensor, Tensor, Tensor, Tensor> verify_drafts(const Tensor& logits, const Tensor& ids, const Tensor& query_offsets,
                                                          const Tensor& uniforms, const OptTensor& draft_probs,
                                                          const OptTensor& temperature, double temperature_default,
@@ -571,6 +651,11 @@ Tensor rotary_append_meta(const Tensor& q, const Tensor&, const Tensor&, const T
                           const Tensor&, at::IntArrayRef, bool, bool, double, OptTensor) {
   return at::empty(q.sizes(), q.options());
 }
+std::tuple<Tensor, Tensor> chunk_attention_meta(const Tensor& q, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                const Tensor&, const OptTensor&, int64_t, int64_t, c10::optional<double>,
+                                                OptTensor, const OptTensor&) {
+  return {at::empty(q.sizes(), q.options()), at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat))};
+}
 std::tuple<Tensor, Tensor, Tensor, Tensor> verify_drafts_meta(const Tensor&, const Tensor& ids, const Tensor& offsets,
                                                               const Tensor&, const OptTensor&, const OptTensor&, double,
                                                               const OptTensor&, OptTensor) {
@@ -605,6 +690,9 @@ TORCH_LIBRARY_FRAGMENT(q3s, m) {
   m.def("rotary_append(Tensor q, Tensor k, Tensor v, Tensor positions, Tensor inv_freq, Tensor(a!) k_cache, "
         "Tensor(b!) v_cache, Tensor slot_map, int[] sections, bool interleaved=False, bool adjacent=False, "
         "float scale=1.0, Tensor(c!)? error_word=None) -> Tensor");
+  m.def("chunk_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor query_offsets, Tensor block_table, "
+        "Tensor lengths, Tensor? prefix_blocks=None, int prefix_length=0, int window=0, float? scale=None, "
+        "Tensor(a!)? error_word=None, Tensor? slot_map=None) -> (Tensor, Tensor)");
   m.def("verify_drafts(Tensor logits, Tensor ids, Tensor query_offsets, Tensor uniforms, Tensor? draft_probs=None, "
         "Tensor? temperature=None, float temperature_default=1.0, Tensor? slot_map=None, Tensor(a!)? error_word=None) -> "
         "(Tensor, Tensor, Tensor, Tensor)");
@@ -621,6 +709,7 @@ TORCH_LIBRARY_IMPL(q3s, CUDA, m) {
   m.impl("int8_linear", &int8_linear);
   m.impl("rotary", &rotary);
   m.impl("rotary_append", &rotary_append);
+  m.impl("chunk_attention", &chunk_attention);
   m.impl("verify_drafts", &verify_drafts);
   m.impl("cache_trim", &cache_trim);
 }
@@ -634,6 +723,7 @@ TORCH_LIBRARY_IMPL(q3s, Meta, m) {
   m.impl("int8_linear", &int8_linear_meta);
   m.impl("rotary", &rotary_meta);
   m.impl("rotary_append", &rotary_append_meta);
+  m.impl("chunk_attention", &chunk_attention_meta);
   m.impl("verify_drafts", &verify_drafts_meta);
   m.impl("cache_trim", &cache_trim_meta);
 }

@@ -14,6 +14,7 @@ from .decode import (
     cache_append,
     cache_tables,
     cache_trim,
+    chunk_attention,
     int8_linear,
     int8_matmul,
     prefix_attention,
@@ -51,6 +52,7 @@ __all__ = [
     "cache_append",
     "cache_tables",
     "cache_trim",
+    "chunk_attention",
     "int8_linear",
     "int8_matmul",
     "prefix_attention",

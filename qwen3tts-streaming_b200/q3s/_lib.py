@@ -167,7 +167,7 @@ class HeadDesc(C.Structure):
 
 # the decode step's operators (include/q3s_decode.h)
 ELEM_F32, ELEM_BF16, ELEM_F16 = 0, 1, 2
-MAX_CACHE_ROWS, MAX_QUERY_GROUP = 65536, 16
+MAX_CACHE_ROWS, MAX_QUERY_GROUP, MAX_CHUNK_GROUP = 65536, 16, 128
 TABLES_WHOLE_ROWS = 1
 ROTARY_ADJACENT, ROTARY_INTERLEAVED, MAX_ROTARY_AXES = 1, 2, 4
 MAX_VERIFY_VOCAB = 1 << 24
@@ -392,8 +392,51 @@ class CacheTrimDesc(C.Structure):
     ]
 
 
+class ChunkAttentionDesc(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("batch", C.c_int32),
+        ("tokens", C.c_int32),
+        ("q_heads", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("dim", C.c_int32),
+        ("block_size", C.c_int32),
+        ("blocks", C.c_int32),
+        ("elem", C.c_int32),
+        ("max_blocks", C.c_int32),
+        ("prefix_length", C.c_int32),
+        ("window", C.c_int32),
+        ("scale", C.c_float),
+        ("reserved0", C.c_int32),
+        ("q", _p),
+        ("q_token_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("k_cache", _p),
+        ("v_cache", _p),
+        ("k_block_stride", C.c_int64),
+        ("k_head_stride", C.c_int64),
+        ("k_place_stride", C.c_int64),
+        ("v_block_stride", C.c_int64),
+        ("v_head_stride", C.c_int64),
+        ("v_place_stride", C.c_int64),
+        ("query_offsets", _p),
+        ("block_table", _p),
+        ("block_table_stride", C.c_int64),
+        ("lengths", _p),
+        ("prefix_blocks", _p),
+        ("out", _p),
+        ("out_token_stride", C.c_int64),
+        ("out_head_stride", C.c_int64),
+        ("lse", _p),
+        ("workspace", _p),
+        ("workspace_bytes", C.c_int64),
+        ("error_word", _p),
+        ("slot_map", _p),
+    ]
+
+
 DECODE_DESCS = (CacheTablesDesc, CacheAppendDesc, PrefixAttentionDesc, QuantizeRowsDesc, Int8MatmulDesc,
-                RotaryDesc, VerifyDraftsDesc, CacheTrimDesc)
+                RotaryDesc, VerifyDraftsDesc, CacheTrimDesc, ChunkAttentionDesc)
 # every symbol include/q3s_decode.h declares
 DECODE_EXPORTS = (
     "q3s_cache_tables",
@@ -406,6 +449,8 @@ DECODE_EXPORTS = (
     "q3s_rotary",
     "q3s_verify_drafts",
     "q3s_cache_trim",
+    "q3s_chunk_attention_workspace",
+    "q3s_chunk_attention",
     "q3s_decode_desc_size",
 )
 
@@ -462,13 +507,16 @@ def load(path: str | Path | None = None) -> C.CDLL:
         lib.q3s_head_sample.argtypes = [C.POINTER(HeadDesc), _p]
         lib.q3s_head_sample.restype = C.c_int
         for name, st in zip(("q3s_cache_tables", "q3s_cache_append", "q3s_prefix_attention", "q3s_quantize_rows",
-                             "q3s_int8_matmul", "q3s_rotary", "q3s_verify_drafts", "q3s_cache_trim"), DECODE_DESCS):
+                             "q3s_int8_matmul", "q3s_rotary", "q3s_verify_drafts", "q3s_cache_trim",
+                             "q3s_chunk_attention"), DECODE_DESCS):
             getattr(lib, name).argtypes = [C.POINTER(st), _p]
             getattr(lib, name).restype = C.c_int
         lib.q3s_int8_linear.argtypes = [C.POINTER(QuantizeRowsDesc), C.POINTER(Int8MatmulDesc), _p]
         lib.q3s_int8_linear.restype = C.c_int
         lib.q3s_prefix_attention_workspace.argtypes = [C.POINTER(PrefixAttentionDesc), C.POINTER(C.c_int64)]
         lib.q3s_prefix_attention_workspace.restype = C.c_int
+        lib.q3s_chunk_attention_workspace.argtypes = [C.POINTER(ChunkAttentionDesc), C.POINTER(C.c_int64)]
+        lib.q3s_chunk_attention_workspace.restype = C.c_int
         lib.q3s_decode_desc_size.argtypes = [C.c_int32]
         lib.q3s_decode_desc_size.restype = C.c_uint32
         if lib.q3s_abi_version() != Q3S_ABI_VERSION:

@@ -1,5 +1,7 @@
 """The decode step's operators beside the sampler: the paged key/value cache's
-tables and append, attention over a shared prefix, and 8-bit projections.
+tables and append, attention over a shared prefix, 8-bit projections, and what a
+step of several tokens a row needs: rotary positions, attention of chunks,
+drafts verified, rows cut back.
 
 A step runs them in this order, from device lengths alone (no host read)::
 
@@ -10,6 +12,17 @@ A step runs them in this order, from device lengths alone (no host read)::
                                prefix_blocks=voice_blocks, prefix_length=voice_tokens, slot_map=t.slot_map)
     hidden = projection(out)                 # q3s.Int8Linear
     # then the codec head, the sampler and the epilogue (q3s.head_sample, q3s.StepGuard)
+
+A step whose rows bring several tokens (drafts, a prompt in chunks)::
+
+    t = q3s.cache_tables(...)                # new: 1 + drafts, or the chunk's length
+    # for every layer:
+    q = q3s.rotary_append(q, k, v, t.positions + voice_tokens, inv_freq, k_cache, v_cache, t.slot_map)
+    out = q3s.chunk_attention(q, k_cache, v_cache, t.query_offsets, table, t.lengths,
+                              prefix_blocks=voice_blocks, prefix_length=voice_tokens, slot_map=t.slot_map)
+    # then the head's logits, and
+    r = q3s.verify_drafts(logits, ids, t.query_offsets, uniforms, draft_probs=proposed, slot_map=t.slot_map)
+    c = q3s.cache_trim(t.lengths, r.rejected, table, ring, t.free_state, block_size=16)
 
 ``PagedCache`` keeps the state that such a program carries from step to step.
 The functions are thin: they call ``torch.ops.q3s.*`` (C++: argument checks,
@@ -179,6 +192,24 @@ class Rotary:
         return rotary_append(q, k, v, positions, self.inv_freq, k_cache, v_cache, slot_map, error_word=error_word, **self.how)
 
 
+def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, query_offsets: torch.Tensor,
+                    block_table: torch.Tensor, lengths: torch.Tensor, *, prefix_blocks: Optional[torch.Tensor] = None,
+                    prefix_length: int = 0, window: int = 0, scale: Optional[float] = None, return_lse: bool = False,
+                    error_word: Optional[torch.Tensor] = None, slot_map: Optional[torch.Tensor] = None):
+    """Attention of every row's chunk of new tokens over the shared prefix and
+    its own pages: ``prefix_attention`` for rows of many query tokens (a prompt
+    in chunks, drafts), with an optional sliding window.
+
+    Arguments and results as there, up to 128 query heads for a key/value head,
+    ``scale`` positive.  With ``window`` a query sees the ``window`` keys up to
+    its own, counted over prefix and own tokens together.  Every row's query
+    tokens are taken in tiles of 128 (tokens times heads of a group), so it is
+    the faster one where rows have more than about 16 of them."""
+    out, lse = _op("chunk_attention")(q, k_cache, v_cache, query_offsets, block_table, lengths, prefix_blocks,
+                                      prefix_length, window, scale, error_word, slot_map)
+    return (out, lse) if return_lse else out
+
+
 class VerifiedDrafts(NamedTuple):
     """What ``verify_drafts`` decides (device tensors)."""
 
@@ -262,7 +293,8 @@ class Int8Linear:
 
 class PagedCache:
     """The state of a paged key/value cache of ``layers`` layers for ``batch``
-    rows, and the three calls of a step on it.
+    rows, and the calls of a step on it: ``step``, ``append`` or
+    ``append_rotary``, ``attend`` or ``attend_chunk``, and ``trim``.
 
     ``blocks`` blocks of ``block_size`` tokens; the first ``prefix_blocks`` of
     them are set aside for a prefix that all rows share (``prefix``), the rest
@@ -325,3 +357,31 @@ class PagedCache:
         return prefix_attention(q, self.k[layer], self.v[layer], self.tables.query_offsets, self.table, self.lengths,
                                 prefix_blocks=self.prefix, prefix_length=self.prefix_length,
                                 **{"error_word": self.error_word, "slot_map": slots, **kw})
+
+    @property
+    def positions(self) -> torch.Tensor:
+        """Places of the step's tokens behind the prefix (int32 [max_tokens]): what a rotary turns them by."""
+        return self.tables.positions + self.prefix_length
+
+    def append_rotary(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rotary: Rotary,
+                      positions: torch.Tensor) -> torch.Tensor:
+        """``append`` of keys that ``rotary`` turns by ``positions`` (``self.positions``, or [axes, max_tokens]), and the
+        queries turned likewise, in one launch."""
+        return rotary.append(q, k, v, positions, self.k[layer], self.v[layer], self.tables.slot_map, error_word=self.error_word)
+
+    def attend_chunk(self, layer: int, q: torch.Tensor, *, window: int = 0, **kw):
+        """``attend`` for rows that bring many tokens (a prompt, drafts), with an optional sliding window over prefix and row."""
+        slots = self.tables.slot_map
+        if q.shape[0] != slots.shape[0]:
+            slots = torch.nn.functional.pad(slots, (0, q.shape[0] - slots.shape[0]), value=-1)
+        return chunk_attention(q, self.k[layer], self.v[layer], self.tables.query_offsets, self.table, self.lengths,
+                               prefix_blocks=self.prefix, prefix_length=self.prefix_length, window=window,
+                               **{"error_word": self.error_word, "slot_map": slots, **kw})
+
+    def trim(self, removed: torch.Tensor) -> None:
+        """Take the last ``removed[b]`` tokens of every row back out (``verify_drafts``' rejected ones): lengths and the ring
+        go on without them.  ``error_word`` collects what ``cache_trim`` reports."""
+        t = cache_trim(self.lengths, removed, self.table, self.ring, self.ring_state, block_size=self.block_size)
+        self.lengths.copy_(t.lengths)  # in place, as step does
+        self.ring_state.copy_(t.free_state)
+        self.error_word.bitwise_or_(t.error_word)

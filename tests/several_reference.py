@@ -119,3 +119,45 @@ def verify_drafts(logits, ids, offsets, uniforms, probs=None, temperature=None, 
             error |= 64
         accepted[b], rejected[b], fresh[b] = t - start, end - 1 - t, tokens[t]
     return dict(tokens=tokens, accepted=accepted, rejected=rejected, next_ids=fresh, error=error)
+
+
+def chunk_attention(q, k_cache, v_cache, offsets, table, lengths, prefix_blocks, prefix_length, scale, window=0, slot_map=None):
+    """(out, lse, spread, mass) in float64 on the tensors' device: spread = sum p |v - out|, which bounds what rounding p
+    moves where out is divided by the sum of the rounded p, and mass = sum p |v|."""
+    T, Hq, D = q.shape
+    H, bs = k_cache.shape[1], k_cache.shape[2]
+    G = Hq // H
+    zero = dict(dtype=torch.float64, device=q.device)
+    out, spread, mass = (torch.zeros(T, Hq, D, **zero) for _ in range(3))
+    lse = torch.full((T, Hq), -math.inf, **zero)
+
+    def gather(cache, blocks, n):
+        nb = ceil_div(n, bs)
+        return cache[blocks[:nb].long()].double().transpose(1, 2).reshape(-1, H, D)[:n]
+
+    for b in range(len(lengths)):
+        t0, t1, length = int(offsets[b]), int(offsets[b + 1]), int(lengths[b])
+        n = t1 - t0
+        if n <= 0:
+            continue
+        k, v = (torch.cat([gather(x, prefix_blocks, prefix_length), gather(x, table[b], length)]) for x in (k_cache, v_cache))
+        key = torch.arange(len(k), device=q.device)
+        own = length - n + torch.arange(n, device=q.device) + 1  # own tokens that each query sees
+        pos = prefix_length + own - 1
+        seen = (key < prefix_length) | (key - prefix_length < own[:, None])
+        if window:
+            seen &= key > pos[:, None] - window
+        if slot_map is not None:
+            seen &= (slot_map[t0:t1] >= 0)[:, None]
+        for h in range(Hq):
+            s = torch.where(seen, scale * (q[t0:t1, h].double() @ k[:, h // G].t()), -math.inf)
+            any_key = seen.any(1)
+            p = torch.where(any_key[:, None], torch.softmax(s, 1), 0.0)
+            lse[t0:t1, h] = torch.logsumexp(s, 1)
+            vh = torch.where(seen.any(0)[:, None], v[:, h // G], 0.0)  # what nobody sees counts for nothing
+            o = p @ vh
+            out[t0:t1, h] = o
+            mass[t0:t1, h] = p @ vh.abs()
+            for c in range(0, n, 16):
+                spread[t0 + c:min(t0 + c + 16, t1), h] = torch.einsum("nk,nkd->nd", p[c:c + 16], (vh[None] - o[c:c + 16, None]).abs())
+    return out, lse, spread, mass

@@ -457,3 +457,72 @@ def test_verify_captured_step_follows_its_inputs(dev):
         want = R.verify_drafts(logits.cpu().numpy(), ids.tolist(), c["offsets"].tolist(), u.tolist(), probs.cpu().numpy(), [heat] * 6)
         assert r.next_ids.tolist() == want["next_ids"] and r.rejected.tolist() == want["rejected"] and r.tokens.tolist() == want["tokens"]
         assert t.lengths.tolist() == [64 - x for x in want["rejected"]]
+
+
+# ---- a step of several tokens, as it is used ----------------------------------------
+
+def test_steps_with_drafts_on_a_paged_cache(dev):
+    """Prompt, then steps of drafts: tables, turn and append, attention, verification and cut, each against its definition
+    on the state that the step has."""
+    B, hq, hk, dim, bs, V, prefix = 5, 4, 2, 64, 16, 300, 20
+    rng = np.random.RandomState(0)
+    g = torch.Generator(device=dev).manual_seed(0)
+    cache = q3s.PagedCache(B, 60, layers=1, kv_heads=hk, dim=dim, block_size=bs, max_blocks=9, prefix_blocks=2, device=dev)
+    rotary = q3s.Rotary(dim, device=dev)
+    kv = torch.randn(2, prefix, hk, dim, device=dev, generator=g).bfloat16()
+    cache.write_prefix(0, kv[0], kv[1])
+    rows = [torch.zeros(0, hk, dim, dtype=torch.bfloat16, device=dev) for _ in range(B)]  # turned keys, as they should be stored
+    for step in range(6):
+        new = rng.randint(20, 60, B) if step == 0 else rng.randint(0, 5, B)
+        new[0] = max(new[0], 1)
+        T = int(new.sum())
+        t = cache.step(i32(new, dev), max_tokens=T + 3)
+        qkv = torch.randn(T + 3, hq + 2 * hk, dim, device=dev, generator=g).bfloat16()
+        q, k, v = qkv[:, :hq], qkv[:, hq:hq + hk], qkv[:, hq + hk:]
+        turned = cache.append_rotary(0, q, k, v, rotary, cache.positions)
+        before = [len(r) for r in rows]
+        pos = np.concatenate([prefix + before[b] + np.arange(new[b]) for b in range(B)] + [np.full(3, prefix)])
+        check_turned(turned, q, i32(pos, dev), rotary.inv_freq)
+        off = np.concatenate([[0], np.cumsum(new)])
+        stored = q3s.rotary(k, i32(pos, dev), rotary.inv_freq)
+        for b in range(B):
+            rows[b] = torch.cat([rows[b], stored[off[b]:off[b + 1]]])
+        window = 0 if step % 2 else 50
+        out = cache.attend_chunk(0, turned, window=window)
+        want, _, spread, mass = R.chunk_attention(turned, cache.k[0], cache.v[0], off.tolist(), cache.table, cache.lengths.tolist(),
+                                                  cache.prefix, prefix, dim ** -0.5, window)
+        tol = 2.0 ** -8 * want.abs() + 1.02 * 2.0 ** -8 * spread + 2.0 ** -16 * mass
+        assert bool(((out.double() - want).abs() <= tol).all()) and not out[T:].any()
+        for b in range(B):  # the row's keys are where its table says
+            j = torch.arange(len(rows[b]), device=dev)
+            assert torch.equal(cache.k[0][cache.table[b, j // bs].long(), :, j % bs], rows[b])
+        c = dict(logits=torch.randn(T + 3, V, generator=torch.Generator().manual_seed(step)) * 2, offsets=off, slot_map=t.slot_map.cpu(),
+                 uniforms=torch.rand(T + 3, generator=torch.Generator().manual_seed(step)), probs=None, heat=np.full(B, 0.5, np.float32))
+        c["ids"] = c["logits"].argmax(1).roll(1, 0)
+        verdict = check_verify(c, dev)
+        r = q3s.verify_drafts(c["logits"].to(dev), c["ids"].to(dev), t.query_offsets, c["uniforms"].to(dev), temperature=0.5,
+                              slot_map=t.slot_map)
+        assert r.rejected.tolist() == verdict["rejected"]
+        cache.trim(r.rejected)
+        for b in range(B):
+            rows[b] = rows[b][:len(rows[b]) - verdict["rejected"][b]]
+        assert cache.lengths.tolist() == [len(r) for r in rows]
+        held = [int(cache.table[b, j]) for b in range(B) for j in range(R.ceil_div(len(rows[b]), bs))]
+        head, count = cache.ring_state.tolist()
+        free = [int(cache.ring[(head + j) % 58]) for j in range(count)]
+        assert sorted(held + free) == list(range(2, 60)) and int(cache.error_word) == 0 == int(t.error_word)
+
+
+def test_example_of_draft_steps_runs(dev):
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "examples" / "draft_step.py"
+    spec = importlib.util.spec_from_file_location("draft_step", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    tokens, held, cache = module.main(rows=6, steps=4, drafts=3, prompt=21)
+    assert tokens.shape == (6, 1 + 4 * 4) and held.shape == (4, 6) and int(held.min()) >= 0 and int(held.max()) <= 3
+    # the prompt, and of each step the token that was settled and the drafts that held
+    assert cache.lengths.tolist() == (21 + 4 + held.sum(0)).tolist()
+    assert (tokens >= 0).sum(1).tolist() == (1 + 4 + held.sum(0)).tolist() and int(tokens.max()) < 1024

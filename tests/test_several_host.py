@@ -31,6 +31,10 @@ GOOD = {
     "q3s_verify_drafts": (_lib.VerifyDraftsDesc, dict(
         batch=2, tokens=5, vocab=100, elem=1, temperature_default=1.0, logits=P, logits_row_stride=100, ids=P, query_offsets=P,
         uniforms=P, draft_probs=P, draft_row_stride=100, tokens_out=P + 4096, accepted=P, rejected=P, next_ids=P)),
+    "q3s_chunk_attention": (_lib.ChunkAttentionDesc, dict(
+        batch=2, tokens=20, q_heads=8, kv_heads=4, dim=64, block_size=16, blocks=9, elem=1, max_blocks=4, prefix_length=20, scale=0.1,
+        q=P, k_cache=P, v_cache=P, query_offsets=P, block_table=P, block_table_stride=4, lengths=P, prefix_blocks=P, out=P,
+        workspace=P, workspace_bytes=1 << 40)),
     "q3s_cache_trim": (_lib.CacheTrimDesc, dict(
         batch=4, block_size=16, max_blocks=8, lengths=P, removed=P + 64, block_table=P, block_table_stride=8, free_blocks=P,
         free_state=P, free_state_out=P + 64, lengths_out=P + 128, ring_size=10)),
@@ -81,6 +85,31 @@ def _call(lib, name, **kw):
     ("q3s_verify_drafts", dict(logits_row_stride=99), "strides"),
     ("q3s_verify_drafts", dict(draft_row_stride=99), "strides"),
     ("q3s_verify_drafts", dict(tokens_out=P), "tokens_out"),
+    ("q3s_chunk_attention", dict(struct_size=8), "struct_size"),
+    ("q3s_chunk_attention", dict(batch=-1), "batch"),
+    ("q3s_chunk_attention", dict(batch=65537), "batch"),
+    ("q3s_chunk_attention", dict(tokens=-1), "tokens"),
+    ("q3s_chunk_attention", dict(q_heads=6), "query heads"),
+    ("q3s_chunk_attention", dict(q_heads=129, kv_heads=1), "query heads"),
+    ("q3s_chunk_attention", dict(q_heads=65536, kv_heads=65536), "too many"),
+    ("q3s_chunk_attention", dict(dim=96), "dim"),
+    ("q3s_chunk_attention", dict(block_size=256), "block_size"),
+    ("q3s_chunk_attention", dict(elem=0), "elem"),
+    ("q3s_chunk_attention", dict(blocks=0), "blocks"),
+    ("q3s_chunk_attention", dict(window=-1), "window"),
+    ("q3s_chunk_attention", dict(prefix_length=-1), "prefix_length"),
+    ("q3s_chunk_attention", dict(scale=0.0), "scale"),
+    ("q3s_chunk_attention", dict(scale=-0.1), "scale"),
+    ("q3s_chunk_attention", dict(scale=float("nan")), "scale"),
+    ("q3s_chunk_attention", dict(scale=float("inf")), "scale"),
+    ("q3s_chunk_attention", dict(tokens=1 << 28), "2^31"),
+    ("q3s_chunk_attention", dict(prefix_length=(1 << 31) - 65600), "2^31"),
+    ("q3s_chunk_attention", dict(prefix_blocks=None), "prefix_blocks"),
+    ("q3s_chunk_attention", dict(out=None), "required"),
+    ("q3s_chunk_attention", dict(lengths=None), "lengths"),
+    ("q3s_chunk_attention", dict(q=P + 8), "16-byte"),
+    ("q3s_chunk_attention", dict(k_place_stride=100), "multiples of 8"),
+    ("q3s_chunk_attention", dict(workspace_bytes=100), "workspace of 100"),
     ("q3s_cache_trim", dict(struct_size=8), "struct_size"),
     ("q3s_cache_trim", dict(batch=-1), "batch"),
     ("q3s_cache_trim", dict(batch=65537), "batch"),
@@ -100,7 +129,7 @@ def test_bad_arguments_are_refused_on_the_host(lib, name, kw, msg):
 
 
 @pytest.mark.parametrize("name,kw", [("q3s_rotary", dict(tokens=0)), ("q3s_rotary", dict(q_heads=0, kv_heads=0)),
-                                     ("q3s_verify_drafts", dict(batch=0, tokens=0))])
+                                     ("q3s_verify_drafts", dict(batch=0, tokens=0)), ("q3s_chunk_attention", dict(tokens=0))])
 def test_empty_calls_do_nothing(lib, name, kw):
     assert _call(lib, name, **kw)[0] == _lib.OK
     assert getattr(lib, name)(None, None) == _lib.ERR_INVALID_ARGUMENT
@@ -126,6 +155,8 @@ def test_python_calls_refuse_cpu_tensors_and_trace_on_meta():
                           temperature=torch.empty(3, **m))
     assert r.tokens.shape == (6,) and r.tokens.dtype == torch.int64 and r.accepted.shape == (3,) and r.accepted.dtype == torch.int32
     assert r.rejected.shape == r.next_ids.shape == (3,) and r.next_ids.dtype == torch.int64
+    out, lse = q3s.chunk_attention(q, cache, cache, torch.empty(6, **n), torch.empty(5, 8, **n), torch.empty(5, **n), window=7, return_lse=True)
+    assert out.shape == q.shape and lse.shape == (6, 8) and lse.dtype == torch.float32
     t = q3s.cache_trim(torch.empty(5, **n), torch.empty(5, **n), torch.empty(5, 8, **n), torch.empty(9, **n), torch.empty(2, **n), block_size=16)
     assert t.lengths.shape == (5,) and t.free_state.shape == (2,) and t.error_word.shape == (1,)
 
@@ -170,3 +201,38 @@ def test_verified_tokens_have_the_targets_distribution():
             for w in grid:
                 count[R.verify_drafts(logits, [0, d], [0, 2], [w, u], np.stack([q, q]), [1.0])["tokens"][0]] += 1
     assert np.abs(count / n ** 3 - p).max() < 4 * 3 / n
+
+
+def test_chunk_kernel_shares_no_multiprocessor_with_another_that_takes_tensor_memory(tmp_path):
+    """It takes all 512 columns, so no CTA that takes some may fit beside it (228 KB of shared memory)."""
+    import subprocess
+    from pathlib import Path
+
+    from q3s import build
+
+    src, exe = tmp_path / "chunk.cu", tmp_path / "chunk"
+    src.write_text('#include <cstdio>\n#include "q3s_chunk.cuh"\nint main() { printf("%d %d %d", q3s::ChunkTile<64>::SMEM, '
+                   'q3s::ChunkTile<128>::SMEM, q3s::TMEM_PART_SMEM); }\n')
+    csrc = Path(__file__).resolve().parents[1] / "qwen3tts-streaming_b200" / "csrc"
+    subprocess.run([build.nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", f"-I{csrc}", f"-I{build.INCLUDE}",
+                    "-o", str(exe), str(src)], check=True, capture_output=True)
+    a, b, part = map(int, subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split())
+    assert min(a, b) + part > 228 * 1024 and max(a, b) <= 227 * 1024
+
+
+def test_chunk_operator_takes_an_error_word():
+    q3s.load_torch_ops()
+    for name in ("chunk_attention", "rotary_append", "verify_drafts"):
+        arg = {a.name: a for a in getattr(torch.ops.q3s, name).default._schema.arguments}["error_word"]
+        assert arg.alias_info is not None and arg.alias_info.is_write and arg.default_value is None
+
+
+def test_reference_chunk_attention_by_hand():
+    """Two queries of one row on two keys with equal scores: the first sees one, the second both; a window of one, its own."""
+    k, v, q = torch.zeros(1, 1, 16, 64), torch.zeros(1, 1, 16, 64), torch.ones(2, 1, 64)
+    v[0, 0, 0], v[0, 0, 1] = 1.0, 3.0
+    args = ([0, 2], torch.tensor([[0]]), [2], torch.zeros(0, dtype=torch.int32), 0, 1.0)
+    out, lse, spread, mass = R.chunk_attention(q, k, v, *args)
+    assert out[:, 0, 0].tolist() == [1.0, 2.0] and np.allclose(lse[:, 0], [0.0, np.log(2)])
+    assert spread[:, 0, 0].tolist() == [0.0, 1.0] and mass[:, 0, 0].tolist() == [1.0, 2.0]
+    assert R.chunk_attention(q, k, v, *args, window=1)[0][:, 0, 0].tolist() == [1.0, 3.0]
