@@ -22,11 +22,16 @@
 namespace q3s {
 
 constexpr int CH_M = PX_M, CH_KEYS = PX_KEYS;
-constexpr int CH_NT = 320;      // two softmax warpgroups (a tile each), the copy warp, the matrix warp
+constexpr int CH_NT = 384;      // two softmax warpgroups, and one with the copy warp and the matrix warp
 constexpr int CH_SEGS = 64;     // segments of a CTA's range that are listed at a time
+// Registers a thread: a softmax thread holds a row of 128 scores.  Launched with 168 a thread, which is what the shares add up to.
+constexpr int CH_REGS_SOFTMAX = 216, CH_REGS_OTHER = 72;
+static_assert(2 * CH_REGS_SOFTMAX + CH_REGS_OTHER <= 3 * 168, "what the CTA is launched with");
 constexpr int CH_START = 6;     // cost of an item's start and end, where a step of two tiles costs 3 and one of one tile 2
 constexpr int CH_MAX_STEP = 3;  // the largest cost of a step
 constexpr int CH_JOIN_NT = 256, CH_JOIN_ROWS = 32;  // threads and query rows of a CTA of the joining kernel
+
+constexpr int CH_UNSEEN = -0x7fffffff - 1;  // in place of how many own tokens a query sees: there is none, or it sees nothing
 
 // A CTA's piece of an item.
 struct ChunkSeg {
@@ -57,7 +62,7 @@ struct ChunkTile {
   static constexpr int STAGES = D == 64 ? 4 : 2;  // steps of K (and of V) in shared memory
   static constexpr int Q_BYTES = CH_M * D * 2;
   static constexpr int KV_BYTES = CH_KEYS * D * 2;
-  static constexpr int LIST = CH_SEGS * static_cast<int>(sizeof(ChunkSeg)) + CH_NT * static_cast<int>(sizeof(ChunkRow));
+  static constexpr int LIST = CH_SEGS * static_cast<int>(sizeof(ChunkSeg)) + CH_NT * static_cast<int>(sizeof(ChunkRow)) + CH_M * 12;
   static constexpr int USED = 1024 + 2 * Q_BYTES + 2 * STAGES * KV_BYTES + LIST + 512;
   static constexpr int SMEM = USED > TMEM_ALL_SMEM ? USED : TMEM_ALL_SMEM;  // all of the tensor memory
   static_assert(SMEM <= HEAD_SMEM_LIMIT, "shared memory");
@@ -84,7 +89,10 @@ Q3S_DEV ChunkRow chunk_row(const AttnArgs& a, int b) {
 // Steps of the item of tokens [i0, i0 + m) of a row: first and count (0: its queries see nothing).
 Q3S_DEV int2 chunk_steps(const ChunkArgs& c, const ChunkRow& x, int i0, int m) {
   const int L = c.a.L;
-  auto step_of = [&](int p) { return p < L ? p / CH_KEYS : (L + CH_KEYS - 1) / CH_KEYS + (p - L) / CH_KEYS; };
+  auto step_of = [&](int p) {  // p >= 0
+    const uint32_t own = static_cast<uint32_t>(p - L);
+    return static_cast<int>(p < L ? static_cast<uint32_t>(p) / CH_KEYS : static_cast<uint32_t>(L + CH_KEYS - 1) / CH_KEYS + own / CH_KEYS);
+  };
   const int hi = L + max(x.len - x.n + i0 + m, 0) - 1;  // the last position that is seen
   if (hi < 0) return make_int2(0, 0);
   const int64_t lo = c.window ? static_cast<int64_t>(L) + x.len - x.n + i0 - c.window + 1 : 0;
@@ -94,18 +102,38 @@ Q3S_DEV int2 chunk_steps(const ChunkArgs& c, const ChunkRow& x, int i0, int m) {
 
 // Where a CTA is in the list.
 struct ChunkWalk {
-  int b, i, h;  // row, first token in it, head: the item that starts at `at`
+  int b, item;  // row, item in it (token pair times heads, and head), or -1: at the row's start
   int written, cut, more;
-  long long at, all;
+  int ctas;
+  long long at, all;  // where that item (the row) starts; the list's length, for `ctas` CTAs
 };
 
 // Boundaries of the CTAs' ranges: CTA i has [all * i / ctas, all * (i + 1) / ctas).
 struct ChunkCutting {
   long long all;
   int ctas;
-  Q3S_DEV long long start(int i) const { return all * i / ctas; }
-  Q3S_DEV int cta_of(long long at) const { return static_cast<int>(((at + 1) * ctas + all - 1) / all) - 1; }
+  Q3S_DEV long long start(int i) const { return div_nonneg(all * i, ctas); }
+  Q3S_DEV int cta_of(long long at) const { return static_cast<int>(div_nonneg((at + 1) * ctas + all - 1, all)) - 1; }
 };
+
+// 16 consecutive columns of this thread's TMEM lane; a store is complete after tmem_st_wait.
+Q3S_DEV void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+}
+Q3S_DEV void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+      "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+Q3S_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // One query row of a segment again, key by key: what it does not see is left out
 // instead of taken times p = 0, where an infinity or NaN in V would reach it.
@@ -164,20 +192,21 @@ Q3S_DEV void chunk_row_by_key(const ChunkArgs& c, const ChunkSeg& g, int token, 
 Q3S_DEV float chunk_inverse(float l) { return l > 0.0f ? 1.0f / l : l == l ? 0.0f : l; }
 Q3S_DEV float chunk_lse(float m, float l) { return l > 0.0f ? (m + log2f(l)) * 0.69314718055994531f : l == l ? -INFINITY : l; }
 
-// The matrix warp alternates between the two tiles as the shared-prefix kernel
-// does (q3s_attn_prefix.cuh), here over the steps of one segment after another:
-//   O0 += P0 V, S0 = Q0 K'^T, O1 += P1 V, S1 = Q1 K'^T,
-// where K' is the next step's, of the next segment after a segment's last, so
-// that a segment's start overlaps the end of the one before.  A tile's O is taken
-// out by its softmax warps before they write the next segment's first P, which
-// is what the next product into O waits for; Q is replaced once the
-// last scores of a segment are complete.  A softmax thread owns a query row; m, l and the
-// sum of the rounded p are in registers.  TMEM: S0 S1 O0 O1, 128 columns each.
+// The two softmax warpgroups take turns: unit u of the CTA's work, 128 query rows
+// against 128 keys, is that of warpgroup u % 2, whose scores, probabilities and sums have
+// their place in TMEM (S0 S1 O0 O1, 128 columns each).  A step of a segment of two tiles
+// is two units; a segment of one tile (a few drafts) has a unit a step, so the two
+// warpgroups share its keys, odd and even steps, and the one that began joins the
+// other's sums to its own at the end.  The matrix warp keeps two units on their way,
+//   O(u) += P(u) V, S(u + 2) = Q K'^T,
+// over the segments without a pause: a warpgroup's O is taken out before it hands over the
+// next segment's first P, which is what the next product into O waits for, and the two tiles of Q are a ring.
+// A softmax thread owns a query row; m, l and the sum of the rounded p (q3s_attn_prefix.cuh says why) are in registers.
 //
-// Masks are a range of columns a row and step (behind the query's own place, before the window, past the prefix's end); steps
-// that all rows of a warp see whole skip them.  V is cleared past the end of a
-// row's (or the prefix's) last step by the softmax warps of tile 0 before they hand over their first P of it;
-// whole pages past the end read as zeros.
+// Masks are a range of columns a row and step (behind the query's own place,
+// before the window, past the prefix's end), applied by quarters of a step that some row of the
+// warp does not see whole.  V is cleared past the end of a row's (or the prefix's)
+// last step by the softmax warps that hand over its first P; whole pages past the end read as zeros.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(CH_NT, 1)
     attn_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -191,26 +220,28 @@ __global__ void __launch_bounds__(CH_NT, 1)
   unsigned char* s_q = smem;
   unsigned char* s_k = s_q + 2 * Tile::Q_BYTES;
   unsigned char* s_v = s_k + STAGES * Tile::KV_BYTES;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(s_v + STAGES * Tile::KV_BYTES);
-  uint64_t* q_empty = q_full + 1;
-  uint64_t* k_full = q_empty + 1;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(s_v + STAGES * Tile::KV_BYTES);  // [2]
+  uint64_t* q_empty = q_full + 2;                                                 // [2]
+  uint64_t* k_full = q_empty + 2;
   uint64_t* k_empty = k_full + STAGES;
   uint64_t* v_full = k_empty + STAGES;
   uint64_t* v_empty = v_full + STAGES;
-  uint64_t* s_full = v_empty + STAGES;  // [2] scores of a tile are in TMEM
+  uint64_t* s_full = v_empty + STAGES;  // [2] scores of a warpgroup's unit are in TMEM
   uint64_t* p_half = s_full + 2;        // [2] the probabilities of its first 64 keys are
   uint64_t* p_full = p_half + 2;        // [2] all are
   uint64_t* o_done = p_full + 2;        // [2] its second product is complete
-  uint64_t* done = o_done + 2;          // behind a wait that gave up
+  uint64_t* given = o_done + 2;         // a shared tile's second sums may be read, and have been
+  uint64_t* taken = given + 1;
+  uint64_t* done = taken + 1;           // behind a wait that gave up
   long long* s_sum = reinterpret_cast<long long*>(done + 1);  // [CH_NT / 32]
-  long long* s_at = s_sum + CH_NT / 32;
-  ChunkWalk* walker = reinterpret_cast<ChunkWalk*>(s_at + 1);
+  ChunkWalk* walker = reinterpret_cast<ChunkWalk*>(s_sum + CH_NT / 32);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(walker + 1);
   int* failed = reinterpret_cast<int*>(tmem_slot + 1);
-  int *s_row = failed + 1, *s_segs = s_row + 1, *s_more = s_segs + 1;
-  static_assert((2 + 4 * STAGES + 8 + 1 + CH_NT / 32 + 1) * 8 + sizeof(ChunkWalk) + 5 * 4 <= 512, "room for the barriers and counts");
+  int* s_segs = failed + 1;
+  static_assert((4 + 4 * STAGES + 8 + 3 + CH_NT / 32) * 8 + sizeof(ChunkWalk) + 3 * 4 <= 512, "room for the barriers and counts");
   ChunkSeg* s_list = reinterpret_cast<ChunkSeg*>(reinterpret_cast<unsigned char*>(q_full) + 512);
   ChunkRow* s_rows = reinterpret_cast<ChunkRow*>(s_list + CH_SEGS);  // the first CH_NT rows
+  float* s_ml = reinterpret_cast<float*>(s_rows + CH_NT);            // [128][3] m, l and the sum of the rounded p of a shared tile's second sums
   const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
   const int cta = static_cast<int>(blockIdx.x);
   const int pair = 2 * c.per_tile;  // tokens of an item
@@ -221,21 +252,23 @@ __global__ void __launch_bounds__(CH_NT, 1)
   if (w == 8) {
     if (lane < 3) prefetch_map(lane == 0 ? &tm_q : lane == 1 ? &tm_k : &tm_v);
     if (lane == 0) {
-      mbar_init(q_full, 1);
-      mbar_init(q_empty, 1);
-      mbar_init(done, 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&q_full[i], 1);
+        mbar_init(&q_empty[i], 1);
+        mbar_init(&s_full[i], 1);
+        mbar_init(&p_half[i], 128);
+        mbar_init(&p_full[i], 128);
+        mbar_init(&o_done[i], 1);
+      }
       for (int s = 0; s < STAGES; ++s) {
         mbar_init(&k_full[s], 1);
         mbar_init(&k_empty[s], 1);
         mbar_init(&v_full[s], 1);
         mbar_init(&v_empty[s], 1);
       }
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&s_full[i], 1);
-        mbar_init(&p_half[i], 128);
-        mbar_init(&p_full[i], 128);
-        mbar_init(&o_done[i], 1);
-      }
+      mbar_init(given, 128);
+      mbar_init(taken, 128);
+      mbar_init(done, 1);
       *failed = 0;
       fence_mbar_init();
     }
@@ -249,27 +282,48 @@ __global__ void __launch_bounds__(CH_NT, 1)
 
   // ---- the list's length, and this CTA's range of it ----
   auto step_cost = [&](int m) { return m > c.per_tile ? 3 : 2; };
+  auto item_cost = [&](const ChunkRow& x, int i0) {  // of tokens [i0, i0 + pair), for one head; 0: nothing is seen
+    const int m = min(pair, x.n - i0), steps = chunk_steps(c, x, i0, m).y;
+    return steps ? CH_START + static_cast<long long>(steps) * step_cost(m) : 0ll;
+  };
+  auto warp_scan = [&](long long up) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long o = __shfl_up_sync(FULL, up, d);
+      if (lane >= d) up += o;
+    }
+    return up;
+  };
+  // a row's cost; a whole warp calls (a row of many items is its 32 lanes' work)
   auto row_cost = [&](const ChunkRow& x) {
     long long r = 0;
-    for (int i0 = 0; i0 < x.n; i0 += pair) {
-      const int m = min(pair, x.n - i0), steps = chunk_steps(c, x, i0, m).y;
-      if (steps) r += static_cast<long long>(a.H) * (CH_START + static_cast<long long>(steps) * step_cost(m));
+    const bool large = x.n > 4 * pair;
+    for (int i0 = 0; i0 < x.n && !large; i0 += pair) r += item_cost(x, i0);
+    for (unsigned rest = __ballot_sync(FULL, large); rest; rest &= rest - 1) {
+      const int src = __ffs(rest) - 1;
+      const ChunkRow y = {0, __shfl_sync(FULL, x.n, src), __shfl_sync(FULL, x.len, src)};
+      long long sum = 0;
+      for (int64_t i0 = static_cast<int64_t>(lane) * pair; i0 < y.n; i0 += 32 * pair) sum += item_cost(y, static_cast<int>(i0));
+#pragma unroll
+      for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(FULL, sum, d);
+      if (lane == src) r = sum;
     }
-    return r;
+    return r * a.H;
   };
   long long mine = 0, all = 0;  // this thread's row of the first CH_NT, all of its rows
-  for (int b = t; b < a.B; b += CH_NT) {
-    const ChunkRow x = chunk_row(a, b);
+  for (int b0 = 0; b0 < a.B; b0 += CH_NT) {
+    const ChunkRow x = b0 + t < a.B ? chunk_row(a, b0 + t) : ChunkRow{0, 0, 0};
     const long long r = row_cost(x);
-    if (b == t) {
+    if (b0 == 0) {
       mine = r;
       s_rows[t] = x;
     }
     all += r;
   }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(FULL, all, d);
-  if (lane == 0) s_sum[w] = all;
+  {
+    const long long up = warp_scan(all);
+    if (lane == 31) s_sum[w] = up;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -278,103 +332,100 @@ __global__ void __launch_bounds__(CH_NT, 1)
 #pragma unroll
   for (int i = 0; i < CH_NT / 32; ++i) all += s_sum[i];
   // as many CTAs as every range holds the start of a step for
-  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), max(all / CH_MAX_STEP, 1ll)));
+  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), max(div_nonneg(all, CH_MAX_STEP), 1ll)));
   const bool works = all > 0 && cta < ctas;
   if (works) {  // the row in which the range starts
     const long long range0 = ChunkCutting{all, ctas}.start(cta);
     long long carry = 0;
     for (int b0 = 0; b0 < a.B && carry <= range0; b0 += CH_NT) {
-      const long long r = b0 == 0 ? mine : b0 + t < a.B ? row_cost(chunk_row(a, b0 + t)) : 0;
-      long long up = r;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const long long o = __shfl_up_sync(FULL, up, d);
-        if (lane >= d) up += o;
+      long long r = mine;
+      if (b0) r = row_cost(b0 + t < a.B ? chunk_row(a, b0 + t) : ChunkRow{0, 0, 0});
+      const long long up = warp_scan(r);
+      if (a.B > CH_NT) {  // the sums in s_sum are of all rows
+        __syncthreads();
+        if (lane == 31) s_sum[w] = up;
+        __syncthreads();
       }
-      __syncthreads();  // the sums before have been read
-      if (lane == 31) s_sum[w] = up;
-      __syncthreads();
       long long at = carry + up - r;
 #pragma unroll
       for (int i = 0; i < CH_NT / 32; ++i) {
         if (i < w) at += s_sum[i];
         carry += s_sum[i];
       }
-      if (at <= range0 && range0 < at + r) {
-        *s_row = b0 + t;
-        *s_at = at;
-      }
+      if (at <= range0 && range0 < at + r) *walker = {b0 + t, -1, 0, 0, 1, ctas, at, all};
     }
-    __syncthreads();
+  } else if (t == 0) {
+    c.cuts[cta].parts = 0;
   }
-  // Thread 0 walks the list from there and writes the segments, CH_SEGS at a time
-  // (where it is stands in shared memory: the registers are the softmax's).
-  if (t == 0) {
-    if (works) *walker = {*s_row, 0, 0, 0, 0, 1, *s_at, all};
-    else c.cuts[cta].parts = 0;
-  }
-  auto walk = [&]() {  // thread 0
+  __syncthreads();
+
+  // Warp 0 lists the CTA's segments, up to CH_SEGS at a time: 32 items at once, a lane each.
+  auto walk = [&]() {
     ChunkWalk k = *walker;
-    const ChunkCutting cut = {k.all, ctas};
+    __syncwarp();
+    const ChunkCutting cut = {k.all, k.ctas};
+    const int cta = static_cast<int>(blockIdx.x);
     const long long range0 = cut.start(cta), range1 = cut.start(cta + 1);
-    auto row_at = [&](int b) { return b < CH_NT ? s_rows[b] : chunk_row(a, b); };
-    ChunkRow x = k.b < a.B ? row_at(k.b) : ChunkRow{0, 0, 0};
     int n = 0;
-    while (k.more && n < CH_SEGS) {
-      if (k.i >= x.n) {  // the next row
-        if (++k.b >= a.B) {
-          k.more = 0;
-          break;
-        }
-        x = row_at(k.b);
-        k.i = 0;
-        continue;
-      }
-      const int m = min(pair, x.n - k.i), each = step_cost(m);
-      const int2 steps = chunk_steps(c, x, k.i, m);
-      const long long cost = steps.y ? CH_START + static_cast<long long>(steps.y) * each : 0;
-      if (steps.y == 0 || (k.h == 0 && k.at + a.H * cost <= range0)) {  // nothing to see, or before the range
-        k.at += a.H * cost;
-        k.i += pair;
-        continue;
-      }
-      if (k.h == 0 && k.at < range0) {
-        k.h = static_cast<int>((range0 - k.at) / cost);
-        k.at += k.h * cost;
-      }
-      if (k.at >= range1) {
+    while (k.more && n + 32 <= CH_SEGS) {
+      if (k.b >= a.B) {
         k.more = 0;
         break;
       }
-      const long long start = k.at + CH_START;  // of its first step
-      auto steps_before = [&](long long y) {    // that start before y
-        return y <= start ? 0 : static_cast<int>(min((y - start + each - 1) / each, static_cast<long long>(steps.y)));
+      const ChunkRow x = k.b < CH_NT ? s_rows[k.b] : chunk_row(a, k.b);
+      const int pairs = (x.n + pair - 1) / pair;
+      const long long items = static_cast<long long>(pairs) * a.H;
+      if (k.item < 0) {  // the range starts in this row: skip to the tokens where it does
+        int p0 = 0;
+        for (; p0 < pairs; p0 += 32) {
+          const long long cost = p0 + lane < pairs ? item_cost(x, (p0 + lane) * pair) * a.H : 0;
+          const long long up = warp_scan(cost);
+          const unsigned past = __ballot_sync(FULL, k.at + up > range0);
+          if (past) {
+            const int f = __ffs(past) - 1;
+            p0 += f;
+            k.at += __shfl_sync(FULL, up - cost, f);
+            break;
+          }
+          k.at += __shfl_sync(FULL, up, 31);
+        }
+        k.item = p0 * a.H;
+      }
+      const int item = k.item + lane, p = item / a.H, h = item - p * a.H;
+      const int i0 = p * pair, m = min(pair, x.n - i0);
+      int2 steps = make_int2(0, 0);
+      if (item < items) steps = chunk_steps(c, x, i0, m);
+      const int each = step_cost(m);
+      const long long cost = steps.y ? CH_START + static_cast<long long>(steps.y) * each : 0;
+      const long long up = warp_scan(cost), start = k.at + up - cost;
+      auto steps_before = [&](long long y) {  // that start before y
+        const long long past = min(max(y - start - CH_START, 0ll), static_cast<long long>(steps.y) * each);
+        return static_cast<int>(div_nonneg(past + each - 1, each));
       };
       const int lo = steps_before(range0), hi = steps_before(range1);
+      const unsigned live = __ballot_sync(FULL, lo < hi);
+      const bool whole = lo == 0 && hi == steps.y;
+      const int rank = __popc(live & ((1u << lane) - 1u));
       if (lo < hi) {
-        ChunkSeg& g = s_list[n++];
-        g.b = k.b;
-        g.h = k.h;
-        g.token = x.t0 + k.i;
-        g.tokens = m;
-        g.i_key = x.len - x.n + k.i + 1;
-        g.len = x.len;
-        g.step0 = steps.x + lo;
-        g.steps = hi - lo;
-        g.slot = lo == 0 && hi == steps.y ? -1 : 2 * cta + (k.written ? 1 : 0);
-        k.written = 1;
-        if (lo == 0 && hi < steps.y) {
-          c.cuts[cta] = {cut.cta_of(start + static_cast<long long>(steps.y - 1) * each) - cta + 1, g.slot, cta, k.h, g.token, m};
-          k.cut = 1;
-        }
+        const int slot = whole ? -1 : 2 * cta + (k.written + rank > 0 ? 1 : 0);
+        s_list[n + rank] = {k.b, h, x.t0 + i0, m, x.len - x.n + i0 + 1, x.len, steps.x + lo, hi - lo, slot};
+        if (lo == 0 && !whole)
+          c.cuts[cta] = {cut.cta_of(start + CH_START + static_cast<long long>(steps.y - 1) * each) - cta + 1, slot, cta, h, x.t0 + i0, m};
       }
-      k.at += cost;
-      if (++k.h == a.H) k.h = 0, k.i += pair;
+      k.cut |= __any_sync(FULL, lo < hi && lo == 0 && !whole);
+      k.written += __popc(live);
+      n += __popc(live);
+      if (__any_sync(FULL, item < items && start >= range1)) k.more = 0;
+      k.at += __shfl_sync(FULL, up, 31);
+      k.item += 32;
+      if (k.item >= items) ++k.b, k.item = 0;
     }
-    if (!k.more && !k.cut) c.cuts[cta].parts = 0;
-    *walker = k;
-    *s_segs = n;
-    *s_more = k.more;
+    if (!k.more && !k.cut && lane == 0) c.cuts[cta].parts = 0;
+    __syncwarp();
+    if (lane == 0) {
+      *walker = k;
+      *s_segs = n;
+    }
   };
 
   // a wait that gives up marks the CTA; every role then stops at its next wait
@@ -385,178 +436,70 @@ __global__ void __launch_bounds__(CH_NT, 1)
     atomicOr(failed, 1);
     return false;
   };
-  const int rows = min(a.bs, CH_KEYS), pages = CH_KEYS / rows;
-  int kv = 0, segs = 0;  // steps and segments so far (softmax warps: kv counts the steps of their tile)
-  int cnt[2] = {0, 0};   // the matrix warp's steps of each tile
-  int k_copies = 0, v_copies = 0, q_copies = 0, bad = 0;
+  int kv = 0, units = 0, tiles_q = 0;  // steps, units and tiles of Q so far (the matrix warp: before this batch of segments)
   bool ok = true;
+  auto tiles_of = [&](const ChunkSeg& g) { return g.tokens > c.per_tile ? 2 : 1; };
 
-  for (bool again = works; again;) {
-    if (t == 0) walk();
-    __syncthreads();
-    const int n = *s_segs;
-    again = *s_more;
-    if (w == 8) {
-      // ---- copies: lane l copies box l of a step (a page, or 128 tokens of one) ----
-      auto block_of = [&](const ChunkSeg& g, int j) {  // past the cache (it reads as zeros) where there is none
-        const int s = g.step0 + j;
-        const bool prefix = s < before;
-        const int key = (prefix ? s : s - before) * CH_KEYS + lane * rows;
-        if (lane >= pages || key >= (prefix ? a.L : g.len)) return a.blocks;
-        const int32_t* ids = prefix ? a.prefix_blocks : a.table + g.b * a.table_stride;
-        return ids[key >> a.bs_log2];
-      };
-      auto copy = [&](const CUtensorMap* map, unsigned char* ring, uint64_t* full, int h, int block) {
-        const int s = kv % STAGES, place = (lane * rows) & (a.bs - 1);
-        if (lane == 0) mbar_expect_tx(&full[s], Tile::KV_BYTES);
-        __syncwarp();
-        if (lane < pages)
-          for (int x = 0; x < HALVES; ++x)
-            tma_load_slice(smem_u32(ring + s * Tile::KV_BYTES + x * CH_KEYS * 128 + lane * rows * 128), map, x, place, h, block, &full[s]);
-      };
-      int next = n ? block_of(s_list[0], 0) : 0;
-      for (int e = 0; ok && e < n; ++e) {
-        const ChunkSeg g = s_list[e];
-        const int tiles = g.tokens > c.per_tile ? 2 : 1;
-        for (int j = 0; ok && j < g.steps; ++j) {
-          const bool inside = static_cast<unsigned>(next) < static_cast<unsigned>(a.blocks);
-          bad |= !inside && next != a.blocks;
-          const int block = inside ? next : a.blocks;
-          if (j + 1 < g.steps) next = block_of(g, j + 1);
-          else if (e + 1 < n) next = block_of(s_list[e + 1], 0);
-          const int s = kv % STAGES;
-          const uint32_t parity = static_cast<uint32_t>(kv / STAGES - 1) & 1u;
-          if (kv >= STAGES && !(ok = __all_sync(FULL, wait(&k_empty[s], parity)))) break;
-          copy(&tm_k, s_k, k_full, g.h, block);
-          ++k_copies;
-          if (j == 0) {
-            if (segs && !(ok = __all_sync(FULL, wait(q_empty, static_cast<uint32_t>(segs - 1) & 1u)))) break;
-            if (lane == 0) {
-              mbar_expect_tx(q_full, static_cast<uint32_t>(tiles * HALVES * c.per_tile * a.G * 128));
-              for (int i = 0; i < tiles; ++i)
-                for (int x = 0; x < HALVES; ++x)
-                  tma_load_3d(smem_u32(s_q + i * Tile::Q_BYTES + x * CH_M * 128), &tm_q, 64 * x, g.h * a.G, g.token + i * c.per_tile, q_full);
-            }
-            __syncwarp();
-            ++q_copies;
-            ++segs;
-          }
-          if (kv >= STAGES && !(ok = __all_sync(FULL, wait(&v_empty[s], parity)))) break;
-          copy(&tm_v, s_v, v_full, g.h, block);
-          ++v_copies;
-          ++kv;
-        }
-      }
-    } else if (w == 9) {
-      // ---- products --------------------------------------------------------------
-      constexpr uint32_t FMT = BF16 ? 1u : 0u;
-      constexpr uint32_t ID_S = (1u << 4) | (FMT << 7) | (FMT << 10) | (static_cast<uint32_t>(CH_KEYS >> 3) << 17) |
-                                (static_cast<uint32_t>(CH_M >> 4) << 24);
-      constexpr uint32_t ID_O = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) |
-                                (static_cast<uint32_t>(CH_M >> 4) << 24);  // bit 16: B's rows are the contraction
-      const int kv0 = kv, segs0 = segs, cnt0[2] = {cnt[0], cnt[1]};
-      if (elect_one()) {
-        const uint64_t q_desc = head_smem_desc(smem_u32(s_q)), k_desc = head_smem_desc(smem_u32(s_k)), v_desc = v_smem_desc(smem_u32(s_v));
-        auto scores = [&](int i, int s) {  // S_i = Q_i K^T
-          const uint64_t dq = q_desc + static_cast<uint64_t>(i * (Tile::Q_BYTES >> 4)), dk = k_desc + static_cast<uint64_t>(s * (Tile::KV_BYTES >> 4));
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            constexpr int SLICE = (CH_KEYS * 128) >> 4;
-            umma_f16(tmem + static_cast<uint32_t>(128 * i), dq + (k / 4) * SLICE + (k % 4) * 2, dk + (k / 4) * SLICE + (k % 4) * 2, ID_S, k != 0);
-          }
-          umma_commit(&s_full[i]);
-        };
-        // the scores of a step: its first tile waits for their operands
-        auto next_scores = [&](int i, int tiles, int step, bool first, bool last) {
-          const int s = step % STAGES;
-          if (i == 0) {
-            if (first) ok = ok && wait(q_full, static_cast<uint32_t>(segs++) & 1u);
-            ok = ok && wait(&k_full[s], static_cast<uint32_t>(step / STAGES) & 1u);
-            if (!ok) return;
-            tc_fence_after();
-          }
-          scores(i, s);
-          if (i == tiles - 1) {
-            umma_commit(&k_empty[s]);
-            if (last) umma_commit(q_empty);
-          }
-        };
-        auto tiles_of = [&](int e) { return s_list[e].tokens > c.per_tile ? 2 : 1; };
-        if (n) {
-          const int tiles = tiles_of(0);
-          for (int i = 0; ok && i < tiles; ++i) next_scores(i, tiles, kv, true, s_list[0].steps == 1);
-        }
-        for (int e = 0; ok && e < n; ++e) {
-          const int steps = s_list[e].steps, tiles = tiles_of(e);
-          for (int j = 0; ok && j < steps; ++j, ++kv) {
-            const int s = kv % STAGES;
-            const bool fresh = j + 1 == steps;  // the next step is the next segment's first
-            const int following = fresh ? (e + 1 < n ? s_list[e + 1].steps : 0) : steps - j - 1;  // steps from the next on
-            const int next_tiles = following == 0 ? 0 : fresh ? tiles_of(e + 1) : tiles;
-            ok = wait(&v_full[s], static_cast<uint32_t>(kv / STAGES) & 1u);
-            for (int i = 0; ok && i < 2; ++i) {
-              if (i < tiles) {
-                const uint64_t dv = v_desc + static_cast<uint64_t>(s * (Tile::KV_BYTES >> 4));
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {  // O_i += P_i V
-                  ok = ok && wait(half ? &p_full[i] : &p_half[i], static_cast<uint32_t>(cnt[i]) & 1u);
-                  if (!ok) break;
-                  tc_fence_after();
-#pragma unroll
-                  for (int q = 0; q < CH_KEYS / 32; ++q) {
-                    const int k = half * (CH_KEYS / 32) + q;
-                    umma_f16_ta(tmem + static_cast<uint32_t>(256 + 128 * i), tmem + static_cast<uint32_t>(128 * i + 8 * k),
-                                dv + k * ((16 * 128) >> 4), ID_O, (j | k) != 0);
-                  }
-                }
-                if (!ok) break;
-                if (i == tiles - 1) umma_commit(&v_empty[s]);
-                umma_commit(&o_done[i]);
-                ++cnt[i];
-              }
-              if (i < next_tiles) next_scores(i, next_tiles, kv + 1, fresh, following == 1);
-            }
-          }
-        }
-      }
-      __syncwarp();
-      // the counts, for whichever lane is elected next
-      kv = kv0, segs = segs0 + n, cnt[0] = cnt0[0], cnt[1] = cnt0[1];
-      for (int e = 0; e < n; ++e) {
-        kv += s_list[e].steps;
-        cnt[0] += s_list[e].steps;
-        if (s_list[e].tokens > c.per_tile) cnt[1] += s_list[e].steps;
-      }
-    } else {
+  // Each role with a loop of its own over the batches of segments, so that it has its own number of registers.
+  if (w < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CH_REGS_SOFTMAX));
+    int cnt = 0;           // this warpgroup's units
+    int shared = 0;        // tiles so far whose keys the two warpgroups shared
+    bool pending = false;  // the sums given for the last of them must have been taken before the next product into them
+    for (bool again = works; again;) {
+      if (w == 0) walk();
+      __syncthreads();  // the segments are listed
+      const int n = *s_segs;
+      again = walker->more != 0;
       // ---- softmax ----------------------------------------------------------------
       const int i = w >> 2, row = (w & 3) * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>((w & 3) * 32) << 16;
       const uint32_t ts = tmem + lanes + static_cast<uint32_t>(128 * i), to = tmem + lanes + static_cast<uint32_t>(256 + 128 * i);
       for (int e = 0; ok && e < n; ++e) {
         const ChunkSeg& g = s_list[e];
-        if (i > 0 && g.tokens <= c.per_tile) continue;
-        const int token = i * c.per_tile + row / a.G, gq = row % a.G;
-        const bool exists = row < c.per_tile * a.G && token < g.tokens;
-        const bool sees = exists && (!a.slot_map || a.slot_map[g.token + token] >= 0);
-        const int own = sees ? g.i_key + token : 0;  // own tokens that this query sees, and the first position
-        const int64_t first = sees && c.window ? max(static_cast<int64_t>(a.L) + own - c.window, static_cast<int64_t>(0)) : 0;
+        const int turn = (i - units) & 1;  // this warpgroup's first unit in the segment
+        const int stage0 = kv;             // steps before the segment
+        const int tile = tiles_of(g) == 2 ? turn : 0;
+        units += tiles_of(g) * g.steps;
+        kv += g.steps;
         float m = -INFINITY, l = 0.0f, lr = 0.0f;  // lr: of the rounded p
-        for (int j = 0; j < g.steps; ++j, ++kv) {
-          const int s = g.step0 + j;
-          const bool prefix = s < before;
-          const int key0 = (prefix ? s : s - before) * CH_KEYS;  // of the prefix or of the row's own
-          ok = __all_sync(FULL, wait(&s_full[i], static_cast<uint32_t>(kv) & 1u));
+        int own, from = 0;  // own tokens that this row's query sees (none where there is no such query), and the first position
+        {
+          const int token = tile * c.per_tile + row / a.G;
+          const bool sees = row < c.per_tile * a.G && token < g.tokens && (!a.slot_map || a.slot_map[g.token + token] >= 0);
+          own = sees ? g.i_key + token : CH_UNSEEN;
+          if (sees && c.window) from = max(a.L + own - c.window, 0);
+        }
+        const bool alone = tiles_of(g) == 2;
+        if (!alone && turn >= g.steps) continue;
+        for (int j = alone ? 0 : turn; j < g.steps; j += alone ? 1 : 2, ++cnt) {
+          bool prefix;
+          int key0;  // of the prefix or of the row's own
+          {
+            const int s = g.step0 + j;
+            prefix = s < before;
+            key0 = (prefix ? s : s - before) * CH_KEYS;
+          }
+          ok = __all_sync(FULL, wait(&s_full[i], static_cast<uint32_t>(cnt) & 1u));
           if (!ok) break;
           tc_fence_after();
           uint32_t r[128];
           tmem_ld128(ts, r);
-          // the columns that are seen: [c_lo, c_hi)
-          const int c_hi = sees ? (prefix ? a.L : own) - key0 : 0;
-          const int c_lo = static_cast<int>(min(max(first - key0 - (prefix ? 0 : a.L), static_cast<int64_t>(0)), static_cast<int64_t>(CH_KEYS)));
-          if (__any_sync(FULL, c_hi < CH_KEYS || c_lo > 0)) {
+          {
+            // the columns that are seen, [c_lo, c_hi), as a bit each
+            const int c_hi = own == CH_UNSEEN ? 0 : min(max((prefix ? a.L : own) - key0, 0), CH_KEYS);
+            const int c_lo = min(max(from - key0 - (prefix ? 0 : a.L), 0), CH_KEYS);
+            if (__any_sync(FULL, c_hi < CH_KEYS || c_lo > 0)) {
 #pragma unroll
-            for (int x = 0; x < 128; ++x)
-              if (x >= c_hi || x < c_lo) r[x] = 0xff800000u;
+              for (int y = 0; y < 4; ++y) {
+                const int lo = min(max(c_lo - 32 * y, 0), 32), hi = min(max(c_hi - 32 * y, 0), 32);
+                const uint32_t seen = (hi == 32 ? 0xffffffffu : (1u << hi) - 1u) & (lo == 32 ? 0u : 0xffffffffu << lo);
+                if (__any_sync(FULL, seen != 0xffffffffu)) {
+#pragma unroll
+                  for (int x = 0; x < 32; ++x) r[32 * y + x] = seen & (1u << x) ? r[32 * y + x] : 0xff800000u;
+                }
+              }
+            }
           }
           auto f = [&](int x) { return __uint_as_float(r[x]); };
           float x4[4] = {f(0), f(1), f(2), f(3)};
@@ -568,48 +511,56 @@ __global__ void __launch_bounds__(CH_NT, 1)
 #pragma unroll
           for (int y = 0; y < 4; ++y) x4[y] = fmaxf(x4[y], f(124 + y));
           const float top = max3(fmaxf(x4[0], x4[1]), x4[2], x4[3]) * a.scale_log2;
-          const bool rise = top > m + PX_SLACK || (j == 0 && top > m);
+          const bool start = j < 2 - (alone ? 1 : 0);  // this warpgroup's first unit of the segment
+          const bool rise = top > m + PX_SLACK || (start && top > m);
           if (__any_sync(FULL, rise)) {
             const float nm = rise ? top : m;
             const float k = rise ? ex2(m - nm) : 1.0f;  // 0 from -inf
             l *= k;
             lr *= k;
             m = nm;
-            if (j > 0) {
-              ok = __all_sync(FULL, wait(&o_done[i], static_cast<uint32_t>(kv - 1) & 1u));
+            if (!start) {
+              ok = __all_sync(FULL, wait(&o_done[i], static_cast<uint32_t>(cnt - 1) & 1u));
               if (!ok) break;
               tc_fence_after();
 #pragma unroll 1
-              for (int y = 0; y < D / 32; ++y) {
-                float v[32];
-                tmem_ld32(to + static_cast<uint32_t>(32 * y), v);
-                uint32_t u[32];
+              for (int y = 0; y < D / 16; ++y) {
+                uint32_t v[16];
+                tmem_ld16(to + static_cast<uint32_t>(16 * y), v);
 #pragma unroll
-                for (int x = 0; x < 32; ++x) u[x] = __float_as_uint(v[x] * k);
-                tmem_st32(to + static_cast<uint32_t>(32 * y), u);
+                for (int x = 0; x < 16; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * k);
+                tmem_st16(to + static_cast<uint32_t>(16 * y), v);
               }
+              tmem_st_wait();
             }
           }
-          const int valid = (prefix ? a.L : g.len) - key0, end = min((valid + rows - 1) / rows * rows, CH_KEYS);
-          if (i == 0 && valid < end) {  // V past the end, up to the end of its box
-            const int stage = kv % STAGES;
-            ok = __all_sync(FULL, wait(&v_full[stage], static_cast<uint32_t>(kv / STAGES) & 1u));
-            if (!ok) break;
-            for (int x = t; x < (end - valid) * 8 * HALVES; x += 128) {
-              const int half = x / ((end - valid) * 8), at = x - half * (end - valid) * 8;
-              *reinterpret_cast<uint4*>(s_v + stage * Tile::KV_BYTES + half * CH_KEYS * 128 + valid * 128 + at * 16) = make_uint4(0, 0, 0, 0);
+          if (tile == 0) {
+            const int rows = min(a.bs, CH_KEYS);
+            const int valid = (prefix ? a.L : g.len) - key0, end = min((valid + rows - 1) & ~(rows - 1), CH_KEYS);
+            if (valid < end) {  // V past the end, up to the end of its box
+              const int stage = (stage0 + j) % STAGES;
+              ok = __all_sync(FULL, wait(&v_full[stage], static_cast<uint32_t>((stage0 + j) / STAGES) & 1u));
+              if (!ok) break;
+              for (int x = row; x < (end - valid) * 8; x += 128)
+                for (int y = 0; y < HALVES; ++y)
+                  *reinterpret_cast<uint4*>(s_v + stage * Tile::KV_BYTES + y * CH_KEYS * 128 + valid * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+              fence_proxy_async_smem();
             }
-            fence_proxy_async_smem();
+          }
+          if (pending) {  // the sums given at the end of the last shared tile
+            ok = __all_sync(FULL, wait(taken, static_cast<uint32_t>(shared - 1) & 1u));
+            if (!ok) break;
+            pending = false;
           }
           const float base = m == -INFINITY ? 0.0f : m;
           const float2 sc = make_float2(a.scale_log2, a.scale_log2), nb = make_float2(-base, -base);
           float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0, rounded0 = sum0, rounded1 = sum0;
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t pk[32];
+          for (int quarter = 0; quarter < 4; ++quarter) {
+            uint32_t pk[16];
 #pragma unroll
-            for (int x = 0; x < 32; ++x) {
-              float2 p = __ffma2_rn(make_float2(f(64 * half + 2 * x), f(64 * half + 2 * x + 1)), sc, nb);
+            for (int x = 0; x < 16; ++x) {
+              float2 p = __ffma2_rn(make_float2(f(32 * quarter + 2 * x), f(32 * quarter + 2 * x + 1)), sc, nb);
               p.x = ex2(p.x);
               p.y = ex2(p.y);
               if (x & 1) sum1 = __fadd2_rn(sum1, p); else sum0 = __fadd2_rn(sum0, p);
@@ -617,23 +568,53 @@ __global__ void __launch_bounds__(CH_NT, 1)
               const float2 r2 = unpack2<BF16>(pk[x]);
               if (x & 1) rounded1 = __fadd2_rn(rounded1, r2); else rounded0 = __fadd2_rn(rounded0, r2);
             }
-            tmem_st32(ts + static_cast<uint32_t>(32 * half), pk);
-            tc_fence_before();
-            mbar_arrive(half ? &p_full[i] : &p_half[i]);
+            tmem_st16(ts + static_cast<uint32_t>(16 * quarter), pk);
+            if (quarter & 1) {
+              tmem_st_wait();
+              tc_fence_before();
+              mbar_arrive(quarter == 1 ? &p_half[i] : &p_full[i]);
+            }
           }
           l += (sum0.x + sum1.x) + (sum0.y + sum1.y);
           lr += (rounded0.x + rounded1.x) + (rounded0.y + rounded1.y);
         }
         if (!ok) break;
-        ok = __all_sync(FULL, wait(&o_done[i], static_cast<uint32_t>(kv - 1) & 1u));
+        ok = __all_sync(FULL, wait(&o_done[i], static_cast<uint32_t>(cnt - 1) & 1u));
         if (!ok) break;
         tc_fence_after();
+        float even = lr > 0.0f ? l / lr : 1.0f;  // O times this: what the unrounded p would have summed, but for its direction
+        float other = 0.0f;                      // the same for the other warpgroup's O
+        const bool both = !alone && g.steps > 1;
+        if (both) {
+          ++shared;
+          if (turn) {  // it has this one's sums: m, l and the sum of the rounded p here, O where it is
+            s_ml[3 * row] = m, s_ml[3 * row + 1] = l, s_ml[3 * row + 2] = lr;
+            mbar_arrive(given);
+            pending = true;
+            continue;
+          }
+          ok = __all_sync(FULL, wait(given, static_cast<uint32_t>(shared - 1) & 1u));
+          if (!ok) break;
+          tc_fence_after();
+          const float m2 = s_ml[3 * row], l2 = s_ml[3 * row + 1], lr2 = s_ml[3 * row + 2];
+          const float nm = fmaxf(m, m2), base = nm == -INFINITY ? 0.0f : nm, k = ex2(m - base), k2 = ex2(m2 - base);
+          even = l == 0.0f ? 0.0f : even * k;
+          other = l2 == 0.0f ? 0.0f : (lr2 > 0.0f ? l2 / lr2 : 1.0f) * k2;
+          m = nm;
+          l = l * k + l2 * k2;
+        }
         // out = O / (sum of the rounded p); a part: O times l over that sum, with m and l
         const bool whole = g.slot < 0;
-        const bool some = !(l == 0.0f);  // (a NaN is some)
-        const float even = lr > 0.0f ? l / lr : 1.0f, factor = whole ? even * chunk_inverse(l) : even;
+        if (whole) {
+          const float inv = chunk_inverse(l);
+          even *= inv;
+          other *= inv;
+        }
+        const int token = tile * c.per_tile + row / a.G, gq = row % a.G;
+        const bool exists = row < c.per_tile * a.G && token < g.tokens, sees = own != CH_UNSEEN;
         const int64_t out_at = static_cast<int64_t>(g.token + token) * a.ot + (static_cast<int64_t>(g.h) * a.G + gq) * a.oh;
-        const int64_t part_at = static_cast<int64_t>(max(g.slot, 0)) * c.slot_rows + i * c.per_tile * a.G + row;
+        const int64_t part_at = static_cast<int64_t>(max(g.slot, 0)) * c.slot_rows + tile * c.per_tile * a.G + row;
+        const uint32_t to2 = tmem + lanes + static_cast<uint32_t>(256 + 128 * (i ^ 1));
         float odd = 0.0f;  // a NaN where a value is not finite
 #pragma unroll 1
         for (int y = 0; y < D / 32; ++y) {
@@ -641,8 +622,17 @@ __global__ void __launch_bounds__(CH_NT, 1)
           tmem_ld32(to + static_cast<uint32_t>(32 * y), v);
 #pragma unroll
           for (int x = 0; x < 32; ++x) {
-            odd = fmaf(v[x], 0.0f, odd);
-            v[x] = some ? v[x] * factor : 0.0f;
+            odd = fmaf(v[x], 0.0f, odd);  // (a NaN from an infinity, too)
+            v[x] = l == 0.0f || even == 0.0f ? 0.0f : v[x] * even;  // (0 times what nobody saw)
+          }
+          if (both) {
+            float z[32];
+            tmem_ld32(to2 + static_cast<uint32_t>(32 * y), z);
+#pragma unroll
+            for (int x = 0; x < 32; ++x) {
+              odd = fmaf(z[x], 0.0f, odd);
+              v[x] = other == 0.0f ? v[x] : fmaf(z[x], other, v[x]);
+            }
           }
           if (exists) {
             if (whole) {
@@ -658,7 +648,8 @@ __global__ void __launch_bounds__(CH_NT, 1)
             }
           }
         }
-        tc_fence_before();  // O has been read: the next P of this tile (its barrier) lets the next product into it start
+        tc_fence_before();  // O has been read: the next P (its barrier) lets the next product into it start
+        if (both) mbar_arrive(taken);
         if (exists) {
           if (!whole) c.part_ml[part_at] = make_float2(m, l);
           else if (a.lse) a.lse[static_cast<int64_t>(g.token + token) * a.Hq + g.h * a.G + gq] = chunk_lse(m, l);
@@ -669,7 +660,8 @@ __global__ void __launch_bounds__(CH_NT, 1)
           const int src = __ffs(redo) - 1;
           redo &= redo - 1;
           const int tk = __shfl_sync(FULL, token, src), q = __shfl_sync(FULL, gq, src), ow = __shfl_sync(FULL, own, src);
-          const int64_t fi = __shfl_sync(FULL, first, src), at = __shfl_sync(FULL, part_at, src), oat = __shfl_sync(FULL, out_at, src);
+          const int fi = __shfl_sync(FULL, from, src);
+          const int64_t at = __shfl_sync(FULL, part_at, src), oat = __shfl_sync(FULL, out_at, src);
           constexpr int E = D / 32;
           float acc[E], km, kl;
           chunk_row_by_key<D, BF16>(c, g, g.token + tk, q, ow, fi, lane, acc, km, kl);
@@ -686,20 +678,176 @@ __global__ void __launch_bounds__(CH_NT, 1)
           }
         }
       }
+      __syncthreads();  // the segments have been taken, the next ones may be listed
+      if (*reinterpret_cast<volatile int*>(failed)) break;
     }
-    __syncthreads();  // the segments have been taken, the next ones may be listed
-    if (*reinterpret_cast<volatile int*>(failed)) break;
-  }
-
-  if (w == 8) {
-    if (bad && a.error_word) atomicOr(a.error_word, Q3S_DECERR_BLOCK_ID);
-    // no copy may be in flight when the CTA leaves: wait for each stage's last one
-    if (lane == 0) {
-      if (q_copies) (void)mbar_wait_bounded(q_full, static_cast<uint32_t>(q_copies - 1) & 1u);
-      for (int i = max(0, k_copies - STAGES); i < k_copies; ++i)
-        (void)mbar_wait_bounded(&k_full[i % STAGES], static_cast<uint32_t>(i / STAGES) & 1u);
-      for (int i = max(0, v_copies - STAGES); i < v_copies; ++i)
-        (void)mbar_wait_bounded(&v_full[i % STAGES], static_cast<uint32_t>(i / STAGES) & 1u);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CH_REGS_OTHER));
+    if (w == 8) {
+      int copies = 0, v_copies = 0, q_copies = 0, bad = 0;  // (V's may be one behind K's where a wait gave up)
+    for (bool again = works; again;) {
+      __syncthreads();  // the segments are listed
+      const int n = *s_segs;
+      again = walker->more != 0;
+      // ---- copies: lane l copies box l of a step (a page, or 128 tokens of one) ----
+      const int rows = min(a.bs, CH_KEYS), pages = CH_KEYS / rows;
+      auto block_of = [&](const ChunkSeg& g, int j) {  // past the cache (it reads as zeros) where there is none
+        const int s = g.step0 + j;
+        const bool prefix = s < before;
+        const int key = (prefix ? s : s - before) * CH_KEYS + lane * rows;
+        if (lane >= pages || key >= (prefix ? a.L : g.len)) return a.blocks;
+        const int32_t* ids = prefix ? a.prefix_blocks : a.table + g.b * a.table_stride;
+        return ids[key >> a.bs_log2];
+      };
+      auto copy = [&](const CUtensorMap* map, unsigned char* ring, uint64_t* full, int s, int h, int block) {
+        const int place = (lane * rows) & (a.bs - 1);
+        if (lane == 0) mbar_expect_tx(&full[s], Tile::KV_BYTES);
+        __syncwarp();
+        if (lane < pages)
+          for (int x = 0; x < HALVES; ++x)
+            tma_load_slice(smem_u32(ring + s * Tile::KV_BYTES + x * CH_KEYS * 128 + lane * rows * 128), map, x, place, h, block, &full[s]);
+      };
+      int next = n ? block_of(s_list[0], 0) : 0;
+      for (int e = 0; ok && e < n; ++e) {
+        const ChunkSeg& g = s_list[e];
+        const int steps = g.steps, h = g.h, tiles = tiles_of(g);
+        for (int j = 0; ok && j < steps; ++j) {
+          const bool inside = static_cast<unsigned>(next) < static_cast<unsigned>(a.blocks);
+          bad |= !inside && next != a.blocks;
+          const int block = inside ? next : a.blocks;
+          if (j + 1 < steps) next = block_of(g, j + 1);
+          else if (e + 1 < n) next = block_of(s_list[e + 1], 0);
+          const int s = copies % STAGES;
+          const uint32_t parity = static_cast<uint32_t>(copies / STAGES - 1) & 1u;
+          if (copies >= STAGES && !(ok = __all_sync(FULL, wait(&k_empty[s], parity)))) break;
+          copy(&tm_k, s_k, k_full, s, h, block);
+          ++copies;
+          if (j == 0) {
+            for (int i = 0; i < tiles; ++i) {
+              const int place = q_copies & 1;
+              if (q_copies >= 2 && !(ok = __all_sync(FULL, wait(&q_empty[place], static_cast<uint32_t>((q_copies >> 1) - 1) & 1u)))) break;
+              if (lane == 0) {
+                mbar_expect_tx(&q_full[place], static_cast<uint32_t>(HALVES * c.per_tile * a.G * 128));
+                for (int x = 0; x < HALVES; ++x)
+                  tma_load_3d(smem_u32(s_q + place * Tile::Q_BYTES + x * CH_M * 128), &tm_q, 64 * x, h * a.G, g.token + i * c.per_tile,
+                              &q_full[place]);
+              }
+              __syncwarp();
+              ++q_copies;
+            }
+            if (!ok) break;
+          }
+          if (copies > STAGES && !(ok = __all_sync(FULL, wait(&v_empty[s], parity)))) break;
+          copy(&tm_v, s_v, v_full, s, h, block);
+          ++v_copies;
+        }
+      }
+      __syncthreads();  // the segments have been taken, the next ones may be listed
+      if (*reinterpret_cast<volatile int*>(failed)) break;
+    }
+      if (bad && a.error_word) atomicOr(a.error_word, Q3S_DECERR_BLOCK_ID);
+      // no copy may be in flight when the CTA leaves: wait for each place's last one
+      if (lane == 0) {
+        for (int i = max(0, q_copies - 2); i < q_copies; ++i) (void)mbar_wait_bounded(&q_full[i & 1], static_cast<uint32_t>(i >> 1) & 1u);
+        for (int i = max(0, copies - STAGES); i < copies; ++i)
+          (void)mbar_wait_bounded(&k_full[i % STAGES], static_cast<uint32_t>(i / STAGES) & 1u);
+        for (int i = max(0, v_copies - STAGES); i < v_copies; ++i)
+          (void)mbar_wait_bounded(&v_full[i % STAGES], static_cast<uint32_t>(i / STAGES) & 1u);
+      }
+    } else if (w == 9) {
+    for (bool again = works; again;) {
+      __syncthreads();  // the segments are listed
+      const int n = *s_segs;
+      again = walker->more != 0;
+      // ---- products --------------------------------------------------------------
+      constexpr uint32_t FMT = BF16 ? 1u : 0u;
+      constexpr uint32_t ID_S = (1u << 4) | (FMT << 7) | (FMT << 10) | (static_cast<uint32_t>(CH_KEYS >> 3) << 17) |
+                                (static_cast<uint32_t>(CH_M >> 4) << 24);
+      constexpr uint32_t ID_O = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) |
+                                (static_cast<uint32_t>(CH_M >> 4) << 24);  // bit 16: B's rows are the contraction
+      if (elect_one()) {
+        const uint64_t q_desc = head_smem_desc(smem_u32(s_q)), k_desc = head_smem_desc(smem_u32(s_k)), v_desc = v_smem_desc(smem_u32(s_v));
+        // A place in the sequence of units: segment, unit in it, its tiles and steps, the steps and tiles of Q before it.
+        struct Place {
+          int e, x, tiles, steps, kv, q, u;
+        };
+        auto at_segment = [&](Place& p) {
+          if (p.e < n) p.tiles = tiles_of(s_list[p.e]), p.steps = s_list[p.e].steps;
+        };
+        auto advance = [&](Place& p) {
+          ++p.u;
+          if (++p.x < p.steps * p.tiles) return;
+          p.kv += p.steps;
+          p.q += p.tiles;
+          ++p.e;
+          p.x = 0;
+          at_segment(p);
+        };
+        auto scores = [&](Place& p) {  // S = Q K^T of its unit
+          const int j = p.tiles == 2 ? p.x >> 1 : p.x, tile = p.tiles == 2 ? p.x & 1 : 0;
+          const int s = (p.kv + j) % STAGES, q = (p.q + tile) & 1, i = p.u & 1;
+          if (j == 0) ok = ok && wait(&q_full[q], static_cast<uint32_t>((p.q + tile) >> 1) & 1u);
+          if (tile == 0) ok = ok && wait(&k_full[s], static_cast<uint32_t>((p.kv + j) / STAGES) & 1u);
+          if (!ok) return;
+          tc_fence_after();
+          const uint64_t dq = q_desc + static_cast<uint64_t>(q * (Tile::Q_BYTES >> 4)), dk = k_desc + static_cast<uint64_t>(s * (Tile::KV_BYTES >> 4));
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            constexpr int SLICE = (CH_KEYS * 128) >> 4;
+            umma_f16(tmem + static_cast<uint32_t>(128 * i), dq + (k / 4) * SLICE + (k % 4) * 2, dk + (k / 4) * SLICE + (k % 4) * 2, ID_S, k != 0);
+          }
+          umma_commit(&s_full[i]);
+          if (tile == p.tiles - 1) umma_commit(&k_empty[s]);
+          if (j == p.steps - 1) umma_commit(&q_empty[q]);
+          advance(p);
+        };
+        Place ahead = {0, 0, 1, 1, kv, tiles_q, units};
+        at_segment(ahead);
+        Place now = ahead;
+        for (int i = 0; i < 2 && ok && ahead.e < n; ++i) scores(ahead);
+        while (ok && now.e < n) {
+          const int j = now.tiles == 2 ? now.x >> 1 : now.x, tile = now.tiles == 2 ? now.x & 1 : 0;
+          const int s = (now.kv + j) % STAGES, i = now.u & 1;
+          const uint32_t parity = static_cast<uint32_t>(now.u >> 1) & 1u;  // of the warpgroup's units
+          const bool first = now.x < 2;  // into this O
+          if (tile == 0) ok = wait(&v_full[s], static_cast<uint32_t>((now.kv + j) / STAGES) & 1u);
+          const uint64_t dv = v_desc + static_cast<uint64_t>(s * (Tile::KV_BYTES >> 4));
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {  // O += P V
+            ok = ok && wait(half ? &p_full[i] : &p_half[i], parity);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int q = 0; q < CH_KEYS / 32; ++q) {
+              const int k = half * (CH_KEYS / 32) + q;
+              umma_f16_ta(tmem + static_cast<uint32_t>(256 + 128 * i), tmem + static_cast<uint32_t>(128 * i + 8 * k),
+                          dv + k * ((16 * 128) >> 4), ID_O, !first || k != 0);
+            }
+          }
+          if (!ok) break;
+          if (tile == now.tiles - 1) umma_commit(&v_empty[s]);
+          umma_commit(&o_done[i]);
+          if (ahead.e < n) scores(ahead);
+          advance(now);
+        }
+      }
+      __syncwarp();
+      for (int e = 0; e < n; ++e) {  // what came before the next batch
+        const int tiles = tiles_of(s_list[e]);
+        kv += s_list[e].steps;
+        units += s_list[e].steps * tiles;
+        tiles_q += tiles;
+      }
+      __syncthreads();  // the segments have been taken, the next ones may be listed
+      if (*reinterpret_cast<volatile int*>(failed)) break;
+    }
+    } else {  // makes the warpgroup whole
+    for (bool again = works; again;) {
+      __syncthreads();  // the segments are listed
+      again = walker->more != 0;
+      __syncthreads();  // the segments have been taken, the next ones may be listed
+      if (*reinterpret_cast<volatile int*>(failed)) break;
+    }
     }
   }
   __syncwarp();
