@@ -22,10 +22,10 @@
 namespace q3s {
 
 constexpr int CH_M = PX_M, CH_KEYS = PX_KEYS;
-constexpr int CH_NT = 384;      // two softmax warpgroups, and one with the copy warp and the matrix warp
+constexpr int CH_NT = 384;      // two softmax warpgroups, and one with the copy warp and three matrix warps
 constexpr int CH_SEGS = 64;     // segments of a CTA's range that are listed at a time
 // Registers a thread: a softmax thread holds a row of 128 scores.  Launched with 168 a thread, which is what the shares add up to.
-constexpr int CH_REGS_SOFTMAX = 216, CH_REGS_OTHER = 72;
+constexpr int CH_REGS_SOFTMAX = 184, CH_REGS_OTHER = 136;
 static_assert(2 * CH_REGS_SOFTMAX + CH_REGS_OTHER <= 3 * 168, "what the CTA is launched with");
 constexpr int CH_START = 6;     // cost of an item's start and end, where a step of two tiles costs 3 and one of one tile 2
 constexpr int CH_MAX_STEP = 3;  // the largest cost of a step
@@ -60,6 +60,11 @@ template <int D>
 struct ChunkTile {
   static constexpr int HALVES = D / 64;
   static constexpr int STAGES = D == 64 ? 4 : 2;  // steps of K (and of V) in shared memory
+  static constexpr int KEYS = 64;                  // keys of a unit
+  static constexpr int PIECES = CH_KEYS / KEYS;    // units that a step's keys are cut into
+  static_assert(PIECES == 2, "each softmax warpgroup has a unit of every step");
+  static constexpr int BUFFERS = D == 64 ? 6 : 4;  // places for scores in TMEM
+  static_assert(BUFFERS * KEYS + 2 * D == 512, "columns");
   static constexpr int Q_BYTES = CH_M * D * 2;
   static constexpr int KV_BYTES = CH_KEYS * D * 2;
   static constexpr int LIST = CH_SEGS * static_cast<int>(sizeof(ChunkSeg)) + CH_NT * static_cast<int>(sizeof(ChunkRow)) + CH_M * 12;
@@ -115,6 +120,28 @@ struct ChunkCutting {
   Q3S_DEV long long start(int i) const { return div_nonneg(all * i, ctas); }
   Q3S_DEV int cta_of(long long at) const { return static_cast<int>(div_nonneg((at + 1) * ctas + all - 1, all)) - 1; }
 };
+
+// Products and commits of one lane of a converged warp, under a predicate and not a branch: their operands are
+// then computed once for the warp (in a branch each product took three times as many issue slots).
+Q3S_DEV void umma_ss_if(uint32_t leader, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], %2, %3, %4, p;\n}" ::"r"(leader),
+      "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+Q3S_DEV void umma_ts_if(uint32_t leader, uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], %3, %4, p;\n}" ::"r"(leader),
+      "r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+Q3S_DEV void umma_commit_if(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n}" ::"r"(leader),
+      "r"(smem_u32(bar))
+      : "memory");
+}
 
 // 16 consecutive columns of this thread's TMEM lane; a store is complete after tmem_st_wait.
 Q3S_DEV void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
@@ -193,18 +220,20 @@ Q3S_DEV float chunk_inverse(float l) { return l > 0.0f ? 1.0f / l : l == l ? 0.0
 Q3S_DEV float chunk_lse(float m, float l) { return l > 0.0f ? (m + log2f(l)) * 0.69314718055994531f : l == l ? -INFINITY : l; }
 
 // The two softmax warpgroups take turns: unit u of the CTA's work, 128 query rows
-// against 128 keys, is that of warpgroup u % 2, whose scores, probabilities and sums have
-// their place in TMEM (S0 S1 O0 O1, 128 columns each).  A step of a segment of two tiles
-// is two units; a segment of one tile (a few drafts) has a unit a step, so the two
-// warpgroups share its keys, odd and even steps, and the one that began joins the
-// other's sums to its own at the end.  The matrix warp keeps two units on their way,
-//   O(u) += P(u) V, S(u + 2) = Q K'^T,
-// over the segments without a pause: a warpgroup's O is taken out before it hands over the
-// next segment's first P, which is what the next product into O waits for, and the two tiles of Q are a ring.
-// A softmax thread owns a query row; m, l and the sum of the rounded p (q3s_attn_prefix.cuh says why) are in registers.
+// against half of a step's keys, is that of warpgroup u % 2.  With two tiles of query rows
+// each has one; with one tile (a few drafts) the two share its keys in turn, and the one that began joins the
+// other's sums to its own at the end.  Scores have BUFFERS places in TMEM, which the probabilities take over
+// (16-bit, the second product's A operand), so that the scores of up to BUFFERS units are on their way or waiting:
+//   O(u) += P(u) V, then S(u + BUFFERS) = Q K^T into the place that this frees,
+// over the segments without a pause.  (With one place of 128 keys a warpgroup, its softmax waited for two products
+// at each step: 2 rows of 4096 tokens took 252 us.)  A warpgroup's O, D more columns each, is taken out before it hands
+// over the next segment's first P, which is what the next product into O waits for, and the two tiles of Q are a ring.
+// A softmax thread owns a query row; m, l and the sum of the rounded p (q3s_attn_prefix.cuh says why) are in
+// registers.  It takes its exponentials with the maximum so far while it looks for the unit's own; where a score
+// rises above that by more than 8, which after a segment's first unit is rare, O is rescaled and the unit taken again.
 //
-// Masks are a range of columns a row and step (behind the query's own place,
-// before the window, past the prefix's end), applied by quarters of a step that some row of the
+// Masks are a range of columns a row and unit (behind the query's own place,
+// before the window, past the prefix's end), applied by 32 columns that some row of the
 // warp does not see whole.  V is cleared past the end of a row's (or the prefix's)
 // last step by the softmax warps that hand over its first P; whole pages past the end read as zeros.
 template <int D, bool BF16>
@@ -212,7 +241,7 @@ __global__ void __launch_bounds__(CH_NT, 1)
     attn_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const ChunkArgs c) {
   using Tile = ChunkTile<D>;
-  constexpr int HALVES = Tile::HALVES, STAGES = Tile::STAGES;
+  constexpr int HALVES = Tile::HALVES, STAGES = Tile::STAGES, KEYS = Tile::KEYS, PIECES = Tile::PIECES, BUFFERS = Tile::BUFFERS;
   const AttnArgs& a = c.a;
   extern __shared__ __align__(1024) unsigned char ch_smem[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ch_smem) + 1023) &
@@ -226,11 +255,10 @@ __global__ void __launch_bounds__(CH_NT, 1)
   uint64_t* k_empty = k_full + STAGES;
   uint64_t* v_full = k_empty + STAGES;
   uint64_t* v_empty = v_full + STAGES;
-  uint64_t* s_full = v_empty + STAGES;  // [2] scores of a warpgroup's unit are in TMEM
-  uint64_t* p_half = s_full + 2;        // [2] the probabilities of its first 64 keys are
-  uint64_t* p_full = p_half + 2;        // [2] all are
-  uint64_t* o_done = p_full + 2;        // [2] its second product is complete
-  uint64_t* given = o_done + 2;         // a shared tile's second sums may be read, and have been
+  uint64_t* s_full = v_empty + STAGES;  // [BUFFERS] a unit's scores are in TMEM
+  uint64_t* p_full = s_full + BUFFERS;  // [BUFFERS] its probabilities are
+  uint64_t* o_done = p_full + BUFFERS;  // [BUFFERS] its second product is complete
+  uint64_t* given = o_done + BUFFERS;         // a shared tile's second sums may be read, and have been
   uint64_t* taken = given + 1;
   uint64_t* done = taken + 1;           // behind a wait that gave up
   long long* s_sum = reinterpret_cast<long long*>(done + 1);  // [CH_NT / 32]
@@ -238,7 +266,7 @@ __global__ void __launch_bounds__(CH_NT, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(walker + 1);
   int* failed = reinterpret_cast<int*>(tmem_slot + 1);
   int* s_segs = failed + 1;
-  static_assert((4 + 4 * STAGES + 8 + 3 + CH_NT / 32) * 8 + sizeof(ChunkWalk) + 3 * 4 <= 512, "room for the barriers and counts");
+  static_assert((4 + 4 * STAGES + 3 * BUFFERS + 3 + CH_NT / 32) * 8 + sizeof(ChunkWalk) + 3 * 4 <= 512, "room for the barriers and counts");
   ChunkSeg* s_list = reinterpret_cast<ChunkSeg*>(reinterpret_cast<unsigned char*>(q_full) + 512);
   ChunkRow* s_rows = reinterpret_cast<ChunkRow*>(s_list + CH_SEGS);  // the first CH_NT rows
   float* s_ml = reinterpret_cast<float*>(s_rows + CH_NT);            // [128][3] m, l and the sum of the rounded p of a shared tile's second sums
@@ -249,32 +277,33 @@ __global__ void __launch_bounds__(CH_NT, 1)
 
   grid_wait();
   grid_release();
-  if (w == 8) {
+  if (w == 0) {
     if (lane < 3) prefetch_map(lane == 0 ? &tm_q : lane == 1 ? &tm_k : &tm_v);
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&q_full[i], 1);
-        mbar_init(&q_empty[i], 1);
+        mbar_init(&q_empty[i], 2);
+      }
+      for (int i = 0; i < BUFFERS; ++i) {
         mbar_init(&s_full[i], 1);
-        mbar_init(&p_half[i], 128);
         mbar_init(&p_full[i], 128);
         mbar_init(&o_done[i], 1);
       }
       for (int s = 0; s < STAGES; ++s) {
         mbar_init(&k_full[s], 1);
-        mbar_init(&k_empty[s], 1);
+        mbar_init(&k_empty[s], 2);
         mbar_init(&v_full[s], 1);
         mbar_init(&v_empty[s], 1);
       }
       mbar_init(given, 128);
       mbar_init(taken, 128);
-      mbar_init(done, 1);
+      mbar_init(done, 3);
       *failed = 0;
       fence_mbar_init();
     }
     __syncwarp();
   }
-  if (w == 9) {
+  if (w == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -436,91 +465,118 @@ __global__ void __launch_bounds__(CH_NT, 1)
     atomicOr(failed, 1);
     return false;
   };
-  int kv = 0, units = 0, tiles_q = 0;  // steps, units and tiles of Q so far (the matrix warp: before this batch of segments)
+  int kv = 0, units = 0, tiles_q = 0;  // steps, units and tiles of Q so far
   bool ok = true;
   auto tiles_of = [&](const ChunkSeg& g) { return g.tokens > c.per_tile ? 2 : 1; };
 
   // Each role with a loop of its own over the batches of segments, so that it has its own number of registers.
-  if (w < 8) {
+  if (w >= 4) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CH_REGS_SOFTMAX));
-    int cnt = 0;           // this warpgroup's units
     int shared = 0;        // tiles so far whose keys the two warpgroups shared
     bool pending = false;  // the sums given for the last of them must have been taken before the next product into them
     for (bool again = works; again;) {
-      if (w == 0) walk();
       __syncthreads();  // the segments are listed
       const int n = *s_segs;
       again = walker->more != 0;
       // ---- softmax ----------------------------------------------------------------
-      const int i = w >> 2, row = (w & 3) * 32 + lane;
+      const int i = (w >> 2) - 1, row = (w & 3) * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>((w & 3) * 32) << 16;
-      const uint32_t ts = tmem + lanes + static_cast<uint32_t>(128 * i), to = tmem + lanes + static_cast<uint32_t>(256 + 128 * i);
+      const uint32_t ts = tmem + lanes, to = ts + static_cast<uint32_t>(BUFFERS * KEYS + D * i);
       for (int e = 0; ok && e < n; ++e) {
         const ChunkSeg& g = s_list[e];
-        const int turn = (i - units) & 1;  // this warpgroup's first unit in the segment
-        const int stage0 = kv;             // steps before the segment
-        const int tile = tiles_of(g) == 2 ? turn : 0;
-        units += tiles_of(g) * g.steps;
+        const bool alone = tiles_of(g) == 2;  // with its tile
+        const int turn = (i - units) & 1;     // this warpgroup's first unit in the segment
+        const int tile = alone ? turn : 0, stage0 = kv, end = g.steps * PIECES * (alone ? 2 : 1);  // steps before the segment; its units
+        int buffer = (units + turn) % BUFFERS;
+        uint32_t parity = static_cast<uint32_t>((units + turn) / BUFFERS) & 1u;
+        units += end;
         kv += g.steps;
+        if (turn >= end) continue;
+        int last_buffer = buffer;
+        uint32_t last_parity = parity;
         float m = -INFINITY, l = 0.0f, lr = 0.0f;  // lr: of the rounded p
-        int own, from = 0;  // own tokens that this row's query sees (none where there is no such query), and the first position
+        // Own tokens that this row's query sees, and the first position.  A row without a query, or whose query sees
+        // nothing, goes along: it is told apart at the end.
+        int own = CH_UNSEEN, from = 0;
         {
           const int token = tile * c.per_tile + row / a.G;
-          const bool sees = row < c.per_tile * a.G && token < g.tokens && (!a.slot_map || a.slot_map[g.token + token] >= 0);
-          own = sees ? g.i_key + token : CH_UNSEEN;
-          if (sees && c.window) from = max(a.L + own - c.window, 0);
-        }
-        const bool alone = tiles_of(g) == 2;
-        if (!alone && turn >= g.steps) continue;
-        for (int j = alone ? 0 : turn; j < g.steps; j += alone ? 1 : 2, ++cnt) {
-          bool prefix;
-          int key0;  // of the prefix or of the row's own
-          {
-            const int s = g.step0 + j;
-            prefix = s < before;
-            key0 = (prefix ? s : s - before) * CH_KEYS;
+          if (row < c.per_tile * a.G && token < g.tokens && (!a.slot_map || a.slot_map[g.token + token] >= 0)) {
+            own = g.i_key + token;
+            if (c.window) from = max(a.L + own - c.window, 0);
           }
-          ok = __all_sync(FULL, wait(&s_full[i], static_cast<uint32_t>(cnt) & 1u));
-          if (!ok) break;
-          tc_fence_after();
-          uint32_t r[128];
-          tmem_ld128(ts, r);
-          {
-            // the columns that are seen, [c_lo, c_hi), as a bit each
-            const int c_hi = own == CH_UNSEEN ? 0 : min(max((prefix ? a.L : own) - key0, 0), CH_KEYS);
-            const int c_lo = min(max(from - key0 - (prefix ? 0 : a.L), 0), CH_KEYS);
-            if (__any_sync(FULL, c_hi < CH_KEYS || c_lo > 0)) {
-#pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                const int lo = min(max(c_lo - 32 * y, 0), 32), hi = min(max(c_hi - 32 * y, 0), 32);
-                const uint32_t seen = (hi == 32 ? 0xffffffffu : (1u << hi) - 1u) & (lo == 32 ? 0u : 0xffffffffu << lo);
-                if (__any_sync(FULL, seen != 0xffffffffu)) {
-#pragma unroll
-                  for (int x = 0; x < 32; ++x) r[32 * y + x] = seen & (1u << x) ? r[32 * y + x] : 0xff800000u;
+        }
+        // The pieces that all rows of the warp see whole: [full0, full1) of the prefix, [full2, full3) of the row's own.
+        int full0, full1, full2, full3;
+        {
+          const int least = __reduce_min_sync(FULL, own == CH_UNSEEN ? 0x7fffffff : own), most = __reduce_max_sync(FULL, from);
+          const int own0 = (before - g.step0) * PIECES;
+          full0 = (most + KEYS - 1) / KEYS - g.step0 * PIECES;
+          full1 = a.L / KEYS - g.step0 * PIECES;
+          full2 = own0 + (max(most - a.L, 0) + KEYS - 1) / KEYS;
+          full3 = own0 + min(max(least, 0), g.len) / KEYS;
+        }
+        for (int x = turn; x < end; x += 2) {
+          const int piece = alone ? x >> 1 : x;
+          const bool whole_piece = (piece >= full0 && piece < full1) || (piece >= full2 && piece < full3);
+          int c_hi = KEYS, c_lo = 0;  // the columns that are seen: [c_lo, c_hi)
+          if (!whole_piece) {
+            const int step = g.step0 + piece / PIECES;
+            const bool prefix = step < before;
+            const int key0 = (prefix ? step : step - before) * CH_KEYS + piece % PIECES * KEYS;  // of the prefix or of the row's own
+            c_hi = min(max((prefix ? a.L : own == CH_UNSEEN ? g.len : own) - key0, 0), KEYS);
+            c_lo = min(max(from - key0 - (prefix ? 0 : a.L), 0), KEYS);
+            if (tile == 0) {
+              // of the step's keys: behind the last one, up to the end of its box, in this piece
+              const int rows = min(a.bs, CH_KEYS), first = piece % PIECES * KEYS, valid = (prefix ? a.L : g.len) - key0 + first;
+              const int clear = max(valid, first), last = min(min((valid + rows - 1) & ~(rows - 1), CH_KEYS), first + KEYS);
+              if (clear < last) {
+                const int kv_step = stage0 + piece / PIECES, stage = kv_step % STAGES;
+                ok = __all_sync(FULL, wait(&v_full[stage], static_cast<uint32_t>(kv_step / STAGES) & 1u));
+                if (!ok) break;
+                for (int y = row; y < (last - clear) * 8 * HALVES; y += 128) {
+                  const int half = HALVES == 1 || y < (last - clear) * 8 ? 0 : 1, at = y - half * (last - clear) * 8;
+                  *reinterpret_cast<uint4*>(s_v + stage * Tile::KV_BYTES + half * CH_KEYS * 128 + clear * 128 + at * 16) =
+                      make_uint4(0, 0, 0, 0);
                 }
+                fence_proxy_async_smem();
               }
             }
           }
-          auto f = [&](int x) { return __uint_as_float(r[x]); };
+          ok = __all_sync(FULL, wait(&s_full[buffer], parity));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t place = ts + static_cast<uint32_t>(KEYS * buffer);
+          uint32_t r[KEYS];
+          tmem_ld64(place, r);
+          if (!whole_piece) {
+#pragma unroll
+            for (int y = 0; y < KEYS / 32; ++y) {
+              const int lo = min(max(c_lo - 32 * y, 0), 32), hi = min(max(c_hi - 32 * y, 0), 32);
+              const uint32_t seen = (hi == 32 ? 0xffffffffu : (1u << hi) - 1u) & (lo == 32 ? 0u : 0xffffffffu << lo);
+#pragma unroll
+              for (int z = 0; z < 32; ++z) r[32 * y + z] = seen & (1u << z) ? r[32 * y + z] : 0xff800000u;
+            }
+          }
+          auto f = [&](int z) { return __uint_as_float(r[z]); };
           float x4[4] = {f(0), f(1), f(2), f(3)};
 #pragma unroll
-          for (int x = 4; x + 8 <= 128; x += 8) {
+          for (int z = 4; z + 8 <= KEYS; z += 8) {
 #pragma unroll
-            for (int y = 0; y < 4; ++y) x4[y] = max3(x4[y], f(x + 2 * y), f(x + 2 * y + 1));
+            for (int y = 0; y < 4; ++y) x4[y] = max3(x4[y], f(z + 2 * y), f(z + 2 * y + 1));
           }
 #pragma unroll
-          for (int y = 0; y < 4; ++y) x4[y] = fmaxf(x4[y], f(124 + y));
+          for (int y = 0; y < 4; ++y) x4[y] = fmaxf(x4[y], f(KEYS - 4 + y));
           const float top = max3(fmaxf(x4[0], x4[1]), x4[2], x4[3]) * a.scale_log2;
-          const bool start = j < 2 - (alone ? 1 : 0);  // this warpgroup's first unit of the segment
-          const bool rise = top > m + PX_SLACK || (start && top > m);
+          const bool rise = top > m + PX_SLACK || (x < 2 && top > m);
           if (__any_sync(FULL, rise)) {
             const float nm = rise ? top : m;
             const float k = rise ? ex2(m - nm) : 1.0f;  // 0 from -inf
             l *= k;
             lr *= k;
             m = nm;
-            if (!start) {
-              ok = __all_sync(FULL, wait(&o_done[i], static_cast<uint32_t>(cnt - 1) & 1u));
+            if (x >= 2) {
+              // the product before is this warpgroup's unit before: two buffers back
+              ok = __all_sync(FULL, wait(&o_done[buffer >= 2 ? buffer - 2 : buffer - 2 + BUFFERS], buffer >= 2 ? parity : parity ^ 1u));
               if (!ok) break;
               tc_fence_after();
 #pragma unroll 1
@@ -528,63 +584,48 @@ __global__ void __launch_bounds__(CH_NT, 1)
                 uint32_t v[16];
                 tmem_ld16(to + static_cast<uint32_t>(16 * y), v);
 #pragma unroll
-                for (int x = 0; x < 16; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * k);
+                for (int z = 0; z < 16; ++z) v[z] = __float_as_uint(__uint_as_float(v[z]) * k);
                 tmem_st16(to + static_cast<uint32_t>(16 * y), v);
               }
               tmem_st_wait();
             }
           }
-          if (tile == 0) {
-            const int rows = min(a.bs, CH_KEYS);
-            const int valid = (prefix ? a.L : g.len) - key0, end = min((valid + rows - 1) & ~(rows - 1), CH_KEYS);
-            if (valid < end) {  // V past the end, up to the end of its box
-              const int stage = (stage0 + j) % STAGES;
-              ok = __all_sync(FULL, wait(&v_full[stage], static_cast<uint32_t>((stage0 + j) / STAGES) & 1u));
-              if (!ok) break;
-              for (int x = row; x < (end - valid) * 8; x += 128)
-                for (int y = 0; y < HALVES; ++y)
-                  *reinterpret_cast<uint4*>(s_v + stage * Tile::KV_BYTES + y * CH_KEYS * 128 + valid * 128 + x * 16) = make_uint4(0, 0, 0, 0);
-              fence_proxy_async_smem();
-            }
+          uint32_t pk[KEYS / 2];
+          const float base = m == -INFINITY ? 0.0f : m;
+          const float2 sc = make_float2(a.scale_log2, a.scale_log2), nb = make_float2(-base, -base);
+          float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0, rounded0 = sum0, rounded1 = sum0;
+#pragma unroll
+          for (int z = 0; z < KEYS / 2; ++z) {
+            float2 p = __ffma2_rn(make_float2(f(2 * z), f(2 * z + 1)), sc, nb);
+            p.x = ex2(p.x);
+            p.y = ex2(p.y);
+            if (z & 1) sum1 = __fadd2_rn(sum1, p); else sum0 = __fadd2_rn(sum0, p);
+            pk[z] = pack2<BF16>(p.x, p.y);
+            const float2 r2 = unpack2<BF16>(pk[z]);
+            if (z & 1) rounded1 = __fadd2_rn(rounded1, r2); else rounded0 = __fadd2_rn(rounded0, r2);
           }
+          tmem_st32(place, pk);
           if (pending) {  // the sums given at the end of the last shared tile
             ok = __all_sync(FULL, wait(taken, static_cast<uint32_t>(shared - 1) & 1u));
             if (!ok) break;
             pending = false;
           }
-          const float base = m == -INFINITY ? 0.0f : m;
-          const float2 sc = make_float2(a.scale_log2, a.scale_log2), nb = make_float2(-base, -base);
-          float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0, rounded0 = sum0, rounded1 = sum0;
-#pragma unroll
-          for (int quarter = 0; quarter < 4; ++quarter) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              float2 p = __ffma2_rn(make_float2(f(32 * quarter + 2 * x), f(32 * quarter + 2 * x + 1)), sc, nb);
-              p.x = ex2(p.x);
-              p.y = ex2(p.y);
-              if (x & 1) sum1 = __fadd2_rn(sum1, p); else sum0 = __fadd2_rn(sum0, p);
-              pk[x] = pack2<BF16>(p.x, p.y);
-              const float2 r2 = unpack2<BF16>(pk[x]);
-              if (x & 1) rounded1 = __fadd2_rn(rounded1, r2); else rounded0 = __fadd2_rn(rounded0, r2);
-            }
-            tmem_st16(ts + static_cast<uint32_t>(16 * quarter), pk);
-            if (quarter & 1) {
-              tmem_st_wait();
-              tc_fence_before();
-              mbar_arrive(quarter == 1 ? &p_half[i] : &p_full[i]);
-            }
-          }
+          tc_fence_before();
+          mbar_arrive(&p_full[buffer]);
           l += (sum0.x + sum1.x) + (sum0.y + sum1.y);
           lr += (rounded0.x + rounded1.x) + (rounded0.y + rounded1.y);
+          last_buffer = buffer, last_parity = parity;
+          buffer += 2;
+          if (buffer >= BUFFERS) buffer -= BUFFERS, parity ^= 1u;
         }
         if (!ok) break;
-        ok = __all_sync(FULL, wait(&o_done[i], static_cast<uint32_t>(cnt - 1) & 1u));
+        ok = __all_sync(FULL, wait(&o_done[last_buffer], last_parity));
         if (!ok) break;
         tc_fence_after();
+        if (own == CH_UNSEEN) m = -INFINITY, l = lr = 0.0f;
         float even = lr > 0.0f ? l / lr : 1.0f;  // O times this: what the unrounded p would have summed, but for its direction
         float other = 0.0f;                      // the same for the other warpgroup's O
-        const bool both = !alone && g.steps > 1;
+        const bool both = !alone && end > 1;
         if (both) {
           ++shared;
           if (turn) {  // it has this one's sums: m, l and the sum of the rounded p here, O where it is
@@ -614,7 +655,7 @@ __global__ void __launch_bounds__(CH_NT, 1)
         const bool exists = row < c.per_tile * a.G && token < g.tokens, sees = own != CH_UNSEEN;
         const int64_t out_at = static_cast<int64_t>(g.token + token) * a.ot + (static_cast<int64_t>(g.h) * a.G + gq) * a.oh;
         const int64_t part_at = static_cast<int64_t>(max(g.slot, 0)) * c.slot_rows + tile * c.per_tile * a.G + row;
-        const uint32_t to2 = tmem + lanes + static_cast<uint32_t>(256 + 128 * (i ^ 1));
+        const uint32_t to2 = ts + static_cast<uint32_t>(BUFFERS * KEYS + D * (i ^ 1));
         float odd = 0.0f;  // a NaN where a value is not finite
 #pragma unroll 1
         for (int y = 0; y < D / 32; ++y) {
@@ -683,9 +724,10 @@ __global__ void __launch_bounds__(CH_NT, 1)
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CH_REGS_OTHER));
-    if (w == 8) {
+    if (w == 0) {
       int copies = 0, v_copies = 0, q_copies = 0, bad = 0;  // (V's may be one behind K's where a wait gave up)
     for (bool again = works; again;) {
+      walk();
       __syncthreads();  // the segments are listed
       const int n = *s_segs;
       again = walker->more != 0;
@@ -754,114 +796,96 @@ __global__ void __launch_bounds__(CH_NT, 1)
         for (int i = max(0, v_copies - STAGES); i < v_copies; ++i)
           (void)mbar_wait_bounded(&v_full[i % STAGES], static_cast<uint32_t>(i / STAGES) & 1u);
       }
-    } else if (w == 9) {
-    for (bool again = works; again;) {
-      __syncthreads();  // the segments are listed
-      const int n = *s_segs;
-      again = walker->more != 0;
-      // ---- products --------------------------------------------------------------
+    } else {
+      // ---- products: warp 1 the second one, O += P V, warps 2 and 3 the scores of a softmax warpgroup each ----
+      // (one warp for all scores took 450 clocks to issue a unit's eight products beside the softmax warps and 500 more for
+      // its waits and loop: 2 rows of 4096 tokens 271 us)
       constexpr uint32_t FMT = BF16 ? 1u : 0u;
-      constexpr uint32_t ID_S = (1u << 4) | (FMT << 7) | (FMT << 10) | (static_cast<uint32_t>(CH_KEYS >> 3) << 17) |
+      constexpr uint32_t ID_S = (1u << 4) | (FMT << 7) | (FMT << 10) | (static_cast<uint32_t>(KEYS >> 3) << 17) |
                                 (static_cast<uint32_t>(CH_M >> 4) << 24);
       constexpr uint32_t ID_O = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) |
                                 (static_cast<uint32_t>(CH_M >> 4) << 24);  // bit 16: B's rows are the contraction
-      if (elect_one()) {
-        const uint64_t q_desc = head_smem_desc(smem_u32(s_q)), k_desc = head_smem_desc(smem_u32(s_k)), v_desc = v_smem_desc(smem_u32(s_v));
-        // A place in the sequence of units: segment, unit in it, its tiles and steps, the steps and tiles of Q before it.
-        struct Place {
-          int e, x, tiles, steps, kv, q, u;
-        };
-        auto at_segment = [&](Place& p) {
-          if (p.e < n) p.tiles = tiles_of(s_list[p.e]), p.steps = s_list[p.e].steps;
-        };
-        auto advance = [&](Place& p) {
-          ++p.u;
-          if (++p.x < p.steps * p.tiles) return;
-          p.kv += p.steps;
-          p.q += p.tiles;
-          ++p.e;
-          p.x = 0;
-          at_segment(p);
-        };
-        auto scores = [&](Place& p) {  // S = Q K^T of its unit
-          const int j = p.tiles == 2 ? p.x >> 1 : p.x, tile = p.tiles == 2 ? p.x & 1 : 0;
-          const int s = (p.kv + j) % STAGES, q = (p.q + tile) & 1, i = p.u & 1;
-          if (j == 0) ok = ok && wait(&q_full[q], static_cast<uint32_t>((p.q + tile) >> 1) & 1u);
-          if (tile == 0) ok = ok && wait(&k_full[s], static_cast<uint32_t>((p.kv + j) / STAGES) & 1u);
-          if (!ok) return;
-          tc_fence_after();
-          const uint64_t dq = q_desc + static_cast<uint64_t>(q * (Tile::Q_BYTES >> 4)), dk = k_desc + static_cast<uint64_t>(s * (Tile::KV_BYTES >> 4));
+      constexpr uint64_t DESC_HI = (1024ull >> 4 << 32) | (1ull << 46) | (2ull << 61);  // of both kinds of descriptor
+      const uint32_t leader = elect_one() ? 1u : 0u;
+      const uint32_t q_lo = static_cast<uint32_t>(head_smem_desc(smem_u32(s_q))), k_lo = static_cast<uint32_t>(head_smem_desc(smem_u32(s_k)));
+      const uint32_t v_lo = static_cast<uint32_t>(v_smem_desc(smem_u32(s_v)));
+      for (bool again = works; again;) {
+        __syncthreads();  // the segments are listed
+        const int n = *s_segs;
+        again = walker->more != 0;
+        for (int e = 0; ok && e < n; ++e) {
+          const int steps = s_list[e].steps, tiles = tiles_of(s_list[e]);
+          const bool alone = tiles == 2;
+          const int end = steps * PIECES * tiles, stride = w == 1 ? 1 : 2;
+          const int x0 = w == 1 ? 0 : (w - units) & 1;  // warp 2 has the even units
+          int buffer = (units + x0) % BUFFERS;
+          uint32_t parity = static_cast<uint32_t>((units + x0) / BUFFERS) & 1u;
+          bool used = units + x0 >= BUFFERS;  // the buffer, before
+          int stage = kv % STAGES, step = -1;
+          uint32_t stage_parity = static_cast<uint32_t>(kv / STAGES) & 1u;
+          for (int x = x0; x < end; x += stride) {
+            const int piece = alone ? x >> 1 : x, part = piece % PIECES;
+            if (piece / PIECES != step) {
+              if (step >= 0 && ++stage == STAGES) stage = 0, stage_parity ^= 1u;
+              step = piece / PIECES;
+              ok = __all_sync(FULL, wait(w == 1 ? &v_full[stage] : &k_full[stage], stage_parity));
+              if (!ok) break;
+            }
+            if (w == 1) {
+              ok = __all_sync(FULL, wait(&p_full[buffer], parity));
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t dv = v_lo + static_cast<uint32_t>(stage * (Tile::KV_BYTES >> 4) + part * ((KEYS * 128) >> 4));
+              const uint32_t to = tmem + static_cast<uint32_t>(BUFFERS * KEYS + D * ((units + x) & 1)), p = tmem + static_cast<uint32_t>(KEYS * buffer);
+              const bool first = x < 2;  // into this O
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            constexpr int SLICE = (CH_KEYS * 128) >> 4;
-            umma_f16(tmem + static_cast<uint32_t>(128 * i), dq + (k / 4) * SLICE + (k % 4) * 2, dk + (k / 4) * SLICE + (k % 4) * 2, ID_S, k != 0);
-          }
-          umma_commit(&s_full[i]);
-          if (tile == p.tiles - 1) umma_commit(&k_empty[s]);
-          if (j == p.steps - 1) umma_commit(&q_empty[q]);
-          advance(p);
-        };
-        Place ahead = {0, 0, 1, 1, kv, tiles_q, units};
-        at_segment(ahead);
-        Place now = ahead;
-        for (int i = 0; i < 2 && ok && ahead.e < n; ++i) scores(ahead);
-        while (ok && now.e < n) {
-          const int j = now.tiles == 2 ? now.x >> 1 : now.x, tile = now.tiles == 2 ? now.x & 1 : 0;
-          const int s = (now.kv + j) % STAGES, i = now.u & 1;
-          const uint32_t parity = static_cast<uint32_t>(now.u >> 1) & 1u;  // of the warpgroup's units
-          const bool first = now.x < 2;  // into this O
-          if (tile == 0) ok = wait(&v_full[s], static_cast<uint32_t>((now.kv + j) / STAGES) & 1u);
-          const uint64_t dv = v_desc + static_cast<uint64_t>(s * (Tile::KV_BYTES >> 4));
+              for (int k = 0; k < KEYS / 16; ++k)
+                umma_ts_if(leader, to, p + static_cast<uint32_t>(8 * k), DESC_HI | (dv + static_cast<uint32_t>(k * ((16 * 128) >> 4))), ID_O, !first || k != 0);
+              umma_commit_if(leader, &o_done[buffer]);
+              if (part == PIECES - 1 && (!alone || (x & 1))) umma_commit_if(leader, &v_empty[stage]);
+              if (++buffer == BUFFERS) buffer = 0, parity ^= 1u;
+            } else {
+              const uint32_t tile_q = static_cast<uint32_t>(tiles_q + (alone ? x & 1 : 0)), q = tile_q & 1u;
+              if (x < 2) ok = __all_sync(FULL, wait(&q_full[q], (tile_q >> 1) & 1u));
+              // the probabilities that were there have been taken
+              if (ok && used) ok = __all_sync(FULL, wait(&o_done[buffer], parity ^ 1u));
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t to = tmem + static_cast<uint32_t>(KEYS * buffer), dq = q_lo + q * static_cast<uint32_t>(Tile::Q_BYTES >> 4);
+              const uint32_t dk = k_lo + static_cast<uint32_t>(stage * (Tile::KV_BYTES >> 4) + part * ((KEYS * 128) >> 4));
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {  // O += P V
-            ok = ok && wait(half ? &p_full[i] : &p_half[i], parity);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int q = 0; q < CH_KEYS / 32; ++q) {
-              const int k = half * (CH_KEYS / 32) + q;
-              umma_f16_ta(tmem + static_cast<uint32_t>(256 + 128 * i), tmem + static_cast<uint32_t>(128 * i + 8 * k),
-                          dv + k * ((16 * 128) >> 4), ID_O, !first || k != 0);
+              for (int k = 0; k < D / 16; ++k) {
+                constexpr int SLICE = (CH_KEYS * 128) >> 4;
+                umma_ss_if(leader, to, DESC_HI | (dq + static_cast<uint32_t>((k / 4) * SLICE + (k % 4) * 2)),
+                           DESC_HI | (dk + static_cast<uint32_t>((k / 4) * SLICE + (k % 4) * 2)), ID_S, k != 0);
+              }
+              umma_commit_if(leader, &s_full[buffer]);
+              // each of the two warps frees a stage, and a tile of Q (one that only this warp has twice)
+              if (!alone || part == PIECES - 1) umma_commit_if(leader, &k_empty[stage]);
+              if (x + 2 >= end) {
+                umma_commit_if(leader, &q_empty[q]);
+                if (alone) umma_commit_if(leader, &q_empty[q]);
+              }
+              buffer += 2;
+              if (buffer >= BUFFERS) buffer -= BUFFERS, parity ^= 1u, used = true;
             }
           }
-          if (!ok) break;
-          if (tile == now.tiles - 1) umma_commit(&v_empty[s]);
-          umma_commit(&o_done[i]);
-          if (ahead.e < n) scores(ahead);
-          advance(now);
+          units += end;
+          kv += steps;
+          tiles_q += tiles;
         }
+        __syncthreads();  // the segments have been taken, the next ones may be listed
+        if (*reinterpret_cast<volatile int*>(failed)) break;
       }
-      __syncwarp();
-      for (int e = 0; e < n; ++e) {  // what came before the next batch
-        const int tiles = tiles_of(s_list[e]);
-        kv += s_list[e].steps;
-        units += s_list[e].steps * tiles;
-        tiles_q += tiles;
-      }
-      __syncthreads();  // the segments have been taken, the next ones may be listed
-      if (*reinterpret_cast<volatile int*>(failed)) break;
-    }
-    } else {  // makes the warpgroup whole
-    for (bool again = works; again;) {
-      __syncthreads();  // the segments are listed
-      again = walker->more != 0;
-      __syncthreads();  // the segments have been taken, the next ones may be listed
-      if (*reinterpret_cast<volatile int*>(failed)) break;
-    }
+      if (*failed) umma_commit_if(leader, done);  // products may still be running
     }
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (w == 9) {
+  if (w == 1) {
     tc_fence_after();
-    if (*failed) {  // products may still be running: a commit behind them (bounded) before the columns go
-      if (elect_one()) {
-        umma_commit(done);
-        (void)mbar_wait_bounded(done, 0);
-      }
-      __syncwarp();
-    }
+    if (*failed) (void)mbar_wait_bounded(done, 0);  // (bounded) before the columns go
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
   if (t == 0 && *failed && a.error_word) atomicOr(a.error_word, Q3S_DECERR_WAIT);
