@@ -11,6 +11,7 @@
 #pragma once
 
 #include <cuda.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -116,10 +117,8 @@ Q3S_DEV float2 unpack2(uint32_t p) {
   if constexpr (BF16) {
     return make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
   } else {
-    float2 r;
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n}"
-        : "=f"(r.x), "=f"(r.y) : "r"(p));
-    return r;
+    // both at once: single conversions go through the unit that the exponentials need
+    return __half22float2(*reinterpret_cast<const __half2*>(&p));
   }
 }
 Q3S_DEV float ex2(float x) {

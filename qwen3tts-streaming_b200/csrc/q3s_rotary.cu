@@ -20,7 +20,6 @@ struct RotaryArgs {
   bool interleaved;
   float scale;
   int turned, copied;  // units of a head that turn (pairs of vectors with HALF) and that are only copied
-  int per;             // head rows that a pass of the CTA takes
   const int32_t* positions;
   int64_t position_stride;
   const float* inv_freq;
@@ -31,7 +30,7 @@ struct RotaryArgs {
   int32_t* error_word;
 };
 
-constexpr int RO_NT = 256;
+constexpr int RO_MAX_NT = 256;
 constexpr int RO_ANGLES = 512;  // cos and sin that a CTA holds: its tokens times the pairs
 constexpr int RO_TOKENS = 4;    // the most tokens of a CTA
 
@@ -50,14 +49,17 @@ Q3S_DEV float2 rotary_angle(int pos, float freq, float scale) {
   return make_float2((quadrant == 1 || quadrant == 2 ? -x : x) * scale, (quadrant >= 2 ? -y : y) * scale);
 }
 
-template <typename T>
-Q3S_DEV float to_f32(T x) {
-  return static_cast<float>(x);
+// Two neighbouring values, converted together: single conversions to or from 16 bits go through
+// the unit of the transcendental functions, a quarter as fast (8191 tokens 39 us).
+Q3S_DEV float2 to_f32(const float* x) { return make_float2(x[0], x[1]); }
+Q3S_DEV float2 to_f32(const __nv_bfloat16* x) {
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(x);
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
-template <typename T>
-Q3S_DEV T from_f32(float x) {
-  return static_cast<T>(x);  // to nearest even
-}
+Q3S_DEV float2 to_f32(const __half* x) { return __half22float2(*reinterpret_cast<const __half2*>(x)); }
+Q3S_DEV void from_f32(float* x, float2 f) { x[0] = f.x, x[1] = f.y; }
+Q3S_DEV void from_f32(__nv_bfloat16* x, float2 f) { *reinterpret_cast<__nv_bfloat162*>(x) = __floats2bfloat162_rn(f.x, f.y); }
+Q3S_DEV void from_f32(__half* x, float2 f) { *reinterpret_cast<__half2*>(x) = __floats2half2_rn(f.x, f.y); }
 
 template <typename T, int E>
 struct alignas(sizeof(T) * E) RotaryVec {
@@ -85,18 +87,34 @@ struct RotaryUnit {
   // cs: cos and sin of the token's pairs
   Q3S_DEV void turn(const float2* cs, int u, int turned) {
     if (u >= turned) return;
-    if constexpr (TWO) {
+    // pair i of a unit is at i * units, so that neighbouring lanes read neighbouring places
+    if constexpr (E == 1) {
+      const float2 c = cs[u];
+      float p = static_cast<float>(a.x[0]), q = static_cast<float>(b.x[0]);
+      one(c, p, q);
+      a.x[0] = static_cast<T>(p), b.x[0] = static_cast<T>(q);
+    } else if constexpr (TWO) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) one(cs[u * E + e], a.x[e], b.x[e]);
+      for (int e = 0; e < E; e += 2) {
+        float2 p = to_f32(a.x + e), q = to_f32(b.x + e);
+        one(cs[u + e * turned], p.x, q.x);
+        one(cs[u + (e + 1) * turned], p.y, q.y);
+        from_f32(a.x + e, p), from_f32(b.x + e, q);
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < E / 2; ++e) one(cs[u * (E / 2) + e], a.x[2 * e], a.x[2 * e + 1]);
+      for (int e = 0; e < E / 2; ++e) {
+        float2 p = to_f32(a.x + 2 * e);
+        one(cs[u + e * turned], p.x, p.y);
+        from_f32(a.x + 2 * e, p);
+      }
     }
   }
-  Q3S_DEV static void one(float2 c, T& x, T& y) {
-    const float p = to_f32(x), q = to_f32(y);
-    x = from_f32<T>(fmaf(p, c.x, -(q * c.y)));
-    y = from_f32<T>(fmaf(p, c.y, q * c.x));
+  static constexpr int PAIRS = TWO ? E : E / 2;  // of a unit
+  Q3S_DEV static void one(float2 c, float& x, float& y) {
+    const float p = x, q = y;
+    x = fmaf(p, c.x, -(q * c.y));
+    y = fmaf(p, c.y, q * c.x);
   }
   Q3S_DEV void store(T* to, int u, int turned, int pairs) const {
     if (u < turned) {
@@ -109,108 +127,100 @@ struct RotaryUnit {
   }
 };
 
-// A CTA takes TT tokens and one share of their heads (blockIdx.y).  Its threads
-// first compute the cos and sin of the tokens' pairs, one each, into shared memory:
-// all heads share them, and one evaluation a thread is the shortest way to the first
-// store.  Then a thread keeps its unit of a head row (two 16-byte vectors) and
-// walks the rows, queries, keys and values after one another, two at a time so that
-// four to six loads are on their way.  Bound by HBM: every byte is read and written once.
+// A CTA takes up to four neighbouring tokens and one share of their heads
+// (blockIdx.y); a thread keeps a unit of a head (two 16-byte vectors) for all of
+// them, so that addresses are counted up and not divided out (one unit after another of
+// tokens times heads took 39 us for 8191 tokens, bound by instructions).  The units of queries or keys and of values are requested before
+// anything else; while they are on their way the threads compute the cos and sin of the
+// tokens' pairs, one each, into shared memory, where all heads find them.  Bound by HBM: every byte is read and written once.
 template <typename T, int E, bool ADJ>
-__global__ void __launch_bounds__(RO_NT) rotary_kernel(const RotaryArgs a, int tokens) {
+__global__ void __launch_bounds__(RO_MAX_NT) rotary_kernel(const RotaryArgs a, int tokens) {
   using Unit = RotaryUnit<T, E, ADJ>;
+  using Vec = RotaryVec<T, E>;
   __shared__ float2 s_cs[RO_ANGLES];
   __shared__ int64_t s_k[RO_TOKENS], s_v[RO_TOKENS];  // offsets of a token's place in the caches; -1: none
-  const int t = static_cast<int>(threadIdx.x);
+  const int t = static_cast<int>(threadIdx.x), nt = static_cast<int>(blockDim.x);
+  const int first = static_cast<int>(blockIdx.y) * nt + t, all = static_cast<int>(gridDim.y) * nt;  // of a unit a thread
   const int64_t token0 = static_cast<int64_t>(blockIdx.x) * tokens;
   const int n = static_cast<int>(min(static_cast<int64_t>(tokens), a.T - token0));
+  const int units = a.turned + a.copied, items = (a.Hq + a.Hk) * units, vunits = a.dim / E, vitems = a.Hk * vunits;
   grid_wait();
   grid_release();
-  for (int i = t; i < n * a.pairs; i += RO_NT) {
+
+  Unit x[RO_TOKENS];
+  Vec y[RO_TOKENS];
+  auto fetch = [&](int item) {
+    const int h = item / units, u = item - h * units;
+    const bool query = h < a.Hq;
+    const T* from = query ? static_cast<const T*>(a.q) + token0 * a.qt + h * a.qh : static_cast<const T*>(a.k) + token0 * a.kt + (h - a.Hq) * a.kh;
+    const int64_t stride = query ? a.qt : a.kt;
+#pragma unroll
+    for (int i = 0; i < RO_TOKENS; ++i)
+      if (i < n) x[i].load(from + i * stride, u, a.turned, a.pairs);
+  };
+  auto finish = [&](int item) {
+    const int h = item / units, u = item - h * units;
+    const bool query = h < a.Hq;
+    T* to = query ? static_cast<T*>(a.out) + token0 * a.ot + h * a.oh : static_cast<T*>(a.kc) + (h - a.Hq) * a.kch;
+#pragma unroll
+    for (int i = 0; i < RO_TOKENS; ++i) {
+      if (i >= n || (!query && s_k[i] < 0)) continue;
+      x[i].turn(s_cs + i * a.pairs, u, a.turned);
+      x[i].store(to + (query ? i * a.ot : s_k[i]), u, a.turned, a.pairs);
+    }
+  };
+  auto fetch_v = [&](int item) {  // values are copied whole
+    const int h = item / vunits, u = item - h * vunits;
+    const T* from = static_cast<const T*>(a.v) + token0 * a.vt + h * a.vh + u * E;
+#pragma unroll
+    for (int i = 0; i < RO_TOKENS; ++i)
+      if (i < n) y[i] = *reinterpret_cast<const Vec*>(from + i * a.vt);
+  };
+  auto finish_v = [&](int item) {
+    const int h = item / vunits, u = item - h * vunits;
+    T* to = static_cast<T*>(a.vc) + h * a.vch + u * E;
+#pragma unroll
+    for (int i = 0; i < RO_TOKENS; ++i)
+      if (i < n && s_v[i] >= 0) *reinterpret_cast<Vec*>(to + s_v[i]) = y[i];
+  };
+  if (first < items) fetch(first);
+  if (first < vitems) fetch_v(first);
+
+  for (int i = t; i < n * a.pairs; i += nt) {
     const int tok = i / a.pairs, p = i - tok * a.pairs;
     int axis = 0;
-    if (a.interleaved) {
-      const int m = p % a.axes;
-      axis = p < a.axes * a.sections[m] ? m : 0;
-    } else {
-      int end = a.sections[0];
-      while (p >= end && axis + 1 < a.axes) end += a.sections[++axis];
-    }
-    s_cs[i] = rotary_angle(a.positions[axis * a.position_stride + token0 + tok], a.inv_freq[p], a.scale);
-  }
-  if (a.Hk)
-    for (int i = t; i < n; i += RO_NT) {
-      const int64_t slot = a.slots[token0 + i];
-      s_k[i] = s_v[i] = -1;
-      if (slot >= static_cast<int64_t>(a.blocks) * a.bs) {
-        if (a.error_word && blockIdx.y == 0) atomicOr(a.error_word, Q3S_DECERR_BLOCK_ID);
-      } else if (slot >= 0) {
-        const int64_t block = slot / a.bs, place = slot - block * a.bs;
-        s_k[i] = block * a.kb + place * a.kp;
-        s_v[i] = block * a.vb + place * a.vp;
+    if (a.axes > 1) {
+      if (a.interleaved) {
+        const int m = p % a.axes;
+        axis = p < a.axes * a.sections[m] ? m : 0;
+      } else {
+        int end = a.sections[0];
+        while (p >= end && axis + 1 < a.axes) end += a.sections[++axis];
       }
     }
-  __syncthreads();
-  const int units = a.turned + a.copied, per = a.per;
-  {
-    const int row0 = t / units, first = t - row0 * units;
-    const int heads = a.Hq + a.Hk, rows = n * heads, step = per * static_cast<int>(gridDim.y);
-    if (row0 < per)
-      for (int u = first; u < units; u += RO_NT)
-        for (int r = static_cast<int>(blockIdx.y) * per + row0; r < rows; r += 2 * step) {
-          Unit x[2];
-          T* to[2];
-          int tok[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int at = r + i * step;
-            to[i] = nullptr;
-            if (at >= rows) continue;
-            tok[i] = at / heads;
-            const int h = at - tok[i] * heads;
-            const int64_t token = token0 + tok[i];
-            const T* from;
-            if (h < a.Hq) {
-              from = static_cast<const T*>(a.q) + token * a.qt + h * a.qh;
-              to[i] = static_cast<T*>(a.out) + token * a.ot + h * a.oh;
-            } else {
-              if (s_k[tok[i]] < 0) continue;
-              from = static_cast<const T*>(a.k) + token * a.kt + (h - a.Hq) * a.kh;
-              to[i] = static_cast<T*>(a.kc) + s_k[tok[i]] + (h - a.Hq) * a.kch;
-            }
-            x[i].load(from, u, a.turned, a.pairs);
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (to[i]) {
-              x[i].turn(s_cs + tok[i] * a.pairs, u, a.turned);
-              x[i].store(to[i], u, a.turned, a.pairs);
-            }
-        }
+    s_cs[tok * a.pairs + p / Unit::PAIRS + p % Unit::PAIRS * a.turned] = rotary_angle(a.positions[axis * a.position_stride + token0 + tok], a.inv_freq[p], a.scale);
   }
-  if (a.Hk) {  // values: copied whole
-    using Vec = RotaryVec<T, E>;
-    const int vu = a.dim / E, vper = max(RO_NT / vu, 1);
-    const int row0 = t / vu, first = t - row0 * vu;
-    const int rows = n * a.Hk, step = vper * static_cast<int>(gridDim.y);
-    if (row0 < vper)
-      for (int u = first; u < vu; u += RO_NT)
-        for (int r = static_cast<int>(blockIdx.y) * vper + row0; r < rows; r += 4 * step) {
-          Vec x[4];
-          T* to[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int at = r + i * step;
-            to[i] = nullptr;
-            if (at >= rows) continue;
-            const int tok = at / a.Hk, h = at - tok * a.Hk;
-            if (s_v[tok] < 0) continue;
-            to[i] = static_cast<T*>(a.vc) + s_v[tok] + h * a.vch + u * E;
-            x[i] = *reinterpret_cast<const Vec*>(static_cast<const T*>(a.v) + (token0 + tok) * a.vt + h * a.vh + u * E);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (to[i]) *reinterpret_cast<Vec*>(to[i]) = x[i];
-        }
+  if (a.Hk && nt - 1 - t < n) {  // the last threads, which have the fewest angles
+    const int i = nt - 1 - t;
+    const int64_t slot = a.slots[token0 + i];
+    s_k[i] = s_v[i] = -1;
+    if (slot >= static_cast<int64_t>(a.blocks) * a.bs) {
+      if (a.error_word && blockIdx.y == 0) atomicOr(a.error_word, Q3S_DECERR_BLOCK_ID);
+    } else if (slot >= 0) {
+      const int64_t block = (slot >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(a.bs)) : slot / a.bs;
+      const int64_t place = slot - block * a.bs;
+      s_k[i] = block * a.kb + place * a.kp;
+      s_v[i] = block * a.vb + place * a.vp;
+    }
+  }
+  __syncthreads();
+  for (int item = first; item < items; item += all) {
+    if (item != first) fetch(item);
+    finish(item);
+  }
+  for (int item = first; item < vitems; item += all) {
+    if (item != first) fetch_v(item);
+    finish_v(item);
   }
 }
 
@@ -220,19 +230,17 @@ cudaError_t launch_rotary(RotaryArgs a, cudaStream_t st) {
   const int turned = !ADJ || E == 1 ? a.pairs / E : 2 * a.pairs / E;
   a.turned = turned;
   a.copied = (a.dim - 2 * a.pairs) / E;
-  a.per = std::max(RO_NT / (turned + a.copied), 1);
-  // Tokens a CTA: one while that leaves SMs without a CTA, up to four (and what its angles have room for).
+  // Threads: a unit each, up to 256 (more units: several in turn).
+  const int64_t items = std::max<int64_t>(static_cast<int64_t>(a.Hq + a.Hk) * (turned + a.copied), static_cast<int64_t>(a.Hk) * (a.dim / E));
+  const int nt = static_cast<int>(std::min<int64_t>((items + 31) / 32 * 32, RO_MAX_NT));
+  // Tokens a CTA: up to four (and what its angles have room for) while there are four CTAs a SM.
   const int sms = sm_count();
-  const int room = std::max(RO_ANGLES / a.pairs, 1);
-  int tokens = 1;
-  while (tokens < RO_TOKENS && 2 * tokens <= room && a.T / (2 * tokens) >= 4 * sms) tokens *= 2;
-  // shares of the heads while there are fewer CTAs than SMs
-  const int rows = tokens * (a.Hq + a.Hk);
+  const int tokens = std::max(std::min(std::min(RO_ANGLES / a.pairs, RO_TOKENS), a.T / (4 * sms)), 1);
+  // shares of the units while there are fewer CTAs than SMs
   const int64_t ctas = (static_cast<int64_t>(a.T) + tokens - 1) / tokens;
-  int64_t shares = std::min<int64_t>((rows + a.per - 1) / a.per, std::max<int64_t>(sms / ctas, 1));
-  shares = std::max<int64_t>(std::min<int64_t>(shares, 65535), 1);
-  return launch_maybe_pdl(rotary_kernel<T, E, ADJ>, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(shares)), dim3(RO_NT), 0, st,
-                          true, a, tokens);
+  const int64_t shares = std::max<int64_t>(std::min<int64_t>(std::min<int64_t>((items + nt - 1) / nt, sms / ctas), 65535), 1);
+  return launch_maybe_pdl(rotary_kernel<T, E, ADJ>, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(shares)), dim3(nt), 0, st, true, a,
+                          tokens);
 }
 
 template <typename T>

@@ -7,11 +7,13 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "q3s_args.cuh"
 #include "q3s_decode.h"
 #include "q3s_device.cuh"
 #include "q3s_pdl.cuh"
+#include "q3s_tma.cuh"
 
 namespace q3s {
 
@@ -21,6 +23,7 @@ struct VerifyArgs {
   int B, T, V;
   int slice;   // entries of the vocabulary that a CTA of a row's cluster takes
   int places;  // places that a CTA looks at together: a power of two, 1..VF_WARPS
+  bool held;   // what a draw is made from is held in shared memory (`slice` 64-bit values)
   float temperature_default;
   const void* logits;
   int64_t logits_stride;
@@ -40,6 +43,7 @@ struct VerifyArgs {
 
 constexpr int VF_NT = 512, VF_WARPS = VF_NT / 32;
 constexpr int VF_MAX_CLUSTER = 8;
+constexpr int VF_SLICE = 8192;  // entries of the vocabulary that a CTA takes, while the cluster grows; it holds so many for the draw
 // Relative error that a 32-bit probability may have, besides its distance (in
 // log2 units) from the largest one times VF_GAP.  An exponential is off by 2^-22
 // (its instruction) and by the rounding of its argument, 2^-24 ln 2 times its
@@ -83,6 +87,24 @@ Q3S_DEV VerifyStat verify_shfl_xor(const VerifyStat& a, int d) {
 }
 // Whether the logits have a distribution.
 Q3S_DEV bool verify_defined(const VerifyStat& s) { return s.sum == s.sum && fabsf(s.best) < INFINITY; }
+// 2^(t / 32) for t <= 0 in 64 bits, by a whole warp: with t = 32 n + j + f, j in
+// [0, 32) and |f| <= 1/2, 2^n 2^(j/32) e^z, z = f ln 2 / 32, where 2^(j/32) is
+// lane j's `root` and e^z its series up to z^5 / 120 (|z| < 0.0109: off by
+// z^6 / 720, 2.3e-15).  14 operations in place of exp2's 40 or so.
+Q3S_DEV double vf_exp2_64(double t, double root) {
+  constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer, in the low word
+  const bool some = t > -32000.0;               // 2^-1000 and less count as 0
+  const double shifted = (some ? t : 0.0) + MAGIC;
+  const int k = __double2loint(shifted);
+  const double z = ((some ? t : 0.0) - (shifted - MAGIC)) * 0.021660849392498290;  // ln 2 / 32
+  double p = fma(z, 1.0 / 120, 1.0 / 24);
+  p = fma(z, p, 1.0 / 6);
+  p = fma(z, p, 0.5);
+  p = fma(z, p, 1.0);
+  p = fma(z, p, 1.0);
+  const double r = __shfl_sync(FULL, root, k & 31) * p;
+  return some ? __hiloint2double(__double2hiint(r) + (k >> 5) * (1 << 20), __double2loint(r)) : 0.0;
+}
 Q3S_DEV float vf_ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -173,6 +195,7 @@ struct VerifyShared {
 template <typename T>
 __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
   __shared__ VerifyShared sh;
+  extern __shared__ double held[];  // [slice], if they are held
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
@@ -222,15 +245,14 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
   const int v0 = min(rank * a.slice, a.V), v1 = min(v0 + a.slice, a.V);
   const T* logits = static_cast<const T*>(a.logits);
 
-  // ---- 64-bit passes over one place: each warp's neighbouring entries ----
+  // ---- 64-bit passes over one place: each warp's neighbouring entries, 32 at a time ----
   const int share = ((v1 - v0 + VF_WARPS - 1) / VF_WARPS + 31) & ~31;
   const int w0 = min(v0 + w * share, v1), w1 = min(w0 + share, v1);
-  // e(v) = 2^((x_v - largest) log2(e) / temperature)
-  auto weight = [&](const T* x, int v, double best) { return exp2((static_cast<double>(static_cast<float>(x[v])) - best) * c64); };
-  // f summed over the vocabulary: the warps' sums meet in every CTA
-  auto sum_all = [&](auto f) {
-    double s = 0.0;
-    for (int v = w0 + lane; v < w1; v += 32) s += f(v);
+  const double root = exp2(lane / 32.0), steep = 32.0 * c64;
+  // e(v) = 2^((x_v - largest) log2(e) / temperature); a whole warp calls
+  auto weight = [&](float x, double best) { return vf_exp2_64((static_cast<double>(x) - best) * steep, root); };
+  // the warps' sums meet in every CTA
+  auto meet = [&](double s) {
 #pragma unroll
     for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(FULL, s, d);
     sync();  // the sums of the pass before have been read
@@ -244,6 +266,18 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
       total += x;
     }
     return total;
+  };
+  // f(v, x_v) of all entries of this warp in turn, x_v requested AHEAD at a time (a float of `from`, -infinity past the end); f is called by the whole warp
+  auto each = [&](const auto* from, auto f) {
+    constexpr int AHEAD = 8;
+    for (int v = w0; v < w1; v += 32 * AHEAD) {
+      float x[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) x[i] = v + 32 * i + lane < w1 ? static_cast<float>(from[v + 32 * i + lane]) : -INFINITY;
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (v + 32 * i < w1) f(v + 32 * i + lane, x[i]);
+    }
   };
 
   // ---- which drafts hold ----
@@ -275,6 +309,18 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
         verify_take<1>(s, one, rest, c);
       }
     }
+    // what warp 0 decides with: the draft behind place first + lane
+    int64_t draft = -1;
+    double aim = 0.0;
+    float draft_x = 0.0f;
+    if (w == 0 && lane < a.places && first + lane + 1 < n) {
+      const int64_t at = t0 + first + lane + 1;
+      draft = a.ids[at];
+      if (draft >= 0 && draft < a.V) {
+        aim = static_cast<double>(a.uniforms[at]) * (a.probs ? static_cast<double>(a.probs[at * a.probs_stride + draft]) : 1.0);
+        draft_x = static_cast<float>(logits[(at - 1) * a.logits_stride + draft]);
+      }
+    }
 #pragma unroll
     for (int d = 16; d; d >>= 1) s = verify_join(s, verify_shfl_xor(s, d));
     if (lane == 0) sh.warp[w] = s;
@@ -297,23 +343,17 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
           p = sh.part[lane][0];
           for (int r = 1; r < ctas; ++r) p = verify_join(p, sh.part[lane][r]);
           verdict = 0;
-          if (i + 1 < n && verify_defined(p)) {
-            const int64_t d = a.ids[t0 + i + 1];
-            if (d >= 0 && d < a.V) {
-              const double q = a.probs ? static_cast<double>(a.probs[(t0 + i + 1) * a.probs_stride + d]) : 1.0;
-              const double aim = static_cast<double>(a.uniforms[t0 + i + 1]) * q;
-              if (greedy) {
-                verdict = aim < (d == p.index ? 1.0 : 0.0);
-              } else {
-                const float x = static_cast<float>(logits[(t0 + i) * a.logits_stride + d]);
-                const double y = static_cast<double>(x) * static_cast<double>(c) - static_cast<double>(p.k);
-                const double left = aim * p.sum, right = exp2(y);
-                const double error = (VF_BOUND - VF_GAP * fmin(y, 0.0)) * (left + right);
-                verdict = !(p.sum > 0.0) || fabsf(p.k) > VF_LARGE ? 2
-                          : !(right > 0.0)                        ? 0
-                          : fabs(left - right) <= error           ? 2
-                                                                  : left < right;
-              }
+          if (i + 1 < n && verify_defined(p) && draft >= 0 && draft < a.V) {
+            if (greedy) {
+              verdict = aim < (draft == p.index ? 1.0 : 0.0);
+            } else {
+              const double y = static_cast<double>(draft_x) * static_cast<double>(c) - static_cast<double>(p.k);
+              const double left = aim * p.sum, right = exp2(y);
+              const double error = (VF_BOUND - VF_GAP * fmin(y, 0.0)) * (left + right);
+              verdict = !(p.sum > 0.0) || fabsf(p.k) > VF_LARGE ? 2
+                        : !(right > 0.0)                        ? 0
+                        : fabs(left - right) <= error           ? 2
+                                                                : left < right;
             }
           }
         }
@@ -335,10 +375,12 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
       } else {
         const T* x = logits + (t0 + place) * a.logits_stride;
         const double best = static_cast<double>(sh.stat.best);
-        const double total = sum_all([&](int v) { return weight(x, v, best); });
+        double sum = 0.0;
+        each(x, [&](int, float y) { sum += weight(y, best); });
+        const double total = meet(sum);
         const int64_t d = a.ids[t0 + place + 1];
         const double q = a.probs ? static_cast<double>(a.probs[(t0 + place + 1) * a.probs_stride + d]) : 1.0;
-        stop = !(static_cast<double>(a.uniforms[t0 + place + 1]) * q * total < weight(x, static_cast<int>(d), best));
+        stop = !(static_cast<double>(a.uniforms[t0 + place + 1]) * q * total < weight(static_cast<float>(x[d]), best));
         from = at + 1;
       }
       __syncthreads();  // before warp 0 writes the next verdict
@@ -371,18 +413,49 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
   }
   const double best = static_cast<double>(stat.best);
   const float* q = a.probs && place + 1 < n ? a.probs + (t0 + place + 1) * a.probs_stride : nullptr;
-  double mass = 0.0;  // sum of e: q is taken times it
-  if (q) mass = sum_all([&](int v) { return weight(x, v, best); });
-  int mode = q ? 2 : place + 1 < n && draft >= 0 && draft < a.V ? 1 : 0;  // what p loses: q, the draft, nothing
-  auto left = [&](int v) {
-    const double e = weight(x, v, best);
-    return mode == 2 ? fmax(e - static_cast<double>(q[v]) * mass, 0.0) : mode == 1 && v == static_cast<int>(draft) ? 0.0 : e;
-  };
-  double total = sum_all(left);
-  if (!(total > 0.0)) {  // nothing is left: from p
-    mode = 0;
-    total = sum_all(left);
+  const int gone = place + 1 < n && !a.probs && draft >= 0 && draft < a.V ? static_cast<int>(draft) : -1;  // a draft that was certain
+  if (q)  // on its way while the weights are taken
+    for (int v = w0 + 32 * lane; v < w1; v += 1024) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + v));
+  // What is drawn from, `left`: e without the draft; with probabilities e - q times the sum of e, where that is positive.
+  // A CTA that holds its slice takes each exponential once.
+  double mass = 0.0, sum = 0.0;
+  each(x, [&](int v, float y) {
+    double e = weight(y, best);  // (every lane: its root goes around)
+    if (v == gone) e = 0.0;
+    if (a.held && v < w1) held[v - v0] = e;
+    sum += e;
+  });
+  double total = meet(sum);
+  bool minus = false;
+  if (q) {
+    mass = total;
+    minus = true;
+    sum = 0.0;
+    each(q, [&](int v, float y) {
+      const double e = a.held ? (v < w1 ? held[v - v0] : 0.0) : weight(v < w1 ? static_cast<float>(x[v]) : -INFINITY, best);
+      const double r = fmax(e - (v < w1 ? static_cast<double>(y) : 0.0) * mass, 0.0);
+      if (a.held && v < w1) held[v - v0] = r;
+      sum += r;
+    });
+    total = meet(sum);
   }
+  const bool again = !(total > 0.0);  // nothing is left: from p
+  if (again) {
+    minus = false;
+    sum = 0.0;
+    each(x, [&](int v, float y) {
+      const double e = weight(y, best);
+      if (a.held && v < w1) held[v - v0] = e;
+      sum += e;
+    });
+    total = meet(sum);
+  }
+  auto left = [&](int v) {  // a whole warp calls
+    if (a.held) return v < w1 ? held[v - v0] : 0.0;
+    double e = weight(v < w1 ? static_cast<float>(x[v]) : -INFINITY, best);
+    if (v == gone && !again) e = 0.0;
+    return minus && v < w1 ? fmax(e - static_cast<double>(q[v]) * mass, 0.0) : e;
+  };
   if (w == 0) {  // the warp (of all CTAs') whose entries reach u * total: its number, and the sum before it
     const double aim = static_cast<double>(a.uniforms[t0]) * total;
     const int warps = ctas * VF_WARPS;
@@ -419,7 +492,7 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
     const double aim = sh.aim;
     int id = -1, last = v0;
     for (int v = w0; v < w1 && id < 0; v += 32) {
-      const double s = v + lane < w1 ? left(v + lane) : 0.0;
+      const double s = left(v + lane);
       double up = s;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -437,9 +510,14 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
 
 template <typename T>
 cudaError_t launch_verify(const VerifyArgs& a, int ctas, cudaStream_t st) {
+  const int smem = a.held ? a.slice * static_cast<int>(sizeof(double)) : 0;
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t allowed = allow_smem(verify_kernel<T>, VF_SLICE * static_cast<int>(sizeof(double)), done);
+  if (allowed != cudaSuccess) return allowed;
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3(static_cast<unsigned>(std::max(a.B, 1)) * ctas);
   lc.blockDim = dim3(VF_NT);
+  lc.dynamicSmemBytes = static_cast<size_t>(smem);
   lc.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -497,8 +575,9 @@ extern "C" q3s_status q3s_verify_drafts(const q3s_verify_drafts_desc* d, void* s
   a.next_ids = d->next_ids;
   a.error_word = d->error_word;
   int ctas = 1;
-  while (ctas < q3s::VF_MAX_CLUSTER && static_cast<int64_t>(ctas) * 8192 < a.V) ctas *= 2;
+  while (ctas < q3s::VF_MAX_CLUSTER && static_cast<int64_t>(ctas) * q3s::VF_SLICE < a.V) ctas *= 2;
   a.slice = ((a.V + ctas - 1) / ctas + 31) & ~31;
+  a.held = a.slice <= q3s::VF_SLICE;
   // as many places at once as a row of the batch has on average
   const int mean = (a.T + std::max(a.B, 1) - 1) / std::max(a.B, 1);
   a.places = 1;
