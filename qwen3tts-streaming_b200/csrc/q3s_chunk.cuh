@@ -143,6 +143,15 @@ Q3S_DEV void umma_commit_if(uint32_t leader, uint64_t* bar) {
       : "memory");
 }
 
+// s += the two 16-bit values of p, each to its own sum (one instruction a value; unpacked first they were three a pair).
+template <bool BF16>
+Q3S_DEV void add_rounded(float2& s, uint32_t p) {
+  if constexpr (BF16)
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.f32.bf16 %0, l, %0;\n\tadd.f32.bf16 %1, h, %1;\n}" : "+f"(s.x), "+f"(s.y) : "r"(p));
+  else
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.f32.f16 %0, l, %0;\n\tadd.f32.f16 %1, h, %1;\n}" : "+f"(s.x), "+f"(s.y) : "r"(p));
+}
+
 // 16 consecutive columns of this thread's TMEM lane; a store is complete after tmem_st_wait.
 Q3S_DEV void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
@@ -601,8 +610,7 @@ __global__ void __launch_bounds__(CH_NT, 1)
             p.y = ex2(p.y);
             if (z & 1) sum1 = __fadd2_rn(sum1, p); else sum0 = __fadd2_rn(sum0, p);
             pk[z] = pack2<BF16>(p.x, p.y);
-            const float2 r2 = unpack2<BF16>(pk[z]);
-            if (z & 1) rounded1 = __fadd2_rn(rounded1, r2); else rounded0 = __fadd2_rn(rounded0, r2);
+            if (z & 1) add_rounded<BF16>(rounded1, pk[z]); else add_rounded<BF16>(rounded0, pk[z]);
           }
           tmem_st32(place, pk);
           if (pending) {  // the sums given at the end of the last shared tile
@@ -891,59 +899,88 @@ __global__ void __launch_bounds__(CH_NT, 1)
   if (t == 0 && *failed && a.error_word) atomicOr(a.error_word, Q3S_DECERR_WAIT);
 }
 
-// Joins the parts of the items that were cut, a warp a query row; blocks behind
-// those write 0 and -inf for the tokens that no item has (of no row, or that see nothing).
+// ROWS query rows of a cut item, STEP apart, by one warp, D / 32 dims a lane: PARTS of their parts requested at a time, of all rows together.
+template <int D, bool BF16, int ROWS, int PARTS, int STEP>
+Q3S_DEV void chunk_join_rows(const ChunkArgs& c, const ChunkCut& k, int r0, int rows, int lane) {
+  constexpr int E = D / 32;
+  const AttnArgs& a = c.a;
+  float acc[ROWS][E], m[ROWS], l[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    m[i] = -INFINITY, l[i] = 0.0f;
+#pragma unroll
+    for (int x = 0; x < E; ++x) acc[i][x] = 0.0f;
+  }
+  for (int p = 0; p < k.parts; p += PARTS) {
+    float y[PARTS][ROWS][E];
+    float2 ml[PARTS][ROWS];
+#pragma unroll
+    for (int j = 0; j < PARTS; ++j) {
+      const int64_t slot = static_cast<int64_t>(p + j == 0 ? k.slot : 2 * (k.cta + p + j)) * c.slot_rows;
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        ml[j][i] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+        for (int x = 0; x < E; ++x) y[j][i][x] = 0.0f;
+        const int r = r0 + i * STEP;
+        if (p + j < k.parts && r < rows) {
+          ml[j][i] = c.part_ml[slot + r];
+          const float* src = c.part_o + (slot + r) * D + lane * E;
+          if constexpr (E == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(src);
+            y[j][i][0] = f.x, y[j][i][1] = f.y, y[j][i][2] = f.z, y[j][i][3] = f.w;
+          } else {
+            const float2 f = *reinterpret_cast<const float2*>(src);
+            y[j][i][0] = f.x, y[j][i][1] = f.y;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < PARTS; ++j)
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const float nm = fmaxf(m[i], ml[j][i].x), base = nm == -INFINITY ? 0.0f : nm;
+        const float wm = ex2(m[i] - base), wp = ex2(ml[j][i].x - base);
+        m[i] = nm;
+        l[i] = l[i] * wm + wp * ml[j][i].y;
+#pragma unroll
+        for (int x = 0; x < E; ++x) acc[i][x] = acc[i][x] * wm + wp * y[j][i][x];
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = r0 + i * STEP;
+    if (r >= rows) continue;
+    const int token = k.token + r / a.G, head = k.h * a.G + r % a.G;
+    const float inv = chunk_inverse(l[i]);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + token * a.ot + head * a.oh + lane * E);
+#pragma unroll
+    for (int x = 0; x < E; x += 2) dst[x / 2] = pack2<BF16>(acc[i][x] * inv, acc[i][x + 1] * inv);
+    if (a.lse && lane == 0) a.lse[static_cast<int64_t>(token) * a.Hq + head] = chunk_lse(m[i], l[i]);
+  }
+}
+
+// Joins the parts of the items that were cut, a warp four query rows at once (most items have two parts; of one
+// with more a warp takes a row and eight parts at once); blocks behind those write 0 and -inf for the tokens that
+// no item has (of no row, or that see nothing).  Bound by latency: a row after the other took 15 us of the 2 rows' 245.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(CH_JOIN_NT) attn_chunk_join_kernel(const ChunkArgs c, int join_blocks, int blocks_each) {
-  constexpr int E = D / 32, AHEAD = 4;
   const AttnArgs& a = c.a;
   const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31, block = static_cast<int>(blockIdx.x);
+  constexpr int WARPS = CH_JOIN_NT / 32;
   grid_wait();
   grid_release();
   if (block < join_blocks) {
     const ChunkCut k = c.cuts[block / blocks_each];
     if (k.parts == 0) return;
-    const int rows = k.tokens * a.G, row0 = (block % blocks_each) * CH_JOIN_ROWS;
-    for (int r = row0 + w; r < min(rows, row0 + CH_JOIN_ROWS); r += CH_JOIN_NT / 32) {
-      float acc[E], m = -INFINITY, l = 0.0f;
-#pragma unroll
-      for (int x = 0; x < E; ++x) acc[x] = 0.0f;
-      for (int i = 0; i < k.parts; i += AHEAD) {
-        float y[AHEAD][E];
-        float2 ml[AHEAD];
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-          ml[j] = make_float2(-INFINITY, 0.0f);
-          if (i + j < k.parts) {
-            const int64_t at = static_cast<int64_t>(i + j == 0 ? k.slot : 2 * (k.cta + i + j)) * c.slot_rows + r;
-            ml[j] = c.part_ml[at];
-            const float* src = c.part_o + at * D + lane * E;
-            if constexpr (E == 4) {
-              const float4 f = *reinterpret_cast<const float4*>(src);
-              y[j][0] = f.x, y[j][1] = f.y, y[j][2] = f.z, y[j][3] = f.w;
-            } else {
-              const float2 f = *reinterpret_cast<const float2*>(src);
-              y[j][0] = f.x, y[j][1] = f.y;
-            }
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-          if (i + j >= k.parts) break;
-          const float nm = fmaxf(m, ml[j].x), base = nm == -INFINITY ? 0.0f : nm;
-          const float wm = ex2(m - base), wp = ex2(ml[j].x - base);
-          m = nm;
-          l = l * wm + wp * ml[j].y;
-#pragma unroll
-          for (int x = 0; x < E; ++x) acc[x] = acc[x] * wm + wp * y[j][x];
-        }
-      }
-      const int token = k.token + r / a.G, head = k.h * a.G + r % a.G;
-      const float inv = chunk_inverse(l);
-      uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + token * a.ot + head * a.oh + lane * E);
-#pragma unroll
-      for (int x = 0; x < E; x += 2) dst[x / 2] = pack2<BF16>(acc[x] * inv, acc[x + 1] * inv);
-      if (a.lse && lane == 0) a.lse[static_cast<int64_t>(token) * a.Hq + head] = chunk_lse(m, l);
+    const int row0 = (block % blocks_each) * CH_JOIN_ROWS, rows = min(k.tokens * a.G, row0 + CH_JOIN_ROWS);
+    static_assert(CH_JOIN_ROWS == 4 * WARPS, "a warp's rows");
+    if (row0 + w >= rows) return;
+    if (k.parts <= 2) {
+      chunk_join_rows<D, BF16, 4, 2, WARPS>(c, k, row0 + w, rows, lane);
+    } else {
+      for (int r = row0 + w; r < rows; r += WARPS) chunk_join_rows<D, BF16, 1, 8, WARPS>(c, k, r, rows, lane);
     }
     return;
   }
