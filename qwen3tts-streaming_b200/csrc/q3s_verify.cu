@@ -12,6 +12,7 @@
 #include "q3s_args.cuh"
 #include "q3s_decode.h"
 #include "q3s_device.cuh"
+#include "q3s_head.cuh"
 #include "q3s_pdl.cuh"
 #include "q3s_tma.cuh"
 
@@ -56,37 +57,42 @@ constexpr int VF_SLICE = 8192;  // entries of the vocabulary that a CTA takes, w
 constexpr double VF_BOUND = 1.0 / (1 << 18), VF_GAP = 1.0 / (1 << 22);
 
 // Beyond this |x c| its rounding is too coarse for the 32-bit sum to say anything.
-constexpr float VF_LARGE = 1048576.0f;
+constexpr int VF_LARGE = 1 << 20;
 
 // sum_v 2^(x_v c - k) over some entries, k an integer above their largest
-// x c (however large that is: no term overflows), with the largest logit and its
+// x c (however large that is: no term overflows; VF_NONE: only entries without a
+// probability), with the largest logit as a key that orders like it and its
 // lowest index.  A NaN among the entries makes the sum one; nothing else does
 // where the largest logit is finite.
 struct VerifyStat {
   double sum;
-  float k, best;
+  int k;
+  uint32_t best;
   int index;
 };
+constexpr int VF_NONE = -(1 << 30);
+Q3S_DEV VerifyStat verify_nothing() { return {0.0, VF_NONE, f2key(-INFINITY), 0x7fffffff}; }
 
 // 2^d for an integer d <= 0 (0 below -1000), exactly.
-Q3S_DEV double pow2_int(float d) { return d < -1000.0f ? 0.0 : __hiloint2double((1023 + static_cast<int>(d)) << 20, 0); }
+Q3S_DEV double pow2_int(int d) { return d < -1000 ? 0.0 : __hiloint2double((1023 + d) << 20, 0); }
 
-Q3S_DEV VerifyStat verify_join(const VerifyStat& a, const VerifyStat& b) {
+// All lanes' together, in every lane.
+Q3S_DEV VerifyStat verify_join(const VerifyStat& s) {
   VerifyStat r;
-  r.k = fmaxf(a.k, b.k);
-  // -inf: nothing there, or only entries that have no probability (sum 0)
-  r.sum = a.sum * (a.k == r.k ? 1.0 : pow2_int(a.k - r.k)) + b.sum * (b.k == r.k ? 1.0 : pow2_int(b.k - r.k));
-  const bool first = a.best > b.best || (a.best == b.best && a.index < b.index);
-  r.best = first ? a.best : b.best;
-  r.index = first ? a.index : b.index;
+  r.k = __reduce_max_sync(FULL, s.k);
+  r.best = __reduce_max_sync(FULL, s.best);
+  r.index = static_cast<int>(__reduce_min_sync(FULL, s.best == r.best ? static_cast<uint32_t>(s.index) : 0x7fffffffu));
+  r.sum = s.sum * pow2_int(s.k - r.k);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) r.sum += __shfl_xor_sync(FULL, r.sum, d);
   return r;
 }
-Q3S_DEV VerifyStat verify_shfl_xor(const VerifyStat& a, int d) {
-  return {__shfl_xor_sync(FULL, a.sum, d), __shfl_xor_sync(FULL, a.k, d), __shfl_xor_sync(FULL, a.best, d),
-          __shfl_xor_sync(FULL, a.index, d)};
+Q3S_DEV VerifyStat verify_shfl(const VerifyStat& s, int lane) {
+  return {__shfl_sync(FULL, s.sum, lane), __shfl_sync(FULL, s.k, lane), __shfl_sync(FULL, s.best, lane), __shfl_sync(FULL, s.index, lane)};
 }
 // Whether the logits have a distribution.
-Q3S_DEV bool verify_defined(const VerifyStat& s) { return s.sum == s.sum && fabsf(s.best) < INFINITY; }
+Q3S_DEV bool verify_defined(const VerifyStat& s) { return s.sum == s.sum && fabsf(key2f(s.best)) < INFINITY; }
+
 // 2^(t / 32) for t <= 0 in 64 bits, by a whole warp: with t = 32 n + j + f, j in
 // [0, 32) and |f| <= 1/2, 2^n 2^(j/32) e^z, z = f ln 2 / 32, where 2^(j/32) is
 // lane j's `root` and e^z its series up to z^5 / 120 (|z| < 0.0109: off by
@@ -111,9 +117,15 @@ Q3S_DEV float vf_ex2(float x) {
   return r;
 }
 
+// A thread's sums on the way.
+struct VerifyRun {
+  double sum;
+  float k, best;  // k: -infinity before the first entry with a probability
+  int index;
+};
 // N neighbouring entries, the first at index v.
 template <int N>
-Q3S_DEV void verify_take(VerifyStat& s, const float (&x)[N], int v, float c) {
+Q3S_DEV void verify_take(VerifyRun& s, const float (&x)[N], int v, float c) {
   float top = x[0];
 #pragma unroll
   for (int e = 1; e < N; ++e) top = fmaxf(top, x[e]);
@@ -125,7 +137,7 @@ Q3S_DEV void verify_take(VerifyStat& s, const float (&x)[N], int v, float c) {
     s.index = v + at;
     const float y = top * c, k = ceilf(fmaf(fabsf(y), 2.384185791015625e-07f, y));  // 2^-22: above the rounding of y
     if (k > s.k) {
-      s.sum = s.k == -INFINITY ? 0.0 : s.sum * pow2_int(fmaxf(s.k - k, -2000.0f));
+      s.sum = s.k == -INFINITY ? 0.0 : s.sum * pow2_int(static_cast<int>(fmaxf(s.k - k, -2000.0f)));
       s.k = k;
     }
   }
@@ -139,22 +151,25 @@ Q3S_DEV void verify_take(VerifyStat& s, const float (&x)[N], int v, float c) {
     for (int i = 0; i + w < N; i += 2 * w) e[i] += e[i + w];
   s.sum += static_cast<double>(e[0]);  // a NaN among the entries stays one
 }
+Q3S_DEV VerifyStat verify_stat(const VerifyRun& s) {
+  // (beyond VF_LARGE k only says that it is)
+  return {s.sum, s.k == -INFINITY ? VF_NONE : static_cast<int>(fminf(fmaxf(s.k, -1.0e9f), 1.0e9f)), f2key(s.best), s.index};
+}
 
+// A 16-byte vector of logits, as fp32.
 template <typename T>
 struct VerifyVec;
 template <>
 struct VerifyVec<float> {
   static constexpr int N = 4;
-  Q3S_DEV static void load(const float* p, float (&x)[4]) {
-    const float4 f = *reinterpret_cast<const float4*>(p);
-    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+  Q3S_DEV static void widen(const uint4& f, float (&x)[4]) {
+    x[0] = __uint_as_float(f.x), x[1] = __uint_as_float(f.y), x[2] = __uint_as_float(f.z), x[3] = __uint_as_float(f.w);
   }
 };
 template <>
 struct VerifyVec<__nv_bfloat16> {
   static constexpr int N = 8;
-  Q3S_DEV static void load(const __nv_bfloat16* p, float (&x)[8]) {
-    const uint4 f = *reinterpret_cast<const uint4*>(p);
+  Q3S_DEV static void widen(const uint4& f, float (&x)[8]) {
     const uint32_t w[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
@@ -163,8 +178,7 @@ struct VerifyVec<__nv_bfloat16> {
 template <>
 struct VerifyVec<__half> {
   static constexpr int N = 8;
-  Q3S_DEV static void load(const __half* p, float (&x)[8]) {
-    const uint4 f = *reinterpret_cast<const uint4*>(p);
+  Q3S_DEV static void widen(const uint4& f, float (&x)[8]) {
     const uint32_t w[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -176,9 +190,9 @@ struct VerifyVec<__half> {
 
 // One row's shared state of a CTA.
 struct VerifyShared {
-  VerifyStat warp[VF_WARPS];
-  VerifyStat part[VF_WARPS][VF_MAX_CLUSTER];  // [place][CTA of the cluster], written by that CTA
-  double sums[VF_MAX_CLUSTER * VF_WARPS];     // a pass's sums, CTA by CTA and warp by warp
+  VerifyStat part[VF_MAX_CLUSTER][VF_WARPS];  // [CTA of the cluster][warp], written by that CTA
+  VerifyStat place_stat[VF_WARPS];            // of a place
+  double sums[2][VF_MAX_CLUSTER * VF_WARPS];  // a pass's sums, CTA by CTA and warp by warp; passes take turns
   VerifyStat stat;                            // of the place that is being decided
   int verdict, place, winner;
   double before, aim;
@@ -193,7 +207,7 @@ struct VerifyShared {
 // decided again from a 64-bit sum.  Then the place where the row stops is drawn from: each warp sums its
 // neighbouring entries in 64 bits, the sums meet, and the one warp whose entries reach u * total looks for the entry.
 template <typename T>
-__global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(VF_NT, 2) verify_kernel(const VerifyArgs a) {
   __shared__ VerifyShared sh;
   extern __shared__ double held[];  // [slice], if they are held
   cg::cluster_group cluster = cg::this_cluster();
@@ -203,6 +217,7 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
   auto sync = [&]() {
     if (ctas > 1) cluster.sync(); else __syncthreads();
   };
+  if (ctas > 1) cluster_arrive_relaxed();  // this CTA has begun: its shared memory may be written (waited for before that)
   grid_wait();
   grid_release();
 
@@ -227,6 +242,7 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
     if (without) sh.refused = 1;  // every writer writes 1
     __syncthreads();
   }
+  if (ctas > 1) cluster_wait();
   if (n == 0 || sh.refused) {  // the same in all CTAs of the cluster
     if (rank == 0) {
       for (int i = t; i < n; i += VF_NT) a.tokens_out[t0 + i] = -1;
@@ -238,6 +254,7 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
     }
     return;
   }
+  const double row_uniform = static_cast<double>(a.uniforms[t0]);
   const float heat = a.temperature ? a.temperature[b] : a.temperature_default;
   const bool greedy = !(heat >= 7.888609052210118e-31f);  // 2^-100
   const float c = greedy ? 1.0f : 1.4426950408889634f / heat;
@@ -252,24 +269,22 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
   // e(v) = 2^((x_v - largest) log2(e) / temperature); a whole warp calls
   auto weight = [&](float x, double best) { return vf_exp2_64((static_cast<double>(x) - best) * steep, root); };
   // the warps' sums meet in every CTA
+  int pass = 0;
   auto meet = [&](double s) {
 #pragma unroll
     for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(FULL, s, d);
-    sync();  // the sums of the pass before have been read
-    for (int r = lane; r < ctas; r += 32) cluster.map_shared_rank(&sh, r)->sums[rank * VF_WARPS + w] = s;
+    ++pass;  // (the sums of the pass before the last were read before the last one's barrier)
+    if (lane < ctas) cluster.map_shared_rank(&sh, lane)->sums[pass & 1][rank * VF_WARPS + w] = s;
     sync();
     double total = 0.0;
-    for (int i = 0; i < ctas * VF_WARPS; i += 32) {
-      double x = i + lane < ctas * VF_WARPS ? sh.sums[i + lane] : 0.0;
+    for (int i = lane; i < ctas * VF_WARPS; i += 32) total += sh.sums[pass & 1][i];
 #pragma unroll
-      for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(FULL, x, d);
-      total += x;
-    }
+    for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(FULL, total, d);
     return total;
   };
   // f(v, x_v) of all entries of this warp in turn, x_v requested AHEAD at a time (a float of `from`, -infinity past the end); f is called by the whole warp
   auto each = [&](const auto* from, auto f) {
-    constexpr int AHEAD = 8;
+    constexpr int AHEAD = 4;
     for (int v = w0; v < w1; v += 32 * AHEAD) {
       float x[AHEAD];
 #pragma unroll
@@ -285,28 +300,36 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
   const int group = VF_WARPS / a.places;
   for (int first = 0;; first += a.places) {
     const int mine = first + w / group;
-    VerifyStat s = {0.0, -INFINITY, -INFINITY, 0x7fffffff};
+    VerifyRun run = {0.0, -INFINITY, -INFINITY, 0x7fffffff};
     if (mine < n) {
-      constexpr int N = VerifyVec<T>::N;
+      constexpr int N = VerifyVec<T>::N, AHEAD = 4;
       const T* x = logits + (t0 + mine) * a.logits_stride;
       const int lanes = group * 32, l = (w % group) * 32 + lane;
-      // single entries up to the first 16-byte boundary, vectors, single entries
+      // single entries up to the first 16-byte boundary, vectors (several requested at a time), single entries
       const int head = static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(x + v0) & 15)) & 15) / sizeof(T));
       const int vec0 = min(v0 + head, v1), vecs = (v1 - vec0) / N;
       if (l < vec0 - v0) {
         const float one[1] = {static_cast<float>(x[v0 + l])};
-        verify_take<1>(s, one, v0 + l, c);
+        verify_take<1>(run, one, v0 + l, c);
       }
-#pragma unroll 4
-      for (int i = l; i < vecs; i += lanes) {
-        float y[N];
-        VerifyVec<T>::load(x + vec0 + i * N, y);
-        verify_take<N>(s, y, vec0 + i * N, c);
+      const uint4* vectors = reinterpret_cast<const uint4*>(x + vec0);
+      for (int i = l; i < vecs; i += AHEAD * lanes) {
+        uint4 f[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+          if (i + j * lanes < vecs) f[j] = vectors[i + j * lanes];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+          if (i + j * lanes < vecs) {
+            float y[N];
+            VerifyVec<T>::widen(f[j], y);
+            verify_take<N>(run, y, vec0 + (i + j * lanes) * N, c);
+          }
       }
       const int rest = vec0 + vecs * N + l;
       if (rest < v1) {
         const float one[1] = {static_cast<float>(x[rest])};
-        verify_take<1>(s, one, rest, c);
+        verify_take<1>(run, one, rest, c);
       }
     }
     // what warp 0 decides with: the draft behind place first + lane
@@ -321,27 +344,32 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
         draft_x = static_cast<float>(logits[(at - 1) * a.logits_stride + draft]);
       }
     }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) s = verify_join(s, verify_shfl_xor(s, d));
-    if (lane == 0) sh.warp[w] = s;
-    sync();  // and the parts of the turn before have been read
-    if (t < a.places) {
-      VerifyStat p = sh.warp[t * group];
-      for (int i = 1; i < group; ++i) p = verify_join(p, sh.warp[t * group + i]);
-      for (int r = 0; r < ctas; ++r) cluster.map_shared_rank(&sh, r)->part[t][rank] = p;
-    }
+    const VerifyStat warp_stat = verify_join(verify_stat(run));
+    if (first > 0) sync();  // the parts of the turn before have been read
+    if (lane < ctas) cluster.map_shared_rank(&sh, lane)->part[rank][w] = warp_stat;
     sync();
+    if (w < a.places) {  // a warp joins the parts of a place: of `group` warps of every CTA, up to four a lane
+      VerifyStat p = verify_nothing();
+      for (int i = 0; i < ctas * group; i += 32) {
+        VerifyStat o = verify_nothing();
+        if (i + lane < ctas * group) o = sh.part[(i + lane) / group][w * group + (i + lane) % group];
+        o = verify_join(o);
+        if (lane == i / 32) p = o;
+      }
+      p = ctas * group > 32 ? verify_join(p) : verify_shfl(p, 0);
+      if (lane == 0) sh.place_stat[w] = p;
+    }
+    __syncthreads();
     int from = 0;  // places of this turn that are decided
     bool stop = false;
     while (!stop) {
       if (w == 0) {
         const int i = first + lane;
         const bool live = lane < a.places && i < n;
-        VerifyStat p = {0.0, -INFINITY, -INFINITY, 0x7fffffff};
+        VerifyStat p = verify_nothing();
         int verdict = 1;  // 0: the row stops here, 1: the draft holds, 2: too close
         if (live) {
-          p = sh.part[lane][0];
-          for (int r = 1; r < ctas; ++r) p = verify_join(p, sh.part[lane][r]);
+          p = sh.place_stat[lane];
           verdict = 0;
           if (i + 1 < n && verify_defined(p) && draft >= 0 && draft < a.V) {
             if (greedy) {
@@ -350,7 +378,7 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
               const double y = static_cast<double>(draft_x) * static_cast<double>(c) - static_cast<double>(p.k);
               const double left = aim * p.sum, right = exp2(y);
               const double error = (VF_BOUND - VF_GAP * fmin(y, 0.0)) * (left + right);
-              verdict = !(p.sum > 0.0) || fabsf(p.k) > VF_LARGE ? 2
+              verdict = !(p.sum > 0.0) || abs(p.k) > VF_LARGE ? 2
                         : !(right > 0.0)                        ? 0
                         : fabs(left - right) <= error           ? 2
                                                                 : left < right;
@@ -374,7 +402,7 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
         stop = true;
       } else {
         const T* x = logits + (t0 + place) * a.logits_stride;
-        const double best = static_cast<double>(sh.stat.best);
+        const double best = static_cast<double>(key2f(sh.stat.best));
         double sum = 0.0;
         each(x, [&](int, float y) { sum += weight(y, best); });
         const double total = meet(sum);
@@ -411,7 +439,7 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
     if (rank == 0 && t == 0) finish(stat.index == 0x7fffffff ? 0 : stat.index);
     return;
   }
-  const double best = static_cast<double>(stat.best);
+  const double best = static_cast<double>(key2f(stat.best));
   const float* q = a.probs && place + 1 < n ? a.probs + (t0 + place + 1) * a.probs_stride : nullptr;
   const int gone = place + 1 < n && !a.probs && draft >= 0 && draft < a.V ? static_cast<int>(draft) : -1;  // a draft that was certain
   if (q)  // on its way while the weights are taken
@@ -457,31 +485,38 @@ __global__ void __launch_bounds__(VF_NT) verify_kernel(const VerifyArgs a) {
     return minus && v < w1 ? fmax(e - static_cast<double>(q[v]) * mass, 0.0) : e;
   };
   if (w == 0) {  // the warp (of all CTAs') whose entries reach u * total: its number, and the sum before it
-    const double aim = static_cast<double>(a.uniforms[t0]) * total;
+    const double aim = row_uniform * total;
     const int warps = ctas * VF_WARPS;
-    double carry = 0.0, before = 0.0;
-    int winner = -1, last = 0;  // last: the last warp with a sum
-    for (int i = 0; i < warps; i += 32) {
-      const double s = i + lane < warps ? sh.sums[i + lane] : 0.0;
-      double up = s;
+    constexpr int EACH = VF_MAX_CLUSTER * VF_WARPS / 32;  // neighbouring sums of a lane
+    double at[EACH], up = 0.0;
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const double o = __shfl_up_sync(FULL, up, d);
-        if (lane >= d) up += o;
-      }
-      const double at = carry + up;
-      const double prior = __shfl_up_sync(FULL, at, 1);
-      const unsigned over = __ballot_sync(FULL, s > 0.0 && at > aim), some = __ballot_sync(FULL, s > 0.0);
-      if (winner < 0 && over) {
-        const int src = __ffs(over) - 1;
-        winner = i + src;
-        before = src ? __shfl_sync(FULL, prior, src) : carry;
-      }
-      if (some) last = i + 31 - __clz(some);
-      carry = __shfl_sync(FULL, at, 31);
+    for (int j = 0; j < EACH; ++j) {
+      at[j] = lane * EACH + j < warps ? sh.sums[pass & 1][lane * EACH + j] : 0.0;
+      up += at[j];
     }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const double o = __shfl_up_sync(FULL, up, d);
+      if (lane >= d) up += o;
+    }
+    double edge = __shfl_up_sync(FULL, up, 1), mine_before = 0.0;
+    if (lane == 0) edge = 0.0;
+    int mine = -1, last = -1;  // this lane's first sum that reaches the aim, its last that is not 0
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      if (at[j] > 0.0) {
+        last = lane * EACH + j;
+        if (mine < 0 && edge + at[j] > aim) mine = last, mine_before = edge;
+      }
+      edge += at[j];
+    }
+    const unsigned over = __ballot_sync(FULL, mine >= 0), some = __ballot_sync(FULL, last >= 0);
+    const int src = over ? __ffs(over) - 1 : 0;
+    const int winner = over ? __shfl_sync(FULL, mine, src) : -1;
+    const double before = __shfl_sync(FULL, mine_before, src);
+    last = __shfl_sync(FULL, last, some ? 31 - __clz(some) : 0);
     if (lane == 0) {
-      sh.winner = winner < 0 ? last : winner;
+      sh.winner = winner < 0 ? max(last, 0) : winner;
       sh.before = before;
       sh.aim = winner < 0 ? INFINITY : aim;  // rounding left the aim at or above the sum: the last entry that has any
     }
@@ -574,8 +609,12 @@ extern "C" q3s_status q3s_verify_drafts(const q3s_verify_drafts_desc* d, void* s
   a.rejected = d->rejected;
   a.next_ids = d->next_ids;
   a.error_word = d->error_word;
+  // CTAs of a row: so many that each holds its slice; and more, down to slices of 1024 entries, while
+  // all rows' fit the SMs together, two each.  One CTA against eight, 8192 entries: 1 row 19.2 against 9.8 us,
+  // 16 rows 17.8 against 10.7, 64 rows 18.2 against 21.9, 200 rows 24.7 against 60.9.
   int ctas = 1;
   while (ctas < q3s::VF_MAX_CLUSTER && static_cast<int64_t>(ctas) * q3s::VF_SLICE < a.V) ctas *= 2;
+  while (ctas < q3s::VF_MAX_CLUSTER && ctas * 1024 < a.V && static_cast<int64_t>(a.B) * ctas <= q3s::sm_count()) ctas *= 2;
   a.slice = ((a.V + ctas - 1) / ctas + 31) & ~31;
   a.held = a.slice <= q3s::VF_SLICE;
   // as many places at once as a row of the batch has on average
