@@ -27,8 +27,7 @@ constexpr int CH_SEGS = 64;     // segments of a CTA's range that are listed at 
 // Registers a thread: a softmax thread holds a row of 128 scores.  Launched with 168 a thread, which is what the shares add up to.
 constexpr int CH_REGS_SOFTMAX = 184, CH_REGS_OTHER = 136;
 static_assert(2 * CH_REGS_SOFTMAX + CH_REGS_OTHER <= 3 * 168, "what the CTA is launched with");
-constexpr int CH_START = 6;     // cost of an item's start and end, where a step of two tiles costs 3 and one of one tile 2
-constexpr int CH_MAX_STEP = 3;  // the largest cost of a step
+constexpr int CH_START = 2;     // cost of an item's start and end, in steps (2 rows of 4096 tokens: 0.7 261 us, 2 248, 4 251, 8 264)
 constexpr int CH_JOIN_NT = 256, CH_JOIN_ROWS = 32;  // threads and query rows of a CTA of the joining kernel
 
 constexpr int CH_UNSEEN = -0x7fffffff - 1;  // in place of how many own tokens a query sees: there is none, or it sees nothing
@@ -319,10 +318,9 @@ __global__ void __launch_bounds__(CH_NT, 1)
   }
 
   // ---- the list's length, and this CTA's range of it ----
-  auto step_cost = [&](int m) { return m > c.per_tile ? 3 : 2; };
   auto item_cost = [&](const ChunkRow& x, int i0) {  // of tokens [i0, i0 + pair), for one head; 0: nothing is seen
-    const int m = min(pair, x.n - i0), steps = chunk_steps(c, x, i0, m).y;
-    return steps ? CH_START + static_cast<long long>(steps) * step_cost(m) : 0ll;
+    const int steps = chunk_steps(c, x, i0, min(pair, x.n - i0)).y;
+    return steps ? CH_START + static_cast<long long>(steps) : 0ll;
   };
   auto warp_scan = [&](long long up) {
 #pragma unroll
@@ -369,8 +367,8 @@ __global__ void __launch_bounds__(CH_NT, 1)
   all = 0;
 #pragma unroll
   for (int i = 0; i < CH_NT / 32; ++i) all += s_sum[i];
-  // as many CTAs as every range holds the start of a step for
-  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), max(div_nonneg(all, CH_MAX_STEP), 1ll)));
+  // (a range within an item's steps holds at least one)
+  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), max(all, 1ll)));
   const bool works = all > 0 && cta < ctas;
   if (works) {  // the row in which the range starts
     const long long range0 = ChunkCutting{all, ctas}.start(cta);
@@ -433,12 +431,10 @@ __global__ void __launch_bounds__(CH_NT, 1)
       const int i0 = p * pair, m = min(pair, x.n - i0);
       int2 steps = make_int2(0, 0);
       if (item < items) steps = chunk_steps(c, x, i0, m);
-      const int each = step_cost(m);
-      const long long cost = steps.y ? CH_START + static_cast<long long>(steps.y) * each : 0;
+      const long long cost = steps.y ? CH_START + static_cast<long long>(steps.y) : 0;
       const long long up = warp_scan(cost), start = k.at + up - cost;
       auto steps_before = [&](long long y) {  // that start before y
-        const long long past = min(max(y - start - CH_START, 0ll), static_cast<long long>(steps.y) * each);
-        return static_cast<int>(div_nonneg(past + each - 1, each));
+        return static_cast<int>(min(max(y - start - CH_START, 0ll), static_cast<long long>(steps.y)));
       };
       const int lo = steps_before(range0), hi = steps_before(range1);
       const unsigned live = __ballot_sync(FULL, lo < hi);
@@ -448,7 +444,7 @@ __global__ void __launch_bounds__(CH_NT, 1)
         const int slot = whole ? -1 : 2 * cta + (k.written + rank > 0 ? 1 : 0);
         s_list[n + rank] = {k.b, h, x.t0 + i0, m, x.len - x.n + i0 + 1, x.len, steps.x + lo, hi - lo, slot};
         if (lo == 0 && !whole)
-          c.cuts[cta] = {cut.cta_of(start + CH_START + static_cast<long long>(steps.y - 1) * each) - cta + 1, slot, cta, h, x.t0 + i0, m};
+          c.cuts[cta] = {cut.cta_of(start + CH_START + steps.y - 1) - cta + 1, slot, cta, h, x.t0 + i0, m};
       }
       k.cut |= __any_sync(FULL, lo < hi && lo == 0 && !whole);
       k.written += __popc(live);
