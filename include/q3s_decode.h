@@ -284,10 +284,11 @@ q3s_status q3s_rotary(const q3s_rotary_desc* desc, void* stream);
  * [query_offsets[b], query_offsets[b+1])) stands at position
  *   p = prefix_length + lengths[b] - n + i
  * and sees the keys at positions (p - window, p], all up to p where window is 0.
- * Otherwise as q3s_prefix_attention: the same result without a window, computed
- * by a kernel whose tiles are 128 query rows of one row of the batch and not 16,
- * for chunks from some tens of query rows on.  Probabilities are rounded to the cache's type for the product
- * with v, as described there for the prefix of a large batch. */
+ * Otherwise as q3s_prefix_attention: the same without a window, computed by a
+ * kernel whose tiles are 128 query rows of one row of the batch and not 16 (with
+ * few query rows and no window by q3s_prefix_attention's own).  Probabilities
+ * are rounded to the cache's type for the product with v, as described there for
+ * the prefix of a large batch. */
 #define Q3S_MAX_CHUNK_GROUP 128 /* query heads per key/value head */
 
 typedef struct q3s_chunk_attention_desc {

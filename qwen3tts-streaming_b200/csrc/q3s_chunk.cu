@@ -64,6 +64,56 @@ q3s_status check_sizes(const q3s_chunk_attention_desc* d) {
   return Q3S_OK;
 }
 
+// Whether the kernels of q3s_prefix_attention, whose tiles are 16 query rows, are the faster ones: few query rows, together or
+// a row of the batch, and no window.  They against the kernel here, us, 8 key/value heads of 128, query rows a row of the
+// batch: 1 row of 8000 keys, 64: 31 and 35, 128: 43 and 43, 256: 78 and 49; 1 row of 200 keys, 128: 14 and 21, 512: 24 and 28;
+// 16 rows of 2000 keys, 16: 33 and 38, 32: 49 and 40; 64 rows of 1000 keys, 16: 52 and 60, 32: 83 and 61; 16 rows of 8000
+// keys, 8: 81 and 79, 16: 86 and 82; 4 heads of 64, 16 rows of 2000 keys, 16: 15 and 24, 64: 29 and 27.
+bool few_queries(const q3s_chunk_attention_desc* d) {
+  const int64_t G = d->q_heads / d->kv_heads;
+  return d->window == 0 && G <= Q3S_MAX_QUERY_GROUP && d->tokens * G <= std::max<int64_t>(160, static_cast<int64_t>(d->batch) * 20);
+}
+q3s_prefix_attention_desc few_queries_desc(const q3s_chunk_attention_desc* d) {
+  q3s_prefix_attention_desc p = {};
+  p.struct_size = sizeof(p);
+  p.batch = d->batch;
+  p.tokens = d->tokens;
+  p.q_heads = d->q_heads;
+  p.kv_heads = d->kv_heads;
+  p.dim = d->dim;
+  p.block_size = d->block_size;
+  p.blocks = d->blocks;
+  p.elem = d->elem;
+  p.max_blocks = d->max_blocks;
+  p.prefix_length = d->prefix_length;
+  p.scale = d->scale;
+  p.q = d->q;
+  p.q_token_stride = d->q_token_stride;
+  p.q_head_stride = d->q_head_stride;
+  p.k_cache = d->k_cache;
+  p.v_cache = d->v_cache;
+  p.k_block_stride = d->k_block_stride;
+  p.k_head_stride = d->k_head_stride;
+  p.k_place_stride = d->k_place_stride;
+  p.v_block_stride = d->v_block_stride;
+  p.v_head_stride = d->v_head_stride;
+  p.v_place_stride = d->v_place_stride;
+  p.query_offsets = d->query_offsets;
+  p.block_table = d->block_table;
+  p.block_table_stride = d->block_table_stride;
+  p.lengths = d->lengths;
+  p.prefix_blocks = d->prefix_blocks;
+  p.out = d->out;
+  p.out_token_stride = d->out_token_stride;
+  p.out_head_stride = d->out_head_stride;
+  p.lse = d->lse;
+  p.workspace = d->workspace;
+  p.workspace_bytes = d->workspace_bytes;
+  p.error_word = d->error_word;
+  p.slot_map = d->slot_map;
+  return p;
+}
+
 template <int D, bool BF16>
 cudaError_t launch(const q3s::ChunkArgs& c, const Layout& l, cudaStream_t st) {
   auto kernel = q3s::attn_chunk_kernel<D, BF16>;
@@ -87,6 +137,10 @@ extern "C" q3s_status q3s_chunk_attention_workspace(const q3s_chunk_attention_de
   const q3s_status s = check_sizes(d);
   if (s != Q3S_OK) return s;
   if (!bytes) return q3s::report(Q3S_ERR_INVALID_ARGUMENT, "q3s_chunk_attention_workspace: bytes is NULL");
+  if (few_queries(d)) {
+    const q3s_prefix_attention_desc p = few_queries_desc(d);
+    return q3s_prefix_attention_workspace(&p, bytes);
+  }
   *bytes = layout_of(d).bytes;
   return q3s::report(Q3S_OK, "");
 }
@@ -110,6 +164,15 @@ extern "C" q3s_status q3s_chunk_attention(const q3s_chunk_attention_desc* d, voi
                     d->k_head_stride, d->k_place_stride, d->v_block_stride, d->v_head_stride, d->v_place_stride})
     if (x % 8)
       return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_chunk_attention: strides must be multiples of 8 elements");
+  if (few_queries(d)) {
+    int64_t needed = 0;
+    const q3s_prefix_attention_desc p = few_queries_desc(d);
+    const q3s_status sized = q3s_prefix_attention_workspace(&p, &needed);
+    if (sized != Q3S_OK) return sized;
+    if (d->workspace_bytes >= needed) return q3s_prefix_attention(&p, stream);
+    return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_chunk_attention: workspace of %lld bytes, %lld needed",
+                  static_cast<long long>(d->workspace_bytes), static_cast<long long>(needed));
+  }
   const Layout l = layout_of(d);
   if (d->workspace_bytes < l.bytes)
     return report(Q3S_ERR_INVALID_ARGUMENT, "q3s_chunk_attention: workspace of %lld bytes, %lld needed",

@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(CH_NT, 1)
           const int token = tile * c.per_tile + row / a.G;
           if (row < c.per_tile * a.G && token < g.tokens && (!a.slot_map || a.slot_map[g.token + token] >= 0)) {
             own = g.i_key + token;
-            if (c.window) from = max(a.L + own - c.window, 0);
+            if (c.window) from = static_cast<int>(max(static_cast<int64_t>(a.L) + own - c.window, static_cast<int64_t>(0)));
           }
         }
         // The pieces that all rows of the warp see whole: [full0, full1) of the prefix, [full2, full3) of the row's own.

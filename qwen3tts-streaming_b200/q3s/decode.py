@@ -203,8 +203,9 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Arguments and results as there, up to 128 query heads for a key/value head,
     ``scale`` positive.  With ``window`` a query sees the ``window`` keys up to
     its own, counted over prefix and own tokens together.  Every row's query
-    tokens are taken in tiles of 128 (tokens times heads of a group), so it is
-    the faster one where rows have more than about 16 of them."""
+    tokens are taken in tiles of 128 (tokens times heads of a group); where they
+    are too few for that (about 20 a row of the batch), without a window, the
+    call is ``prefix_attention``'s."""
     out, lse = _op("chunk_attention")(q, k_cache, v_cache, query_offsets, block_table, lengths, prefix_blocks,
                                       prefix_length, window, scale, error_word, slot_map)
     return (out, lse) if return_lse else out

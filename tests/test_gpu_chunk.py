@@ -59,8 +59,14 @@ def run(c, **kw):
                                prefix_length=c["prefix"], return_lse=True, **kw)
 
 
+EVERYTHING = 2 ** 31 - 1  # a window that leaves nothing out: always the kernel with tiles of 128 query rows
+
+
 def check(c, window=0, scale=None, slot_map=None, k=None, v=None):
-    """`k`, `v`: what the definition reads in place of the caches."""
+    """`k`, `v`: what the definition reads in place of the caches.  Without a window both kernels: few queries go to the
+    one of prefix_attention otherwise."""
+    if window == 0:
+        check(c, EVERYTHING, scale, slot_map, k, v)
     D = c["q"].shape[2]
     err = torch.zeros(1, dtype=torch.int32, device=c["q"].device)
     out, lse = run(c, window=window, scale=scale, error_word=err, slot_map=slot_map)
@@ -158,10 +164,11 @@ def test_queries_without_a_slot_and_tokens_of_no_row(dev):
 def test_no_rows_no_tokens_no_keys(dev):
     c = make(dev, 11, [4], [0])
     z = dict(c, off=i32([0], dev), table=c["table"][:0], len=i32([], dev))
-    out, lse = run(z)
-    assert not out.any() and bool((lse == -float("inf")).all())
-    out, lse = run(dict(c, len=i32([0], dev)))
-    assert not out.any() and bool((lse == -float("inf")).all())
+    for window in (0, EVERYTHING):
+        out, lse = run(z, window=window)
+        assert not out.any() and bool((lse == -float("inf")).all())
+        out, lse = run(dict(c, len=i32([0], dev)), window=window)
+        assert not out.any() and bool((lse == -float("inf")).all())
     out, lse = run(dict(c, q=c["q"][:0], off=i32([0, 0], dev)))
     assert out.shape == (0, 8, 128) and lse.shape == (0, 8)
 
@@ -196,7 +203,7 @@ def test_values_that_a_query_does_not_see_do_not_reach_it(dev, news, owns, prefi
     where = (c["table"][0, last // 32], slice(None), last % 32)
     v[where] = value
     n = news[0]
-    out, lse = run(dict(c, k=k, v=v), window=window)
+    out, lse = run(dict(c, k=k, v=v), window=window or EVERYTHING)
     keep = torch.ones(out.shape[0], dtype=torch.bool, device=dev)
     keep[n - 1] = False
     want, want_lse, spread, mass = R.chunk_attention(c["q"], c["k"], c["v"], c["off"].tolist(), c["table"], c["len"].tolist(), c["shared"],
@@ -212,7 +219,7 @@ def test_peaked_scores_and_large_ones(dev):
     for factor in (8.0, 40.0):
         c = make(dev, 14, [150, 20], [300, 100], hq=4, hk=2)
         c["q"] = (c["q"].float() * factor).bfloat16()
-        out, _ = run(c)
+        out, _ = run(c, window=EVERYTHING)
         want, _, spread, mass = R.chunk_attention(c["q"], c["k"], c["v"], c["off"].tolist(), c["table"], c["len"].tolist(), c["shared"], 0,
                                                   128 ** -0.5)
         U = ROUNDOFF[torch.bfloat16]
@@ -226,26 +233,26 @@ def test_bad_block_ids_read_as_zeros(dev):
     bad = c["table"].clone()
     bad[0, 2], bad[0, 4] = 10 ** 6, -1
     err = torch.zeros(1, dtype=torch.int32, device=dev)
-    out, lse = run(dict(c, table=bad), error_word=err)
+    out, lse = run(dict(c, table=bad), error_word=err, window=EVERYTHING)
     assert int(err) == q3s.decode.DECERR_BLOCK_ID
     k, v = c["k"].clone(), c["v"].clone()
     for j in (2, 4):
         k[c["table"][0, j]] = 0
         v[c["table"][0, j]] = 0
-    want, want_lse = run(dict(c, k=k, v=v))
+    want, want_lse = run(dict(c, k=k, v=v), window=EVERYTHING)
     assert torch.equal(out, want) and torch.equal(lse, want_lse)
 
 
 def test_same_call_same_result_and_side_stream(dev):
     c = make(dev, 16, [300, 20, 7], [900, 100, 2000], hq=8, hk=4, prefix=100)
-    first = run(c)
+    first = run(c, window=EVERYTHING)
     for _ in range(5):
-        again = run(c)
+        again = run(c, window=EVERYTHING)
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
-        other = run(c)
+        other = run(c, window=EVERYTHING)
     s.synchronize()
     assert torch.equal(first[0], other[0])
 
@@ -267,27 +274,27 @@ def test_two_streams_at_once(dev):
 
 def test_captured_call_follows_the_lengths(dev):
     c = make(dev, 19, [40, 30], [10, 900], hq=4, hk=2, prefix=64)
-    run(c)
+    run(c, window=EVERYTHING)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        out, lse = run(c)
+        out, lse = run(c, window=EVERYTHING)
     for lengths, off in (([50, 930], [0, 40, 70]), ([45, 100], [0, 5, 70]), ([50, 930], [0, 0, 30])):
         c["len"].copy_(i32(lengths, dev))
         c["off"].copy_(i32(off, dev))
         graph.replay()
-        o, l = run(c)
+        o, l = run(c, window=EVERYTHING)
         assert torch.equal(out, o) and torch.equal(lse, l)
         check(c)
 
 
 def test_output_strides_through_the_c_abi(dev):
-    c = make(dev, 20, [40, 7], [100, 900], hq=4, hk=2)
+    c = make(dev, 20, [140, 7], [100, 900], hq=4, hk=2)
     want, want_lse = run(c)
     lib, L = q3s._lib.load(), q3s._lib
-    out = torch.zeros(47, 9, 136, dtype=torch.bfloat16, device=dev)
+    out = torch.zeros(147, 9, 136, dtype=torch.bfloat16, device=dev)
     d = L.ChunkAttentionDesc(
-        struct_size=C.sizeof(L.ChunkAttentionDesc), batch=2, tokens=47, q_heads=4, kv_heads=2, dim=128, block_size=16,
+        struct_size=C.sizeof(L.ChunkAttentionDesc), batch=2, tokens=147, q_heads=4, kv_heads=2, dim=128, block_size=16,
         blocks=c["k"].shape[0], elem=L.ELEM_BF16, max_blocks=c["table"].shape[1], scale=128 ** -0.5, q=c["q"].data_ptr(),
         q_token_stride=512, q_head_stride=128, k_cache=c["k"].data_ptr(), v_cache=c["v"].data_ptr(), query_offsets=c["off"].data_ptr(),
         block_table=c["table"].data_ptr(), block_table_stride=c["table"].stride(0), lengths=c["len"].data_ptr(), out=out.data_ptr(),
