@@ -11,6 +11,12 @@
 // with at most two cut items a CTA.  Each CTA derives its range from the device's lengths, so no host
 // plan is needed and a captured graph follows the lengths.  A whole item is written as
 // it ends; the parts (m, l, o) of a cut one are joined by the second kernel (q3s_attn.cuh has the mathematics).
+//
+// Measured on the device: 2 rows of 4096 tokens behind up to 3650 keys, 16 and 8 heads of 128, 246 us (920 TFLOP/s;
+// 280 us in a long run under the power limit); 13 rows of up to 700 tokens in a window of 512, 16 and 4 heads of 64,
+// 57 us; 48 rows of up to 9 tokens and 1533 keys, 32 and 8 heads of 128, 60 us (54 by the other kernels).  A long row is bound by the softmax and its hand-overs: two units
+// of 64 keys take 2100 clocks, of which the tensor cores run 1300.  Short rows are bound by what each
+// range and item begins and ends with (the list, the first loads, the sums taken out) and by the join, 7 to 15 us together.
 #pragma once
 
 #include <cuda.h>
@@ -234,7 +240,7 @@ Q3S_DEV float chunk_lse(float m, float l) { return l > 0.0f ? (m + log2f(l)) * 0
 // (16-bit, the second product's A operand), so that the scores of up to BUFFERS units are on their way or waiting:
 //   O(u) += P(u) V, then S(u + BUFFERS) = Q K^T into the place that this frees,
 // over the segments without a pause.  (With one place of 128 keys a warpgroup, its softmax waited for two products
-// at each step: 2 rows of 4096 tokens took 252 us.)  A warpgroup's O, D more columns each, is taken out before it hands
+// at each step: 2 rows of 4096 tokens took 252 us, with these 244.)  A warpgroup's O, D more columns each, is taken out before it hands
 // over the next segment's first P, which is what the next product into O waits for, and the two tiles of Q are a ring.
 // A softmax thread owns a query row; m, l and the sum of the rounded p (q3s_attn_prefix.cuh says why) are in
 // registers.  It takes its exponentials with the maximum so far while it looks for the unit's own; where a score
@@ -730,67 +736,67 @@ __global__ void __launch_bounds__(CH_NT, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CH_REGS_OTHER));
     if (w == 0) {
       int copies = 0, v_copies = 0, q_copies = 0, bad = 0;  // (V's may be one behind K's where a wait gave up)
-    for (bool again = works; again;) {
-      walk();
-      __syncthreads();  // the segments are listed
-      const int n = *s_segs;
-      again = walker->more != 0;
-      // ---- copies: lane l copies box l of a step (a page, or 128 tokens of one) ----
-      const int rows = min(a.bs, CH_KEYS), pages = CH_KEYS / rows;
-      auto block_of = [&](const ChunkSeg& g, int j) {  // past the cache (it reads as zeros) where there is none
-        const int s = g.step0 + j;
-        const bool prefix = s < before;
-        const int key = (prefix ? s : s - before) * CH_KEYS + lane * rows;
-        if (lane >= pages || key >= (prefix ? a.L : g.len)) return a.blocks;
-        const int32_t* ids = prefix ? a.prefix_blocks : a.table + g.b * a.table_stride;
-        return ids[key >> a.bs_log2];
-      };
-      auto copy = [&](const CUtensorMap* map, unsigned char* ring, uint64_t* full, int s, int h, int block) {
-        const int place = (lane * rows) & (a.bs - 1);
-        if (lane == 0) mbar_expect_tx(&full[s], Tile::KV_BYTES);
-        __syncwarp();
-        if (lane < pages)
-          for (int x = 0; x < HALVES; ++x)
-            tma_load_slice(smem_u32(ring + s * Tile::KV_BYTES + x * CH_KEYS * 128 + lane * rows * 128), map, x, place, h, block, &full[s]);
-      };
-      int next = n ? block_of(s_list[0], 0) : 0;
-      for (int e = 0; ok && e < n; ++e) {
-        const ChunkSeg& g = s_list[e];
-        const int steps = g.steps, h = g.h, tiles = tiles_of(g);
-        for (int j = 0; ok && j < steps; ++j) {
-          const bool inside = static_cast<unsigned>(next) < static_cast<unsigned>(a.blocks);
-          bad |= !inside && next != a.blocks;
-          const int block = inside ? next : a.blocks;
-          if (j + 1 < steps) next = block_of(g, j + 1);
-          else if (e + 1 < n) next = block_of(s_list[e + 1], 0);
-          const int s = copies % STAGES;
-          const uint32_t parity = static_cast<uint32_t>(copies / STAGES - 1) & 1u;
-          if (copies >= STAGES && !(ok = __all_sync(FULL, wait(&k_empty[s], parity)))) break;
-          copy(&tm_k, s_k, k_full, s, h, block);
-          ++copies;
-          if (j == 0) {
-            for (int i = 0; i < tiles; ++i) {
-              const int place = q_copies & 1;
-              if (q_copies >= 2 && !(ok = __all_sync(FULL, wait(&q_empty[place], static_cast<uint32_t>((q_copies >> 1) - 1) & 1u)))) break;
-              if (lane == 0) {
-                mbar_expect_tx(&q_full[place], static_cast<uint32_t>(HALVES * c.per_tile * a.G * 128));
-                for (int x = 0; x < HALVES; ++x)
-                  tma_load_3d(smem_u32(s_q + place * Tile::Q_BYTES + x * CH_M * 128), &tm_q, 64 * x, h * a.G, g.token + i * c.per_tile,
-                              &q_full[place]);
+      for (bool again = works; again;) {
+        walk();
+        __syncthreads();  // the segments are listed
+        const int n = *s_segs;
+        again = walker->more != 0;
+        // ---- copies: lane l copies box l of a step (a page, or 128 tokens of one) ----
+        const int rows = min(a.bs, CH_KEYS), pages = CH_KEYS / rows;
+        auto block_of = [&](const ChunkSeg& g, int j) {  // past the cache (it reads as zeros) where there is none
+          const int s = g.step0 + j;
+          const bool prefix = s < before;
+          const int key = (prefix ? s : s - before) * CH_KEYS + lane * rows;
+          if (lane >= pages || key >= (prefix ? a.L : g.len)) return a.blocks;
+          const int32_t* ids = prefix ? a.prefix_blocks : a.table + g.b * a.table_stride;
+          return ids[key >> a.bs_log2];
+        };
+        auto copy = [&](const CUtensorMap* map, unsigned char* ring, uint64_t* full, int s, int h, int block) {
+          const int place = (lane * rows) & (a.bs - 1);
+          if (lane == 0) mbar_expect_tx(&full[s], Tile::KV_BYTES);
+          __syncwarp();
+          if (lane < pages)
+            for (int x = 0; x < HALVES; ++x)
+              tma_load_slice(smem_u32(ring + s * Tile::KV_BYTES + x * CH_KEYS * 128 + lane * rows * 128), map, x, place, h, block, &full[s]);
+        };
+        int next = n ? block_of(s_list[0], 0) : 0;
+        for (int e = 0; ok && e < n; ++e) {
+          const ChunkSeg& g = s_list[e];
+          const int steps = g.steps, h = g.h, tiles = tiles_of(g);
+          for (int j = 0; ok && j < steps; ++j) {
+            const bool inside = static_cast<unsigned>(next) < static_cast<unsigned>(a.blocks);
+            bad |= !inside && next != a.blocks;
+            const int block = inside ? next : a.blocks;
+            if (j + 1 < steps) next = block_of(g, j + 1);
+            else if (e + 1 < n) next = block_of(s_list[e + 1], 0);
+            const int s = copies % STAGES;
+            const uint32_t parity = static_cast<uint32_t>(copies / STAGES - 1) & 1u;
+            if (copies >= STAGES && !(ok = __all_sync(FULL, wait(&k_empty[s], parity)))) break;
+            copy(&tm_k, s_k, k_full, s, h, block);
+            ++copies;
+            if (j == 0) {
+              for (int i = 0; i < tiles; ++i) {
+                const int place = q_copies & 1;
+                if (q_copies >= 2 && !(ok = __all_sync(FULL, wait(&q_empty[place], static_cast<uint32_t>((q_copies >> 1) - 1) & 1u)))) break;
+                if (lane == 0) {
+                  mbar_expect_tx(&q_full[place], static_cast<uint32_t>(HALVES * c.per_tile * a.G * 128));
+                  for (int x = 0; x < HALVES; ++x)
+                    tma_load_3d(smem_u32(s_q + place * Tile::Q_BYTES + x * CH_M * 128), &tm_q, 64 * x, h * a.G, g.token + i * c.per_tile,
+                                &q_full[place]);
+                }
+                __syncwarp();
+                ++q_copies;
               }
-              __syncwarp();
-              ++q_copies;
+              if (!ok) break;
             }
-            if (!ok) break;
+            if (copies > STAGES && !(ok = __all_sync(FULL, wait(&v_empty[s], parity)))) break;
+            copy(&tm_v, s_v, v_full, s, h, block);
+            ++v_copies;
           }
-          if (copies > STAGES && !(ok = __all_sync(FULL, wait(&v_empty[s], parity)))) break;
-          copy(&tm_v, s_v, v_full, s, h, block);
-          ++v_copies;
         }
+        __syncthreads();  // the segments have been taken, the next ones may be listed
+        if (*reinterpret_cast<volatile int*>(failed)) break;
       }
-      __syncthreads();  // the segments have been taken, the next ones may be listed
-      if (*reinterpret_cast<volatile int*>(failed)) break;
-    }
       if (bad && a.error_word) atomicOr(a.error_word, Q3S_DECERR_BLOCK_ID);
       // no copy may be in flight when the CTA leaves: wait for each place's last one
       if (lane == 0) {
@@ -803,7 +809,7 @@ __global__ void __launch_bounds__(CH_NT, 1)
     } else {
       // ---- products: warp 1 the second one, O += P V, warps 2 and 3 the scores of a softmax warpgroup each ----
       // (one warp for all scores took 450 clocks to issue a unit's eight products beside the softmax warps and 500 more for
-      // its waits and loop: 2 rows of 4096 tokens 271 us)
+      // its waits and loop: 2 rows of 4096 tokens 271 us, with two 244)
       constexpr uint32_t FMT = BF16 ? 1u : 0u;
       constexpr uint32_t ID_S = (1u << 4) | (FMT << 7) | (FMT << 10) | (static_cast<uint32_t>(KEYS >> 3) << 17) |
                                 (static_cast<uint32_t>(CH_M >> 4) << 24);
