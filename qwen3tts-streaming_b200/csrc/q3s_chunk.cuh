@@ -72,7 +72,7 @@ struct ChunkTile {
   static_assert(BUFFERS * KEYS + 2 * D == 512, "columns");
   static constexpr int Q_BYTES = CH_M * D * 2;
   static constexpr int KV_BYTES = CH_KEYS * D * 2;
-  static constexpr int LIST = CH_SEGS * static_cast<int>(sizeof(ChunkSeg)) + CH_NT * static_cast<int>(sizeof(ChunkRow)) + CH_M * 12;
+  static constexpr int LIST = CH_SEGS * static_cast<int>(sizeof(ChunkSeg)) + CH_NT * static_cast<int>(sizeof(ChunkRow) + 8) + CH_M * 12;
   static constexpr int USED = 1024 + 2 * Q_BYTES + 2 * STAGES * KV_BYTES + LIST + 512;
   static constexpr int SMEM = USED > TMEM_ALL_SMEM ? USED : TMEM_ALL_SMEM;  // all of the tensor memory
   static_assert(SMEM <= HEAD_SMEM_LIMIT, "shared memory");
@@ -83,7 +83,7 @@ struct ChunkArgs {
   int per_tile;      // tokens of a tile: 128 / G
   int window;        // 0: none
   int slot_rows;     // query rows of a part in the workspace
-  float* part_o;     // [2 * CTAs][slot_rows][D]
+  float* part_o;     // [2 * CTAs][D / 4][slot_rows][4]: neighbouring rows, which are neighbouring threads', side by side
   float2* part_ml;   // [2 * CTAs][slot_rows]
   ChunkCut* cuts;    // [CTAs]
 };
@@ -283,7 +283,8 @@ __global__ void __launch_bounds__(CH_NT, 1)
   static_assert((4 + 4 * STAGES + 3 * BUFFERS + 3 + CH_NT / 32) * 8 + sizeof(ChunkWalk) + 3 * 4 <= 512, "room for the barriers and counts");
   ChunkSeg* s_list = reinterpret_cast<ChunkSeg*>(reinterpret_cast<unsigned char*>(q_full) + 512);
   ChunkRow* s_rows = reinterpret_cast<ChunkRow*>(s_list + CH_SEGS);  // the first CH_NT rows
-  float* s_ml = reinterpret_cast<float*>(s_rows + CH_NT);            // [128][3] m, l and the sum of the rounded p of a shared tile's second sums
+  long long* s_cost = reinterpret_cast<long long*>(s_rows + CH_NT);  // theirs
+  float* s_ml = reinterpret_cast<float*>(s_cost + CH_NT);            // [128][3] m, l and the sum of the rounded p of a shared tile's second sums
   const int t = static_cast<int>(threadIdx.x), w = t >> 5, lane = t & 31;
   const int cta = static_cast<int>(blockIdx.x);
   const int pair = 2 * c.per_tile;  // tokens of an item
@@ -352,13 +353,14 @@ __global__ void __launch_bounds__(CH_NT, 1)
     }
     return r * a.H;
   };
-  long long mine = 0, all = 0;  // this thread's row of the first CH_NT, all of its rows
+  long long all = 0;
+  const int turn_row = lane * (CH_NT / 32) + w;  // neighbouring rows to different warps (13 rows of one warp: 2 us)
   for (int b0 = 0; b0 < a.B; b0 += CH_NT) {
-    const ChunkRow x = b0 + t < a.B ? chunk_row(a, b0 + t) : ChunkRow{0, 0, 0};
+    const ChunkRow x = b0 + turn_row < a.B ? chunk_row(a, b0 + turn_row) : ChunkRow{0, 0, 0};
     const long long r = row_cost(x);
     if (b0 == 0) {
-      mine = r;
-      s_rows[t] = x;
+      s_cost[turn_row] = r;
+      s_rows[turn_row] = x;
     }
     all += r;
   }
@@ -380,14 +382,12 @@ __global__ void __launch_bounds__(CH_NT, 1)
     const long long range0 = ChunkCutting{all, ctas}.start(cta);
     long long carry = 0;
     for (int b0 = 0; b0 < a.B && carry <= range0; b0 += CH_NT) {
-      long long r = mine;
+      long long r = s_cost[t];  // in order
       if (b0) r = row_cost(b0 + t < a.B ? chunk_row(a, b0 + t) : ChunkRow{0, 0, 0});
       const long long up = warp_scan(r);
-      if (a.B > CH_NT) {  // the sums in s_sum are of all rows
-        __syncthreads();
-        if (lane == 31) s_sum[w] = up;
-        __syncthreads();
-      }
+      __syncthreads();
+      if (lane == 31) s_sum[w] = up;
+      __syncthreads();
       long long at = carry + up - r;
 #pragma unroll
       for (int i = 0; i < CH_NT / 32; ++i) {
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(CH_NT, 1)
         const int token = tile * c.per_tile + row / a.G, gq = row % a.G;
         const bool exists = row < c.per_tile * a.G && token < g.tokens, sees = own != CH_UNSEEN;
         const int64_t out_at = static_cast<int64_t>(g.token + token) * a.ot + (static_cast<int64_t>(g.h) * a.G + gq) * a.oh;
-        const int64_t part_at = static_cast<int64_t>(max(g.slot, 0)) * c.slot_rows + tile * c.per_tile * a.G + row;
+        const int part_row = tile * c.per_tile * a.G + row;
         const uint32_t to2 = ts + static_cast<uint32_t>(BUFFERS * KEYS + D * (i ^ 1));
         float odd = 0.0f;  // a NaN where a value is not finite
 #pragma unroll 1
@@ -693,16 +693,16 @@ __global__ void __launch_bounds__(CH_NT, 1)
                 dst[x] = make_uint4(pack2<BF16>(v[8 * x], v[8 * x + 1]), pack2<BF16>(v[8 * x + 2], v[8 * x + 3]),
                                     pack2<BF16>(v[8 * x + 4], v[8 * x + 5]), pack2<BF16>(v[8 * x + 6], v[8 * x + 7]));
             } else {
-              float4* dst = reinterpret_cast<float4*>(c.part_o + part_at * D + 32 * y);
+              float4* dst = reinterpret_cast<float4*>(c.part_o) + (static_cast<int64_t>(g.slot) * (D / 4) + 8 * y) * c.slot_rows + part_row;
 #pragma unroll
-              for (int x = 0; x < 8; ++x) dst[x] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+              for (int x = 0; x < 8; ++x) dst[x * c.slot_rows] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
             }
           }
         }
         tc_fence_before();  // O has been read: the next P (its barrier) lets the next product into it start
         if (both) mbar_arrive(taken);
         if (exists) {
-          if (!whole) c.part_ml[part_at] = make_float2(m, l);
+          if (!whole) c.part_ml[static_cast<int64_t>(g.slot) * c.slot_rows + part_row] = make_float2(m, l);
           else if (a.lse) a.lse[static_cast<int64_t>(g.token + token) * a.Hq + g.h * a.G + gq] = chunk_lse(m, l);
         }
         // sums that are not finite though the scores are: V holds an infinity or a NaN
@@ -712,7 +712,8 @@ __global__ void __launch_bounds__(CH_NT, 1)
           redo &= redo - 1;
           const int tk = __shfl_sync(FULL, token, src), q = __shfl_sync(FULL, gq, src), ow = __shfl_sync(FULL, own, src);
           const int fi = __shfl_sync(FULL, from, src);
-          const int64_t at = __shfl_sync(FULL, part_at, src), oat = __shfl_sync(FULL, out_at, src);
+          const int64_t oat = __shfl_sync(FULL, out_at, src);
+          const int pr = __shfl_sync(FULL, part_row, src);
           constexpr int E = D / 32;
           float acc[E], km, kl;
           chunk_row_by_key<D, BF16>(c, g, g.token + tk, q, ow, fi, lane, acc, km, kl);
@@ -724,8 +725,11 @@ __global__ void __launch_bounds__(CH_NT, 1)
             for (int x = 0; x < E; x += 2) dst[x / 2] = pack2<BF16>(acc[x] * inv, acc[x + 1] * inv);
           } else {
 #pragma unroll
-            for (int x = 0; x < E; ++x) c.part_o[at * D + lane * E + x] = acc[x];
-            if (lane == 0) c.part_ml[at] = make_float2(km, kl);
+            for (int x = 0; x < E; ++x) {
+              const int d = lane * E + x;
+              c.part_o[((static_cast<int64_t>(g.slot) * (D / 4) + d / 4) * c.slot_rows + pr) * 4 + d % 4] = acc[x];
+            }
+            if (lane == 0) c.part_ml[static_cast<int64_t>(g.slot) * c.slot_rows + pr] = make_float2(km, kl);
           }
         }
       }
@@ -901,71 +905,56 @@ __global__ void __launch_bounds__(CH_NT, 1)
   if (t == 0 && *failed && a.error_word) atomicOr(a.error_word, Q3S_DECERR_WAIT);
 }
 
-// ROWS query rows of a cut item, STEP apart, by one warp, D / 32 dims a lane: PARTS of their parts requested at a time, of all rows together.
-template <int D, bool BF16, int ROWS, int PARTS, int STEP>
-Q3S_DEV void chunk_join_rows(const ChunkArgs& c, const ChunkCut& k, int r0, int rows, int lane) {
-  constexpr int E = D / 32;
+// A query row of a cut item (8 rows a warp) and TILES times 4 dims of it a lane, 16 dims apart, the first at `dim`:
+// PARTS of its parts requested at a time.
+template <int D, bool BF16, int TILES, int PARTS>
+Q3S_DEV void chunk_join_row(const ChunkArgs& c, const ChunkCut& k, int r, int dim) {
   const AttnArgs& a = c.a;
-  float acc[ROWS][E], m[ROWS], l[ROWS];
+  float4 acc[TILES];
+  float m = -INFINITY, l = 0.0f;
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    m[i] = -INFINITY, l[i] = 0.0f;
-#pragma unroll
-    for (int x = 0; x < E; ++x) acc[i][x] = 0.0f;
-  }
+  for (int i = 0; i < TILES; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int p = 0; p < k.parts; p += PARTS) {
-    float y[PARTS][ROWS][E];
-    float2 ml[PARTS][ROWS];
+    float4 y[PARTS][TILES];
+    float2 ml[PARTS];
 #pragma unroll
     for (int j = 0; j < PARTS; ++j) {
-      const int64_t slot = static_cast<int64_t>(p + j == 0 ? k.slot : 2 * (k.cta + p + j)) * c.slot_rows;
+      const int64_t slot = p + j == 0 ? k.slot : 2 * (k.cta + p + j);
+      const bool live = p + j < k.parts;
+      ml[j] = live ? c.part_ml[slot * c.slot_rows + r] : make_float2(-INFINITY, 0.0f);
 #pragma unroll
-      for (int i = 0; i < ROWS; ++i) {
-        ml[j][i] = make_float2(-INFINITY, 0.0f);
-#pragma unroll
-        for (int x = 0; x < E; ++x) y[j][i][x] = 0.0f;
-        const int r = r0 + i * STEP;
-        if (p + j < k.parts && r < rows) {
-          ml[j][i] = c.part_ml[slot + r];
-          const float* src = c.part_o + (slot + r) * D + lane * E;
-          if constexpr (E == 4) {
-            const float4 f = *reinterpret_cast<const float4*>(src);
-            y[j][i][0] = f.x, y[j][i][1] = f.y, y[j][i][2] = f.z, y[j][i][3] = f.w;
-          } else {
-            const float2 f = *reinterpret_cast<const float2*>(src);
-            y[j][i][0] = f.x, y[j][i][1] = f.y;
-          }
-        }
-      }
+      for (int i = 0; i < TILES; ++i)
+        y[j][i] = live ? reinterpret_cast<const float4*>(c.part_o)[(slot * (D / 4) + dim / 4 + 4 * i) * c.slot_rows + r]
+                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
 #pragma unroll
-    for (int j = 0; j < PARTS; ++j)
+    for (int j = 0; j < PARTS; ++j) {
+      const float nm = fmaxf(m, ml[j].x), base = nm == -INFINITY ? 0.0f : nm;
+      const float wm = ex2(m - base), wp = ex2(ml[j].x - base);
+      m = nm;
+      l = l * wm + wp * ml[j].y;
 #pragma unroll
-      for (int i = 0; i < ROWS; ++i) {
-        const float nm = fmaxf(m[i], ml[j][i].x), base = nm == -INFINITY ? 0.0f : nm;
-        const float wm = ex2(m[i] - base), wp = ex2(ml[j][i].x - base);
-        m[i] = nm;
-        l[i] = l[i] * wm + wp * ml[j][i].y;
-#pragma unroll
-        for (int x = 0; x < E; ++x) acc[i][x] = acc[i][x] * wm + wp * y[j][i][x];
+      for (int i = 0; i < TILES; ++i) {
+        acc[i].x = acc[i].x * wm + wp * y[j][i].x;
+        acc[i].y = acc[i].y * wm + wp * y[j][i].y;
+        acc[i].z = acc[i].z * wm + wp * y[j][i].z;
+        acc[i].w = acc[i].w * wm + wp * y[j][i].w;
       }
+    }
   }
+  const int64_t token = k.token + r / a.G;
+  const int head = k.h * a.G + r % a.G;
+  const float inv = chunk_inverse(l);
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const int r = r0 + i * STEP;
-    if (r >= rows) continue;
-    const int token = k.token + r / a.G, head = k.h * a.G + r % a.G;
-    const float inv = chunk_inverse(l[i]);
-    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + token * a.ot + head * a.oh + lane * E);
-#pragma unroll
-    for (int x = 0; x < E; x += 2) dst[x / 2] = pack2<BF16>(acc[i][x] * inv, acc[i][x + 1] * inv);
-    if (a.lse && lane == 0) a.lse[static_cast<int64_t>(token) * a.Hq + head] = chunk_lse(m[i], l[i]);
-  }
+  for (int i = 0; i < TILES; ++i)
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + token * a.ot + head * a.oh + dim + 16 * i) =
+        make_uint2(pack2<BF16>(acc[i].x * inv, acc[i].y * inv), pack2<BF16>(acc[i].z * inv, acc[i].w * inv));
+  if (a.lse && dim == 0) a.lse[token * a.Hq + head] = chunk_lse(m, l);
 }
 
-// Joins the parts of the items that were cut, a warp four query rows at once (most items have two parts; of one
-// with more a warp takes a row and eight parts at once); blocks behind those write 0 and -inf for the tokens that
-// no item has (of no row, or that see nothing).  Bound by latency: a row after the other took 15 us of the 2 rows' 245.
+// Joins the parts of the items that were cut: 32 query rows a CTA, a warp 8 of them and half the dims, all of them at
+// once and two parts (most items have two; of one with more a warp takes 16 dims and eight parts at once).  Blocks behind those
+// write 0 and -inf for the tokens that no item has (of no row, or that see nothing).  Bound by latency.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(CH_JOIN_NT) attn_chunk_join_kernel(const ChunkArgs c, int join_blocks, int blocks_each) {
   const AttnArgs& a = c.a;
@@ -977,12 +966,14 @@ __global__ void __launch_bounds__(CH_JOIN_NT) attn_chunk_join_kernel(const Chunk
     const ChunkCut k = c.cuts[block / blocks_each];
     if (k.parts == 0) return;
     const int row0 = (block % blocks_each) * CH_JOIN_ROWS, rows = min(k.tokens * a.G, row0 + CH_JOIN_ROWS);
-    static_assert(CH_JOIN_ROWS == 4 * WARPS, "a warp's rows");
-    if (row0 + w >= rows) return;
+    static_assert(CH_JOIN_ROWS == 8 * WARPS / 2, "a warp's rows");
+    const int r = row0 + (w & 3) * 8 + (lane & 7), dim = (w >> 2) * (D / 2) + (lane >> 3) * 4;
+    if (r >= rows) return;
+    constexpr int TILES = D / 32;
     if (k.parts <= 2) {
-      chunk_join_rows<D, BF16, 4, 2, WARPS>(c, k, row0 + w, rows, lane);
+      chunk_join_row<D, BF16, TILES, 2>(c, k, r, dim);
     } else {
-      for (int r = row0 + w; r < rows; r += WARPS) chunk_join_rows<D, BF16, 1, 8, WARPS>(c, k, r, rows, lane);
+      for (int i = 0; i < TILES; ++i) chunk_join_row<D, BF16, 1, 8>(c, k, r, dim + 16 * i);
     }
     return;
   }
