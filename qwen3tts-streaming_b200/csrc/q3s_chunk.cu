@@ -66,12 +66,12 @@ q3s_status check_sizes(const q3s_chunk_attention_desc* d) {
 
 // Whether the kernels of q3s_prefix_attention, whose tiles are 16 query rows, are the faster ones: few query rows, together or
 // a row of the batch, and no window.  They against the kernel here, us, 8 key/value heads of 128, query rows a row of the
-// batch: 1 row of 8000 keys, 64: 31 and 35, 128: 43 and 43, 256: 78 and 49; 1 row of 200 keys, 128: 14 and 21, 512: 24 and 28;
-// 16 rows of 2000 keys, 16: 33 and 38, 32: 49 and 40; 64 rows of 1000 keys, 16: 52 and 60, 32: 83 and 61; 16 rows of 8000
-// keys, 8: 81 and 79, 16: 86 and 82; 4 heads of 64, 16 rows of 2000 keys, 16: 15 and 24, 64: 29 and 27.
+// batch: 1 row of 8000 keys, 64: 31 and 36, 128: 43 and 39, 256: 78 and 43; 1 row of 200 keys, 128: 14 and 17, 512: 24 and 21;
+// 16 rows of 2000 keys, 15: 33 and 38, 31: 49 and 39; 64 rows of 1000 keys, 15: 52 and 59, 31: 82 and 60; 16 rows of 8000
+// keys, 7: 71 and 77, 15: 86 and 80; 4 heads of 64, 16 rows of 2000 keys, 15: 15 and 22, 63: 29 and 23.
 bool few_queries(const q3s_chunk_attention_desc* d) {
   const int64_t G = d->q_heads / d->kv_heads;
-  return d->window == 0 && G <= Q3S_MAX_QUERY_GROUP && d->tokens * G <= std::max<int64_t>(160, static_cast<int64_t>(d->batch) * 20);
+  return d->window == 0 && G <= Q3S_MAX_QUERY_GROUP && d->tokens * G <= std::max<int64_t>(112, static_cast<int64_t>(d->batch) * 20);
 }
 q3s_prefix_attention_desc few_queries_desc(const q3s_chunk_attention_desc* d) {
   q3s_prefix_attention_desc p = {};

@@ -12,11 +12,12 @@
 // plan is needed and a captured graph follows the lengths.  A whole item is written as
 // it ends; the parts (m, l, o) of a cut one are joined by the second kernel (q3s_attn.cuh has the mathematics).
 //
-// Measured on the device: 2 rows of 4096 tokens behind up to 3650 keys, 16 and 8 heads of 128, 246 us (920 TFLOP/s;
-// 280 us in a long run under the power limit); 13 rows of up to 700 tokens in a window of 512, 16 and 4 heads of 64,
-// 57 us; 48 rows of up to 9 tokens and 1533 keys, 32 and 8 heads of 128, 60 us (54 by the other kernels).  A long row is bound by the softmax and its hand-overs: two units
-// of 64 keys take 2100 clocks, of which the tensor cores run 1300.  Short rows are bound by what each
-// range and item begins and ends with (the list, the first loads, the sums taken out) and by the join, 7 to 15 us together.
+// Measured on the device: 2 rows of 4096 tokens behind up to 3650 keys, 16 and 8 heads of 128, 239 us (950 TFLOP/s;
+// 273 us in a long run under the power limit); 13 rows of up to 700 tokens in a window of 512, 16 and 4 heads of 64,
+// 50 us; 48 rows of up to 9 tokens and 1533 keys, 32 and 8 heads of 128, 60 us at first (54 by the other kernels).
+// A long row is bound by the softmax and its hand-overs: two units of 64 keys take 2100 clocks, of which the tensor
+// cores run 1300.  Short rows are bound by what each range and item begins and ends with: 7 us until the first scores
+// (lengths, list, loads), 3 us from an item's last unit to the next one's first, and the join.
 #pragma once
 
 #include <cuda.h>
@@ -84,6 +85,7 @@ struct ChunkArgs {
   int window;        // 0: none
   int slot_rows;     // query rows of a part in the workspace
   float* part_o;     // [2 * CTAs][D / 4][slot_rows][4]: neighbouring rows, which are neighbouring threads', side by side
+                     // (a store takes a clock for each line it touches: row after row, a part's took 3 to 4 us)
   float2* part_ml;   // [2 * CTAs][slot_rows]
   ChunkCut* cuts;    // [CTAs]
 };
@@ -354,7 +356,7 @@ __global__ void __launch_bounds__(CH_NT, 1)
     return r * a.H;
   };
   long long all = 0;
-  const int turn_row = lane * (CH_NT / 32) + w;  // neighbouring rows to different warps (13 rows of one warp: 2 us)
+  const int turn_row = lane * (CH_NT / 32) + w;  // neighbouring rows to different warps (13 rows of one warp, one after another: about 2 us)
   for (int b0 = 0; b0 < a.B; b0 += CH_NT) {
     const ChunkRow x = b0 + turn_row < a.B ? chunk_row(a, b0 + turn_row) : ChunkRow{0, 0, 0};
     const long long r = row_cost(x);
@@ -952,8 +954,8 @@ Q3S_DEV void chunk_join_row(const ChunkArgs& c, const ChunkCut& k, int r, int di
   if (a.lse && dim == 0) a.lse[token * a.Hq + head] = chunk_lse(m, l);
 }
 
-// Joins the parts of the items that were cut: 32 query rows a CTA, a warp 8 of them and half the dims, all of them at
-// once and two parts (most items have two; of one with more a warp takes 16 dims and eight parts at once).  Blocks behind those
+// Joins the parts of the items that were cut: 32 query rows a CTA, a warp 8 of them and half the dims, four parts at
+// once (most items have two; eight parts, 16 dims at a time: 1 row of 300 tokens, 20000 keys, 87 us against 81).  Blocks behind those
 // write 0 and -inf for the tokens that no item has (of no row, or that see nothing).  Bound by latency.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(CH_JOIN_NT) attn_chunk_join_kernel(const ChunkArgs c, int join_blocks, int blocks_each) {
@@ -970,11 +972,7 @@ __global__ void __launch_bounds__(CH_JOIN_NT) attn_chunk_join_kernel(const Chunk
     const int r = row0 + (w & 3) * 8 + (lane & 7), dim = (w >> 2) * (D / 2) + (lane >> 3) * 4;
     if (r >= rows) return;
     constexpr int TILES = D / 32;
-    if (k.parts <= 2) {
-      chunk_join_row<D, BF16, TILES, 2>(c, k, r, dim);
-    } else {
-      for (int i = 0; i < TILES; ++i) chunk_join_row<D, BF16, 1, 8>(c, k, r, dim + 16 * i);
-    }
+    chunk_join_row<D, BF16, TILES, 4>(c, k, r, dim);
     return;
   }
   const int token = (block - join_blocks) * CH_JOIN_NT + t;
