@@ -369,7 +369,7 @@ typedef struct q3s_verify_drafts_desc {
   int64_t draft_row_stride;     /* elements, >= V */
   const float* temperature;     /* optional [B] */
   const int64_t* slot_map;      /* optional [T]: a row with a token without a slot (negative) is left out, like an idle one */
-  int64_t* tokens_out;          /* [T] from each row's first place on: its accepted drafts, then what it drew; -1 behind that and past the last row */
+  int64_t* tokens_out;          /* [T] from each row's first place on: its accepted drafts, then what it drew; -1 behind that, before the first row and past the last */
   int32_t* accepted;            /* [B] drafts accepted; 0 for a row without tokens */
   int32_t* rejected;            /* [B] drafts not accepted; 0 for a row without tokens */
   int64_t* next_ids;            /* [B] what the row drew; -1 for a row without tokens */

@@ -241,6 +241,8 @@ __global__ void __launch_bounds__(VF_NT, 2) verify_kernel(const VerifyArgs a) {
     const int last = a.B ? t0 + n : 0;
     for (int i = last + t; i < a.T; i += VF_NT) a.tokens_out[i] = -1;
   }
+  if (rank == 0 && b == 0 && a.B > 0)  // and before the first
+    for (int i = t; i < t0; i += VF_NT) a.tokens_out[i] = -1;
   if (a.slot_map) {
     bool without = false;
     for (int i = t; i < n; i += VF_NT) without |= a.slot_map[t0 + i] < 0;

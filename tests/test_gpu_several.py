@@ -321,6 +321,19 @@ def test_verify_idle_and_refused_rows_and_padding(dev):
     assert 0 in want["accepted"] and want["tokens"][-17:] == [-1] * 17
 
 
+def test_verify_places_before_the_first_row(dev):
+    g = torch.Generator().manual_seed(44)
+    logits, ids, u = torch.randn(600, 50, generator=g) * 2, torch.randint(0, 50, (600,), generator=g), torch.rand(600, generator=g)
+    for offsets in ([530, 540, 540, 541], [600, 600]):
+        rows = len(offsets) - 1
+        want = R.verify_drafts(logits.numpy(), ids.tolist(), offsets, u.tolist(), None, [1.0] * rows)
+        on_gpu = logits.to(dev), ids.to(dev), i32(offsets, dev), u.to(dev)
+        torch.full((600,), 7, dtype=torch.int64, device=dev)  # freed: what the next allocation of that size finds
+        r = q3s.verify_drafts(*on_gpu)
+        for name in ("accepted", "rejected", "next_ids", "tokens"):
+            assert getattr(r, name).tolist() == want[name], name
+
+
 def test_verify_no_rows(dev):
     z = torch.zeros(3, 10, device=dev)
     r = q3s.verify_drafts(z, torch.zeros(3, dtype=torch.int64, device=dev), i32([0], dev), z[:, 0].contiguous())
