@@ -137,7 +137,7 @@ Q3S_DEV void verify_take(VerifyRun& s, const float (&x)[N], int v, float c) {
     s.index = v + at;
     const float y = top * c, k = ceilf(fmaf(fabsf(y), 2.384185791015625e-07f, y));  // 2^-22: above the rounding of y
     if (k > s.k) {
-      s.sum = s.k == -INFINITY ? 0.0 : s.sum * pow2_int(static_cast<int>(fmaxf(s.k - k, -2000.0f)));
+      s.sum *= pow2_int(static_cast<int>(fmaxf(s.k - k, -2000.0f)));  // from -infinity times 0: a NaN that came first stays one
       s.k = k;
     }
   }

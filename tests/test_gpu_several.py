@@ -426,6 +426,32 @@ def test_verify_logits_without_a_distribution(dev):
     assert check_verify(c, dev)["error"] == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("vocab,places", [
+    (2051, (0, 1, 2, 3, 2047, 2050)),  # places that do not begin on 16 bytes: the first entries, taken alone, and the last
+    (2048, (0, 5, 1023, 2047)),
+    (40001, (0, 1, 39999, 40000))])
+@pytest.mark.parametrize("around", ["finite", "left out", "nothing else"])
+def test_verify_a_nan_wherever_it_stands(dev, dtype, vocab, places, around):
+    """A place that holds a NaN has no distribution: also where the NaN is the first entry that a thread sees, alone or among
+    what top-k left out (-inf)."""
+    c = make_verify(45, 2 * len(places), 3, vocab, dtype=dtype, probs=False)
+    logits, first = c["logits"], c["offsets"][:-1]
+    for i, at in enumerate(places):
+        for t in (int(first[2 * i]), int(first[2 * i + 1])):  # two rows, whose places begin at other addresses
+            if around == "left out":
+                logits[t, max(at - 300, 0):at + 300] = -torch.inf
+            elif around == "nothing else":
+                keep = (at + vocab // 2) % vocab
+                x = float(logits[t, keep])
+                logits[t] = -torch.inf
+                logits[t, keep] = x
+            logits[t, at] = float("nan")
+    c["heat"][1::4] = 0.0  # some greedy
+    want = check_verify(c, dev)
+    assert want["error"] == 64 and want["accepted"] == [0] * (2 * len(places))
+
+
 @pytest.mark.parametrize("probs", [True, False])
 def test_verify_drafts_outside_the_vocabulary(dev, probs):
     c = make_verify(11, 20, 4, 200, probs=probs)
