@@ -225,14 +225,14 @@ __global__ void __launch_bounds__(PX_NT, 1)
 
   // ---- copies: lane l copies box l of a step (a page, or 128 tokens of one) ----
   const int rows = min(a.bs, PX_KEYS), pages = PX_KEYS / rows;
+  auto has_block = [&](int j) { return j < steps && lane < pages && (step0 + j) * PX_KEYS + lane * rows < a.L; };
   auto block_of = [&](int j) {  // lane's block of step j; past the cache (it reads as zeros) where there is none
-    const int key = (step0 + j) * PX_KEYS + lane * rows;
-    return j < steps && lane < pages && key < a.L ? a.prefix_blocks[key >> a.bs_log2] : a.blocks;
+    return has_block(j) ? a.prefix_blocks[((step0 + j) * PX_KEYS + lane * rows) >> a.bs_log2] : a.blocks;
   };
   int bad = 0;
   auto copy = [&](const CUtensorMap* map, unsigned char* ring, uint64_t* full, int j, int block) {
     const bool inside = static_cast<unsigned>(block) < static_cast<unsigned>(a.blocks);
-    bad |= !inside && block != a.blocks;
+    bad |= !inside && has_block(j);
     const int id = inside ? block : a.blocks, place = ((step0 + j) * PX_KEYS + lane * rows) & (a.bs - 1), s = j % PX_STAGES;
     if (lane == 0) mbar_expect_tx(&full[s], Tile::KV_BYTES);
     __syncwarp();

@@ -749,12 +749,16 @@ __global__ void __launch_bounds__(CH_NT, 1)
         again = walker->more != 0;
         // ---- copies: lane l copies box l of a step (a page, or 128 tokens of one) ----
         const int rows = min(a.bs, CH_KEYS), pages = CH_KEYS / rows;
-        auto block_of = [&](const ChunkSeg& g, int j) {  // past the cache (it reads as zeros) where there is none
+        auto key_of = [&](const ChunkSeg& g, int j) {  // the box's first key, of the prefix or of the row's own; -1: there is none
           const int s = g.step0 + j;
           const bool prefix = s < before;
           const int key = (prefix ? s : s - before) * CH_KEYS + lane * rows;
-          if (lane >= pages || key >= (prefix ? a.L : g.len)) return a.blocks;
-          const int32_t* ids = prefix ? a.prefix_blocks : a.table + g.b * a.table_stride;
+          return lane < pages && key < (prefix ? a.L : g.len) ? key : -1;
+        };
+        auto block_of = [&](const ChunkSeg& g, int j) {  // past the cache (it reads as zeros) where there is none
+          const int key = key_of(g, j);
+          if (key < 0) return a.blocks;
+          const int32_t* ids = g.step0 + j < before ? a.prefix_blocks : a.table + g.b * a.table_stride;
           return ids[key >> a.bs_log2];
         };
         auto copy = [&](const CUtensorMap* map, unsigned char* ring, uint64_t* full, int s, int h, int block) {
@@ -771,7 +775,7 @@ __global__ void __launch_bounds__(CH_NT, 1)
           const int steps = g.steps, h = g.h, tiles = tiles_of(g);
           for (int j = 0; ok && j < steps; ++j) {
             const bool inside = static_cast<unsigned>(next) < static_cast<unsigned>(a.blocks);
-            bad |= !inside && next != a.blocks;
+            bad |= !inside && key_of(g, j) >= 0;
             const int block = inside ? next : a.blocks;
             if (j + 1 < steps) next = block_of(g, j + 1);
             else if (e + 1 < n) next = block_of(s_list[e + 1], 0);

@@ -243,6 +243,42 @@ def test_bad_block_ids_read_as_zeros(dev):
     assert torch.equal(out, want) and torch.equal(lse, want_lse)
 
 
+@pytest.mark.parametrize("window", [0, EVERYTHING])
+@pytest.mark.parametrize("news,hq", [([5], 2), ([200, 3], 2)])
+@pytest.mark.parametrize("past", [0, 1, 5])
+def test_the_first_id_past_the_cache_is_reported(dev, news, hq, window, past):
+    """An id equal to the number of blocks is outside too, in a row's table and in the prefix, whichever kernel a call goes to."""
+    c = make(dev, 21, news, [90] * len(news), hq=hq, hk=1, dim=64, prefix=40)
+    blocks = c["k"].shape[0]
+    k, v = c["k"].clone(), c["v"].clone()
+    bad, shared = c["table"].clone(), c["shared"].clone()
+    where = {"table": (bad, (0, 2)), "prefix": (shared, (1,))}
+    for name, (ids, at) in where.items():
+        was, block = int(ids[at]), int(ids[at])
+        ids[at] = blocks + past
+        err = torch.zeros(1, dtype=torch.int32, device=dev)
+        out, lse = run(dict(c, table=bad, shared=shared), error_word=err, window=window)
+        assert int(err) == q3s.decode.DECERR_BLOCK_ID, name
+        kept = k[block].clone(), v[block].clone()
+        k[block], v[block] = 0, 0
+        want, want_lse = run(dict(c, k=k, v=v), window=window)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+        k[block], v[block] = kept
+        ids[at] = was
+
+
+@pytest.mark.parametrize("queries", [5, 90])
+def test_prefix_attention_reports_the_first_id_past_the_cache(dev, queries):
+    """With few queries the prefix is read by the key-split kernel, with many by the kernel of its own."""
+    c = make(dev, 22, [1] * queries, [3] * queries, hq=8, hk=2, dim=64, prefix=2000)
+    for past in (0, 1):
+        shared = c["shared"].clone()
+        shared[7] = c["k"].shape[0] + past
+        err = torch.zeros(1, dtype=torch.int32, device=dev)
+        q3s.prefix_attention(c["q"], c["k"], c["v"], c["off"], c["table"], c["len"], prefix_blocks=shared, prefix_length=2000, error_word=err)
+        assert int(err) == q3s.decode.DECERR_BLOCK_ID
+
+
 def test_same_call_same_result_and_side_stream(dev):
     c = make(dev, 16, [300, 20, 7], [900, 100, 2000], hq=8, hk=4, prefix=100)
     first = run(c, window=EVERYTHING)
