@@ -356,16 +356,22 @@ __global__ void __launch_bounds__(CH_NT, 1)
     return r * a.H;
   };
   long long all = 0;
+  bool bad_length = false;
   const int turn_row = lane * (CH_NT / 32) + w;  // neighbouring rows to different warps (13 rows of one warp, one after another: about 2 us)
   for (int b0 = 0; b0 < a.B; b0 += CH_NT) {
     const ChunkRow x = b0 + turn_row < a.B ? chunk_row(a, b0 + turn_row) : ChunkRow{0, 0, 0};
     const long long r = row_cost(x);
+    if (cta == 0 && b0 + turn_row < a.B) {  // what was cut
+      const int b = b0 + turn_row;
+      bad_length |= a.lengths[b] != x.len || a.offsets[b] != x.t0 || a.offsets[b + 1] != x.t0 + x.n;
+    }
     if (b0 == 0) {
       s_cost[turn_row] = r;
       s_rows[turn_row] = x;
     }
     all += r;
   }
+  if (bad_length && a.error_word) atomicOr(a.error_word, Q3S_DECERR_LENGTHS);
   {
     const long long up = warp_scan(all);
     if (lane == 31) s_sum[w] = up;

@@ -279,6 +279,32 @@ def test_prefix_attention_reports_the_first_id_past_the_cache(dev, queries):
         assert int(err) == q3s.decode.DECERR_BLOCK_ID
 
 
+@pytest.mark.parametrize("window", [0, EVERYTHING])
+@pytest.mark.parametrize("rows", [3, 500])
+@pytest.mark.parametrize("what", ["a negative length", "a length past the table", "offsets past the tokens", "offsets that descend", "a negative offset"])
+def test_lengths_that_are_cut_are_reported(dev, rows, what, window):
+    """Whichever kernel a call goes to, and in every row (500: more than a CTA has threads)."""
+    c = make(dev, 23, [2] * rows, [20] * rows, hq=2, hk=1, dim=64)
+    err = torch.zeros(1, dtype=torch.int32, device=dev)
+    run(c, window=window, error_word=err)
+    assert int(err) == 0
+    row, T = rows - 1, 2 * rows
+    length, off = c["len"].clone(), c["off"].clone()
+    if what == "a negative length":
+        length[row] = -3
+    elif what == "a length past the table":
+        length[row] = c["table"].shape[1] * 16 + 1
+        c["table"][row] = 0
+    elif what == "offsets past the tokens":
+        off[-1] = T + 4
+    elif what == "offsets that descend":
+        off[row], off[row + 1] = T, T - 2
+    else:
+        off[0] = -1
+    run(dict(c, len=length, off=off), window=window, error_word=err)
+    assert int(err) == q3s.decode.DECERR_LENGTHS
+
+
 def test_same_call_same_result_and_side_stream(dev):
     c = make(dev, 16, [300, 20, 7], [900, 100, 2000], hq=8, hk=4, prefix=100)
     first = run(c, window=EVERYTHING)
