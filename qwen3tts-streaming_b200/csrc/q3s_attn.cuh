@@ -167,7 +167,7 @@ Q3S_DEV void prefetch_map(const CUtensorMap* map) {
 }
 
 // a / b with b > 0, by 32-bit division where both fit (the 64-bit one costs several times as much).
-Q3S_DEV long long div_nonneg(long long a, long long b) {
+Q3S_HOST_DEV long long div_nonneg(long long a, long long b) {
   if (((a | b) >> 32) == 0) return static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
   return a / b;
 }

@@ -90,7 +90,7 @@ struct ChunkArgs {
   ChunkCut* cuts;    // [CTAs]
 };
 
-Q3S_DEV ChunkRow chunk_row(const AttnArgs& a, int b) {
+Q3S_HOST_DEV ChunkRow chunk_row(const AttnArgs& a, int b) {
   const int o0 = a.offsets[b], o1 = a.offsets[b + 1], len = a.lengths[b];
   ChunkRow x;
   x.t0 = min(max(o0, 0), a.T);
@@ -99,7 +99,7 @@ Q3S_DEV ChunkRow chunk_row(const AttnArgs& a, int b) {
   return x;
 }
 // Steps of the item of tokens [i0, i0 + m) of a row: first and count (0: its queries see nothing).
-Q3S_DEV int2 chunk_steps(const ChunkArgs& c, const ChunkRow& x, int i0, int m) {
+Q3S_HOST_DEV int2 chunk_steps(const ChunkArgs& c, const ChunkRow& x, int i0, int m) {
   const int L = c.a.L;
   auto step_of = [&](int p) {  // p >= 0
     const uint32_t own = static_cast<uint32_t>(p - L);
@@ -124,9 +124,105 @@ struct ChunkWalk {
 struct ChunkCutting {
   long long all;
   int ctas;
-  Q3S_DEV long long start(int i) const { return div_nonneg(all * i, ctas); }
-  Q3S_DEV int cta_of(long long at) const { return static_cast<int>(div_nonneg((at + 1) * ctas + all - 1, all)) - 1; }
+  Q3S_HOST_DEV long long start(int i) const { return div_nonneg(all * i, ctas); }
+  Q3S_HOST_DEV int cta_of(long long at) const { return static_cast<int>(div_nonneg((at + 1) * ctas + all - 1, all)) - 1; }
 };
+
+// Of tokens [i0, i0 + an item's) of a row, for one head; 0: nothing is seen.
+Q3S_HOST_DEV long long chunk_item_cost(const ChunkArgs& c, const ChunkRow& x, int i0) {
+  const int steps = chunk_steps(c, x, i0, min(2 * c.per_tile, x.n - i0)).y;
+  return steps ? CH_START + static_cast<long long>(steps) : 0ll;
+}
+
+// The lanes of a warp as chunk_walk takes them (on the host, a test's).
+struct ChunkLanes {
+  int lane;
+  template <typename T>
+  Q3S_DEV T shfl(T x, int src) const { return __shfl_sync(FULL, x, src); }
+  Q3S_DEV long long scan(long long up) const {  // of the lanes up to this one
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long o = __shfl_up_sync(FULL, up, d);
+      if (lane >= d) up += o;
+    }
+    return up;
+  }
+  Q3S_DEV unsigned ballot(bool x) const { return __ballot_sync(FULL, x); }
+  Q3S_DEV void sync() const { __syncwarp(); }
+  Q3S_DEV static int first(unsigned x) { return __ffs(x) - 1; }
+  Q3S_DEV static int count(unsigned x) { return __popc(x); }
+};
+
+// Lists a CTA's next segments, up to CH_SEGS of them: a warp, 32 items at once, a lane each.  After every call c.cuts[cta]
+// says which cut item starts in the segments so far, or that none does (a CTA that gives up lists no more).
+#pragma nv_exec_check_disable
+template <typename Lanes>
+Q3S_HOST_DEV void chunk_walk(const ChunkArgs& c, int cta, const ChunkRow* rows, ChunkWalk* walker, int* segs, ChunkSeg* list, const Lanes& l) {
+  const AttnArgs& a = c.a;
+  const int pair = 2 * c.per_tile, lane = l.lane;
+  ChunkWalk k = *walker;
+  l.sync();
+  const ChunkCutting cut = {k.all, k.ctas};
+  const long long range0 = cut.start(cta), range1 = cut.start(cta + 1);
+  int n = 0;
+  while (k.more && n + 32 <= CH_SEGS) {
+    if (k.b >= a.B) {
+      k.more = 0;
+      break;
+    }
+    const ChunkRow x = k.b < CH_NT ? rows[k.b] : chunk_row(a, k.b);
+    const int pairs = (x.n + pair - 1) / pair;
+    const long long items = static_cast<long long>(pairs) * a.H;
+    if (k.item < 0) {  // the range starts in this row: skip to the tokens where it does
+      int p0 = 0;
+      for (; p0 < pairs; p0 += 32) {
+        const long long cost = p0 + lane < pairs ? chunk_item_cost(c, x, (p0 + lane) * pair) * a.H : 0;
+        const long long up = l.scan(cost);
+        const unsigned past = l.ballot(k.at + up > range0);
+        if (past) {
+          const int f = l.first(past);
+          p0 += f;
+          k.at += l.shfl(up - cost, f);
+          break;
+        }
+        k.at += l.shfl(up, 31);
+      }
+      k.item = p0 * a.H;
+    }
+    const int item = k.item + lane, p = item / a.H, h = item - p * a.H;
+    const int i0 = p * pair, m = min(pair, x.n - i0);
+    int2 steps = make_int2(0, 0);
+    if (item < items) steps = chunk_steps(c, x, i0, m);
+    const long long cost = steps.y ? CH_START + static_cast<long long>(steps.y) : 0;
+    const long long up = l.scan(cost), start = k.at + up - cost;
+    auto steps_before = [&](long long y) {  // that start before y
+      return static_cast<int>(min(max(y - start - CH_START, 0ll), static_cast<long long>(steps.y)));
+    };
+    const int lo = steps_before(range0), hi = steps_before(range1);
+    const unsigned live = l.ballot(lo < hi);
+    const bool whole = lo == 0 && hi == steps.y;
+    const int rank = l.count(live & ((1u << lane) - 1u));
+    if (lo < hi) {
+      const int slot = whole ? -1 : 2 * cta + (k.written + rank > 0 ? 1 : 0);
+      list[n + rank] = {k.b, h, x.t0 + i0, m, x.len - x.n + i0 + 1, x.len, steps.x + lo, hi - lo, slot};
+      if (lo == 0 && !whole)
+        c.cuts[cta] = {cut.cta_of(start + CH_START + steps.y - 1) - cta + 1, slot, cta, h, x.t0 + i0, m};
+    }
+    k.cut |= l.ballot(lo < hi && lo == 0 && !whole) != 0;
+    k.written += l.count(live);
+    n += l.count(live);
+    if (l.ballot(item < items && start >= range1)) k.more = 0;
+    k.at += l.shfl(up, 31);
+    k.item += 32;
+    if (k.item >= items) ++k.b, k.item = 0;
+  }
+  if (!k.cut && lane == 0) c.cuts[cta].parts = 0;
+  l.sync();
+  if (lane == 0) {
+    *walker = k;
+    *segs = n;
+  }
+}
 
 // Products and commits of one lane of a converged warp, under a predicate and not a branch: their operands are
 // then computed once for the warp (in a branch each product took three times as many issue slots).
@@ -327,28 +423,17 @@ __global__ void __launch_bounds__(CH_NT, 1)
   }
 
   // ---- the list's length, and this CTA's range of it ----
-  auto item_cost = [&](const ChunkRow& x, int i0) {  // of tokens [i0, i0 + pair), for one head; 0: nothing is seen
-    const int steps = chunk_steps(c, x, i0, min(pair, x.n - i0)).y;
-    return steps ? CH_START + static_cast<long long>(steps) : 0ll;
-  };
-  auto warp_scan = [&](long long up) {
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long o = __shfl_up_sync(FULL, up, d);
-      if (lane >= d) up += o;
-    }
-    return up;
-  };
+  const ChunkLanes lanes_of_warp{lane};
   // a row's cost; a whole warp calls (a row of many items is its 32 lanes' work)
   auto row_cost = [&](const ChunkRow& x) {
     long long r = 0;
     const bool large = x.n > 4 * pair;
-    for (int i0 = 0; i0 < x.n && !large; i0 += pair) r += item_cost(x, i0);
+    for (int i0 = 0; i0 < x.n && !large; i0 += pair) r += chunk_item_cost(c, x, i0);
     for (unsigned rest = __ballot_sync(FULL, large); rest; rest &= rest - 1) {
       const int src = __ffs(rest) - 1;
       const ChunkRow y = {0, __shfl_sync(FULL, x.n, src), __shfl_sync(FULL, x.len, src)};
       long long sum = 0;
-      for (int64_t i0 = static_cast<int64_t>(lane) * pair; i0 < y.n; i0 += 32 * pair) sum += item_cost(y, static_cast<int>(i0));
+      for (int64_t i0 = static_cast<int64_t>(lane) * pair; i0 < y.n; i0 += 32 * pair) sum += chunk_item_cost(c, y, static_cast<int>(i0));
 #pragma unroll
       for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(FULL, sum, d);
       if (lane == src) r = sum;
@@ -373,7 +458,7 @@ __global__ void __launch_bounds__(CH_NT, 1)
   }
   if (bad_length && a.error_word) atomicOr(a.error_word, Q3S_DECERR_LENGTHS);
   {
-    const long long up = warp_scan(all);
+    const long long up = lanes_of_warp.scan(all);
     if (lane == 31) s_sum[w] = up;
   }
   tc_fence_before();
@@ -392,7 +477,7 @@ __global__ void __launch_bounds__(CH_NT, 1)
     for (int b0 = 0; b0 < a.B && carry <= range0; b0 += CH_NT) {
       long long r = s_cost[t];  // in order
       if (b0) r = row_cost(b0 + t < a.B ? chunk_row(a, b0 + t) : ChunkRow{0, 0, 0});
-      const long long up = warp_scan(r);
+      const long long up = lanes_of_warp.scan(r);
       __syncthreads();
       if (lane == 31) s_sum[w] = up;
       __syncthreads();
@@ -408,73 +493,6 @@ __global__ void __launch_bounds__(CH_NT, 1)
     c.cuts[cta].parts = 0;
   }
   __syncthreads();
-
-  // Warp 0 lists the CTA's segments, up to CH_SEGS at a time: 32 items at once, a lane each.
-  auto walk = [&]() {
-    ChunkWalk k = *walker;
-    __syncwarp();
-    const ChunkCutting cut = {k.all, k.ctas};
-    const int cta = static_cast<int>(blockIdx.x);
-    const long long range0 = cut.start(cta), range1 = cut.start(cta + 1);
-    int n = 0;
-    while (k.more && n + 32 <= CH_SEGS) {
-      if (k.b >= a.B) {
-        k.more = 0;
-        break;
-      }
-      const ChunkRow x = k.b < CH_NT ? s_rows[k.b] : chunk_row(a, k.b);
-      const int pairs = (x.n + pair - 1) / pair;
-      const long long items = static_cast<long long>(pairs) * a.H;
-      if (k.item < 0) {  // the range starts in this row: skip to the tokens where it does
-        int p0 = 0;
-        for (; p0 < pairs; p0 += 32) {
-          const long long cost = p0 + lane < pairs ? item_cost(x, (p0 + lane) * pair) * a.H : 0;
-          const long long up = warp_scan(cost);
-          const unsigned past = __ballot_sync(FULL, k.at + up > range0);
-          if (past) {
-            const int f = __ffs(past) - 1;
-            p0 += f;
-            k.at += __shfl_sync(FULL, up - cost, f);
-            break;
-          }
-          k.at += __shfl_sync(FULL, up, 31);
-        }
-        k.item = p0 * a.H;
-      }
-      const int item = k.item + lane, p = item / a.H, h = item - p * a.H;
-      const int i0 = p * pair, m = min(pair, x.n - i0);
-      int2 steps = make_int2(0, 0);
-      if (item < items) steps = chunk_steps(c, x, i0, m);
-      const long long cost = steps.y ? CH_START + static_cast<long long>(steps.y) : 0;
-      const long long up = warp_scan(cost), start = k.at + up - cost;
-      auto steps_before = [&](long long y) {  // that start before y
-        return static_cast<int>(min(max(y - start - CH_START, 0ll), static_cast<long long>(steps.y)));
-      };
-      const int lo = steps_before(range0), hi = steps_before(range1);
-      const unsigned live = __ballot_sync(FULL, lo < hi);
-      const bool whole = lo == 0 && hi == steps.y;
-      const int rank = __popc(live & ((1u << lane) - 1u));
-      if (lo < hi) {
-        const int slot = whole ? -1 : 2 * cta + (k.written + rank > 0 ? 1 : 0);
-        s_list[n + rank] = {k.b, h, x.t0 + i0, m, x.len - x.n + i0 + 1, x.len, steps.x + lo, hi - lo, slot};
-        if (lo == 0 && !whole)
-          c.cuts[cta] = {cut.cta_of(start + CH_START + steps.y - 1) - cta + 1, slot, cta, h, x.t0 + i0, m};
-      }
-      k.cut |= __any_sync(FULL, lo < hi && lo == 0 && !whole);
-      k.written += __popc(live);
-      n += __popc(live);
-      if (__any_sync(FULL, item < items && start >= range1)) k.more = 0;
-      k.at += __shfl_sync(FULL, up, 31);
-      k.item += 32;
-      if (k.item >= items) ++k.b, k.item = 0;
-    }
-    if (!k.more && !k.cut && lane == 0) c.cuts[cta].parts = 0;
-    __syncwarp();
-    if (lane == 0) {
-      *walker = k;
-      *s_segs = n;
-    }
-  };
 
   // a wait that gives up marks the CTA; every role then stops at its next wait
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -749,7 +767,7 @@ __global__ void __launch_bounds__(CH_NT, 1)
     if (w == 0) {
       int copies = 0, v_copies = 0, q_copies = 0, bad = 0;  // (V's may be one behind K's where a wait gave up)
       for (bool again = works; again;) {
-        walk();
+        chunk_walk(c, cta, s_rows, walker, s_segs, s_list, lanes_of_warp);
         __syncthreads();  // the segments are listed
         const int n = *s_segs;
         again = walker->more != 0;

@@ -32,6 +32,7 @@ constexpr int MASS_LO_BITS = 18;          // masses split into two 32-bit histog
 constexpr int NBINS = 256;                // radix digits of 8 bits
 
 #define Q3S_DEV __device__ __forceinline__
+#define Q3S_HOST_DEV __host__ __device__ __forceinline__
 
 // ---------------------------------------------------------------------------
 // scalar helpers
