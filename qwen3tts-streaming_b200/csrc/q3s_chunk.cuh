@@ -171,6 +171,12 @@ Q3S_HOST_DEV void chunk_walk(const ChunkArgs& c, int cta, const ChunkRow* rows, 
       break;
     }
     const ChunkRow x = k.b < CH_NT ? rows[k.b] : chunk_row(a, k.b);
+    if (x.n == 0) {  // on to the next row that has tokens, 32 at once (row by row 0.45 us each: 255 idle rows behind one of 300 tokens 141 us, so 31)
+      const int b = k.b + lane;
+      const unsigned next = l.ballot(b < a.B && (b < CH_NT ? rows[b] : chunk_row(a, b)).n > 0);
+      k.b += next ? l.first(next) : 32;
+      continue;
+    }
     const int pairs = (x.n + pair - 1) / pair;
     const long long items = static_cast<long long>(pairs) * a.H;
     if (k.item < 0) {  // the range starts in this row: skip to the tokens where it does
@@ -211,8 +217,8 @@ Q3S_HOST_DEV void chunk_walk(const ChunkArgs& c, int cta, const ChunkRow* rows, 
     k.cut |= l.ballot(lo < hi && lo == 0 && !whole) != 0;
     k.written += l.count(live);
     n += l.count(live);
-    if (l.ballot(item < items && start >= range1)) k.more = 0;
     k.at += l.shfl(up, 31);
+    if (k.at >= range1) k.more = 0;  // no later item starts before
     k.item += 32;
     if (k.item >= items) ++k.b, k.item = 0;
   }

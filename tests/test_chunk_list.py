@@ -38,3 +38,12 @@ def test_cut_items_are_defined_after_every_batch_of_segments(listed, rows, heads
     kernel reads, from a workspace that needs no initial value.  More segments a CTA than it lists at a time."""
     got = listed(rows, rows, 1, 3, 20, heads, 1)
     assert got["batches"] > 148 and got["segments"] > 64 * 148
+
+
+@pytest.mark.parametrize("rows,active,new", [(8000, 0, 300), (8000, 500, 300), (60000, 0, 2000), (2000, 1999, 5)])
+def test_rows_without_tokens_are_passed_over(listed, rows, active, new):
+    """Rows behind the last with tokens cost a CTA nothing, rows between them an operation of its lanes for 32 rows, not the
+    dozen that a row of its own takes: what a CTA does before its first copy goes by the rows that bring tokens."""
+    got = listed(rows, rows, active, new, 2000, 8, 2)
+    ranges = 1 if active == 0 else -(-rows // active)  # rows with tokens
+    assert got["operations"] <= 100 + 40 * ranges + (0 if active == 0 else rows // 32 + 2 * ranges)
