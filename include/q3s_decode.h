@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define Q3S_DECERR_LENGTHS 1   /* a negative length, or offsets that do not ascend (treated as 0 / cut) */
+#define Q3S_DECERR_LENGTHS 1   /* a negative length or one past the table's room, offsets that do not ascend or pass the tokens (treated as 0 / cut) */
 #define Q3S_DECERR_TABLE 2     /* a row outgrew its block table: it got no blocks */
 #define Q3S_DECERR_POOL 4      /* the free ring ran out: this row and later ones that need blocks got none */
 #define Q3S_DECERR_TOKENS 8    /* more new tokens than max_tokens: the rest have no slot (Q3S_TABLES_WHOLE_ROWS) */
@@ -284,11 +284,19 @@ q3s_status q3s_rotary(const q3s_rotary_desc* desc, void* stream);
  * [query_offsets[b], query_offsets[b+1])) stands at position
  *   p = prefix_length + lengths[b] - n + i
  * and sees the keys at positions (p - window, p], all up to p where window is 0.
- * Otherwise as q3s_prefix_attention: the same without a window, computed by a
- * kernel whose tiles are 128 query rows of one row of the batch and not 16 (with
- * few query rows and no window by q3s_prefix_attention's own).  Probabilities
- * are rounded to the cache's type for the product with v, as described there for
- * the prefix of a large batch. */
+ * (A row whose length does not count its new tokens has queries with p below
+ * prefix_length - 1.  The prefix's end does not bound them: as in
+ * q3s_prefix_attention they see all of the prefix, of which a window leaves out
+ * what lies at or before p - window.)
+ * Otherwise as q3s_prefix_attention, error_word included: the same without a
+ * window, computed by a kernel whose tiles are 128 query rows of one row of the
+ * batch and not 16, or, with few query rows (at most 112, or 20 a row of the
+ * batch, rows without tokens counted) and no window, by q3s_prefix_attention's
+ * own.  The kernel here rounds probabilities to the cache's type for the product
+ * with v, as described there for the prefix of a large batch; the other one
+ * holds those over own tokens as the sum of two such values.  So a row's last
+ * bits can depend on the batch around it; a window that leaves nothing out
+ * (2^31 - 1) always takes the kernel here. */
 #define Q3S_MAX_CHUNK_GROUP 128 /* query heads per key/value head */
 
 typedef struct q3s_chunk_attention_desc {

@@ -69,6 +69,11 @@ q3s_status check_sizes(const q3s_chunk_attention_desc* d) {
 // batch: 1 row of 8000 keys, 64: 31 and 36, 128: 43 and 39, 256: 78 and 43; 1 row of 200 keys, 128: 14 and 17, 512: 24 and 21;
 // 16 rows of 2000 keys, 15: 33 and 38, 31: 49 and 39; 64 rows of 1000 keys, 15: 52 and 59, 31: 82 and 60; 16 rows of 8000
 // keys, 7: 71 and 77, 15: 86 and 80; 4 heads of 64, 16 rows of 2000 keys, 15: 15 and 22, 63: 29 and 23.
+// The host knows the totals alone.  256 rows of 4000 keys, 2048 query rows: 8 each 664 and 827; half of them in one row, 4
+// in each of the others 697 and 1013; all in one row, the others without tokens 401 and 59.  A bound on the total that
+// takes the last of these to the kernel here would slow the first two; the caller can leave such rows out, or ask for this
+// kernel by a window that leaves nothing out.  Rows of 17 to 20 each, all alike, are two tiles there (64 rows of 1000 keys,
+// 20: 84 and 76; 256 of 4000: 1336 and 858); ragged ones of that mean are not (48 rows of up to 36: 54 and 60).
 bool few_queries(const q3s_chunk_attention_desc* d) {
   const int64_t G = d->q_heads / d->kv_heads;
   return d->window == 0 && G <= Q3S_MAX_QUERY_GROUP && d->tokens * G <= std::max<int64_t>(112, static_cast<int64_t>(d->batch) * 20);

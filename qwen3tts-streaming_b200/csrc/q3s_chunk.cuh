@@ -31,7 +31,8 @@ namespace q3s {
 constexpr int CH_M = PX_M, CH_KEYS = PX_KEYS;
 constexpr int CH_NT = 384;      // two softmax warpgroups, and one with the copy warp and three matrix warps
 constexpr int CH_SEGS = 64;     // segments of a CTA's range that are listed at a time
-// Registers a thread: a softmax thread holds a row of 128 scores.  Launched with 168 a thread, which is what the shares add up to.
+// Registers a thread: a softmax thread holds a unit's 64 scores of its row and their probabilities.  Launched with 168 a
+// thread, which is what the shares add up to.
 constexpr int CH_REGS_SOFTMAX = 184, CH_REGS_OTHER = 136;
 static_assert(2 * CH_REGS_SOFTMAX + CH_REGS_OTHER <= 3 * 168, "what the CTA is launched with");
 constexpr int CH_START = 2;     // cost of an item's start and end, in steps (2 rows of 4096 tokens: 0.7 261 us, 2 248, 4 251, 8 264)

@@ -204,8 +204,12 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``scale`` positive.  With ``window`` a query sees the ``window`` keys up to
     its own, counted over prefix and own tokens together.  Every row's query
     tokens are taken in tiles of 128 (tokens times heads of a group); where they
-    are too few for that (about 20 a row of the batch), without a window, the
-    call is ``prefix_attention``'s."""
+    are too few for that (at most 112, or 20 a row of the batch), without a
+    window, the call is ``prefix_attention``'s, whose tiles are 16.  Rows without
+    tokens count there: leave them out of a call for one long chunk, or give a
+    window that leaves nothing out (2**31 - 1), which always takes tiles of 128.
+    These round probabilities to the type of ``q`` once, as ``prefix_attention``
+    does over a large batch's prefix."""
     out, lse = _op("chunk_attention")(q, k_cache, v_cache, query_offsets, block_table, lengths, prefix_blocks,
                                       prefix_length, window, scale, error_word, slot_map)
     return (out, lse) if return_lse else out
